@@ -534,6 +534,100 @@ VVH_API int vvh_mirror_f32(const float* host, size_t n, int as_dtype, const void
 /* Drops the mirrors of a host array (both dtypes). */
 VVH_API int vvh_mirror_release(const float* host);
 
+/* ---- a decode step of several sequences ----------------------------------------
+ * The operators a program needs next to those above to decode several
+ * sequences together: a key-value cache in pages, the append to it, attention
+ * of one new token per sequence over it, linears of 4-bit weights, and the
+ * rules between a row of logits and the sampler.  No counterparts in the
+ * reference, which holds one sequence in one contiguous cache
+ * (src/kv_cache/kv_cache_cuda.cc:22-95).  Everything that differs between two
+ * steps (lengths, positions, page tables, histories) is read from device memory,
+ * so a captured step may be replayed with new values. */
+
+/* A paged cache.  Position p of sequence s is row p % page_size of page
+ * page_table[s * max_pages + p / page_size]; an entry outside [0, num_pages)
+ * is no page (not yet allocated, or given back). */
+typedef struct vvh_paged_cache {
+    void* k_pages;             /* device, [num_pages, page_size, num_kv_heads, head_dim] */
+    void* v_pages;             /* the same */
+    const int32_t* page_table; /* device, [num_seqs, max_pages] */
+    uint64_t num_pages;
+    uint64_t page_size;        /* any size >= 1 (num_pages * page_size < 2^31) */
+    uint64_t num_seqs;
+    uint64_t max_pages;
+    uint64_t num_kv_heads;
+    uint64_t head_dim;         /* <= 256 */
+    int32_t dtype;             /* VVH_F32 or VVH_F16: pages, queries and outputs */
+} vvh_paged_cache;
+
+/* Cosine and sine of every rotation pair of vvh_rope at positions [0, positions):
+ * table[(p * head_dim / 2 + i) * 2] and the float after it (device memory,
+ * positions * head_dim floats), for vvh_rope_append_paged. */
+VVH_API int vvh_rope_table(float* table, size_t positions, size_t head_dim, float theta, void* stream);
+/* vvh_rope_append for tokens of any sequences: token t (rows t of q [tokens,
+ * num_heads, head_dim] and of k and v [tokens, num_kv_heads, head_dim]) is
+ * position positions[t] of sequence seqs[t] (seqs NULL: sequence t).  Its
+ * rotated query goes to row t of q_out (q itself, or no overlap), its rotated
+ * key and its value into the cache; k stays as it is.  The rotation is vvh_rope's with the angles
+ * of rope_table ([rope_positions, head_dim / 2, 2], vvh_rope_table; head_dim
+ * even); rope_table NULL stores k as it is, for num_heads = 0 only.  A token whose sequence, position
+ * or page is out of range (-1 by convention: the padding of a captured batch)
+ * is left out: nothing is read or written for it.  No two tokens of a call
+ * may be one row of the cache. */
+VVH_API int vvh_rope_append_paged(const vvh_paged_cache* cache, void* q_out, const void* q, const void* k,
+                                  const void* v, const int32_t* seqs, const int32_t* positions, size_t tokens,
+                                  size_t num_heads, const float* rope_table, size_t rope_positions, void* stream);
+/* Attention of one query per sequence (the decode step of a batch): row s of
+ * q [num_seqs, num_heads, head_dim] attends to positions 0 .. lens[s] - 1 of
+ * sequence s, head h to kv head h / (num_heads / num_kv_heads); out
+ * [num_seqs, num_heads, head_dim], not q.  lens (device) counts positions from
+ * the sequence's start, the new token's among them; a length past the page table's
+ * max_pages * page_size counts as that, a negative one as 0.  Positions on
+ * entries that are no page are left out; a row without any position gives
+ * zeros.  max_len: the longest length to expect, 0 for unknown (the page table's
+ * capacity); it steers how the work is split, longer rows are attended in full
+ * all the same.  Cache rows that no sequence has reached may hold anything.  The
+ * split's partial sums use the stream's workspace, whose size depends only on
+ * num_seqs, the heads and max_len: make one such call before capturing on the stream. */
+VVH_API int vvh_attention_paged(const vvh_paged_cache* cache, void* out, const void* q, const int32_t* lens,
+                                size_t max_len, size_t num_heads, float scale, void* stream);
+/* Linear of 4-bit weights: out[M,N] = inp[M,K] . W[N,K]^T + bias[N] (+
+ * residual[M,N], may alias out), W[n][k] = (c - z) * scales[n][k / group] with
+ * the code c of 4 bits and its group's zero point z.  dev_weight: rows of K / 2
+ * bytes, code k in the low (k even) or high (k odd) half of byte k / 2;
+ * dev_scales: [N, K / group] fp16 bits; dev_zeros: [N, K / group] bytes, or
+ * NULL for 8 everywhere.  group 32, 64 or 128, K a multiple of it; inp and
+ * dev_weight 16-byte aligned.  Activations are used as given, products summed in
+ * fp32, the epilogue rounds once (as vvh_linear_q8).  Made for the few rows of a decode
+ * step; more than 64 are taken 64 at a time, each pass reading the weights again. */
+VVH_API int vvh_linear_q4(void* out, const void* inp, const uint8_t* dev_weight, const uint16_t* dev_scales,
+                          const uint8_t* dev_zeros, const float* dev_bias, const void* residual, size_t M, size_t N,
+                          size_t K, size_t group, int act_dtype, int out_dtype, void* stream);
+
+/* What is done to rows of logits before a token is chosen; every pointer is
+ * device memory and may be NULL where the rule is not wanted. */
+typedef struct vvh_logits_spec {
+    const int32_t* tokens;        /* row r's tokens so far: tokens[r * token_stride ..] */
+    uint64_t token_stride;
+    const int32_t* token_counts;  /* [rows] (clamped to token_stride); needed with tokens */
+    const int32_t* prompt_counts; /* [rows]: how many of them are the prompt's; NULL: none */
+    const float* repetition;      /* [rows]: logit > 0 ? logit / r : logit * r for tokens among them (r > 0) */
+    const float* frequency;       /* [rows]: - f * (times the token is among those after the prompt) */
+    const float* presence;        /* [rows]: - p for tokens among those after the prompt */
+    const int32_t* bias_ids;      /* row r: entries bias_offsets[r] .. bias_offsets[r + 1] - 1 of */
+    const float* bias_values;     /*   ids and values; of a token listed twice the last entry counts */
+    const int32_t* bias_offsets;  /* [rows + 1], clamped to [0, bias_count] */
+    uint64_t bias_count;
+    const uint32_t* mask;         /* row r: bit i % 32 of word mask[r * mask_stride + i / 32] clear: -infinity */
+    uint64_t mask_stride;         /* at least ceil(n / 32), or 0: one mask for all rows */
+} vvh_logits_spec;
+/* out[rows, n] = logits[rows, n] under the rules, in the order repetition,
+ * frequency, presence, bias, mask, in fp32 and rounded once to dtype; out may be
+ * logits itself (then only what a rule changes is written).  Tokens and ids outside [0, n) are ignored.
+ * vvh_argmax or vvh_sample then choose a row's token. */
+VVH_API int vvh_logits_rules(void* out, const void* logits, const vvh_logits_spec* rules, size_t rows, size_t n,
+                             int dtype, void* stream);
+
 typedef enum vvh_kernel {
     VVH_KERNEL_AUTO = 0,      /* size-based choice (default) */
     VVH_KERNEL_GENERIC = 1,   /* any shape / alignment, one thread per output */

@@ -35,6 +35,19 @@ class Q8Problem(ctypes.Structure):
                 ("scales", c_void_p), ("bias", c_void_p), ("M", c_uint64), ("N", c_uint64), ("K", c_uint64)]
 
 
+class PagedCache(ctypes.Structure):
+    _fields_ = [("k_pages", c_void_p), ("v_pages", c_void_p), ("page_table", c_void_p), ("num_pages", c_uint64),
+                ("page_size", c_uint64), ("num_seqs", c_uint64), ("max_pages", c_uint64), ("num_kv_heads", c_uint64),
+                ("head_dim", c_uint64), ("dtype", ctypes.c_int32)]
+
+
+class LogitsRules(ctypes.Structure):
+    _fields_ = [("tokens", c_void_p), ("token_stride", c_uint64), ("token_counts", c_void_p),
+                ("prompt_counts", c_void_p), ("repetition", c_void_p), ("frequency", c_void_p), ("presence", c_void_p),
+                ("bias_ids", c_void_p), ("bias_values", c_void_p), ("bias_offsets", c_void_p), ("bias_count", c_uint64),
+                ("mask", c_void_p), ("mask_stride", c_uint64)]
+
+
 _PP = POINTER(c_void_p)
 # name -> (restype, argtypes); every VVH_API function of include/vvllm_hip.h
 SIGNATURES = {
@@ -111,6 +124,13 @@ SIGNATURES = {
     "vvh_mirror_release": (c_int, [c_void_p]),
     "vvh_memcpy_d2d_async": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),
     "vvh_gemm_variant": (c_int, [c_size_t, c_size_t, c_size_t, POINTER(c_int), POINTER(c_int)]),
+    "vvh_rope_table": (c_int, [c_void_p, c_size_t, c_size_t, c_float, c_void_p]),
+    "vvh_rope_append_paged": (c_int, [POINTER(PagedCache), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                      c_size_t, c_size_t, c_void_p, c_size_t, c_void_p]),
+    "vvh_attention_paged": (c_int, [POINTER(PagedCache), c_void_p, c_void_p, c_void_p, c_size_t, c_size_t, c_float,
+                                    c_void_p]),
+    "vvh_linear_q4": (c_int, [c_void_p] * 7 + [c_size_t] * 4 + [c_int, c_int, c_void_p]),
+    "vvh_logits_rules": (c_int, [c_void_p, c_void_p, POINTER(LogitsRules), c_size_t, c_size_t, c_int, c_void_p]),
 }
 # entries that return a value rather than a vvh_status
 _NOT_STATUS = {"vvh_status_string", "vvh_last_error", "vvh_version", "vvh_device_cu_count",
@@ -238,6 +258,21 @@ def gemm_variant(M, N, K) -> str:
 
 def sync() -> None:
     call("vvh_sync")
+
+
+def quantize_q4(w: np.ndarray, group: int) -> tuple[np.ndarray, np.ndarray]:
+    """fp32 weights [N, K] as vvh_linear_q4 takes them, without zero points: per group of `group` weights of a row
+    scale = absmax / 7 rounded to fp16 and codes 8 + round(w / scale) in [0, 15], two to a byte; a group of zeros has
+    scale 0 and codes 8.  Returns (codes [N, K / 2] uint8, scales [N, K / group] fp16)."""
+    n, k = w.shape
+    if group not in (32, 64, 128) or k % group:
+        raise ValueError(f"groups of {group} over rows of {k}")
+    g = np.asarray(w, np.float32).reshape(n, k // group, group)
+    scales = np.minimum(np.abs(g).max(-1) / np.float32(7), np.float32(65504)).astype(np.float16)
+    s = scales.astype(np.float32)[..., None]
+    q = np.divide(g, s, out=np.zeros_like(g), where=s > 0)
+    c = (8 + np.clip(np.rint(q), -8, 7)).astype(np.uint8).reshape(n, k)
+    return c[:, 0::2] | c[:, 1::2] << 4, scales
 
 
 def plan_kernel(plan: int) -> str:

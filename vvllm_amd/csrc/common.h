@@ -407,6 +407,39 @@ int launch_argmax(const float* x, int64_t n, int32_t* idx, float* ws, void* stre
 int launch_sample(const void* x, int dtype, int64_t n, float temperature, uint64_t seed, int32_t step, int32_t* idx,
                   float* ws, void* stream);
 
+// Paged cache (paged_kernels.hip); slots (pages * page_size) below 2^31.
+struct PagedArgs {
+    void* kp;              // [pages, P, KVH, D]
+    void* vp;
+    const int32_t* table;  // [B, max_pages]
+    int32_t pages, P, B, max_pages, KVH, D;
+};
+// cosine and sine of every pair of vvh_rope at positions [0, positions)
+int launch_rope_table_theta(float* out, int64_t positions, int64_t D, float theta, void* stream);
+int launch_rope_append_paged(const PagedArgs& c, void* q_out, const void* q, const void* k, const void* v,
+                             const int32_t* seqs, const int32_t* positions, int64_t tokens, int64_t H,
+                             const float* rope, int64_t rope_positions, int dtype, void* stream);
+int launch_attention_paged(const PagedArgs& c, void* out, const void* q, const int32_t* lens, int64_t H, float scale,
+                           int dtype, void* stream);
+
+// 4-bit linear (q4_kernels.hip)
+struct Q4Args {
+    void* out;
+    const void* inp;
+    const void* res;       // may be null; may alias out
+    const uint8_t* w;      // [N, K / 2]
+    const uint16_t* scales;  // [N, K / group] fp16
+    const uint8_t* zeros;  // [N, K / group] or null (8)
+    const float* bias;     // [N] or null
+    int64_t M, N, K;
+    int32_t group;
+};
+int launch_linear_q4(const Q4Args& a, int act, int out, void* stream);
+
+// Logit rules (logits_kernels.hip)
+int launch_logits_rules(void* out, const void* logits, const vvh_logits_spec& r, int64_t rows, int64_t n, int dtype,
+                        void* stream);
+
 // Auxiliary kernels (aux_kernels.hip).
 // w: N x K elements of src_dtype (VVH_F32 or VVH_BF16)
 int launch_quantize(const void* w, int src_dtype, int64_t N, int64_t K, int8_t* q, float* scales, void* stream);

@@ -2333,6 +2333,131 @@ VVH_API int vvh_sample(const void* logits, int dtype, size_t n, float temperatur
                       "sample launch");
 }
 
+// ---- a decode step of several sequences -----------------------------------------------------
+// The checks of a paged cache, and its form for the launchers.
+static int paged_args(const vvh_paged_cache* c, PagedArgs* a)
+{
+    if (!c) return fail(VVH_ERR_INVALID_ARG, "cache is null");
+    if (!act_ok(c->dtype)) return fail(VVH_ERR_INVALID_ARG, "bad dtype");
+    if (!c->k_pages || !c->v_pages || !c->page_table) return fail(VVH_ERR_INVALID_ARG, "null pointer");
+    if (c->page_size == 0 || c->num_pages == 0 || c->max_pages == 0)
+        return fail(VVH_ERR_INVALID_ARG, "a cache has pages of at least one row");
+    if (c->num_kv_heads == 0 || c->head_dim == 0 || c->head_dim > 256)
+        return fail(VVH_ERR_INVALID_ARG, "%llu kv heads, head_dim %llu outside 1..256", (unsigned long long)c->num_kv_heads,
+                    (unsigned long long)c->head_dim);
+    if (c->num_pages > INT32_MAX || c->page_size > INT32_MAX / c->num_pages || c->max_pages > INT32_MAX ||
+        c->num_seqs > INT32_MAX || c->num_kv_heads > 65535)
+        return fail(VVH_ERR_UNSUPPORTED, "a cache of 2^31 rows, table columns or sequences, or 65536 kv heads");
+    const uintptr_t e = c->dtype == VVH_F32 ? 3 : 1;
+    if (((uintptr_t)c->k_pages & e) || ((uintptr_t)c->v_pages & e) || ((uintptr_t)c->page_table & 3))
+        return fail(VVH_ERR_INVALID_ARG, "misaligned pointer");
+    *a = PagedArgs{c->k_pages, c->v_pages, c->page_table, (int32_t)c->num_pages, (int32_t)c->page_size,
+                   (int32_t)c->num_seqs, (int32_t)c->max_pages, (int32_t)c->num_kv_heads, (int32_t)c->head_dim};
+    return VVH_OK;
+}
+
+VVH_API int vvh_rope_table(float* table, size_t positions, size_t head_dim, float theta, void* stream)
+{
+    if (head_dim % 2 != 0 || head_dim > 256) return fail(VVH_ERR_INVALID_ARG, "head_dim %zu is odd or above 256", head_dim);
+    if (positions > INT32_MAX) return fail(VVH_ERR_UNSUPPORTED, "%zu positions", positions);
+    if (positions == 0 || head_dim == 0) return VVH_OK;
+    if (!table) return fail(VVH_ERR_INVALID_ARG, "null pointer");
+    if ((uintptr_t)table & 7) return fail(VVH_ERR_INVALID_ARG, "misaligned table");
+    REQUIRE_INIT();
+    return ret_launch(launch_rope_table_theta(table, (int64_t)positions, (int64_t)head_dim, theta, stream),
+                      "rope table launch");
+}
+
+VVH_API int vvh_rope_append_paged(const vvh_paged_cache* cache, void* q_out, const void* q, const void* k, const void* v,
+                                  const int32_t* seqs, const int32_t* positions, size_t tokens, size_t num_heads,
+                                  const float* rope_table, size_t rope_positions, void* stream)
+{
+    PagedArgs a;
+    const int st = paged_args(cache, &a);
+    if (st != VVH_OK || tokens == 0) return st;
+    if (!k || !v || !positions || (num_heads && (!q || !q_out))) return fail(VVH_ERR_INVALID_ARG, "null pointer");
+    if (!seqs && tokens > cache->num_seqs)
+        return fail(VVH_ERR_INVALID_ARG, "%zu tokens of %llu sequences without seqs", tokens, (unsigned long long)cache->num_seqs);
+    if (rope_table ? cache->head_dim % 2 != 0 : num_heads != 0)
+        return fail(VVH_ERR_INVALID_ARG, rope_table ? "odd head_dim" : "queries without a rope table");
+    if (tokens > INT32_MAX || num_heads > 65535) return fail(VVH_ERR_UNSUPPORTED, "%zu tokens, %zu heads", tokens, num_heads);
+    const uintptr_t e = cache->dtype == VVH_F32 ? 3 : 1;
+    if ((((uintptr_t)q | (uintptr_t)q_out | (uintptr_t)k | (uintptr_t)v) & e) || (((uintptr_t)seqs | (uintptr_t)positions) & 3) ||
+        ((uintptr_t)rope_table & 7))
+        return fail(VVH_ERR_INVALID_ARG, "misaligned pointer");
+    REQUIRE_INIT();
+    return ret_launch(launch_rope_append_paged(a, q_out, q, k, v, seqs, positions, (int64_t)tokens, (int64_t)num_heads,
+                                               rope_table, (int64_t)std::min(rope_positions, (size_t)INT32_MAX),
+                                               cache->dtype, stream),
+                      "paged append launch");
+}
+
+VVH_API int vvh_attention_paged(const vvh_paged_cache* cache, void* out, const void* q, const int32_t* lens,
+                                size_t max_len, size_t num_heads, float scale, void* stream)
+{
+    PagedArgs a;
+    const int st = paged_args(cache, &a);
+    if (st != VVH_OK) return st;
+    if (num_heads % cache->num_kv_heads != 0)
+        return fail(VVH_ERR_INVALID_ARG, "num_heads %zu not a multiple of num_kv_heads %llu", num_heads,
+                    (unsigned long long)cache->num_kv_heads);
+    if (cache->num_seqs == 0 || num_heads == 0) return VVH_OK;
+    if (!out || !q || !lens) return fail(VVH_ERR_INVALID_ARG, "null pointer");
+    if (num_heads > 65535) return fail(VVH_ERR_UNSUPPORTED, "%zu heads", num_heads);
+    const uintptr_t e = cache->dtype == VVH_F32 ? 3 : 1;
+    if ((((uintptr_t)q | (uintptr_t)out) & e) || ((uintptr_t)lens & 3)) return fail(VVH_ERR_INVALID_ARG, "misaligned pointer");
+    (void)max_len;
+    REQUIRE_INIT();
+    return ret_launch(launch_attention_paged(a, out, q, lens, (int64_t)num_heads, scale, cache->dtype, stream),
+                      "paged attention launch");
+}
+
+VVH_API int vvh_linear_q4(void* out, const void* inp, const uint8_t* dev_weight, const uint16_t* dev_scales,
+                          const uint8_t* dev_zeros, const float* dev_bias, const void* residual, size_t M, size_t N,
+                          size_t K, size_t group, int act_dtype, int out_dtype, void* stream)
+{
+    if (!act_ok(act_dtype) || !act_ok(out_dtype)) return fail(VVH_ERR_INVALID_ARG, "bad dtype");
+    if (group != 32 && group != 64 && group != 128) return fail(VVH_ERR_INVALID_ARG, "groups of %zu, not 32, 64 or 128", group);
+    if (K % group != 0) return fail(VVH_ERR_INVALID_ARG, "K %zu is not whole groups of %zu", K, group);
+    uint64_t t;
+    if (!mul_ok(M, N, &t) || !mul_ok(N, K, &t) || !mul_ok(M, K, &t)) return fail(VVH_ERR_INVALID_ARG, "size overflow");
+    if (M == 0 || N == 0) return VVH_OK;
+    if (!out || (K > 0 && (!inp || !dev_weight || !dev_scales))) return fail(VVH_ERR_INVALID_ARG, "null pointer");
+    if (!aligned16(inp) || !aligned16(dev_weight) || ((uintptr_t)dev_scales & 1) || ((uintptr_t)dev_bias & 3) ||
+        (((uintptr_t)out | (uintptr_t)residual) & (dsize(out_dtype) - 1)))
+        return fail(VVH_ERR_INVALID_ARG, "misaligned pointer");
+    if (N > INT32_MAX || K > INT32_MAX / 2 || M > 65535 * 16) return fail(VVH_ERR_UNSUPPORTED, "M %zu, N %zu, K %zu", M, N, K);
+    REQUIRE_INIT();
+    const Q4Args a{out, inp, residual, dev_weight, dev_scales, dev_zeros, dev_bias, (int64_t)M, (int64_t)N, (int64_t)K,
+                   (int32_t)group};
+    return ret_launch(launch_linear_q4(a, act_dtype, out_dtype, stream), "4-bit linear launch");
+}
+
+VVH_API int vvh_logits_rules(void* out, const void* logits, const vvh_logits_spec* rules, size_t rows, size_t n,
+                             int dtype, void* stream)
+{
+    if (!act_ok(dtype)) return fail(VVH_ERR_INVALID_ARG, "bad dtype");
+    if (!rules) return fail(VVH_ERR_INVALID_ARG, "rules is null");
+    const vvh_logits_spec& r = *rules;
+    if (r.tokens ? !r.token_counts : r.repetition || r.frequency || r.presence)
+        return fail(VVH_ERR_INVALID_ARG, r.tokens ? "tokens without token_counts" : "penalties without tokens");
+    if (r.bias_offsets && r.bias_count > 0 && (!r.bias_ids || !r.bias_values))
+        return fail(VVH_ERR_INVALID_ARG, "bias_offsets without ids or values");
+    if (r.mask && r.mask_stride != 0 && r.mask_stride < (n + 31) / 32)
+        return fail(VVH_ERR_INVALID_ARG, "mask_stride %llu is short of %zu logits", (unsigned long long)r.mask_stride, n);
+    if (rows == 0 || n == 0) return VVH_OK;
+    if (!out || !logits) return fail(VVH_ERR_INVALID_ARG, "null pointer");
+    if (n > INT32_MAX || rows > 65535 || r.token_stride > INT32_MAX || r.bias_count > INT32_MAX || r.mask_stride > INT32_MAX)
+        return fail(VVH_ERR_UNSUPPORTED, "%zu rows of %zu logits", rows, n);
+    if ((((uintptr_t)out | (uintptr_t)logits) & (dsize(dtype) - 1)) ||
+        (((uintptr_t)r.tokens | (uintptr_t)r.token_counts | (uintptr_t)r.prompt_counts | (uintptr_t)r.repetition |
+          (uintptr_t)r.frequency | (uintptr_t)r.presence | (uintptr_t)r.bias_ids | (uintptr_t)r.bias_values |
+          (uintptr_t)r.bias_offsets | (uintptr_t)r.mask) & 3))
+        return fail(VVH_ERR_INVALID_ARG, "misaligned pointer");
+    REQUIRE_INIT();
+    return ret_launch(launch_logits_rules(out, logits, r, (int64_t)rows, (int64_t)n, dtype, stream), "logit rules launch");
+}
+
 VVH_API int vvh_mirror_f32(const float* host, size_t n, int as_dtype, const void** dev)
 {
     if (!dev) return fail(VVH_ERR_INVALID_ARG, "dev is null");
