@@ -419,8 +419,17 @@ int launch_rope_table_theta(float* out, int64_t positions, int64_t D, float thet
 int launch_rope_append_paged(const PagedArgs& c, void* q_out, const void* q, const void* k, const void* v,
                              const int32_t* seqs, const int32_t* positions, int64_t tokens, int64_t H,
                              const float* rope, int64_t rope_positions, int dtype, void* stream);
-int launch_attention_paged(const PagedArgs& c, void* out, const void* q, const int32_t* lens, int64_t H, float scale,
-                           int dtype, void* stream);
+// How a call is run: tiled on the matrix cores or by the form for any shape; tiled
+// with blocks > 0 split over 4 * blocks waves (ws_floats floats of workspace, a
+// merge launch), else one block per tile of GT heads (`tiles` of a kv head).
+struct AttnPagedPlan {
+    bool tiled;
+    int64_t GT, tiles, blocks, ws_floats;
+};
+AttnPagedPlan attention_paged_plan(const PagedArgs& c, const void* out, const void* q, int64_t max_len, int64_t H, int dtype,
+                                   int64_t cus);
+int launch_attention_paged(const AttnPagedPlan& p, const PagedArgs& c, void* out, const void* q, const int32_t* lens, int64_t H,
+                           float scale, float* ws, int dtype, void* stream);
 
 // 4-bit linear (q4_kernels.hip)
 struct Q4Args {

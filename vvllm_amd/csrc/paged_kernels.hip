@@ -5,6 +5,9 @@
 // [0, pages) is no page.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+#include <type_traits>
+
 #include "common.h"
 #include "device.h"
 
@@ -119,6 +122,470 @@ __global__ __launch_bounds__(256) void k_attention_paged(PagedArgs c, T* __restr
         out[((int64_t)s * H + h) * D + threadIdx.x] = (T)(M == -INFINITY && den == 0.0f ? 0.0f : num / den);
 }
 
+
+// ---------------------------------------------------------------------------
+// The matrix-core form: head_dim 64, 96 or 128, aligned arrays.
+//
+// A tile is up to 16 query heads of one kv head (GT of its G heads; VH = KVH *
+// ceil(G / GT) tiles a sequence).  One wave takes a tile's keys 64 (fp16) or 32
+// (fp32) at a time:
+//   S^T = K . q^T   A = K rows straight from the pages (lane: key l % 16, 8 or 4 dims of
+//                   group l / 16: one 16-byte load), B = the tile's queries in the same
+//                   dims.  A lane then has head l % 16's scores of keys 4 (l / 16) + i.
+//   softmax         online, in log2 units: maximum and sum over the lane's scores and the
+//                   4 lanes of the head; all of it in fp32.
+//   O^T += V^T P^T  B = the lane's own weights (the keys of a product's slots are any as long
+//                   as A has the same), A = V^T: fp16 V rows pass through the wave's LDS
+//                   region and its transposing read, weights as fp16 pairs high + low (22 bits); fp32 V
+//                   rows are loaded in A's layout (lane: 4 or 2 dims of key 4 (l / 16) + i), weights
+//                   as they are, on the fp32 matrix instruction.
+// A lane finds the row of key c0 + lane in the page table and hands it to the lanes that
+// load it.  A key past the end or on no page loads row 0 instead; its score becomes
+// -infinity and its value 0, whatever that row holds.
+// ---------------------------------------------------------------------------
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ h4 lds_tr16(const f16* p)
+{
+    typedef short s4v __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4v*)(p)));
+}
+
+template <typename T>
+struct PagedTile;
+
+template <>
+struct PagedTile<f16> {
+    static constexpr int CH = 64;  // keys at a time
+    template <int D>
+    struct Q {
+        h8 b[D / 32];
+    };
+    template <int D>
+    static constexpr int lds = CH * (D + 4);  // elements of a wave's V region
+};
+template <>
+struct PagedTile<float> {
+    static constexpr int CH = 32;
+    template <int D>
+    struct Q {
+        f4 b[D / 16];
+    };
+    template <int D>
+    static constexpr int lds = 0;
+};
+
+template <int D>
+__device__ __forceinline__ void paged_load_q(const f16* q, int heads, int lane, PagedTile<f16>::Q<D>& x)
+{
+#pragma unroll
+    for (int s = 0; s < D / 32; s++)
+        x.b[s] = (lane & 15) < heads ? *reinterpret_cast<const h8*>(q + (lane & 15) * D + 32 * s + 8 * (lane >> 4)) : h8{};
+}
+template <int D>
+__device__ __forceinline__ void paged_load_q(const float* q, int heads, int lane, PagedTile<float>::Q<D>& x)
+{
+#pragma unroll
+    for (int s = 0; s < D / 16; s++)
+        x.b[s] = (lane & 15) < heads ? *reinterpret_cast<const f4*>(q + (lane & 15) * D + 16 * s + 4 * (lane >> 4)) : f4{};
+}
+
+// Head (lane % 16)'s running maximum, sum and output fragments: o[e][i] is dim
+// paged_dim(e, lane / 16, i).
+template <int D>
+struct PagedAcc {
+    float m, l;
+    f4 o[D / 16];
+    __device__ __forceinline__ void clear()
+    {
+        m = -INFINITY;
+        l = 0.0f;
+#pragma unroll
+        for (int e = 0; e < D / 16; e++) o[e] = f4{};
+    }
+};
+template <typename T, int D>
+__device__ __forceinline__ constexpr int paged_dim(int e, int gr, int i)
+{
+    if (sizeof(T) == 2) return 16 * e + 4 * gr + i;
+    constexpr int VW = D % 64 == 0 ? 4 : 2;  // dims of a lane's V load
+    return 16 * VW * (e / VW) + VW * (4 * gr + i) + e % VW;
+}
+
+// The chunks c0, c0 + cstep, ... below ke of sequence s.  kh, vh: the kv head's column
+// in the pages.
+template <typename T, int D>
+__device__ __forceinline__ void paged_chunks(const PagedArgs& c, const T* kh, const T* vh, int32_t s,
+                                             const typename PagedTile<T>::template Q<D>& q, int32_t c0, int32_t cstep,
+                                             int32_t ke, float scale_log2, f16* vw, int lane, PagedAcc<D>& acc)
+{
+    constexpr int CH = PagedTile<T>::CH, NT = CH / 16;
+    constexpr bool H16 = sizeof(T) == 2;
+    constexpr int DS = H16 ? D / 32 : D / 16, DE = D / 16, VP = D + 4;
+    constexpr int VW = D % 64 == 0 ? 4 : 2, VJ = D / (16 * VW);
+    typedef float vf __attribute__((ext_vector_type(VW)));
+    const int r = lane & 15, gr = lane >> 4;
+    const int64_t kvs = (int64_t)c.KVH * D;
+    const int32_t* table = c.table + (int64_t)s * c.max_pages;
+    // the row of key c0 + lane (lanes past CH: of no key)
+    auto find = [&](int32_t at) {
+        const uint32_t key = (uint32_t)at + (uint32_t)lane;
+        if (lane >= CH || key >= (uint32_t)ke) return -1;
+        const uint32_t pg = key / (uint32_t)c.P;
+        const int32_t page = table[pg];
+        return page < 0 || page >= c.pages ? -1 : page * c.P + (int32_t)(key - pg * (uint32_t)c.P);
+    };
+    int32_t row = c0 < ke ? find(c0) : -1;
+    for (; c0 < ke; c0 += cstep) {
+        const uint64_t live = __ballot(row >= 0);
+        const bool all = live == (CH == 64 ? ~0ull : (1ull << CH) - 1);
+        const int32_t at = row < 0 ? 0 : row;
+        auto row_of = [&](int j) { return (int64_t)__shfl(at, j) * kvs; };
+        f4 sc[NT];
+        typename std::conditional<H16, h8, f4>::type ka[NT][DS];
+        h8 vr[H16 ? CH * D / 512 : 1];
+        vf vv[H16 ? 1 : NT][H16 ? 1 : 4][VJ];
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            const T* kr = kh + row_of(16 * t + r);
+#pragma unroll
+            for (int x = 0; x < DS; x++) {
+                if constexpr (H16) ka[t][x] = *reinterpret_cast<const h8*>(kr + 32 * x + 8 * gr);
+                else ka[t][x] = *reinterpret_cast<const f4*>(kr + 16 * x + 4 * gr);
+            }
+        }
+        if constexpr (H16) {
+#pragma unroll
+            for (int i = 0; i < CH * D / 512; i++) {
+                const int p = i * 64 + lane, j = p / (D / 8), col = p % (D / 8) * 8;
+                vr[i] = *reinterpret_cast<const h8*>(vh + row_of(j) + col);
+            }
+        } else {
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const T* vp = vh + row_of(16 * t + 4 * gr + i) + VW * r;
+#pragma unroll
+                    for (int x = 0; x < VJ; x++) vv[t][i][x] = *reinterpret_cast<const vf*>(vp + 16 * VW * x);
+                }
+        }
+        // the next chunk's rows are on their way while this one is worked on
+        const int32_t next = c0 + cstep < ke ? find(c0 + cstep) : -1;
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            sc[t] = f4{};
+#pragma unroll
+            for (int x = 0; x < DS; x++) {
+                if constexpr (H16) {
+                    sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[t][x], q.b[x], sc[t], 0, 0, 0);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        sc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(ka[t][x][j], q.b[x][j], sc[t], 0, 0, 0);
+                }
+            }
+        }
+        float cm = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float x = sc[t][i] * scale_log2;
+                if (!all && !(live >> (16 * t + 4 * gr + i) & 1)) x = -INFINITY;
+                sc[t][i] = x;
+                cm = fmaxf(cm, x);
+            }
+        cm = max_x32(max_x16(cm));
+        const float mn = fmaxf(acc.m, cm);
+        const float mb = mn == -INFINITY ? 0.0f : mn;  // no key yet: every weight below is 0
+        const float corr = exp2f(acc.m - mb);
+        float ps = 0.0f;
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                sc[t][i] = exp2f(sc[t][i] - mb);
+                ps += sc[t][i];
+            }
+        ps = sum_x32(sum_x16(ps));
+        acc.l = __builtin_fmaf(acc.l, corr, ps);
+        acc.m = mn;
+#pragma unroll
+        for (int e = 0; e < DE; e++) acc.o[e] *= corr;
+        if constexpr (H16) {
+            if (!all) {
+#pragma unroll
+                for (int i = 0; i < CH * D / 512; i++)
+                    if (!(live >> ((i * 64 + lane) / (D / 8)) & 1)) vr[i] = h8{};
+            }
+            // one wave's LDS accesses complete in order: the reads below see these rows,
+            // and the next chunk's writes come after them
+#pragma unroll
+            for (int i = 0; i < CH * D / 512; i++) {
+                const int p = i * 64 + lane, j = p / (D / 8), col = p % (D / 8) * 8;
+                *reinterpret_cast<h4*>(vw + j * VP + col) = h4{vr[i][0], vr[i][1], vr[i][2], vr[i][3]};
+                *reinterpret_cast<h4*>(vw + j * VP + col + 4) = h4{vr[i][4], vr[i][5], vr[i][6], vr[i][7]};
+            }
+#pragma unroll
+            for (int u = 0; u < NT / 2; u++) {
+                h8 hi, lo;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const float w = sc[2 * u + j / 4][j % 4];
+                    hi[j] = (f16)w;
+                    lo[j] = (f16)(w - (float)hi[j]);
+                }
+                // lane (r, gr): V[32 u + 4 gr + j][16 e + r] and the same 16 keys on, j < 4: in each
+                // group of 16 lanes the transposing read gives lane i element i % 4 of lane 4 j + i / 4's
+                // piece, so lane s points at dims 16 e + 4 (s % 4) of key 4 gr + s / 4
+#pragma unroll
+                for (int e = 0; e < DE; e++) {
+                    const f16* src = vw + (32 * u + 4 * gr + (r >> 2)) * VP + 16 * e + 4 * (r & 3);
+                    const h4 a = lds_tr16(src), b = lds_tr16(src + 16 * VP);
+                    const h8 va = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+                    acc.o[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, hi, acc.o[e], 0, 0, 0);
+                    acc.o[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, lo, acc.o[e], 0, 0, 0);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    if (!all && !(live >> (16 * t + 4 * gr + i) & 1)) {
+#pragma unroll
+                        for (int x = 0; x < VJ; x++) vv[t][i][x] = vf{};
+                    }
+#pragma unroll
+                    for (int e = 0; e < DE; e++)
+                        acc.o[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv[t][i][e / VW][e % VW], sc[t][i], acc.o[e], 0, 0, 0);
+                }
+        }
+        row = next;
+    }
+}
+
+// Sequence s's length, as the kernels take it
+__device__ __forceinline__ int32_t paged_len(const PagedArgs& c, const int32_t* lens, int32_t s)
+{
+    const int64_t cap = (int64_t)c.max_pages * c.P;
+    const int32_t n = lens[s];
+    return n < 0 ? 0 : n < cap ? n : (int32_t)cap;
+}
+
+// What tile v of a sequence is: its kv head, first query head and number of heads.
+struct PagedHeads {
+    int32_t G, GT, tiles;  // heads of a kv head, of a tile, tiles of a kv head
+    __device__ __forceinline__ void at(int32_t v, int32_t& g, int32_t& h0, int32_t& n) const
+    {
+        g = v / tiles;
+        const int32_t t = v - g * tiles;
+        h0 = g * G + t * GT;
+        n = G - t * GT < GT ? G - t * GT : GT;
+    }
+};
+
+// One tile of one sequence by one block, its NW waves each every NW-th chunk, merged
+// through LDS: short contexts, in one launch.
+template <typename T, int D, int NW>
+__global__ __launch_bounds__(64 * NW) void k_attention_paged_one(PagedArgs c, T* __restrict__ out, const T* __restrict__ q,
+                                                                 const int32_t* __restrict__ lens, PagedHeads hd, int32_t H,
+                                                                 float scale_log2)
+{
+    constexpr int CH = PagedTile<T>::CH, OP = D + 4;
+    constexpr int VB = PagedTile<T>::template lds<D> * 2, OB = 16 * OP * 4;  // bytes a wave
+    __shared__ __align__(16) char smem[NW * (VB > OB ? VB : OB)];
+    __shared__ float wm[NW][16], wl[NW][16];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r = lane & 15, gr = lane >> 4;
+    const int32_t s = blockIdx.y, len = paged_len(c, lens, s);
+    int32_t g, h0, n;
+    hd.at(blockIdx.x, g, h0, n);
+    const int64_t row0 = (int64_t)s * H + h0;
+    typename PagedTile<T>::template Q<D> x;
+    paged_load_q<D>(q + row0 * D, n, lane, x);
+    PagedAcc<D> acc;
+    acc.clear();
+    paged_chunks<T, D>(c, (const T*)c.kp + g * D, (const T*)c.vp + g * D, s, x, w * CH, NW * CH, len, scale_log2,
+                       reinterpret_cast<f16*>(smem + w * VB), lane, acc);
+    __syncthreads();
+    float* os = reinterpret_cast<float*>(smem);
+    if (gr == 0) {
+        wm[w][r] = acc.m;
+        wl[w][r] = acc.l;
+    }
+#pragma unroll
+    for (int e = 0; e < D / 16; e++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) os[(w * 16 + r) * OP + paged_dim<T, D>(e, gr, i)] = acc.o[e][i];
+    __syncthreads();
+    for (int idx = threadIdx.x; idx < n * D; idx += 64 * NW) {
+        const int h = idx / D, d = idx - h * D;
+        float M = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < NW; i++) M = fmaxf(M, wm[i][h]);
+        const float Mb = M == -INFINITY ? 0.0f : M;
+        float num = 0.0f, den = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NW; i++) attn_merge_add(num, den, wm[i][h], Mb, os[(i * 16 + h) * OP + d], wl[i][h]);
+        out[row0 * D + idx] = (T)(den == 0.0f ? 0.0f : num / den);
+    }
+}
+
+// Chunks of the 64 sequences from s0 on, one a lane, and their sums up to each lane.
+__device__ __forceinline__ int32_t paged_window(const PagedArgs& c, const int32_t* lens, int32_t s0, int lane, int ch)
+{
+    return s0 + lane < c.B ? (paged_len(c, lens, s0 + lane) + ch - 1) / ch : 0;
+}
+__device__ __forceinline__ int64_t wave_scan(int64_t v, int lane)
+{
+    for (int o = 1; o < 64; o <<= 1) {
+        const int64_t u = __shfl_up(v, o);
+        if (lane >= o) v += u;
+    }
+    return v;
+}
+
+// All chunks of all tiles of all sequences in one row (sequence by sequence, tile by
+// tile): wave w of W (all waves, or T) takes units [T w / W, T (w + 1) / W) of its T, so
+// every wave has the same work however ragged the batch.  The part of a tile that a wave has goes
+// straight to out if it is the whole tile, else to the wave's slot 1 (a tile that
+// begins in its range) or 0, a row per head: O, m, l.  k_attention_paged_merge joins them.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void k_attention_paged_split(PagedArgs c, T* __restrict__ out, const T* __restrict__ q,
+                                                               const int32_t* __restrict__ lens, PagedHeads hd, int32_t H,
+                                                               float scale_log2, float* __restrict__ ws, int32_t VH)
+{
+    constexpr int CH = PagedTile<T>::CH;
+    constexpr int VB = PagedTile<T>::template lds<D>;
+    __shared__ __align__(16) f16 vs[VB ? 4 * VB : 4];
+    const int lane = threadIdx.x & 63, r = lane & 15, gr = lane >> 4;
+    const int wb = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t w = (int64_t)blockIdx.x * 4 + wb;
+    int64_t total = 0;
+    for (int32_t s0 = 0; s0 < c.B; s0 += 64) total += paged_window(c, lens, s0, lane, CH);
+    total = __shfl(wave_scan(total, lane), 63) * VH;
+    const int64_t W = total < (int64_t)gridDim.x * 4 ? total : (int64_t)gridDim.x * 4;  // no wave without a unit
+    if (w >= W) return;
+    const int64_t u0 = total * w / W, u1 = total * (w + 1) / W;
+    // the window of sequences that holds unit u0
+    int32_t s0 = 0, n = paged_window(c, lens, 0, lane, CH);
+    int64_t before = 0, upto = wave_scan(n, lane);
+    while ((before + __shfl(upto, 63)) * VH <= u0) {
+        before += __shfl(upto, 63);
+        s0 += 64;
+        n = paged_window(c, lens, s0, lane, CH);
+        upto = wave_scan(n, lane);
+    }
+    int sl = __builtin_ctzll(__ballot((before + upto) * VH > u0));  // the sequence's lane
+    int32_t ns = __shfl(n, sl);
+    int64_t rest = u0 - (before + __shfl(upto, sl) - ns) * VH;  // units before u0 in the sequence
+    int32_t v = (int32_t)(rest / ns), ci = (int32_t)(rest - (int64_t)v * ns);
+    for (int64_t u = u0; u < u1;) {
+        const int32_t s = s0 + sl, cnt = (int32_t)(ns - ci < u1 - u ? ns - ci : u1 - u);
+        int32_t g, h0, nh;
+        hd.at(v, g, h0, nh);
+        const int64_t row0 = (int64_t)s * H + h0;
+        typename PagedTile<T>::template Q<D> x;
+        paged_load_q<D>(q + row0 * D, nh, lane, x);
+        PagedAcc<D> acc;
+        acc.clear();
+        const int32_t len = paged_len(c, lens, s);
+        const int64_t end = (int64_t)(ci + cnt) * CH;
+        paged_chunks<T, D>(c, (const T*)c.kp + g * D, (const T*)c.vp + g * D, s, x, ci * CH, CH,
+                           end < len ? (int32_t)end : len, scale_log2, vs + wb * VB, lane, acc);
+        if (r < nh) {
+            if (cnt == ns) {
+                const float inv = acc.l == 0.0f ? 0.0f : 1.0f / acc.l;
+#pragma unroll
+                for (int e = 0; e < D / 16; e++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        out[(row0 + r) * D + paged_dim<T, D>(e, gr, i)] = (T)(acc.o[e][i] * inv);
+            } else {
+                float* p = ws + ((w * 2 + (ci == 0)) * hd.GT + r) * (D + 4);
+#pragma unroll
+                for (int e = 0; e < D / 16; e++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) p[paged_dim<T, D>(e, gr, i)] = acc.o[e][i];
+                if (gr == 0) {
+                    p[D] = acc.m;
+                    p[D + 1] = acc.l;
+                }
+            }
+        }
+        u += cnt;
+        ci = 0;
+        if (++v == VH && u < u1) {  // the next sequence that has a key: u < u1 <= total, so there is one
+            v = 0;
+            uint64_t more = __ballot(n > 0) & (sl == 63 ? 0 : ~0ull << (sl + 1));
+            while (!more) {
+                s0 += 64;
+                n = paged_window(c, lens, s0, lane, CH);
+                more = __ballot(n > 0);
+            }
+            sl = __builtin_ctzll(more);
+            ns = __shfl(n, sl);
+        }
+    }
+}
+
+// Block (h, s, z): dims 32 z .. of head h of sequence s.  Thread (x, d) merges every
+// S-th part (S = blockDim.x / 32) into a running maximum and sums rescaled to it, the S
+// of a dim merge the same way through LDS.
+template <typename T, int D>
+__global__ __launch_bounds__(1024) void k_attention_paged_merge(PagedArgs c, T* __restrict__ out,
+                                                                const int32_t* __restrict__ lens, PagedHeads hd, int32_t H,
+                                                                const float* __restrict__ ws, int32_t VH, int64_t waves, int32_t CH)
+{
+    __shared__ float sm[1024], sn[1024], sd[1024];
+    const int tid = threadIdx.x, lane = tid & 63, d = blockIdx.z * 32 + (tid & 31), x = tid >> 5, S = blockDim.x >> 5;
+    const int32_t h = blockIdx.x, s = blockIdx.y, g = h / hd.G, t = (h - g * hd.G) / hd.GT, hr = h - g * hd.G - t * hd.GT;
+    const int32_t v = g * hd.tiles + t;
+    int64_t sum = 0, mine = 0;
+    for (int32_t s0 = 0; s0 < c.B; s0 += 64) {
+        const int32_t n = paged_window(c, lens, s0, lane, CH);
+        sum += n;
+        mine += s0 + lane < s ? n : 0;
+    }
+    for (int o = 32; o > 0; o >>= 1) {
+        sum += __shfl_xor(sum, o);
+        mine += __shfl_xor(mine, o);
+    }
+    const int32_t ns = (paged_len(c, lens, s) + CH - 1) / CH;
+    const int64_t at = ((int64_t)s * H + h) * D + d;
+    if (ns == 0) {
+        if (x == 0) out[at] = (T)0.0f;
+        return;
+    }
+    const int64_t total = sum * VH, a = mine * VH + (int64_t)v * ns, b = a + ns - 1;  // first and last unit
+    const int64_t W = total < waves ? total : waves;
+    const int64_t w0 = ((a + 1) * W - 1) / total, w1 = ((b + 1) * W - 1) / total;
+    if (w0 == w1) return;  // one wave had it all
+    float M = -INFINITY, num = 0.0f, den = 0.0f;
+#pragma unroll 4
+    for (int64_t w = w0 + x; w <= w1; w += S) {
+        const float* p = ws + ((w * 2 + (w == w0)) * hd.GT + hr) * (D + 4);
+        const float m = p[D], l = p[D + 1], o = p[d];
+        const float mn = fmaxf(M, m), mb = mn == -INFINITY ? 0.0f : mn;
+        const float f = exp2f(M - mb), e = exp2f(m - mb);
+        num = num * f + o * e;
+        den = den * f + l * e;
+        M = mn;
+    }
+    sm[tid] = M;
+    sn[tid] = num;
+    sd[tid] = den;
+    __syncthreads();
+    if (x) return;
+    float mt = -INFINITY;
+    for (int i = 0; i < S; i++) mt = fmaxf(mt, sm[i * 32 + tid]);
+    const float mb = mt == -INFINITY ? 0.0f : mt;
+    num = den = 0.0f;
+    for (int i = 0; i < S; i++) attn_merge_add(num, den, sm[i * 32 + tid], mb, sn[i * 32 + tid], sd[i * 32 + tid]);
+    out[at] = (T)(den == 0.0f ? 0.0f : num / den);
+}
+
 }  // namespace
 
 int launch_rope_table_theta(float* out, int64_t positions, int64_t D, float theta, void* stream)
@@ -144,16 +611,74 @@ int launch_rope_append_paged(const PagedArgs& c, void* q_out, const void* q, con
     return (int)hipGetLastError();
 }
 
-int launch_attention_paged(const PagedArgs& c, void* out, const void* q, const int32_t* lens, int64_t H, float scale,
-                           int dtype, void* stream)
+
+// Chunks of a context from which its tiles are split over waves.
+constexpr int64_t kPagedOneChunks = 16;
+
+bool attention_paged_tiled(const PagedArgs& c, const void* out, const void* q, int dtype)
 {
-    const dim3 grid((unsigned)H, (unsigned)c.B);
-    auto go = [&](auto kern, auto* t) {
+    const uintptr_t all = (uintptr_t)c.kp | (uintptr_t)c.vp | (uintptr_t)q;
+    (void)out;
+    return (c.D == 64 || c.D == 96 || c.D == 128) && all % 16 == 0 && (dtype == VVH_F16 || dtype == VVH_F32);
+}
+
+AttnPagedPlan attention_paged_plan(const PagedArgs& c, const void* out, const void* q, int64_t max_len, int64_t H, int dtype,
+                                   int64_t cus)
+{
+    AttnPagedPlan p{};
+    const int64_t G = H / c.KVH;
+    p.tiled = attention_paged_tiled(c, out, q, dtype);
+    p.tiles = (G + 15) / 16;
+    p.GT = (G + p.tiles - 1) / p.tiles;
+    if (!p.tiled) return p;
+    const int64_t cap = (int64_t)c.max_pages * c.P;
+    const int64_t len = max_len > 0 && max_len < cap ? max_len : cap;
+    const int64_t chunks = (len + 63) / 64;
+    if (chunks > kPagedOneChunks) {
+        const int64_t units = chunks * c.B * c.KVH * p.tiles;
+        p.blocks = std::min<int64_t>((units + 3) / 4, 2 * cus);
+    }
+    p.ws_floats = p.blocks * 4 * 2 * p.GT * (c.D + 4);
+    return p;
+}
+
+template <typename T, int D>
+static void paged_go(const AttnPagedPlan& p, const PagedArgs& c, T* out, const T* q, const int32_t* lens, int64_t H,
+                     float scale_log2, float* ws, hipStream_t s)
+{
+    const PagedHeads hd{(int32_t)(H / c.KVH), (int32_t)p.GT, (int32_t)p.tiles};
+    const int32_t VH = (int32_t)(c.KVH * p.tiles);
+    if (p.blocks == 0) {
+        hipLaunchKernelGGL((k_attention_paged_one<T, D, 4>), dim3((unsigned)VH, (unsigned)c.B), dim3(256), 0, s, c, out, q, lens,
+                           hd, (int32_t)H, scale_log2);
+        return;
+    }
+    hipLaunchKernelGGL((k_attention_paged_split<T, D>), dim3((unsigned)p.blocks), dim3(256), 0, s, c, out, q, lens, hd,
+                       (int32_t)H, scale_log2, ws, VH);
+    const int64_t W = p.blocks * 4;
+    int64_t S = 2;
+    while (S < 32 && S * 4 < W / ((int64_t)VH * c.B)) S *= 2;
+    hipLaunchKernelGGL((k_attention_paged_merge<T, D>), dim3((unsigned)H, (unsigned)c.B, D / 32), dim3((unsigned)(32 * S)), 0, s,
+                       c, out, lens, hd, (int32_t)H, ws, VH, W, (int32_t)PagedTile<T>::CH);
+}
+
+int launch_attention_paged(const AttnPagedPlan& p, const PagedArgs& c, void* out, const void* q, const int32_t* lens, int64_t H,
+                           float scale, float* ws, int dtype, void* stream)
+{
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    auto go = [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        hipLaunchKernelGGL(kern, grid, dim3(256), 0, static_cast<hipStream_t>(stream), c, (T*)out, (const T*)q, lens,
-                           (int32_t)H, scale);
+        if (p.tiled) {
+            const float sl = (float)((double)scale * 1.4426950408889634);  // scores in log2 units
+            if (c.D == 64) paged_go<T, 64>(p, c, (T*)out, (const T*)q, lens, H, sl, ws, st);
+            else if (c.D == 96) paged_go<T, 96>(p, c, (T*)out, (const T*)q, lens, H, sl, ws, st);
+            else paged_go<T, 128>(p, c, (T*)out, (const T*)q, lens, H, sl, ws, st);
+        } else {
+            hipLaunchKernelGGL(k_attention_paged<T>, dim3((unsigned)H, (unsigned)c.B), dim3(256), 0, st, c, (T*)out,
+                               (const T*)q, lens, (int32_t)H, scale);
+        }
     };
-    dtype == VVH_F16 ? go(k_attention_paged<f16>, (f16*)nullptr) : go(k_attention_paged<float>, (float*)nullptr);
+    dtype == VVH_F16 ? go((f16*)nullptr) : go((float*)nullptr);
     return (int)hipGetLastError();
 }
 

@@ -2345,9 +2345,9 @@ static int paged_args(const vvh_paged_cache* c, PagedArgs* a)
     if (c->num_kv_heads == 0 || c->head_dim == 0 || c->head_dim > 256)
         return fail(VVH_ERR_INVALID_ARG, "%llu kv heads, head_dim %llu outside 1..256", (unsigned long long)c->num_kv_heads,
                     (unsigned long long)c->head_dim);
-    if (c->num_pages > INT32_MAX || c->page_size > INT32_MAX / c->num_pages || c->max_pages > INT32_MAX ||
-        c->num_seqs > INT32_MAX || c->num_kv_heads > 65535)
-        return fail(VVH_ERR_UNSUPPORTED, "a cache of 2^31 rows, table columns or sequences, or 65536 kv heads");
+    if (c->num_pages > INT32_MAX || c->page_size > INT32_MAX / c->num_pages ||
+        c->max_pages > (uint64_t(1) << 30) / c->page_size || c->num_seqs > 65535 || c->num_kv_heads > 65535)
+        return fail(VVH_ERR_UNSUPPORTED, "a cache of 2^31 rows, 2^30 positions a sequence, 65536 sequences or kv heads");
     const uintptr_t e = c->dtype == VVH_F32 ? 3 : 1;
     if (((uintptr_t)c->k_pages & e) || ((uintptr_t)c->v_pages & e) || ((uintptr_t)c->page_table & 3))
         return fail(VVH_ERR_INVALID_ARG, "misaligned pointer");
@@ -2406,9 +2406,15 @@ VVH_API int vvh_attention_paged(const vvh_paged_cache* cache, void* out, const v
     if (num_heads > 65535) return fail(VVH_ERR_UNSUPPORTED, "%zu heads", num_heads);
     const uintptr_t e = cache->dtype == VVH_F32 ? 3 : 1;
     if ((((uintptr_t)q | (uintptr_t)out) & e) || ((uintptr_t)lens & 3)) return fail(VVH_ERR_INVALID_ARG, "misaligned pointer");
-    (void)max_len;
     REQUIRE_INIT();
-    return ret_launch(launch_attention_paged(a, out, q, lens, (int64_t)num_heads, scale, cache->dtype, stream),
+    const AttnPagedPlan p = attention_paged_plan(a, out, q, (int64_t)std::min(max_len, (size_t)INT32_MAX), (int64_t)num_heads,
+                                                 cache->dtype, g_cu_count > 0 ? g_cu_count : 256);
+    float* ws = nullptr;
+    if (p.ws_floats > 0) {
+        const int ws_st = workspace_for(stream, (std::size_t)p.ws_floats * 4, &ws);
+        if (ws_st != VVH_OK) return ws_st;
+    }
+    return ret_launch(launch_attention_paged(p, a, out, q, lens, (int64_t)num_heads, scale, ws, cache->dtype, stream),
                       "paged attention launch");
 }
 
