@@ -443,7 +443,7 @@ struct Q4Args {
     int64_t M, N, K;
     int32_t group;
 };
-int launch_linear_q4(const Q4Args& a, int act, int out, void* stream);
+int launch_linear_q4(const Q4Args& a, int act, int out, int64_t cus, void* stream);
 
 // Logit rules (logits_kernels.hip)
 int launch_logits_rules(void* out, const void* logits, const vvh_logits_spec& r, int64_t rows, int64_t n, int dtype,

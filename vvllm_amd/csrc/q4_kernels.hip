@@ -4,6 +4,8 @@
 // where there are none).
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "common.h"
 #include "device.h"
 
@@ -11,50 +13,302 @@ namespace vvh {
 
 namespace {
 
-// One wave per output channel: lane l takes the 8 codes of dword l, l + 64, ... of
-// the weight row (one group: groups are whole dwords) for up to 8 rows of x.
-template <typename T, typename OT>
-__global__ __launch_bounds__(256) void k_linear_q4(Q4Args a)
+// ---------------------------------------------------------------------------
+// A wave owns a tile of 16 output channels and takes its weight rows 256 codes (one
+// 128-byte line of each) a step; KS waves of a block share a tile's steps, their sums
+// are added through LDS in order.  Up to 16 rows of x are a pass, staged in LDS.
+//
+// Loads: lane l reads the 16-byte piece l % 8 of the lines of rows l / 8 and 8 + l / 8, so
+// that an instruction covers 8 whole lines, kQ4Depth steps ahead of use.  A step's 16 lines go
+// through the wave's LDS tile, whose rows a lane reads back as the matrix instruction
+// wants them: lane (n, g4) 8 codes of channel n, the four lanes of a channel 32 codes of one
+// group, whose sum the instruction gives and the group's scale multiplies in fp32.
+// Codes: a nibble in the low bits of an fp16 of exponent 2^10 is 1024 + c (in the second
+// nibble 1024 + 16 c); one packed subtraction (or multiply-add by 1 / 16) leaves c - z, exactly.
+// The dword of 8 codes gives them in the order 0 4 1 5 2 6 3 7, and x is staged in that order.
+// fp32 rows of x are staged as two fp16 planes, high and low parts of x times a power of two that
+// puts the step's largest |x| into [2^14, 2^15) (22 bits; the sum of a step is multiplied back).
+// ---------------------------------------------------------------------------
+constexpr int kQ4Depth = 4;
+constexpr int kQ4Step = 256;     // codes of a row a step
+constexpr int kQ4WPitch = 144;   // bytes between rows of the LDS weight tile
+constexpr int kQ4SPitch = 12;    // dwords between rows of its scales
+constexpr int kQ4Tile = 16 * kQ4WPitch + 16 * kQ4SPitch * 4;
+constexpr int kQ4Rows = 16;
+
+// What a launch's blocks share out.
+struct Q4Launch {
+    int32_t waves;     // of a block
+    int32_t ks;        // waves that share a tile
+    int32_t seg;       // steps of x in LDS at a time
+    int32_t passes;    // of 16 rows
+    int32_t groups_n;  // blocks of a pass
+    int32_t rows;      // of x in LDS: the largest pass
+    int32_t out_f16;
+};
+
+__device__ __forceinline__ h2 q4_h2(uint32_t v) { return __builtin_bit_cast(h2, v); }
+
+// 8 codes minus their zero point; zl = 1024 + z, zh = 64 + z
+__device__ __forceinline__ h8 q4_codes(uint32_t w, h2 zl, h2 zh)
 {
-    const int lane = threadIdx.x & 63;
-    const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (n >= a.N) return;
-    const int64_t groups = a.K / a.group;
-    for (int64_t m0 = 0; m0 < a.M; m0 += 8) {
-        float acc[8] = {};
-        for (int64_t k = lane * 8; k < a.K; k += 512) {
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(a.w + (n * a.K + k) / 2);
-            const int64_t g = n * groups + k / a.group;
-            const float s = (float)reinterpret_cast<const f16*>(a.scales)[g], z = a.zeros ? (float)a.zeros[g] : 8.0f;
+    const h2 sixteenth = {(f16)0.0625f, (f16)0.0625f};
+    const uint32_t v = w >> 8;
+    const h2 a = q4_h2((w & 0x000F000Fu) | 0x64006400u) - zl;
+    const h2 b = __builtin_elementwise_fma(q4_h2((w & 0x00F000F0u) | 0x64006400u), sixteenth, -zh);
+    const h2 c = q4_h2((v & 0x000F000Fu) | 0x64006400u) - zl;
+    const h2 d = __builtin_elementwise_fma(q4_h2((v & 0x00F000F0u) | 0x64006400u), sixteenth, -zh);
+    return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+template <typename AT, int G, bool ZP>
+__global__ __launch_bounds__(512) void k_linear_q4(Q4Args a, Q4Launch L)
+{
+    constexpr bool F32 = sizeof(AT) == 4;
+    constexpr int PG = kQ4Step / G;                 // groups a step
+    constexpr int NS = PG > 4 ? 2 : 1;              // scales a lane loads a step
+    constexpr int DW = G / 32;                      // dwords of codes a lane reads a group
+    extern __shared__ __align__(16) char smem[];
+    const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g4 = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), threads = L.waves * 64;
+    // blocks go to the 8 XCDs in turn: a tile's passes follow each other on one, whose L2 then has its weights
+    const int32_t xcd = blockIdx.x & 7, idx = blockIdx.x >> 3;
+    const int32_t pass = idx % L.passes, grp = idx / L.passes * 8 + xcd;
+    if (grp >= L.groups_n) return;
+    const int32_t ks = wave % L.ks;
+    const int64_t n0 = ((int64_t)grp * (L.waves / L.ks) + wave / L.ks) * 16, m0 = (int64_t)pass * kQ4Rows;
+    const int32_t rows = (int32_t)(a.M - m0 < kQ4Rows ? a.M - m0 : kQ4Rows);
+    const int32_t K = (int32_t)a.K, steps = (K + kQ4Step - 1) / kQ4Step, groups = K / G;
+    const int32_t pitch = L.seg * kQ4Step + 8;      // halves between rows of x in LDS
+    f16* xs = reinterpret_cast<f16*>(smem);
+    const int32_t plane = L.rows * pitch;           // F32: the low parts' plane is at +plane
+    float* xinv = reinterpret_cast<float*>(xs + (F32 ? 2 : 1) * plane);  // F32: [seg][16] inverse scales
+    char* tile = reinterpret_cast<char*>(xinv + (F32 ? L.seg * kQ4Rows : 0)) + wave * kQ4Tile;
+    uint32_t* stile = reinterpret_cast<uint32_t*>(tile + 16 * kQ4WPitch);
+    const AT* x = (const AT*)a.inp + m0 * a.K;
+
+    // weights: rows past N are row N - 1, pieces past K the last one (met by zeros in x)
+    const int64_t ra = n0 + (lane >> 3) < a.N ? n0 + (lane >> 3) : a.N - 1;
+    const int64_t rb = n0 + 8 + (lane >> 3) < a.N ? n0 + 8 + (lane >> 3) : a.N - 1;
+    const int64_t rn = n0 + n < a.N ? n0 + n : a.N - 1;
+    const uint8_t* wa = a.w + ra * (K / 2);
+    const uint8_t* wb = a.w + rb * (K / 2);
+    const uint16_t* sc = a.scales + rn * groups;
+    const uint8_t* zp = ZP ? a.zeros + rn * groups : nullptr;
+    struct Slot {
+        u4 a, b;
+        uint16_t s[NS];
+        uint8_t z[NS];
+    } ring[kQ4Depth];
+    auto issue = [&](int u, int32_t st) {
+        st = st < steps ? st : steps - 1;  // past the end: the last step again, never used
+        const int32_t at = st * (kQ4Step / 2) + (lane & 7) * 16, last = K / 2 - 16;
+        ring[u].a = *reinterpret_cast<const u4*>(wa + (at < last ? at : last));
+        ring[u].b = *reinterpret_cast<const u4*>(wb + (at < last ? at : last));
 #pragma unroll
-            for (int m = 0; m < 8; m++) {
-                if (m0 + m >= a.M) break;
-                const T* x = (const T*)a.inp + (m0 + m) * a.K + k;
-                float d = 0.0f;
+        for (int i = 0; i < NS; i++) {
+            const int32_t h = st * PG + (g4 * NS + i) % PG, g = h < groups ? h : groups - 1;
+            ring[u].s[i] = sc[g];
+            if (ZP) ring[u].z[i] = zp[g];
+        }
+    };
+
+    // ---- x ----
+    const int32_t row = n < rows ? n : rows - 1;    // rows of the operand past the last are computed and dropped
+    auto order = [](u4 v) {                         // 0 1 2 3 4 5 6 7 -> 0 4 1 5 2 6 3 7
+        return u4{__builtin_amdgcn_perm(v[2], v[0], 0x05040100u), __builtin_amdgcn_perm(v[2], v[0], 0x07060302u),
+                  __builtin_amdgcn_perm(v[3], v[1], 0x05040100u), __builtin_amdgcn_perm(v[3], v[1], 0x07060302u)};
+    };
+    auto stage = [&](int32_t st0, int32_t st1) {
+        if constexpr (!F32) {
+            const int32_t per = (st1 - st0) * (kQ4Step / 8), all = rows * per;
+            for (int32_t i = tid; i < all; i += threads) {
+                const int32_t m = i / per, k = (i - m * per) * 8, at = st0 * kQ4Step + k;
+                u4 v = {};
+                if (at < K) v = *reinterpret_cast<const u4*>(x + (int64_t)m * K + at);
+                *reinterpret_cast<u4*>(xs + m * pitch + k) = order(v);
+            }
+        } else {
+            const int32_t per = st1 - st0;
+            for (int32_t i = wave; i < rows * per; i += L.waves) {  // a wave a row's step: 4 values a lane
+                const int32_t m = i / per, st = i - m * per, at = (st0 + st) * kQ4Step + lane * 4;
+                f4 v = {};
+                if (at < K) v = *reinterpret_cast<const f4*>(x + (int64_t)m * K + at);
+                const float most = group_max(fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))), 64);
+                // 2^(14 - x) for most in [2^x, 2^(x + 1)), at most 2^126; 1 with an infinity or NaN
+                const int b = (int)(__builtin_bit_cast(uint32_t, most) >> 23), e = b < 15 ? 15 : b;
+                const float up = e == 255 ? 1.0f : __builtin_bit_cast(float, (uint32_t)(268 - e) << 23);
+                uint32_t hi[2], lo[2];
 #pragma unroll
-                for (int j = 0; j < 8; j++) d = __builtin_fmaf((float)((w >> (4 * j)) & 15) - z, (float)x[j], d);
-                acc[m] = __builtin_fmaf(s, d, acc[m]);
+                for (int j = 0; j < 2; j++) {
+                    const float p = v[2 * j] * up, q = v[2 * j + 1] * up;
+                    const h2 h = {(f16)p, (f16)q};
+                    h2 l = {(f16)(p - (float)h[0]), (f16)(q - (float)h[1])};
+                    if (e == 255) l = h2{};  // an infinity or NaN is all in its high part
+                    hi[j] = __builtin_bit_cast(uint32_t, h);
+                    lo[j] = __builtin_bit_cast(uint32_t, l);
+                }
+                // lanes of a pair hold values 0-3 and 4-7: the even one stores the high parts, the odd one the low
+                const bool odd = lane & 1;
+                const uint32_t s0 = odd ? hi[0] : lo[0], s1 = odd ? hi[1] : lo[1];
+                const uint32_t r0 = __builtin_amdgcn_mov_dpp((int)s0, 0xB1, 0xF, 0xF, false);
+                const uint32_t r1 = __builtin_amdgcn_mov_dpp((int)s1, 0xB1, 0xF, 0xF, false);
+                const u4 o = order(odd ? u4{r0, r1, lo[0], lo[1]} : u4{hi[0], hi[1], r0, r1});
+                *reinterpret_cast<u4*>(xs + (odd ? plane : 0) + m * pitch + st * kQ4Step + (lane >> 1) * 8) = o;
+                if (lane == 0) xinv[st * kQ4Rows + m] = e == 255 ? 1.0f : __builtin_bit_cast(float, (uint32_t)(e - 14) << 23);
             }
         }
+    };
+
+    f4 acc = {};
+    auto consume = [&](int u, int32_t st) {         // st: the step within x in LDS
+        *reinterpret_cast<u4*>(tile + (lane >> 3) * kQ4WPitch + (lane & 7) * 16) = ring[u].a;
+        *reinterpret_cast<u4*>(tile + (8 + (lane >> 3)) * kQ4WPitch + (lane & 7) * 16) = ring[u].b;
 #pragma unroll
-        for (int m = 0; m < 8; m++) {
-            const float y = wave_sum_xor(acc[m]);
-            if (lane == 0 && m0 + m < a.M) {
-                const int64_t o = (m0 + m) * a.N + n;
-                ((OT*)a.out)[o] = (OT)(y + (a.bias ? a.bias[n] : 0.0f) + (a.res ? (float)((const OT*)a.res)[o] : 0.0f));
+        for (int i = 0; i < NS; i++) {
+            uint32_t v = ring[u].s[i];
+            if (ZP) v |= (uint32_t)__builtin_bit_cast(uint16_t, (f16)(float)ring[u].z[i]) << 16;
+            if (g4 * NS + i < PG) stile[n * kQ4SPitch + g4 * NS + i] = v;
+        }
+        // one wave's LDS accesses complete in order
+        uint32_t sv[PG];
+#pragma unroll
+        for (int g = 0; g < PG; g++) sv[g] = stile[n * kQ4SPitch + g];
+        const f16* xk = xs + row * pitch + st * kQ4Step;
+        f4 part = {};
+#pragma unroll
+        for (int g = 0; g < PG; g++) {
+            uint32_t w[DW];
+            const uint32_t* wr = reinterpret_cast<const uint32_t*>(tile + n * kQ4WPitch) + g * (G / 8) + g4 * DW;
+#pragma unroll
+            for (int j = 0; j < DW; j++) w[j] = wr[j];
+            h2 zl = {(f16)1032.0f, (f16)1032.0f}, zh = {(f16)72.0f, (f16)72.0f};
+            if (ZP) {
+                const f16 z = q4_h2(sv[g])[1];
+                zl = h2{z, z} + h2{(f16)1024.0f, (f16)1024.0f};
+                zh = h2{z, z} + h2{(f16)64.0f, (f16)64.0f};
             }
+            f4 d = {};
+#pragma unroll
+            for (int j = 0; j < DW; j++) {
+                const h8 b = q4_codes(w[j], zl, zh);
+                const f16* xp = xk + g * G + (g4 * DW + j) * 8;
+                if (F32) d = __builtin_amdgcn_mfma_f32_16x16x32_f16(*reinterpret_cast<const h8*>(xp + plane), b, d, 0, 0, 0);
+                d = __builtin_amdgcn_mfma_f32_16x16x32_f16(*reinterpret_cast<const h8*>(xp), b, d, 0, 0, 0);
+            }
+            const float s = (float)q4_h2(sv[g])[0];
+#pragma unroll
+            for (int i = 0; i < 4; i++) part[i] = __builtin_fmaf(s, d[i], part[i]);
+        }
+        if constexpr (F32) {
+            const f4 inv = *reinterpret_cast<const f4*>(xinv + st * kQ4Rows + 4 * g4);  // rows past the last: dropped
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[i] = __builtin_fmaf(part[i], inv[i], acc[i]);
+        } else {
+            acc += part;
+        }
+    };
+
+#pragma unroll
+    for (int u = 0; u < kQ4Depth; u++) issue(u, ks + u * L.ks);
+    // step ks + KS i is the wave's i-th; x is in LDS for L.seg steps at a time, all of them or a
+    // multiple of KS * kQ4Depth
+    for (int32_t st0 = 0; st0 < steps; st0 += L.seg) {
+        const int32_t st1 = st0 + L.seg < steps ? st0 + L.seg : steps;
+        if (st0 > 0) lds_barrier();
+        stage(st0, st1);
+        lds_barrier();
+        for (int32_t st = st0 + ks; st < st1; st += L.ks * kQ4Depth) {
+            if (st + L.ks * kQ4Depth < steps) {     // this ring is full, and steps follow
+#pragma unroll
+                for (int u = 0; u < kQ4Depth; u++) {
+                    consume(u, st - st0 + u * L.ks);
+                    issue(u, st + (u + kQ4Depth) * L.ks);
+                }
+            } else {
+#pragma unroll
+                for (int u = 0; u < kQ4Depth; u++)
+                    if (st + u * L.ks < st1) consume(u, st - st0 + u * L.ks);
+            }
+        }
+    }
+    // ---- the waves' sums, and out ----
+    float* red = reinterpret_cast<float*>(tile);
+    if (L.ks > 1) {
+        lds_barrier();
+        *reinterpret_cast<f4*>(red + lane * 4) = acc;
+        lds_barrier();
+        if (ks != 0) return;
+        for (int i = 1; i < L.ks; i++) acc += *reinterpret_cast<const f4*>(red + i * (kQ4Tile / 4) + lane * 4);
+    }
+    if (n0 + n >= a.N) return;
+    const float bias = a.bias ? a.bias[n0 + n] : 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if (4 * g4 + i >= rows) break;
+        const int64_t o = (m0 + 4 * g4 + i) * a.N + n0 + n;
+        float y = acc[i] + bias;
+        if (L.out_f16) {
+            if (a.res) y += (float)((const f16*)a.res)[o];
+            ((f16*)a.out)[o] = (f16)y;
+        } else {
+            if (a.res) y += ((const float*)a.res)[o];
+            ((float*)a.out)[o] = y;
         }
     }
 }
 
+// K = 0: bias and residual alone.
+template <typename OT>
+__global__ __launch_bounds__(256) void k_linear_q4_none(Q4Args a)
+{
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.M * a.N; i += (int64_t)gridDim.x * 256)
+        ((OT*)a.out)[i] = (OT)((a.bias ? a.bias[i % a.N] : 0.0f) + (a.res ? (float)((const OT*)a.res)[i] : 0.0f));
+}
+
+int64_t q4_lds(int64_t seg, int64_t waves, int64_t rows, bool f32)
+{
+    return (f32 ? 2 : 1) * rows * (seg * kQ4Step + 8) * 2 + (f32 ? seg * kQ4Rows * 4 : 0) + waves * kQ4Tile;
+}
+
 }  // namespace
 
-int launch_linear_q4(const Q4Args& a, int act, int out, void* stream)
+int launch_linear_q4(const Q4Args& a, int act, int out, int64_t cus, void* stream)
 {
-    const dim3 grid((unsigned)((a.N + 3) / 4));
-    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, static_cast<hipStream_t>(stream), a); };
-    if (act == VVH_F16) out == VVH_F16 ? go(k_linear_q4<f16, f16>) : go(k_linear_q4<f16, float>);
-    else out == VVH_F16 ? go(k_linear_q4<float, f16>) : go(k_linear_q4<float, float>);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (a.K == 0) {
+        const dim3 grid((unsigned)std::min<int64_t>((a.M * a.N + 255) / 256, 65536));
+        if (out == VVH_F16) hipLaunchKernelGGL(k_linear_q4_none<f16>, grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL(k_linear_q4_none<float>, grid, dim3(256), 0, st, a);
+        return (int)hipGetLastError();
+    }
+    const bool f32 = act == VVH_F32;
+    const int64_t tiles = (a.N + 15) / 16, steps = (a.K + kQ4Step - 1) / kQ4Step, passes = (a.M + kQ4Rows - 1) / kQ4Rows,
+                  rows = std::min<int64_t>(a.M, kQ4Rows);
+    int64_t ks = 1;
+    while (ks < 8 && ks < steps && tiles * passes * ks < 4 * cus) ks *= 2;
+    const int64_t waves = std::max<int64_t>(4, ks);
+    // x in LDS: all of it, or a multiple of ks * kQ4Depth steps (at least one: 128 KB at 16 steps of fp16,
+    // 8 of fp32)
+    constexpr int64_t kLds = 160 * 1024;
+    int64_t seg = steps;
+    if (q4_lds(seg, waves, rows, f32) > kLds) {
+        while (ks > 1 && q4_lds(ks * kQ4Depth, waves, rows, f32) > kLds) ks /= 2;
+        seg = ks * kQ4Depth;
+        while (q4_lds(seg + ks * kQ4Depth, waves, rows, f32) <= kLds) seg += ks * kQ4Depth;
+    }
+    Q4Launch L{(int32_t)waves, (int32_t)ks, (int32_t)seg, (int32_t)passes, 0, (int32_t)rows, out == VVH_F16};
+    L.groups_n = (int32_t)((tiles + waves / ks - 1) / (waves / ks));
+    const int64_t blocks = (L.groups_n + 7) / 8 * 8 * passes;
+    if (blocks > INT32_MAX) return (int)hipErrorInvalidValue;
+    const size_t lds = (size_t)q4_lds(seg, waves, rows, f32);
+    auto go = [&](auto kern) {
+        hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3((unsigned)(64 * waves)), lds, st, a, L);
+    };
+#define VVH_Q4(AT, G) a.zeros ? go(k_linear_q4<AT, G, true>) : go(k_linear_q4<AT, G, false>)
+    if (f32) a.group == 32 ? (VVH_Q4(float, 32)) : a.group == 64 ? (VVH_Q4(float, 64)) : (VVH_Q4(float, 128));
+    else a.group == 32 ? (VVH_Q4(f16, 32)) : a.group == 64 ? (VVH_Q4(f16, 64)) : (VVH_Q4(f16, 128));
+#undef VVH_Q4
     return (int)hipGetLastError();
 }
 

@@ -2436,7 +2436,7 @@ VVH_API int vvh_linear_q4(void* out, const void* inp, const uint8_t* dev_weight,
     REQUIRE_INIT();
     const Q4Args a{out, inp, residual, dev_weight, dev_scales, dev_zeros, dev_bias, (int64_t)M, (int64_t)N, (int64_t)K,
                    (int32_t)group};
-    return ret_launch(launch_linear_q4(a, act_dtype, out_dtype, stream), "4-bit linear launch");
+    return ret_launch(launch_linear_q4(a, act_dtype, out_dtype, g_cu_count > 0 ? g_cu_count : 256, stream), "4-bit linear launch");
 }
 
 VVH_API int vvh_logits_rules(void* out, const void* logits, const vvh_logits_spec* rules, size_t rows, size_t n,
