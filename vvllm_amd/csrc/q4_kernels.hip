@@ -5,6 +5,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 #include "device.h"
@@ -19,7 +20,7 @@ namespace {
 // are added through LDS in order.  Up to 16 rows of x are a pass, staged in LDS.
 //
 // Loads: lane l reads the 16-byte piece l % 8 of the lines of rows l / 8 and 8 + l / 8, so
-// that an instruction covers 8 whole lines, kQ4Depth steps ahead of use.  A step's 16 lines go
+// that an instruction covers 8 whole lines, DEPTH steps ahead of use.  A step's 16 lines go
 // through the wave's LDS tile, whose rows a lane reads back as the matrix instruction
 // wants them: lane (n, g4) 8 codes of channel n, the four lanes of a channel 32 codes of one
 // group, whose sum the instruction gives and the group's scale multiplies in fp32.
@@ -29,12 +30,12 @@ namespace {
 // fp32 rows of x are staged as two fp16 planes, high and low parts of x times a power of two that
 // puts the step's largest |x| into [2^14, 2^15) (22 bits; the sum of a step is multiplied back).
 // ---------------------------------------------------------------------------
-constexpr int kQ4Depth = 4;
 constexpr int kQ4Step = 256;     // codes of a row a step
 constexpr int kQ4WPitch = 144;   // bytes between rows of the LDS weight tile
 constexpr int kQ4SPitch = 12;    // dwords between rows of its scales
 constexpr int kQ4Tile = 16 * kQ4WPitch + 16 * kQ4SPitch * 4;
 constexpr int kQ4Rows = 16;
+constexpr int kQ4Batch = 4;      // pieces of x a wave loads at a time
 
 // What a launch's blocks share out.
 struct Q4Launch {
@@ -44,24 +45,35 @@ struct Q4Launch {
     int32_t passes;    // of 16 rows
     int32_t groups_n;  // blocks of a pass
     int32_t rows;      // of x in LDS: the largest pass
+    uint32_t inv_per;  // ceil(2^32 / units of a row of x in LDS)
     int32_t out_f16;
 };
 
 __device__ __forceinline__ h2 q4_h2(uint32_t v) { return __builtin_bit_cast(h2, v); }
 
+// The masks of the code conversion, kept in registers: v_and_or_b32 takes no literal.
+struct Q4Masks {
+    uint32_t lo, hi, one;
+};
+__device__ __forceinline__ Q4Masks q4_masks()
+{
+    Q4Masks k{0x000F000Fu, 0x00F000F0u, 0x64006400u};
+    asm("" : "+s"(k.lo), "+s"(k.hi), "+v"(k.one));
+    return k;
+}
 // 8 codes minus their zero point; zl = 1024 + z, zh = 64 + z
-__device__ __forceinline__ h8 q4_codes(uint32_t w, h2 zl, h2 zh)
+__device__ __forceinline__ h8 q4_codes(uint32_t w, h2 zl, h2 zh, const Q4Masks& k)
 {
     const h2 sixteenth = {(f16)0.0625f, (f16)0.0625f};
     const uint32_t v = w >> 8;
-    const h2 a = q4_h2((w & 0x000F000Fu) | 0x64006400u) - zl;
-    const h2 b = __builtin_elementwise_fma(q4_h2((w & 0x00F000F0u) | 0x64006400u), sixteenth, -zh);
-    const h2 c = q4_h2((v & 0x000F000Fu) | 0x64006400u) - zl;
-    const h2 d = __builtin_elementwise_fma(q4_h2((v & 0x00F000F0u) | 0x64006400u), sixteenth, -zh);
+    const h2 a = q4_h2((w & k.lo) | k.one) - zl;
+    const h2 b = __builtin_elementwise_fma(q4_h2((w & k.hi) | k.one), sixteenth, -zh);
+    const h2 c = q4_h2((v & k.lo) | k.one) - zl;
+    const h2 d = __builtin_elementwise_fma(q4_h2((v & k.hi) | k.one), sixteenth, -zh);
     return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-template <typename AT, int G, bool ZP>
+template <typename AT, int G, bool ZP, int DEPTH>
 __global__ __launch_bounds__(512) void k_linear_q4(Q4Args a, Q4Launch L)
 {
     constexpr bool F32 = sizeof(AT) == 4;
@@ -99,7 +111,7 @@ __global__ __launch_bounds__(512) void k_linear_q4(Q4Args a, Q4Launch L)
         u4 a, b;
         uint16_t s[NS];
         uint8_t z[NS];
-    } ring[kQ4Depth];
+    } ring[DEPTH];
     auto issue = [&](int u, int32_t st) {
         st = st < steps ? st : steps - 1;  // past the end: the last step again, never used
         const int32_t at = st * (kQ4Step / 2) + (lane & 7) * 16, last = K / 2 - 16;
@@ -119,34 +131,46 @@ __global__ __launch_bounds__(512) void k_linear_q4(Q4Args a, Q4Launch L)
         return u4{__builtin_amdgcn_perm(v[2], v[0], 0x05040100u), __builtin_amdgcn_perm(v[2], v[0], 0x07060302u),
                   __builtin_amdgcn_perm(v[3], v[1], 0x05040100u), __builtin_amdgcn_perm(v[3], v[1], 0x07060302u)};
     };
-    auto stage = [&](int32_t st0, int32_t st1) {
-        if constexpr (!F32) {
-            const int32_t per = (st1 - st0) * (kQ4Step / 8), all = rows * per;
-            for (int32_t i = tid; i < all; i += threads) {
-                const int32_t m = i / per, k = (i - m * per) * 8, at = st0 * kQ4Step + k;
-                u4 v = {};
-                if (at < K) v = *reinterpret_cast<const u4*>(x + (int64_t)m * K + at);
-                *reinterpret_cast<u4*>(xs + m * pitch + k) = order(v);
-            }
-        } else {
-            const int32_t per = st1 - st0;
-            for (int32_t i = wave; i < rows * per; i += L.waves) {  // a wave a row's step: 4 values a lane
-                const int32_t m = i / per, st = i - m * per, at = (st0 + st) * kQ4Step + lane * 4;
-                f4 v = {};
-                if (at < K) v = *reinterpret_cast<const f4*>(x + (int64_t)m * K + at);
+    // x to LDS.  A unit is 16 bytes of a row: unit i is piece i % per of row i / per (fp32: a wave's unit, 256
+    // values of a row, 4 a lane, whose largest the lanes share).  kQ4Batch of them are loaded together; the
+    // first batch ahead of the weight ring, whose loads it then does not wait for.
+    constexpr int PIECE = F32 ? kQ4Step : 8;            // values a unit
+    const int32_t first = F32 ? wave : tid, stride = F32 ? L.waves : threads;
+    const int32_t per = L.seg * (kQ4Step / PIECE);
+    u4 xr[kQ4Batch];
+    auto load_x = [&](int32_t i0, int32_t st0) {
+#pragma unroll
+        for (int j = 0; j < kQ4Batch; j++) {
+            const int32_t i = i0 + j * stride;
+            if ((F32 ? i : i - first) >= rows * per) break;
+            const int32_t m = (int32_t)__umulhi((uint32_t)i, L.inv_per), at = st0 * kQ4Step + (i - m * per) * PIECE + (F32 ? lane * 4 : 0);
+            xr[j] = u4{};
+            if (m < rows && at < K) xr[j] = *reinterpret_cast<const u4*>(x + (int64_t)m * K + at);
+        }
+    };
+    auto store_x = [&](int32_t i0) {
+#pragma unroll
+        for (int j = 0; j < kQ4Batch; j++) {
+            const int32_t i = i0 + j * stride;
+            if ((F32 ? i : i - first) >= rows * per) break;
+            const int32_t m = (int32_t)__umulhi((uint32_t)i, L.inv_per), k = (i - m * per) * PIECE;
+            if constexpr (!F32) {
+                if (m < rows) *reinterpret_cast<u4*>(xs + m * pitch + k) = order(xr[j]);
+            } else {
+                const f4 v = __builtin_bit_cast(f4, xr[j]);
                 const float most = group_max(fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))), 64);
                 // 2^(14 - x) for most in [2^x, 2^(x + 1)), at most 2^126; 1 with an infinity or NaN
                 const int b = (int)(__builtin_bit_cast(uint32_t, most) >> 23), e = b < 15 ? 15 : b;
                 const float up = e == 255 ? 1.0f : __builtin_bit_cast(float, (uint32_t)(268 - e) << 23);
                 uint32_t hi[2], lo[2];
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const float p = v[2 * j] * up, q = v[2 * j + 1] * up;
+                for (int c = 0; c < 2; c++) {
+                    const float p = v[2 * c] * up, q = v[2 * c + 1] * up;
                     const h2 h = {(f16)p, (f16)q};
                     h2 l = {(f16)(p - (float)h[0]), (f16)(q - (float)h[1])};
                     if (e == 255) l = h2{};  // an infinity or NaN is all in its high part
-                    hi[j] = __builtin_bit_cast(uint32_t, h);
-                    lo[j] = __builtin_bit_cast(uint32_t, l);
+                    hi[c] = __builtin_bit_cast(uint32_t, h);
+                    lo[c] = __builtin_bit_cast(uint32_t, l);
                 }
                 // lanes of a pair hold values 0-3 and 4-7: the even one stores the high parts, the odd one the low
                 const bool odd = lane & 1;
@@ -154,12 +178,13 @@ __global__ __launch_bounds__(512) void k_linear_q4(Q4Args a, Q4Launch L)
                 const uint32_t r0 = __builtin_amdgcn_mov_dpp((int)s0, 0xB1, 0xF, 0xF, false);
                 const uint32_t r1 = __builtin_amdgcn_mov_dpp((int)s1, 0xB1, 0xF, 0xF, false);
                 const u4 o = order(odd ? u4{r0, r1, lo[0], lo[1]} : u4{hi[0], hi[1], r0, r1});
-                *reinterpret_cast<u4*>(xs + (odd ? plane : 0) + m * pitch + st * kQ4Step + (lane >> 1) * 8) = o;
-                if (lane == 0) xinv[st * kQ4Rows + m] = e == 255 ? 1.0f : __builtin_bit_cast(float, (uint32_t)(e - 14) << 23);
+                *reinterpret_cast<u4*>(xs + (odd ? plane : 0) + m * pitch + k + (lane >> 1) * 8) = o;
+                if (lane == 0)
+                    xinv[k / kQ4Step * kQ4Rows + m] = e == 255 ? 1.0f : __builtin_bit_cast(float, (uint32_t)(e - 14) << 23);
             }
         }
     };
-
+    const Q4Masks masks = q4_masks();
     f4 acc = {};
     auto consume = [&](int u, int32_t st) {         // st: the step within x in LDS
         *reinterpret_cast<u4*>(tile + (lane >> 3) * kQ4WPitch + (lane & 7) * 16) = ring[u].a;
@@ -191,7 +216,7 @@ __global__ __launch_bounds__(512) void k_linear_q4(Q4Args a, Q4Launch L)
             f4 d = {};
 #pragma unroll
             for (int j = 0; j < DW; j++) {
-                const h8 b = q4_codes(w[j], zl, zh);
+                const h8 b = q4_codes(w[j], zl, zh, masks);
                 const f16* xp = xk + g * G + (g4 * DW + j) * 8;
                 if (F32) d = __builtin_amdgcn_mfma_f32_16x16x32_f16(*reinterpret_cast<const h8*>(xp + plane), b, d, 0, 0, 0);
                 d = __builtin_amdgcn_mfma_f32_16x16x32_f16(*reinterpret_cast<const h8*>(xp), b, d, 0, 0, 0);
@@ -209,26 +234,37 @@ __global__ __launch_bounds__(512) void k_linear_q4(Q4Args a, Q4Launch L)
         }
     };
 
+    load_x(first, 0);
 #pragma unroll
-    for (int u = 0; u < kQ4Depth; u++) issue(u, ks + u * L.ks);
+    for (int u = 0; u < DEPTH; u++) issue(u, ks + u * L.ks);
     // step ks + KS i is the wave's i-th; x is in LDS for L.seg steps at a time, all of them or a
-    // multiple of KS * kQ4Depth
+    // multiple of KS * DEPTH
     for (int32_t st0 = 0; st0 < steps; st0 += L.seg) {
         const int32_t st1 = st0 + L.seg < steps ? st0 + L.seg : steps;
-        if (st0 > 0) lds_barrier();
-        stage(st0, st1);
+        if (st0 > 0) {
+            load_x(first, st0);
+            lds_barrier();
+        }
+        store_x(first);
+        for (int32_t i = kQ4Batch * stride; i < rows * per; i += kQ4Batch * stride) {
+            load_x(first + i, st0);
+            store_x(first + i);
+        }
         lds_barrier();
-        for (int32_t st = st0 + ks; st < st1; st += L.ks * kQ4Depth) {
-            if (st + L.ks * kQ4Depth < steps) {     // this ring is full, and steps follow
+        for (int32_t st = st0 + ks; st < st1; st += L.ks * DEPTH) {
+            if (st + L.ks * DEPTH < steps) {     // this ring is full, and steps follow
 #pragma unroll
-                for (int u = 0; u < kQ4Depth; u++) {
+                for (int u = 0; u < DEPTH; u++) {
                     consume(u, st - st0 + u * L.ks);
-                    issue(u, st + (u + kQ4Depth) * L.ks);
+                    __builtin_amdgcn_sched_barrier(0);  // no work of the next step ahead of this one's: registers
+                    issue(u, st + (u + DEPTH) * L.ks);
                 }
             } else {
 #pragma unroll
-                for (int u = 0; u < kQ4Depth; u++)
+                for (int u = 0; u < DEPTH; u++) {
                     if (st + u * L.ks < st1) consume(u, st - st0 + u * L.ks);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
         }
     }
@@ -288,27 +324,38 @@ int launch_linear_q4(const Q4Args& a, int act, int out, int64_t cus, void* strea
     int64_t ks = 1;
     while (ks < 8 && ks < steps && tiles * passes * ks < 4 * cus) ks *= 2;
     const int64_t waves = std::max<int64_t>(4, ks);
-    // x in LDS: all of it, or a multiple of ks * kQ4Depth steps (at least one: 128 KB at 16 steps of fp16,
+    // x in LDS: all of it, or a multiple of ks * 4 steps (at least one: 128 KB at 16 steps of fp16,
     // 8 of fp32)
     constexpr int64_t kLds = 160 * 1024;
-    int64_t seg = steps;
+    int64_t seg = std::max<int64_t>(2, steps);
     if (q4_lds(seg, waves, rows, f32) > kLds) {
-        while (ks > 1 && q4_lds(ks * kQ4Depth, waves, rows, f32) > kLds) ks /= 2;
-        seg = ks * kQ4Depth;
-        while (q4_lds(seg + ks * kQ4Depth, waves, rows, f32) <= kLds) seg += ks * kQ4Depth;
+        while (ks > 1 && q4_lds(ks * 4, waves, rows, f32) > kLds) ks /= 2;
+        seg = ks * 4;
+        while (q4_lds(seg + ks * 4, waves, rows, f32) <= kLds) seg += ks * 4;
     }
-    Q4Launch L{(int32_t)waves, (int32_t)ks, (int32_t)seg, (int32_t)passes, 0, (int32_t)rows, out == VVH_F16};
+    Q4Launch L{(int32_t)waves, (int32_t)ks, (int32_t)seg, (int32_t)passes, 0, (int32_t)rows, 0, out == VVH_F16};
     L.groups_n = (int32_t)((tiles + waves / ks - 1) / (waves / ks));
     const int64_t blocks = (L.groups_n + 7) / 8 * 8 * passes;
     if (blocks > INT32_MAX) return (int)hipErrorInvalidValue;
+    L.inv_per = (uint32_t)(((uint64_t(1) << 32) + seg * (f32 ? 1 : 32) - 1) / (seg * (f32 ? 1 : 32)));
+    const int64_t mine = (steps + ks - 1) / ks, depth = mine > 2 ? 4 : mine;  // steps of a wave
     const size_t lds = (size_t)q4_lds(seg, waves, rows, f32);
     auto go = [&](auto kern) {
         hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3((unsigned)(64 * waves)), lds, st, a, L);
     };
-#define VVH_Q4(AT, G) a.zeros ? go(k_linear_q4<AT, G, true>) : go(k_linear_q4<AT, G, false>)
-    if (f32) a.group == 32 ? (VVH_Q4(float, 32)) : a.group == 64 ? (VVH_Q4(float, 64)) : (VVH_Q4(float, 128));
-    else a.group == 32 ? (VVH_Q4(f16, 32)) : a.group == 64 ? (VVH_Q4(f16, 64)) : (VVH_Q4(f16, 128));
-#undef VVH_Q4
+    auto go_depth = [&](auto* t, auto g, auto z) {
+        using AT = std::remove_pointer_t<decltype(t)>;
+        constexpr int G = decltype(g)::value;
+        constexpr bool ZP = decltype(z)::value;
+        depth == 1 ? go(k_linear_q4<AT, G, ZP, 1>) : depth == 2 ? go(k_linear_q4<AT, G, ZP, 2>) : go(k_linear_q4<AT, G, ZP, 4>);
+    };
+    auto go_group = [&](auto* t, auto z) {
+        a.group == 32   ? go_depth(t, std::integral_constant<int, 32>{}, z)
+        : a.group == 64 ? go_depth(t, std::integral_constant<int, 64>{}, z)
+                        : go_depth(t, std::integral_constant<int, 128>{}, z);
+    };
+    auto go_type = [&](auto* t) { a.zeros ? go_group(t, std::true_type{}) : go_group(t, std::false_type{}); };
+    f32 ? go_type((float*)nullptr) : go_type((f16*)nullptr);
     return (int)hipGetLastError();
 }
 
