@@ -85,6 +85,20 @@ def test_short_and_odd_rows(gpu, act, K, group, M):
     Case(M, 37, K, group, act, act, zeros=K % 64 == 32).check()
 
 
+@pytest.mark.parametrize("act", [F16, F32])
+@pytest.mark.parametrize("M,N,K", [(1, 40, 90112), (2, 33, 45056), (16, 130, 8960), (40, 100, 8960), (9, 1, 20480)])
+def test_rows_of_x_past_the_lds(gpu, act, M, N, K):
+    """k shared by several blocks, whose sums a second launch adds."""
+    Case(M, N, K, 128, act, act, zeros=True, bias=True, residual=True).check()
+
+
+@pytest.mark.parametrize("act", [F16, F32])
+@pytest.mark.parametrize("M,N", [(1, 40000), (16, 20011), (33, 9000)])
+def test_many_channels(gpu, act, M, N):
+    """Blocks that take several groups of channels in turn."""
+    Case(M, N, 96, 32, act, act, bias=True).check()
+
+
 @pytest.mark.parametrize("act,outd", [(F16, F32), (F32, F16)])
 @pytest.mark.parametrize("M", [1, 4, 16, 40])
 def test_mixed_types(gpu, act, outd, M):

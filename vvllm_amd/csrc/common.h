@@ -443,7 +443,14 @@ struct Q4Args {
     int64_t M, N, K;
     int32_t group;
 };
-int launch_linear_q4(const Q4Args& a, int act, int out, int64_t cus, void* stream);
+// How a call is run: `waves` waves a block, `ks` of them on a tile, x of `seg` steps in
+// LDS; splits > 1 blocks share a tile's k (ws_floats floats of workspace and a
+// second launch), 0: no k.
+struct Q4Plan {
+    int64_t waves, ks, seg, splits, ws_floats;
+};
+Q4Plan linear_q4_plan(const Q4Args& a, int act, int64_t cus);
+int launch_linear_q4(const Q4Plan& p, const Q4Args& a, int act, int out, float* ws, int64_t cus, void* stream);
 
 // Logit rules (logits_kernels.hip)
 int launch_logits_rules(void* out, const void* logits, const vvh_logits_spec& r, int64_t rows, int64_t n, int dtype,

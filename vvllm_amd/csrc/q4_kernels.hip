@@ -37,16 +37,19 @@ constexpr int kQ4Tile = 16 * kQ4WPitch + 16 * kQ4SPitch * 4;
 constexpr int kQ4Rows = 16;
 constexpr int kQ4Batch = 4;      // pieces of x a wave loads at a time
 
-// What a launch's blocks share out.
+// How a launch's blocks share out the work: block (slot, pass, split) takes the groups slot, slot +
+// slots, ... of `tiles` tiles, 16 rows, and the steps [split * seg, + seg).  Blocks go to the 8 XCDs in
+// turn and gridDim.x is a multiple of 8, so a tile's passes and splits are on one, whose L2 then has its weights.
 struct Q4Launch {
-    int32_t waves;     // of a block
-    int32_t ks;        // waves that share a tile
-    int32_t seg;       // steps of x in LDS at a time
-    int32_t passes;    // of 16 rows
-    int32_t groups_n;  // blocks of a pass
-    int32_t rows;      // of x in LDS: the largest pass
-    uint32_t inv_per;  // ceil(2^32 / units of a row of x in LDS)
+    int32_t waves, tiles;  // of a block: waves a tile = waves / tiles = 1 << log_ks
+    int32_t log_ks;
+    int32_t seg;           // steps of a split, whose x is in LDS
+    int32_t splits;        // > 1: raw sums to ws[split][M][N], for k_linear_q4_join
+    int32_t groups_n, slots;
+    int32_t rows;          // of x in LDS: the largest pass
+    uint32_t inv_per;      // ceil(2^32 / units of a row of x in LDS)
     int32_t out_f16;
+    float* ws;
 };
 
 __device__ __forceinline__ h2 q4_h2(uint32_t v) { return __builtin_bit_cast(h2, v); }
@@ -83,14 +86,15 @@ __global__ __launch_bounds__(512) void k_linear_q4(Q4Args a, Q4Launch L)
     extern __shared__ __align__(16) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g4 = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), threads = L.waves * 64;
-    // blocks go to the 8 XCDs in turn: a tile's passes follow each other on one, whose L2 then has its weights
-    const int32_t xcd = blockIdx.x & 7, idx = blockIdx.x >> 3;
-    const int32_t pass = idx % L.passes, grp = idx / L.passes * 8 + xcd;
-    if (grp >= L.groups_n) return;
-    const int32_t ks = wave % L.ks;
-    const int64_t n0 = ((int64_t)grp * (L.waves / L.ks) + wave / L.ks) * 16, m0 = (int64_t)pass * kQ4Rows;
+    const int32_t slot = blockIdx.x, pass = blockIdx.y, split = blockIdx.z;
+    if (slot >= L.slots) return;
+    const int32_t KS = 1 << L.log_ks, ks = wave & (KS - 1), mytile = wave >> L.log_ks;
+    const int64_t m0 = (int64_t)pass * kQ4Rows;
     const int32_t rows = (int32_t)(a.M - m0 < kQ4Rows ? a.M - m0 : kQ4Rows);
     const int32_t K = (int32_t)a.K, steps = (K + kQ4Step - 1) / kQ4Step, groups = K / G;
+    const int32_t s0 = split * L.seg, s1 = s0 + L.seg < steps ? s0 + L.seg : steps;
+    const int32_t mine = (s1 - s0 - ks + KS - 1) >> L.log_ks;   // steps s0 + ks + KS i of every tile are the wave's
+    const int32_t turns = (mine + DEPTH - 1) / DEPTH * DEPTH;   // whole rings
     const int32_t pitch = L.seg * kQ4Step + 8;      // halves between rows of x in LDS
     f16* xs = reinterpret_cast<f16*>(smem);
     const int32_t plane = L.rows * pitch;           // F32: the low parts' plane is at +plane
@@ -99,21 +103,25 @@ __global__ __launch_bounds__(512) void k_linear_q4(Q4Args a, Q4Launch L)
     uint32_t* stile = reinterpret_cast<uint32_t*>(tile + 16 * kQ4WPitch);
     const AT* x = (const AT*)a.inp + m0 * a.K;
 
-    // weights: rows past N are row N - 1, pieces past K the last one (met by zeros in x)
-    const int64_t ra = n0 + (lane >> 3) < a.N ? n0 + (lane >> 3) : a.N - 1;
-    const int64_t rb = n0 + 8 + (lane >> 3) < a.N ? n0 + 8 + (lane >> 3) : a.N - 1;
-    const int64_t rn = n0 + n < a.N ? n0 + n : a.N - 1;
-    const uint8_t* wa = a.w + ra * (K / 2);
-    const uint8_t* wb = a.w + rb * (K / 2);
-    const uint16_t* sc = a.scales + rn * groups;
-    const uint8_t* zp = ZP ? a.zeros + rn * groups : nullptr;
+    // the weights of a group's tile: rows past N are row N - 1, pieces past K the last one (met by zeros in x)
+    const uint8_t *wa, *wb, *zp = nullptr;
+    const uint16_t* sc;
+    auto first_channel = [&](int32_t grp) { return ((int64_t)grp * L.tiles + mytile) * 16; };
+    auto point = [&](int32_t grp) {
+        const int64_t n0 = first_channel(grp), last = a.N - 1;
+        const int64_t ra = n0 + (lane >> 3), rb = ra + 8, rn = n0 + n;
+        wa = a.w + (ra < last ? ra : last) * (K / 2);
+        wb = a.w + (rb < last ? rb : last) * (K / 2);
+        sc = a.scales + (rn < last ? rn : last) * groups;
+        if (ZP) zp = a.zeros + (rn < last ? rn : last) * groups;
+    };
     struct Slot {
         u4 a, b;
         uint16_t s[NS];
         uint8_t z[NS];
     } ring[DEPTH];
-    auto issue = [&](int u, int32_t st) {
-        st = st < steps ? st : steps - 1;  // past the end: the last step again, never used
+    auto issue = [&](int u, int32_t i) {
+        const int32_t at_step = s0 + ks + (i << L.log_ks), st = at_step < steps ? at_step : steps - 1;  // past the end: never used
         const int32_t at = st * (kQ4Step / 2) + (lane & 7) * 16, last = K / 2 - 16;
         ring[u].a = *reinterpret_cast<const u4*>(wa + (at < last ? at : last));
         ring[u].b = *reinterpret_cast<const u4*>(wb + (at < last ? at : last));
@@ -138,12 +146,12 @@ __global__ __launch_bounds__(512) void k_linear_q4(Q4Args a, Q4Launch L)
     const int32_t first = F32 ? wave : tid, stride = F32 ? L.waves : threads;
     const int32_t per = L.seg * (kQ4Step / PIECE);
     u4 xr[kQ4Batch];
-    auto load_x = [&](int32_t i0, int32_t st0) {
+    auto load_x = [&](int32_t i0) {
 #pragma unroll
         for (int j = 0; j < kQ4Batch; j++) {
             const int32_t i = i0 + j * stride;
             if ((F32 ? i : i - first) >= rows * per) break;
-            const int32_t m = (int32_t)__umulhi((uint32_t)i, L.inv_per), at = st0 * kQ4Step + (i - m * per) * PIECE + (F32 ? lane * 4 : 0);
+            const int32_t m = (int32_t)__umulhi((uint32_t)i, L.inv_per), at = s0 * kQ4Step + (i - m * per) * PIECE + (F32 ? lane * 4 : 0);
             xr[j] = u4{};
             if (m < rows && at < K) xr[j] = *reinterpret_cast<const u4*>(x + (int64_t)m * K + at);
         }
@@ -185,8 +193,9 @@ __global__ __launch_bounds__(512) void k_linear_q4(Q4Args a, Q4Launch L)
         }
     };
     const Q4Masks masks = q4_masks();
-    f4 acc = {};
-    auto consume = [&](int u, int32_t st) {         // st: the step within x in LDS
+    f4 acc;
+    auto consume = [&](int u, int32_t i) {
+        const int32_t st = ks + (i << L.log_ks);           // within x in LDS
         *reinterpret_cast<u4*>(tile + (lane >> 3) * kQ4WPitch + (lane & 7) * 16) = ring[u].a;
         *reinterpret_cast<u4*>(tile + (8 + (lane >> 3)) * kQ4WPitch + (lane & 7) * 16) = ring[u].b;
 #pragma unroll
@@ -234,128 +243,161 @@ __global__ __launch_bounds__(512) void k_linear_q4(Q4Args a, Q4Launch L)
         }
     };
 
-    load_x(first, 0);
+    load_x(first);
+    point(slot);
 #pragma unroll
-    for (int u = 0; u < DEPTH; u++) issue(u, ks + u * L.ks);
-    // step ks + KS i is the wave's i-th; x is in LDS for L.seg steps at a time, all of them or a
-    // multiple of KS * DEPTH
-    for (int32_t st0 = 0; st0 < steps; st0 += L.seg) {
-        const int32_t st1 = st0 + L.seg < steps ? st0 + L.seg : steps;
-        if (st0 > 0) {
-            load_x(first, st0);
-            lds_barrier();
-        }
-        store_x(first);
-        for (int32_t i = kQ4Batch * stride; i < rows * per; i += kQ4Batch * stride) {
-            load_x(first + i, st0);
-            store_x(first + i);
-        }
-        lds_barrier();
-        for (int32_t st = st0 + ks; st < st1; st += L.ks * DEPTH) {
-            if (st + L.ks * DEPTH < steps) {     // this ring is full, and steps follow
+    for (int u = 0; u < DEPTH; u++) issue(u, u);
+    store_x(first);
+    for (int32_t i = kQ4Batch * stride; i < rows * per; i += kQ4Batch * stride) {
+        load_x(first + i);
+        store_x(first + i);
+    }
+    lds_barrier();
+    for (int32_t grp = slot; grp < L.groups_n; grp += L.slots) {
+        const bool next = grp + L.slots < L.groups_n;
+        acc = f4{};
+        for (int32_t i = 0; i < turns; i += DEPTH) {
+            // the ring is refilled with this tile's steps, at their end with the next tile's first ones
+            // (no work of a step ahead of the one before it: registers)
+            if (i + DEPTH < turns) {
 #pragma unroll
                 for (int u = 0; u < DEPTH; u++) {
-                    consume(u, st - st0 + u * L.ks);
-                    __builtin_amdgcn_sched_barrier(0);  // no work of the next step ahead of this one's: registers
-                    issue(u, st + (u + DEPTH) * L.ks);
+                    consume(u, i + u);
+                    __builtin_amdgcn_sched_barrier(0);
+                    issue(u, i + u + DEPTH);
+                }
+            } else if (next) {
+                point(grp + L.slots);
+#pragma unroll
+                for (int u = 0; u < DEPTH; u++) {
+                    if (i + u < mine) consume(u, i + u);
+                    __builtin_amdgcn_sched_barrier(0);
+                    issue(u, u);
                 }
             } else {
 #pragma unroll
                 for (int u = 0; u < DEPTH; u++) {
-                    if (st + u * L.ks < st1) consume(u, st - st0 + u * L.ks);
+                    if (i + u < mine) consume(u, i + u);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
         }
-    }
-    // ---- the waves' sums, and out ----
-    float* red = reinterpret_cast<float*>(tile);
-    if (L.ks > 1) {
-        lds_barrier();
-        *reinterpret_cast<f4*>(red + lane * 4) = acc;
-        lds_barrier();
-        if (ks != 0) return;
-        for (int i = 1; i < L.ks; i++) acc += *reinterpret_cast<const f4*>(red + i * (kQ4Tile / 4) + lane * 4);
-    }
-    if (n0 + n >= a.N) return;
-    const float bias = a.bias ? a.bias[n0 + n] : 0.0f;
+        // the sums of the tile's waves, through their weight tiles
+        if (KS > 1) {
+            *reinterpret_cast<f4*>(tile + lane * 16) = acc;
+            lds_barrier();
+            if (ks == 0)
+                for (int i = 1; i < KS; i++) acc += *reinterpret_cast<const f4*>(tile + i * kQ4Tile + lane * 16);
+            if (next) lds_barrier();  // read before the next tile's weights
+            if (ks != 0) continue;
+        }
+        const int64_t n1 = first_channel(grp) + n;
+        if (n1 >= a.N) continue;
+        const float bias = a.bias ? a.bias[n1] : 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        if (4 * g4 + i >= rows) break;
-        const int64_t o = (m0 + 4 * g4 + i) * a.N + n0 + n;
-        float y = acc[i] + bias;
-        if (L.out_f16) {
-            if (a.res) y += (float)((const f16*)a.res)[o];
-            ((f16*)a.out)[o] = (f16)y;
-        } else {
-            if (a.res) y += ((const float*)a.res)[o];
-            ((float*)a.out)[o] = y;
+        for (int i = 0; i < 4; i++) {
+            if (4 * g4 + i >= rows) break;
+            const int64_t o = (m0 + 4 * g4 + i) * a.N + n1;
+            if (L.splits > 1) {
+                L.ws[(int64_t)split * a.M * a.N + o] = acc[i];
+                continue;
+            }
+            float y = acc[i] + bias;
+            if (L.out_f16) {
+                if (a.res) y += (float)((const f16*)a.res)[o];
+                ((f16*)a.out)[o] = (f16)y;
+            } else {
+                if (a.res) y += ((const float*)a.res)[o];
+                ((float*)a.out)[o] = y;
+            }
         }
     }
 }
 
-// K = 0: bias and residual alone.
+// The sums of the splits, in order, then bias and residual; also K = 0 (no splits).
 template <typename OT>
-__global__ __launch_bounds__(256) void k_linear_q4_none(Q4Args a)
+__global__ __launch_bounds__(256) void k_linear_q4_join(Q4Args a, const float* __restrict__ ws, int32_t splits)
 {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.M * a.N; i += (int64_t)gridDim.x * 256)
-        ((OT*)a.out)[i] = (OT)((a.bias ? a.bias[i % a.N] : 0.0f) + (a.res ? (float)((const OT*)a.res)[i] : 0.0f));
+    const int64_t all = a.M * a.N;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+        float y = 0.0f;
+#pragma unroll 4
+        for (int32_t s = 0; s < splits; s++) y += ws[s * all + i];
+        y += a.bias ? a.bias[i % a.N] : 0.0f;
+        ((OT*)a.out)[i] = (OT)(y + (a.res ? (float)((const OT*)a.res)[i] : 0.0f));
+    }
 }
 
-int64_t q4_lds(int64_t seg, int64_t waves, int64_t rows, bool f32)
+constexpr int64_t kQ4Lds = 160 * 1024;
+
+int64_t q4_lds(const Q4Plan& p, int64_t rows, bool f32)
 {
-    return (f32 ? 2 : 1) * rows * (seg * kQ4Step + 8) * 2 + (f32 ? seg * kQ4Rows * 4 : 0) + waves * kQ4Tile;
+    return (f32 ? 2 : 1) * rows * (p.seg * kQ4Step + 8) * 2 + (f32 ? p.seg * kQ4Rows * 4 : 0) +
+           p.waves * kQ4Tile;
 }
 
 }  // namespace
 
-int launch_linear_q4(const Q4Args& a, int act, int out, int64_t cus, void* stream)
+Q4Plan linear_q4_plan(const Q4Args& a, int act, int64_t cus)
 {
-    hipStream_t st = static_cast<hipStream_t>(stream);
-    if (a.K == 0) {
-        const dim3 grid((unsigned)std::min<int64_t>((a.M * a.N + 255) / 256, 65536));
-        if (out == VVH_F16) hipLaunchKernelGGL(k_linear_q4_none<f16>, grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL(k_linear_q4_none<float>, grid, dim3(256), 0, st, a);
-        return (int)hipGetLastError();
-    }
     const bool f32 = act == VVH_F32;
     const int64_t tiles = (a.N + 15) / 16, steps = (a.K + kQ4Step - 1) / kQ4Step, passes = (a.M + kQ4Rows - 1) / kQ4Rows,
                   rows = std::min<int64_t>(a.M, kQ4Rows);
-    int64_t ks = 1;
-    while (ks < 8 && ks < steps && tiles * passes * ks < 4 * cus) ks *= 2;
-    const int64_t waves = std::max<int64_t>(4, ks);
-    // x in LDS: all of it, or a multiple of ks * 4 steps (at least one: 128 KB at 16 steps of fp16,
-    // 8 of fp32)
-    constexpr int64_t kLds = 160 * 1024;
-    int64_t seg = std::max<int64_t>(2, steps);
-    if (q4_lds(seg, waves, rows, f32) > kLds) {
-        while (ks > 1 && q4_lds(ks * 4, waves, rows, f32) > kLds) ks /= 2;
-        seg = ks * 4;
-        while (q4_lds(seg + ks * 4, waves, rows, f32) <= kLds) seg += ks * 4;
+    Q4Plan p{};
+    if (steps == 0) return p;
+    p.splits = 1;
+    p.ks = 1;
+    p.waves = 8;
+    p.seg = std::max<int64_t>(2, steps);
+    const int64_t most = f32 && rows > 4 ? 96 * 1024 : kQ4Lds;
+    while (q4_lds(p, rows, f32) > most) {
+        p.splits++;
+        p.seg = std::max<int64_t>(2, (steps + p.splits - 1) / p.splits);
     }
-    Q4Launch L{(int32_t)waves, (int32_t)ks, (int32_t)seg, (int32_t)passes, 0, (int32_t)rows, 0, out == VVH_F16};
-    L.groups_n = (int32_t)((tiles + waves / ks - 1) / (waves / ks));
-    const int64_t blocks = (L.groups_n + 7) / 8 * 8 * passes;
-    if (blocks > INT32_MAX) return (int)hipErrorInvalidValue;
-    L.inv_per = (uint32_t)(((uint64_t(1) << 32) + seg * (f32 ? 1 : 32) - 1) / (seg * (f32 ? 1 : 32)));
-    const int64_t mine = (steps + ks - 1) / ks, depth = mine > 2 ? 4 : mine;  // steps of a wave
-    const size_t lds = (size_t)q4_lds(seg, waves, rows, f32);
-    auto go = [&](auto kern) {
-        hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3((unsigned)(64 * waves)), lds, st, a, L);
-    };
-    auto go_depth = [&](auto* t, auto g, auto z) {
-        using AT = std::remove_pointer_t<decltype(t)>;
-        constexpr int G = decltype(g)::value;
-        constexpr bool ZP = decltype(z)::value;
-        depth == 1 ? go(k_linear_q4<AT, G, ZP, 1>) : depth == 2 ? go(k_linear_q4<AT, G, ZP, 2>) : go(k_linear_q4<AT, G, ZP, 4>);
-    };
-    auto go_group = [&](auto* t, auto z) {
-        a.group == 32   ? go_depth(t, std::integral_constant<int, 32>{}, z)
-        : a.group == 64 ? go_depth(t, std::integral_constant<int, 64>{}, z)
-                        : go_depth(t, std::integral_constant<int, 128>{}, z);
-    };
-    auto go_type = [&](auto* t) { a.zeros ? go_group(t, std::true_type{}) : go_group(t, std::false_type{}); };
-    f32 ? go_type((float*)nullptr) : go_type((f16*)nullptr);
+    while (p.ks < 8 && p.ks < p.seg && tiles * passes * p.splits * p.ks < (rows > 4 ? 4 : 8) * cus) p.ks *= 2;
+    p.waves = rows > 4 ? 8 : std::max<int64_t>(4, p.ks);
+    p.splits = (steps + p.seg - 1) / p.seg;
+    p.ws_floats = p.splits > 1 ? p.splits * a.M * a.N : 0;
+    return p;
+}
+
+int launch_linear_q4(const Q4Plan& p, const Q4Args& a, int act, int out, float* ws, int64_t cus, void* stream)
+{
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const bool f32 = act == VVH_F32;
+    if (p.splits > 0) {
+        const int64_t tiles = (a.N + 15) / 16, passes = (a.M + kQ4Rows - 1) / kQ4Rows, rows = std::min<int64_t>(a.M, kQ4Rows);
+        const int64_t per = p.seg * (f32 ? 1 : kQ4Step / 8), lds = q4_lds(p, rows, f32);
+        const int64_t tpb = p.waves / p.ks, groups = (tiles + tpb - 1) / tpb;
+        // Blocks of a group are enough where x costs little to stage; else a block takes several groups with the
+        // x it has, while the blocks still fill the device
+        const int64_t fit = std::max<int64_t>(1, std::min(kQ4Lds / lds, 16 / p.waves));
+        const int64_t worth = (rows * (f32 ? 4 : 2) + tpb - 1) / tpb, full = groups * passes * p.splits / (fit * cus);
+        const int64_t turns = std::max<int64_t>(1, std::min(worth, full)), slots = (groups + turns - 1) / turns;
+        const dim3 grid((unsigned)((slots + 7) / 8 * 8), (unsigned)passes, (unsigned)p.splits);
+        Q4Launch L{(int32_t)p.waves, (int32_t)tpb, 0, (int32_t)p.seg, (int32_t)p.splits, (int32_t)groups, (int32_t)slots, (int32_t)rows,
+                   (uint32_t)(((uint64_t(1) << 32) + per - 1) / per), out == VVH_F16, ws};
+        while ((1 << L.log_ks) < p.ks) L.log_ks++;
+        const bool one = (p.seg + p.ks - 1) / p.ks == 1 && turns == 1;  // a single step a wave
+        auto go = [&](auto kern) {
+            hipLaunchKernelGGL(kern, grid, dim3((unsigned)(64 * p.waves)), (size_t)lds, st, a, L);
+        };
+        auto go_group = [&](auto* t, auto z) {
+            using AT = std::remove_pointer_t<decltype(t)>;
+            constexpr bool ZP = decltype(z)::value;
+            if (one)
+                a.group == 32 ? go(k_linear_q4<AT, 32, ZP, 1>) : a.group == 64 ? go(k_linear_q4<AT, 64, ZP, 1>) : go(k_linear_q4<AT, 128, ZP, 1>);
+            else
+                a.group == 32 ? go(k_linear_q4<AT, 32, ZP, 2>) : a.group == 64 ? go(k_linear_q4<AT, 64, ZP, 2>) : go(k_linear_q4<AT, 128, ZP, 2>);
+        };
+        auto go_type = [&](auto* t) { a.zeros ? go_group(t, std::true_type{}) : go_group(t, std::false_type{}); };
+        f32 ? go_type((float*)nullptr) : go_type((f16*)nullptr);
+    }
+    if (p.splits != 1) {
+        const dim3 grid((unsigned)std::min<int64_t>((a.M * a.N + 255) / 256, 65536));
+        if (out == VVH_F16) hipLaunchKernelGGL(k_linear_q4_join<f16>, grid, dim3(256), 0, st, a, ws, (int32_t)p.splits);
+        else hipLaunchKernelGGL(k_linear_q4_join<float>, grid, dim3(256), 0, st, a, ws, (int32_t)p.splits);
+    }
     return (int)hipGetLastError();
 }
 

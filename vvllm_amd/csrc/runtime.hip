@@ -2436,7 +2436,14 @@ VVH_API int vvh_linear_q4(void* out, const void* inp, const uint8_t* dev_weight,
     REQUIRE_INIT();
     const Q4Args a{out, inp, residual, dev_weight, dev_scales, dev_zeros, dev_bias, (int64_t)M, (int64_t)N, (int64_t)K,
                    (int32_t)group};
-    return ret_launch(launch_linear_q4(a, act_dtype, out_dtype, g_cu_count > 0 ? g_cu_count : 256, stream), "4-bit linear launch");
+    const int64_t cus = g_cu_count > 0 ? g_cu_count : 256;
+    const Q4Plan p = linear_q4_plan(a, act_dtype, cus);
+    float* ws = nullptr;
+    if (p.ws_floats > 0) {
+        const int st = workspace_for(stream, (std::size_t)p.ws_floats * 4, &ws);
+        if (st != VVH_OK) return st;
+    }
+    return ret_launch(launch_linear_q4(p, a, act_dtype, out_dtype, ws, cus, stream), "4-bit linear launch");
 }
 
 VVH_API int vvh_logits_rules(void* out, const void* logits, const vvh_logits_spec* rules, size_t rows, size_t n,
