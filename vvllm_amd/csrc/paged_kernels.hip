@@ -154,18 +154,21 @@ __device__ __forceinline__ h4 lds_tr16(const f16* p)
 template <typename T>
 struct PagedTile;
 
+// CH: keys at a time
 template <>
 struct PagedTile<f16> {
-    static constexpr int CH = 64;  // keys at a time
+    template <int D>
+    static constexpr int CH = D == 64 ? 64 : 32;
     template <int D>
     struct Q {
         h8 b[D / 32];
     };
     template <int D>
-    static constexpr int lds = CH * (D + 4);  // elements of a wave's V region
+    static constexpr int lds = CH<D> * (D + 4);  // elements of a wave's V region
 };
 template <>
 struct PagedTile<float> {
+    template <int D>
     static constexpr int CH = 32;
     template <int D>
     struct Q {
@@ -219,7 +222,7 @@ __device__ __forceinline__ void paged_chunks(const PagedArgs& c, const T* kh, co
                                              const typename PagedTile<T>::template Q<D>& q, int32_t c0, int32_t cstep,
                                              int32_t ke, float scale_log2, f16* vw, int lane, PagedAcc<D>& acc)
 {
-    constexpr int CH = PagedTile<T>::CH, NT = CH / 16;
+    constexpr int CH = PagedTile<T>::template CH<D>, NT = CH / 16;
     constexpr bool H16 = sizeof(T) == 2;
     constexpr int DS = H16 ? D / 32 : D / 16, DE = D / 16, VP = D + 4;
     constexpr int VW = D % 64 == 0 ? 4 : 2, VJ = D / (16 * VW);
@@ -389,11 +392,11 @@ struct PagedHeads {
 // One tile of one sequence by one block, its NW waves each every NW-th chunk, merged
 // through LDS: short contexts, in one launch.
 template <typename T, int D, int NW>
-__global__ __launch_bounds__(64 * NW) void k_attention_paged_one(PagedArgs c, T* __restrict__ out, const T* __restrict__ q,
+__global__ __launch_bounds__(64 * NW, 2) void k_attention_paged_one(PagedArgs c, T* __restrict__ out, const T* __restrict__ q,
                                                                  const int32_t* __restrict__ lens, PagedHeads hd, int32_t H,
                                                                  float scale_log2)
 {
-    constexpr int CH = PagedTile<T>::CH, OP = D + 4;
+    constexpr int CH = PagedTile<T>::template CH<D>, OP = D + 4;
     constexpr int VB = PagedTile<T>::template lds<D> * 2, OB = 16 * OP * 4;  // bytes a wave
     __shared__ __align__(16) char smem[NW * (VB > OB ? VB : OB)];
     __shared__ float wm[NW][16], wl[NW][16];
@@ -452,19 +455,27 @@ __device__ __forceinline__ int64_t wave_scan(int64_t v, int lane)
 // straight to out if it is the whole tile, else to the wave's slot 1 (a tile that
 // begins in its range) or 0, a row per head: O, m, l.  k_attention_paged_merge joins them.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void k_attention_paged_split(PagedArgs c, T* __restrict__ out, const T* __restrict__ q,
+__global__ __launch_bounds__(256, 2) void k_attention_paged_split(PagedArgs c, T* __restrict__ out, const T* __restrict__ q,
                                                                const int32_t* __restrict__ lens, PagedHeads hd, int32_t H,
-                                                               float scale_log2, float* __restrict__ ws, int32_t VH)
+                                                               float scale_log2, int64_t* __restrict__ before_out, float* __restrict__ ws,
+                                                                  int32_t VH)
 {
-    constexpr int CH = PagedTile<T>::CH;
+    constexpr int CH = PagedTile<T>::template CH<D>;
     constexpr int VB = PagedTile<T>::template lds<D>;
     __shared__ __align__(16) f16 vs[VB ? 4 * VB : 4];
     const int lane = threadIdx.x & 63, r = lane & 15, gr = lane >> 4;
     const int wb = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t w = (int64_t)blockIdx.x * 4 + wb;
+    // the sums of the chunks before each sequence, and of all: the first wave keeps them for the merge
     int64_t total = 0;
-    for (int32_t s0 = 0; s0 < c.B; s0 += 64) total += paged_window(c, lens, s0, lane, CH);
-    total = __shfl(wave_scan(total, lane), 63) * VH;
+    for (int32_t s0 = 0; s0 < c.B; s0 += 64) {
+        const int32_t n = paged_window(c, lens, s0, lane, CH);
+        const int64_t upto = total + wave_scan(n, lane);
+        if (w == 0 && s0 + lane < c.B) before_out[s0 + lane + 1] = upto;
+        total = __shfl(upto, 63);
+    }
+    if (w == 0 && lane == 0) before_out[0] = 0;
+    total *= VH;
     const int64_t W = total < (int64_t)gridDim.x * 4 ? total : (int64_t)gridDim.x * 4;  // no wave without a unit
     if (w >= W) return;
     const int64_t u0 = total * w / W, u1 = total * (w + 1) / W;
@@ -530,60 +541,68 @@ __global__ __launch_bounds__(256) void k_attention_paged_split(PagedArgs c, T* _
     }
 }
 
-// Block (h, s, z): dims 32 z .. of head h of sequence s.  Thread (x, d) merges every
-// S-th part (S = blockDim.x / 32) into a running maximum and sums rescaled to it, the S
-// of a dim merge the same way through LDS.
+// Block (h, s) joins the parts of head h of sequence s: D / 4 lanes a part, 4 dims a lane, each
+// group of lanes every S-th part into a running maximum and sums rescaled to it; then the groups of a
+// wave by lane shuffles, and the waves through LDS.
 template <typename T, int D>
-__global__ __launch_bounds__(1024) void k_attention_paged_merge(PagedArgs c, T* __restrict__ out,
-                                                                const int32_t* __restrict__ lens, PagedHeads hd, int32_t H,
-                                                                const float* __restrict__ ws, int32_t VH, int64_t waves, int32_t CH)
+__global__ __launch_bounds__(1024) void k_attention_paged_merge(int32_t B, T* __restrict__ out, PagedHeads hd, int32_t H,
+                                                                const int64_t* __restrict__ before, const float* __restrict__ ws,
+                                                                int32_t VH, int32_t waves)
 {
-    __shared__ float sm[1024], sn[1024], sd[1024];
-    const int tid = threadIdx.x, lane = tid & 63, d = blockIdx.z * 32 + (tid & 31), x = tid >> 5, S = blockDim.x >> 5;
+    constexpr int L = D / 4, GW = 64 / L;  // lanes a part, parts a wave at a time
+    __shared__ f4 so[16][L];
+    __shared__ float sm[16], sl[16];
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, NW = blockDim.x >> 6, grp = lane / L, d = lane - grp * L;
     const int32_t h = blockIdx.x, s = blockIdx.y, g = h / hd.G, t = (h - g * hd.G) / hd.GT, hr = h - g * hd.G - t * hd.GT;
-    const int32_t v = g * hd.tiles + t;
-    int64_t sum = 0, mine = 0;
-    for (int32_t s0 = 0; s0 < c.B; s0 += 64) {
-        const int32_t n = paged_window(c, lens, s0, lane, CH);
-        sum += n;
-        mine += s0 + lane < s ? n : 0;
-    }
-    for (int o = 32; o > 0; o >>= 1) {
-        sum += __shfl_xor(sum, o);
-        mine += __shfl_xor(mine, o);
-    }
-    const int32_t ns = (paged_len(c, lens, s) + CH - 1) / CH;
-    const int64_t at = ((int64_t)s * H + h) * D + d;
+    const int64_t first = before[s], ns = before[s + 1] - first, total = before[B] * VH;
+    T* o4 = out + ((int64_t)s * H + h) * D + 4 * d;
     if (ns == 0) {
-        if (x == 0) out[at] = (T)0.0f;
+        if (wv == 0 && grp == 0)
+#pragma unroll
+            for (int i = 0; i < 4; i++) o4[i] = (T)0.0f;
         return;
     }
-    const int64_t total = sum * VH, a = mine * VH + (int64_t)v * ns, b = a + ns - 1;  // first and last unit
+    const int64_t a = first * VH + (g * hd.tiles + t) * ns, b = a + ns - 1;  // first and last unit
     const int64_t W = total < waves ? total : waves;
     const int64_t w0 = ((a + 1) * W - 1) / total, w1 = ((b + 1) * W - 1) / total;
     if (w0 == w1) return;  // one wave had it all
-    float M = -INFINITY, num = 0.0f, den = 0.0f;
-#pragma unroll 4
-    for (int64_t w = w0 + x; w <= w1; w += S) {
-        const float* p = ws + ((w * 2 + (w == w0)) * hd.GT + hr) * (D + 4);
-        const float m = p[D], l = p[D + 1], o = p[d];
+    float M = -INFINITY, den = 0.0f;
+    f4 num = {};
+    auto join = [&](float m, float l, f4 o) {
         const float mn = fmaxf(M, m), mb = mn == -INFINITY ? 0.0f : mn;
         const float f = exp2f(M - mb), e = exp2f(m - mb);
         num = num * f + o * e;
         den = den * f + l * e;
         M = mn;
+    };
+    if (grp < GW) {
+#pragma unroll 4
+        for (int64_t w = w0 + wv * GW + grp; w <= w1; w += NW * GW) {
+            const float* p = ws + ((w * 2 + (w == w0)) * hd.GT + hr) * (D + 4);
+            join(p[D], p[D + 1], *reinterpret_cast<const f4*>(p + 4 * d));
+        }
     }
-    sm[tid] = M;
-    sn[tid] = num;
-    sd[tid] = den;
-    __syncthreads();
-    if (x) return;
-    float mt = -INFINITY;
-    for (int i = 0; i < S; i++) mt = fmaxf(mt, sm[i * 32 + tid]);
-    const float mb = mt == -INFINITY ? 0.0f : mt;
-    num = den = 0.0f;
-    for (int i = 0; i < S; i++) attn_merge_add(num, den, sm[i * 32 + tid], mb, sn[i * 32 + tid], sd[i * 32 + tid]);
-    out[at] = (T)(den == 0.0f ? 0.0f : num / den);
+#pragma unroll
+    for (int i = 1; i < GW; i++) {  // lanes past the first group's end with sums that nobody reads
+        const int from = (lane + i * L) & 63;
+        const float m = __shfl(M, from), l = __shfl(den, from);
+        const f4 o = {__shfl(num[0], from), __shfl(num[1], from), __shfl(num[2], from), __shfl(num[3], from)};
+        if (lane < L) join(m, l, o);
+    }
+    if (NW > 1) {
+        if (lane < L) so[wv][d] = num;
+        if (lane == 0) {
+            sm[wv] = M;
+            sl[wv] = den;
+        }
+        __syncthreads();
+        if (wv > 0) return;
+        if (lane < L)
+            for (int i = 1; i < NW; i++) join(sm[i], sl[i], so[i][d]);
+    }
+    if (lane < L)
+#pragma unroll
+        for (int i = 0; i < 4; i++) o4[i] = (T)(den == 0.0f ? 0.0f : num[i] / den);
 }
 
 }  // namespace
@@ -615,6 +634,9 @@ int launch_rope_append_paged(const PagedArgs& c, void* q_out, const void* q, con
 // Chunks of a context from which its tiles are split over waves.
 constexpr int64_t kPagedOneChunks = 16;
 
+// Floats of the chunk sums ahead of the parts in the workspace.
+static int64_t paged_before_floats(int64_t B) { return (2 * (B + 1) + 3) / 4 * 4; }
+
 bool attention_paged_tiled(const PagedArgs& c, const void* out, const void* q, int dtype)
 {
     const uintptr_t all = (uintptr_t)c.kp | (uintptr_t)c.vp | (uintptr_t)q;
@@ -638,7 +660,7 @@ AttnPagedPlan attention_paged_plan(const PagedArgs& c, const void* out, const vo
         const int64_t units = chunks * c.B * c.KVH * p.tiles;
         p.blocks = std::min<int64_t>((units + 3) / 4, 2 * cus);
     }
-    p.ws_floats = p.blocks * 4 * 2 * p.GT * (c.D + 4);
+    if (p.blocks > 0) p.ws_floats = paged_before_floats(c.B) + p.blocks * 4 * 2 * p.GT * (c.D + 4);
     return p;
 }
 
@@ -653,13 +675,16 @@ static void paged_go(const AttnPagedPlan& p, const PagedArgs& c, T* out, const T
                            hd, (int32_t)H, scale_log2);
         return;
     }
+    int64_t* before = reinterpret_cast<int64_t*>(ws);
+    float* parts = ws + paged_before_floats(c.B);
     hipLaunchKernelGGL((k_attention_paged_split<T, D>), dim3((unsigned)p.blocks), dim3(256), 0, s, c, out, q, lens, hd,
-                       (int32_t)H, scale_log2, ws, VH);
+                       (int32_t)H, scale_log2, before, parts, VH);
+    // waves of a merge block: about 4 parts a group of lanes if the sequences are alike
     const int64_t W = p.blocks * 4;
-    int64_t S = 2;
-    while (S < 32 && S * 4 < W / ((int64_t)VH * c.B)) S *= 2;
-    hipLaunchKernelGGL((k_attention_paged_merge<T, D>), dim3((unsigned)H, (unsigned)c.B, D / 32), dim3((unsigned)(32 * S)), 0, s,
-                       c, out, lens, hd, (int32_t)H, ws, VH, W, (int32_t)PagedTile<T>::CH);
+    int64_t nw = 1;
+    while (nw < 16 && nw * (256 / D) * 4 < W / ((int64_t)VH * c.B)) nw *= 2;
+    hipLaunchKernelGGL((k_attention_paged_merge<T, D>), dim3((unsigned)H, (unsigned)c.B), dim3((unsigned)(64 * nw)), 0, s,
+                       (int32_t)c.B, out, hd, (int32_t)H, before, parts, VH, (int32_t)W);
 }
 
 int launch_attention_paged(const AttnPagedPlan& p, const PagedArgs& c, void* out, const void* q, const int32_t* lens, int64_t H,
