@@ -421,10 +421,10 @@ int launch_rope_append_paged(const PagedArgs& c, void* q_out, const void* q, con
                              const float* rope, int64_t rope_positions, int dtype, void* stream);
 // How a call is run: tiled on the matrix cores or by the form for any shape; tiled
 // with blocks > 0 split over 4 * blocks waves (ws_floats floats of workspace, a
-// merge launch), else one block per tile of GT heads (`tiles` of a kv head).
+// merge launch), else one block of `waves` waves per tile of GT heads (`tiles` of a kv head).
 struct AttnPagedPlan {
     bool tiled;
-    int64_t GT, tiles, blocks, ws_floats;
+    int64_t GT, tiles, waves, blocks, ws_floats;
 };
 AttnPagedPlan attention_paged_plan(const PagedArgs& c, const void* out, const void* q, int64_t max_len, int64_t H, int dtype,
                                    int64_t cus);

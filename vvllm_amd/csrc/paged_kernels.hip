@@ -169,7 +169,7 @@ struct PagedTile<f16> {
 template <>
 struct PagedTile<float> {
     template <int D>
-    static constexpr int CH = 32;
+    static constexpr int CH = D == 128 ? 16 : 32;
     template <int D>
     struct Q {
         f4 b[D / 16];
@@ -440,13 +440,24 @@ __device__ __forceinline__ int32_t paged_window(const PagedArgs& c, const int32_
 {
     return s0 + lane < c.B ? (paged_len(c, lens, s0 + lane) + ch - 1) / ch : 0;
 }
-__device__ __forceinline__ int64_t wave_scan(int64_t v, int lane)
+// Sums over lanes 0 .. l in lane l (shifts within rows of 16, then the rows' last lanes broadcast).
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v)
 {
-    for (int o = 1; o < 64; o <<= 1) {
-        const int64_t u = __shfl_up(v, o);
-        if (lane >= o) v += u;
-    }
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false);
     return v;
+}
+__device__ __forceinline__ uint32_t lane_of(uint32_t v, int l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); }
+
+// a b / c and a / c, in 32 bits where they fit (a 64-bit division is 100 instructions)
+__device__ __forceinline__ uint64_t muldiv(uint64_t a, uint64_t b, uint64_t c)
+{
+    const uint64_t p = a * b;
+    return (p | c) >> 32 ? p / c : (uint32_t)p / (uint32_t)c;
 }
 
 // All chunks of all tiles of all sequences in one row (sequence by sequence, tile by
@@ -469,29 +480,29 @@ __global__ __launch_bounds__(256, 2) void k_attention_paged_split(PagedArgs c, T
     // the sums of the chunks before each sequence, and of all: the first wave keeps them for the merge
     int64_t total = 0;
     for (int32_t s0 = 0; s0 < c.B; s0 += 64) {
-        const int32_t n = paged_window(c, lens, s0, lane, CH);
-        const int64_t upto = total + wave_scan(n, lane);
-        if (w == 0 && s0 + lane < c.B) before_out[s0 + lane + 1] = upto;
-        total = __shfl(upto, 63);
+        const uint32_t upto = wave_scan((uint32_t)paged_window(c, lens, s0, lane, CH));  // at most 64 * 2^26
+        if (w == 0 && s0 + lane < c.B) before_out[s0 + lane + 1] = total + upto;
+        total += lane_of(upto, 63);
     }
     if (w == 0 && lane == 0) before_out[0] = 0;
     total *= VH;
     const int64_t W = total < (int64_t)gridDim.x * 4 ? total : (int64_t)gridDim.x * 4;  // no wave without a unit
     if (w >= W) return;
-    const int64_t u0 = total * w / W, u1 = total * (w + 1) / W;
+    const int64_t u0 = muldiv(total, w, W), u1 = muldiv(total, w + 1, W);
     // the window of sequences that holds unit u0
     int32_t s0 = 0, n = paged_window(c, lens, 0, lane, CH);
-    int64_t before = 0, upto = wave_scan(n, lane);
-    while ((before + __shfl(upto, 63)) * VH <= u0) {
-        before += __shfl(upto, 63);
+    int64_t before = 0;
+    uint32_t upto = wave_scan((uint32_t)n);
+    while ((before + lane_of(upto, 63)) * VH <= u0) {
+        before += lane_of(upto, 63);
         s0 += 64;
         n = paged_window(c, lens, s0, lane, CH);
-        upto = wave_scan(n, lane);
+        upto = wave_scan((uint32_t)n);
     }
     int sl = __builtin_ctzll(__ballot((before + upto) * VH > u0));  // the sequence's lane
-    int32_t ns = __shfl(n, sl);
-    int64_t rest = u0 - (before + __shfl(upto, sl) - ns) * VH;  // units before u0 in the sequence
-    int32_t v = (int32_t)(rest / ns), ci = (int32_t)(rest - (int64_t)v * ns);
+    int32_t ns = (int32_t)lane_of((uint32_t)n, sl);
+    const int64_t rest = u0 - (before + lane_of(upto, sl) - ns) * VH;  // units before u0 in the sequence
+    int32_t v = (int32_t)muldiv(rest, 1, ns), ci = (int32_t)(rest - (int64_t)v * ns);
     for (int64_t u = u0; u < u1;) {
         const int32_t s = s0 + sl, cnt = (int32_t)(ns - ci < u1 - u ? ns - ci : u1 - u);
         int32_t g, h0, nh;
@@ -536,9 +547,16 @@ __global__ __launch_bounds__(256, 2) void k_attention_paged_split(PagedArgs c, T
                 more = __ballot(n > 0);
             }
             sl = __builtin_ctzll(more);
-            ns = __shfl(n, sl);
+            ns = (int32_t)lane_of((uint32_t)n, sl);
         }
     }
+}
+
+// The wave whose range holds unit u: the last w with floor(total w / W) <= u, that is total w < (u + 1) W.
+__device__ __forceinline__ int64_t last_wave(int64_t u, int64_t W, int64_t total)
+{
+    const uint64_t p = (uint64_t)(u + 1) * (uint64_t)W - 1;
+    return (int64_t)((p | (uint64_t)total) >> 32 ? p / (uint64_t)total : (uint32_t)p / (uint32_t)total);
 }
 
 // Block (h, s) joins the parts of head h of sequence s: D / 4 lanes a part, 4 dims a lane, each
@@ -564,7 +582,7 @@ __global__ __launch_bounds__(1024) void k_attention_paged_merge(int32_t B, T* __
     }
     const int64_t a = first * VH + (g * hd.tiles + t) * ns, b = a + ns - 1;  // first and last unit
     const int64_t W = total < waves ? total : waves;
-    const int64_t w0 = ((a + 1) * W - 1) / total, w1 = ((b + 1) * W - 1) / total;
+    const int64_t w0 = last_wave(a, W, total), w1 = last_wave(b, W, total);
     if (w0 == w1) return;  // one wave had it all
     float M = -INFINITY, den = 0.0f;
     f4 num = {};
@@ -656,6 +674,7 @@ AttnPagedPlan attention_paged_plan(const PagedArgs& c, const void* out, const vo
     const int64_t cap = (int64_t)c.max_pages * c.P;
     const int64_t len = max_len > 0 && max_len < cap ? max_len : cap;
     const int64_t chunks = (len + 63) / 64;
+    p.waves = chunks > 4 ? 8 : 4;
     if (chunks > kPagedOneChunks) {
         const int64_t units = chunks * c.B * c.KVH * p.tiles;
         p.blocks = std::min<int64_t>((units + 3) / 4, 2 * cus);
@@ -671,8 +690,11 @@ static void paged_go(const AttnPagedPlan& p, const PagedArgs& c, T* out, const T
     const PagedHeads hd{(int32_t)(H / c.KVH), (int32_t)p.GT, (int32_t)p.tiles};
     const int32_t VH = (int32_t)(c.KVH * p.tiles);
     if (p.blocks == 0) {
-        hipLaunchKernelGGL((k_attention_paged_one<T, D, 4>), dim3((unsigned)VH, (unsigned)c.B), dim3(256), 0, s, c, out, q, lens,
-                           hd, (int32_t)H, scale_log2);
+        auto one = [&](auto kern) {
+            hipLaunchKernelGGL(kern, dim3((unsigned)VH, (unsigned)c.B), dim3((unsigned)(64 * p.waves)), 0, s, c, out, q, lens, hd,
+                               (int32_t)H, scale_log2);
+        };
+        p.waves == 8 ? one(k_attention_paged_one<T, D, 8>) : one(k_attention_paged_one<T, D, 4>);
         return;
     }
     int64_t* before = reinterpret_cast<int64_t*>(ws);
