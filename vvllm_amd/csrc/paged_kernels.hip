@@ -216,8 +216,9 @@ __device__ __forceinline__ constexpr int paged_dim(int e, int gr, int i)
 }
 
 // The chunks c0, c0 + cstep, ... below ke of sequence s.  kh, vh: the kv head's column
-// in the pages.
-template <typename T, int D>
+// in the pages; vw: the wave's LDS region (fp16).  BIG: the pages of K or V pass 4 GB, the reach of a
+// buffer load's 32-bit offset, and take 64-bit addresses (16 clocks of multiplication a load).
+template <typename T, int D, bool BIG>
 __device__ __forceinline__ void paged_chunks(const PagedArgs& c, const T* kh, const T* vh, int32_t s,
                                              const typename PagedTile<T>::template Q<D>& q, int32_t c0, int32_t cstep,
                                              int32_t ke, float scale_log2, f16* vw, int lane, PagedAcc<D>& acc)
@@ -230,51 +231,71 @@ __device__ __forceinline__ void paged_chunks(const PagedArgs& c, const T* kh, co
     const int r = lane & 15, gr = lane >> 4;
     const int64_t kvs = (int64_t)c.KVH * D;
     const int32_t* table = c.table + (int64_t)s * c.max_pages;
-    // the row of key c0 + lane (lanes past CH: of no key)
-    auto find = [&](int32_t at) {
-        const uint32_t key = (uint32_t)at + (uint32_t)lane;
-        if (lane >= CH || key >= (uint32_t)ke) return -1;
-        const uint32_t pg = key / (uint32_t)c.P;
-        const int32_t page = table[pg];
-        return page < 0 || page >= c.pages ? -1 : page * c.P + (int32_t)(key - pg * (uint32_t)c.P);
+    const uint64_t pool = (uint64_t)c.pages * c.P * kvs;  // values; a resource ends with the pages
+    const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<T*>(kh), 0, BIG ? 0 : (int)(uint32_t)((pool - (uint64_t)(kh - (const T*)c.kp)) * sizeof(T)), 0x00020000);
+    const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<T*>(vh), 0, BIG ? 0 : (int)(uint32_t)((pool - (uint64_t)(vh - (const T*)c.vp)) * sizeof(T)), 0x00020000);
+    const uint32_t stride = (uint32_t)kvs * (uint32_t)sizeof(T);
+    // The page of key at + lane and its row there, looked up a chunk ahead and turned into a row of the
+    // pages (-1: no key, or no page) only when it is used, so that nothing waits for it.
+    struct Spot {
+        int32_t page, in;
     };
-    int32_t row = c0 < ke ? find(c0) : -1;
+    auto look = [&](int32_t at) {
+        const uint32_t key = (uint32_t)(at + lane < ke ? at + lane : ke - 1), pg = key / (uint32_t)c.P;
+        return Spot{table[pg], (int32_t)(key - pg * (uint32_t)c.P)};
+    };
+    if (c0 >= ke) return;
+    Spot spot = look(c0);
     for (; c0 < ke; c0 += cstep) {
+        const int32_t row = lane < CH && c0 + lane < ke && spot.page >= 0 && spot.page < c.pages ? spot.page * c.P + spot.in : -1;
         const uint64_t live = __ballot(row >= 0);
-        const bool all = live == (CH == 64 ? ~0ull : (1ull << CH) - 1);
-        const int32_t at = row < 0 ? 0 : row;
-        auto row_of = [&](int j) { return (int64_t)__shfl(at, j) * kvs; };
+        const bool all = live == ~0ull >> (64 - CH);
+        // every lane's row (its byte offset) to the lanes that load it, all at once
+        const uint32_t at = row < 0 ? 0u : BIG ? (uint32_t)row : (uint32_t)row * stride;
+        constexpr int NVR = H16 ? CH * D / 512 : NT * 4;
+        uint32_t ak[NT], av[NVR];
+#pragma unroll
+        for (int t = 0; t < NT; t++) ak[t] = (uint32_t)__shfl((int)at, 16 * t + r);
+#pragma unroll
+        for (int i = 0; i < NVR; i++) av[i] = (uint32_t)__shfl((int)at, H16 ? (i * 64 + lane) / (D / 8) : 16 * (i / 4) + 4 * gr + i % 4);
+        __builtin_amdgcn_sched_barrier(0);
+        // 16 bytes (or 8) at byte `in` of a row
+        auto load16 = [&](const __amdgpu_buffer_rsrc_t& res, const T* col, uint32_t a, int in) {
+            if constexpr (BIG) return *reinterpret_cast<const u4*>(reinterpret_cast<const char*>(col + (int64_t)a * kvs) + in);
+            else return __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(res, a + in, 0, 0));
+        };
         f4 sc[NT];
         typename std::conditional<H16, h8, f4>::type ka[NT][DS];
         h8 vr[H16 ? CH * D / 512 : 1];
         vf vv[H16 ? 1 : NT][H16 ? 1 : 4][VJ];
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
-            const T* kr = kh + row_of(16 * t + r);
+        for (int t = 0; t < NT; t++)
 #pragma unroll
-            for (int x = 0; x < DS; x++) {
-                if constexpr (H16) ka[t][x] = *reinterpret_cast<const h8*>(kr + 32 * x + 8 * gr);
-                else ka[t][x] = *reinterpret_cast<const f4*>(kr + 16 * x + 4 * gr);
-            }
-        }
+            for (int x = 0; x < DS; x++)
+                ka[t][x] = __builtin_bit_cast(typename std::conditional<H16, h8, f4>::type, load16(rk, kh, ak[t], 64 * x + 16 * gr));
         if constexpr (H16) {
 #pragma unroll
-            for (int i = 0; i < CH * D / 512; i++) {
-                const int p = i * 64 + lane, j = p / (D / 8), col = p % (D / 8) * 8;
-                vr[i] = *reinterpret_cast<const h8*>(vh + row_of(j) + col);
-            }
+            for (int i = 0; i < CH * D / 512; i++)
+                vr[i] = __builtin_bit_cast(h8, load16(rv, vh, av[i], (i * 64 + lane) % (D / 8) * 16));
         } else {
 #pragma unroll
-            for (int t = 0; t < NT; t++)
+            for (int i = 0; i < NT * 4; i++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const T* vp = vh + row_of(16 * t + 4 * gr + i) + VW * r;
-#pragma unroll
-                    for (int x = 0; x < VJ; x++) vv[t][i][x] = *reinterpret_cast<const vf*>(vp + 16 * VW * x);
+                for (int x = 0; x < VJ; x++) {
+                    const int in = (16 * VW * x + VW * r) * 4;
+                    if constexpr (VW == 4) {
+                        vv[i / 4][i % 4][x] = __builtin_bit_cast(vf, load16(rv, vh, av[i], in));
+                    } else if constexpr (BIG) {
+                        vv[i / 4][i % 4][x] = *reinterpret_cast<const vf*>(vh + (int64_t)av[i] * kvs + in / 4);
+                    } else {
+                        const uint32_t off = av[i] + in;
+                        vv[i / 4][i % 4][x] = __builtin_bit_cast(vf, __builtin_amdgcn_raw_buffer_load_b64(rv, off, 0, 0));
+                    }
                 }
         }
-        // the next chunk's rows are on their way while this one is worked on
-        const int32_t next = c0 + cstep < ke ? find(c0 + cstep) : -1;
+        spot = look(c0 + cstep);
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             sc[t] = f4{};
@@ -300,22 +321,23 @@ __device__ __forceinline__ void paged_chunks(const PagedArgs& c, const T* kh, co
                 cm = fmaxf(cm, x);
             }
         cm = max_x32(max_x16(cm));
-        const float mn = fmaxf(acc.m, cm);
-        const float mb = mn == -INFINITY ? 0.0f : mn;  // no key yet: every weight below is 0
-        const float corr = exp2f(acc.m - mb);
+        if (__any(cm > acc.m)) {  // a new maximum for some head
+            const float mn = fmaxf(acc.m, cm), f = acc.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(acc.m - mn);
+            acc.l *= f;
+            acc.m = mn;
+#pragma unroll
+            for (int e = 0; e < DE; e++) acc.o[e] *= f;
+        }
+        const float mb = acc.m == -INFINITY ? 0.0f : acc.m;  // no key yet: every weight below is 0
         float ps = 0.0f;
 #pragma unroll
         for (int t = 0; t < NT; t++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                sc[t][i] = exp2f(sc[t][i] - mb);
+                sc[t][i] = __builtin_amdgcn_exp2f(sc[t][i] - mb);
                 ps += sc[t][i];
             }
-        ps = sum_x32(sum_x16(ps));
-        acc.l = __builtin_fmaf(acc.l, corr, ps);
-        acc.m = mn;
-#pragma unroll
-        for (int e = 0; e < DE; e++) acc.o[e] *= corr;
+        acc.l += sum_x32(sum_x16(ps));
         if constexpr (H16) {
             if (!all) {
 #pragma unroll
@@ -365,7 +387,6 @@ __device__ __forceinline__ void paged_chunks(const PagedArgs& c, const T* kh, co
                         acc.o[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv[t][i][e / VW][e % VW], sc[t][i], acc.o[e], 0, 0, 0);
                 }
         }
-        row = next;
     }
 }
 
@@ -391,7 +412,7 @@ struct PagedHeads {
 
 // One tile of one sequence by one block, its NW waves each every NW-th chunk, merged
 // through LDS: short contexts, in one launch.
-template <typename T, int D, int NW>
+template <typename T, int D, int NW, bool BIG>
 __global__ __launch_bounds__(64 * NW, 2) void k_attention_paged_one(PagedArgs c, T* __restrict__ out, const T* __restrict__ q,
                                                                  const int32_t* __restrict__ lens, PagedHeads hd, int32_t H,
                                                                  float scale_log2)
@@ -400,7 +421,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attention_paged_one(PagedArgs c,
     constexpr int VB = PagedTile<T>::template lds<D> * 2, OB = 16 * OP * 4;  // bytes a wave
     __shared__ __align__(16) char smem[NW * (VB > OB ? VB : OB)];
     __shared__ float wm[NW][16], wl[NW][16];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r = lane & 15, gr = lane >> 4;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, gr = lane >> 4;
     const int32_t s = blockIdx.y, len = paged_len(c, lens, s);
     int32_t g, h0, n;
     hd.at(blockIdx.x, g, h0, n);
@@ -409,7 +430,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attention_paged_one(PagedArgs c,
     paged_load_q<D>(q + row0 * D, n, lane, x);
     PagedAcc<D> acc;
     acc.clear();
-    paged_chunks<T, D>(c, (const T*)c.kp + g * D, (const T*)c.vp + g * D, s, x, w * CH, NW * CH, len, scale_log2,
+    paged_chunks<T, D, BIG>(c, (const T*)c.kp + g * D, (const T*)c.vp + g * D, s, x, w * CH, NW * CH, len, scale_log2,
                        reinterpret_cast<f16*>(smem + w * VB), lane, acc);
     __syncthreads();
     float* os = reinterpret_cast<float*>(smem);
@@ -460,12 +481,18 @@ __device__ __forceinline__ uint64_t muldiv(uint64_t a, uint64_t b, uint64_t c)
     return (p | c) >> 32 ? p / c : (uint32_t)p / (uint32_t)c;
 }
 
+__device__ __forceinline__ int64_t uniform(uint64_t v)
+{
+    return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 |
+                     (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
+}
+
 // All chunks of all tiles of all sequences in one row (sequence by sequence, tile by
 // tile): wave w of W (all waves, or T) takes units [T w / W, T (w + 1) / W) of its T, so
 // every wave has the same work however ragged the batch.  The part of a tile that a wave has goes
 // straight to out if it is the whole tile, else to the wave's slot 1 (a tile that
 // begins in its range) or 0, a row per head: O, m, l.  k_attention_paged_merge joins them.
-template <typename T, int D>
+template <typename T, int D, bool BIG>
 __global__ __launch_bounds__(256, 2) void k_attention_paged_split(PagedArgs c, T* __restrict__ out, const T* __restrict__ q,
                                                                const int32_t* __restrict__ lens, PagedHeads hd, int32_t H,
                                                                float scale_log2, int64_t* __restrict__ before_out, float* __restrict__ ws,
@@ -488,7 +515,7 @@ __global__ __launch_bounds__(256, 2) void k_attention_paged_split(PagedArgs c, T
     total *= VH;
     const int64_t W = total < (int64_t)gridDim.x * 4 ? total : (int64_t)gridDim.x * 4;  // no wave without a unit
     if (w >= W) return;
-    const int64_t u0 = muldiv(total, w, W), u1 = muldiv(total, w + 1, W);
+    const int64_t u0 = uniform(muldiv(total, w, W)), u1 = uniform(muldiv(total, w + 1, W));
     // the window of sequences that holds unit u0
     int32_t s0 = 0, n = paged_window(c, lens, 0, lane, CH);
     int64_t before = 0;
@@ -502,7 +529,8 @@ __global__ __launch_bounds__(256, 2) void k_attention_paged_split(PagedArgs c, T
     int sl = __builtin_ctzll(__ballot((before + upto) * VH > u0));  // the sequence's lane
     int32_t ns = (int32_t)lane_of((uint32_t)n, sl);
     const int64_t rest = u0 - (before + lane_of(upto, sl) - ns) * VH;  // units before u0 in the sequence
-    int32_t v = (int32_t)muldiv(rest, 1, ns), ci = (int32_t)(rest - (int64_t)v * ns);
+    int32_t v = __builtin_amdgcn_readfirstlane((int32_t)muldiv(rest, 1, ns));
+    int32_t ci = __builtin_amdgcn_readfirstlane((int32_t)(rest - (int64_t)v * ns));
     for (int64_t u = u0; u < u1;) {
         const int32_t s = s0 + sl, cnt = (int32_t)(ns - ci < u1 - u ? ns - ci : u1 - u);
         int32_t g, h0, nh;
@@ -512,9 +540,9 @@ __global__ __launch_bounds__(256, 2) void k_attention_paged_split(PagedArgs c, T
         paged_load_q<D>(q + row0 * D, nh, lane, x);
         PagedAcc<D> acc;
         acc.clear();
-        const int32_t len = paged_len(c, lens, s);
+        const int32_t len = __builtin_amdgcn_readfirstlane(paged_len(c, lens, s));
         const int64_t end = (int64_t)(ci + cnt) * CH;
-        paged_chunks<T, D>(c, (const T*)c.kp + g * D, (const T*)c.vp + g * D, s, x, ci * CH, CH,
+        paged_chunks<T, D, BIG>(c, (const T*)c.kp + g * D, (const T*)c.vp + g * D, s, x, ci * CH, CH,
                            end < len ? (int32_t)end : len, scale_log2, vs + wb * VB, lane, acc);
         if (r < nh) {
             if (cnt == ns) {
@@ -677,13 +705,15 @@ AttnPagedPlan attention_paged_plan(const PagedArgs& c, const void* out, const vo
     p.waves = chunks > 4 ? 8 : 4;
     if (chunks > kPagedOneChunks) {
         const int64_t units = chunks * c.B * c.KVH * p.tiles;
-        p.blocks = std::min<int64_t>((units + 3) / 4, 2 * cus);
+        // two blocks a CU; fp16 with few tiles one, whose waves have longer runs and fewer parts (32 contexts of
+        // 4096 keys of 8 heads of 128 107.0 -> 104.8 us; 96 ragged ones 84.5 -> 93; three of fp32 44.0 -> 51.3)
+        p.blocks = std::min<int64_t>((units + 3) / 4, (dtype == VVH_F16 && c.B * c.KVH * p.tiles <= cus ? 1 : 2) * cus);
     }
     if (p.blocks > 0) p.ws_floats = paged_before_floats(c.B) + p.blocks * 4 * 2 * p.GT * (c.D + 4);
     return p;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool BIG>
 static void paged_go(const AttnPagedPlan& p, const PagedArgs& c, T* out, const T* q, const int32_t* lens, int64_t H,
                      float scale_log2, float* ws, hipStream_t s)
 {
@@ -694,12 +724,12 @@ static void paged_go(const AttnPagedPlan& p, const PagedArgs& c, T* out, const T
             hipLaunchKernelGGL(kern, dim3((unsigned)VH, (unsigned)c.B), dim3((unsigned)(64 * p.waves)), 0, s, c, out, q, lens, hd,
                                (int32_t)H, scale_log2);
         };
-        p.waves == 8 ? one(k_attention_paged_one<T, D, 8>) : one(k_attention_paged_one<T, D, 4>);
+        p.waves == 8 ? one(k_attention_paged_one<T, D, 8, BIG>) : one(k_attention_paged_one<T, D, 4, BIG>);
         return;
     }
     int64_t* before = reinterpret_cast<int64_t*>(ws);
     float* parts = ws + paged_before_floats(c.B);
-    hipLaunchKernelGGL((k_attention_paged_split<T, D>), dim3((unsigned)p.blocks), dim3(256), 0, s, c, out, q, lens, hd,
+    hipLaunchKernelGGL((k_attention_paged_split<T, D, BIG>), dim3((unsigned)p.blocks), dim3(256), 0, s, c, out, q, lens, hd,
                        (int32_t)H, scale_log2, before, parts, VH);
     // waves of a merge block: about 4 parts a group of lanes if the sequences are alike
     const int64_t W = p.blocks * 4;
@@ -717,9 +747,13 @@ int launch_attention_paged(const AttnPagedPlan& p, const PagedArgs& c, void* out
         using T = std::remove_pointer_t<decltype(t)>;
         if (p.tiled) {
             const float sl = (float)((double)scale * 1.4426950408889634);  // scores in log2 units
-            if (c.D == 64) paged_go<T, 64>(p, c, (T*)out, (const T*)q, lens, H, sl, ws, st);
-            else if (c.D == 96) paged_go<T, 96>(p, c, (T*)out, (const T*)q, lens, H, sl, ws, st);
-            else paged_go<T, 128>(p, c, (T*)out, (const T*)q, lens, H, sl, ws, st);
+            auto run = [&](auto d) {
+                constexpr int D = decltype(d)::value;
+                const bool big = (uint64_t)c.pages * c.P * c.KVH * D * sizeof(T) > UINT32_MAX;
+                if (big) paged_go<T, D, true>(p, c, (T*)out, (const T*)q, lens, H, sl, ws, st);
+                else paged_go<T, D, false>(p, c, (T*)out, (const T*)q, lens, H, sl, ws, st);
+            };
+            c.D == 64 ? run(std::integral_constant<int, 64>{}) : c.D == 96 ? run(std::integral_constant<int, 96>{}) : run(std::integral_constant<int, 128>{});
         } else {
             hipLaunchKernelGGL(k_attention_paged<T>, dim3((unsigned)H, (unsigned)c.B), dim3(256), 0, st, c, (T*)out,
                                (const T*)q, lens, (int32_t)H, scale);
