@@ -454,7 +454,7 @@ int launch_linear_q4(const Q4Plan& p, const Q4Args& a, int act, int out, float* 
 
 // Logit rules (logits_kernels.hip)
 int launch_logits_rules(void* out, const void* logits, const vvh_logits_spec& r, int64_t rows, int64_t n, int dtype,
-                        void* stream);
+                        int64_t cus, void* stream);
 
 // Auxiliary kernels (aux_kernels.hip).
 // w: N x K elements of src_dtype (VVH_F32 or VVH_BF16)

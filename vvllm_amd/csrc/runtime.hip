@@ -2468,7 +2468,8 @@ VVH_API int vvh_logits_rules(void* out, const void* logits, const vvh_logits_spe
           (uintptr_t)r.bias_offsets | (uintptr_t)r.mask) & 3))
         return fail(VVH_ERR_INVALID_ARG, "misaligned pointer");
     REQUIRE_INIT();
-    return ret_launch(launch_logits_rules(out, logits, r, (int64_t)rows, (int64_t)n, dtype, stream), "logit rules launch");
+    return ret_launch(launch_logits_rules(out, logits, r, (int64_t)rows, (int64_t)n, dtype,
+                                          g_cu_count > 0 ? g_cu_count : 256, stream), "logit rules launch");
 }
 
 VVH_API int vvh_mirror_f32(const float* host, size_t n, int as_dtype, const void** dev)
