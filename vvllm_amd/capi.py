@@ -165,9 +165,9 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
 
 def call(name: str, *args) -> int:
     """Call a status-returning entry point; raise VVHError unless VVH_OK."""
-    lib = load()
+    lib = _lib or load()
     st = getattr(lib, name)(*args)
-    if name not in _NOT_STATUS and st != 0:
+    if st != 0 and name not in _NOT_STATUS:
         raise VVHError(name, st, lib.vvh_last_error().decode(errors="replace"))
     return st
 

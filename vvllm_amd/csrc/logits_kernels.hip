@@ -30,13 +30,18 @@ __global__ __launch_bounds__(1024) void k_logits_rules(T* out, const T* logits, 
     const T* x = logits + (int64_t)r * n + i0;
     T* y = out + (int64_t)r * n + i0;
     const uint8_t* mask = a.mask ? reinterpret_cast<const uint8_t*>(a.mask + (int64_t)r * a.mask_stride) + i0 / 8 : nullptr;
-    // the logits are on their way while the tokens are counted
-    Some<T, 8> v{};
+    // the logits (and mask) are on their way while the tokens are counted: as whole registers and, where the
+    // thread has no 8 of its own, those of another, so that nothing has to wait for them here
+    constexpr int NR = (int)sizeof(T) / 2;
+    typedef u4 __attribute__((aligned(2))) u4t;
+    u4 raw[NR];
     uint32_t bits = 0xFF;
-    if (tid * 8 + 8 <= len) {
-        v = *reinterpret_cast<const Some<T, 8>*>(x + tid * 8);
-        if (mask) bits = mask[tid];
+    if (len >= 8) {
+        const u4t* from = reinterpret_cast<const u4t*>(x + (tid * 8 + 8 <= len ? tid * 8 : 0));
+#pragma unroll
+        for (int k = 0; k < NR; k++) raw[k] = from[k];
     }
+    if (mask) bits = mask[tid * 8 < len ? tid : 0];
     const float rep = a.repetition ? a.repetition[r] : 1.0f, fr = a.frequency ? a.frequency[r] : 0.0f,
                 pr = a.presence ? a.presence[r] : 0.0f;
     int32_t total = 0, prompt = 0;
@@ -89,6 +94,8 @@ __global__ __launch_bounds__(1024) void k_logits_rules(T* out, const T* logits, 
     const bool apart = out != logits;
     const int32_t j = tid * 8;
     if (j + 8 <= len) {
+        Some<T, 8> v;
+        __builtin_memcpy(&v, raw, sizeof(v));
         uint32_t c[8] = {};
         int32_t e[8] = {-1, -1, -1, -1, -1, -1, -1, -1};
         uint32_t any = 0;
