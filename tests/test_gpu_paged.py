@@ -256,6 +256,29 @@ def test_scores_of_any_size(gpu, dtype, D):
     assert (np.abs(run_attention(pg, q) - ref) <= tol).all()
 
 
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("D", [64, 128, 40])
+@pytest.mark.parametrize("n", [500, 3000])
+@pytest.mark.parametrize("at", [0, 250, 499])
+def test_many_small_weights(gpu, dtype, D, n, at):
+    """One key of value 0 whose weight is 2^25.3 times every other's: the outputs are the others' values.  All terms
+    have one sign, so an output's relative error is that of the scores (their D products, in numerator and sum), of the
+    exponentials and weights (2^-20) and of the sums."""
+    rng = np.random.default_rng(D + n)
+    pg = Pages(rng, [n], 16, 2, D, dtype)
+    k, v = (a[pg.table[0, :-(-n // 16)]].reshape(-1, 2, D) for a in (pg.kp, pg.vp))
+    k[:n], v[:n] = 0, rng.uniform(60, 64, (n, 2, D))
+    k[at, :, 0], v[at] = 2.1923828125, 0
+    for a, r in ((pg.kp, k), (pg.vp, v)):
+        a[pg.table[0, :-(-n // 16)]] = r.reshape(-1, 16, 2, D)
+    pg.upload()
+    q = np.zeros((1, 6, D), NP[dtype])
+    q[:, :, 0] = 8
+    ref = attention_ref(pg, q, 1.0, HALF[dtype])[0]
+    rel = HALF[dtype] + 2.0 ** -20 + 2 * (D + 4) * 2.0 ** -24 * 8 * 2.1923828125 + (n / 4 + 16) * 2.0 ** -24
+    assert (np.abs(run_attention(pg, q, scale=1.0) - ref) <= rel * ref).all()
+
+
 def test_offsets_past_32_bits(gpu):
     """A pool of more than 2^31 values: pages at its end, in fp16 (5.4 GB a pool)."""
     rng = np.random.default_rng(1)

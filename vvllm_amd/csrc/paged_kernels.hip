@@ -181,8 +181,10 @@ __global__ __launch_bounds__(256) void k_attention_paged(PagedArgs c, T* __restr
 //   S^T = K . q^T   A = K rows straight from the pages (lane: key l % 16, 8 or 4 dims of
 //                   group l / 16: one 16-byte load), B = the tile's queries in the same
 //                   dims.  A lane then has head l % 16's scores of keys 4 (l / 16) + i.
-//   softmax         online, in log2 units: maximum and sum over the lane's scores and the
-//                   4 lanes of the head; all of it in fp32.
+//   softmax         online, in log2 units: maximum (rounded up to an integer: fewer new ones, whose
+//                   rescaling is exact) and sum over the lane's scores and the 4 lanes of the head; all of
+//                   it in fp32.  fp16: weights are times 2^14, numerators and sums alike, so that those of 2^-38 of the
+//                   largest still have a value in fp16 (thousands of small ones make up for a large one).
 //   O^T += V^T P^T  B = the lane's own weights (the keys of a product's slots are any as long
 //                   as A has the same), A = V^T: fp16 V rows pass through the wave's LDS
 //                   region and its transposing read, weights as fp16 pairs high + low (22 bits); fp32 V
@@ -371,13 +373,13 @@ __device__ __forceinline__ void paged_chunks(const PagedArgs& c, const T* kh, co
             }
         cm = max_x32(max_x16(cm));
         if (__any(cm > acc.m)) {  // a new maximum for some head
-            const float mn = fmaxf(acc.m, cm), f = acc.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(acc.m - mn);
+            const float mn = __builtin_ceilf(fmaxf(acc.m, cm)), f = acc.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(acc.m - mn);
             acc.l *= f;
             acc.m = mn;
 #pragma unroll
             for (int e = 0; e < DE; e++) acc.o[e] *= f;
         }
-        const float mb = acc.m == -INFINITY ? 0.0f : acc.m;  // no key yet: every weight below is 0
+        const float mb = acc.m == -INFINITY ? 0.0f : acc.m - (H16 ? 14.0f : 0.0f);  // no key yet: every weight below is 0
         float ps = 0.0f;
 #pragma unroll
         for (int t = 0; t < NT; t++)
