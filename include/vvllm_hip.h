@@ -23,7 +23,8 @@
  *   - A per-stream workspace that grows on demand (hipMalloc, to at least
  *     twice its size, never below 1 MiB) serves split-K GEMMs and
  *     fp32-activation GEMMs (M * K * 4 + M * 4 bytes for the split activations),
- *     single or in plans, multi-chunk decode attention, multi-block sampling,
+ *     single or in plans, multi-chunk decode attention, vvh_attention_paged and
+ *     vvh_linear_q4 where they split a row, multi-block sampling,
  *     and outside of captures vvh_dense of more than 4 rows and vvh_attention
  *     of several queries, where they split k or the keys.  Under HIP graph
  *     capture it cannot grow: run the same calls once on that stream before
@@ -584,11 +585,15 @@ VVH_API int vvh_rope_append_paged(const vvh_paged_cache* cache, void* q_out, con
  * the sequence's start, the new token's among them; a length past the page table's
  * max_pages * page_size counts as that, a negative one as 0.  Positions on
  * entries that are no page are left out; a row without any position gives
- * zeros.  max_len: the longest length to expect, 0 for unknown (the page table's
- * capacity); it steers how the work is split, longer rows are attended in full
- * all the same.  Cache rows that no sequence has reached may hold anything.  The
- * split's partial sums use the stream's workspace, whose size depends only on
- * num_seqs, the heads and max_len: make one such call before capturing on the stream. */
+ * zeros.  Cache rows that no sequence has reached may hold anything.  Sums and
+ * weights are fp32 (products of fp16 values exact), rounded once to the output;
+ * an infinite value among the rows attended to gives NaN in its dim.  max_len:
+ * the longest length to expect, 0 for unknown (the page table's capacity); it
+ * steers how the work is split, longer rows are attended in full all the same.
+ * Made for head_dim 64, 96 and 128 and 16-byte aligned arrays; others take a
+ * kernel of a block per head, which does not split a long row.  A split's partial
+ * sums use the stream's workspace, whose size depends only on num_seqs, the heads
+ * and max_len: make one such call before capturing on the stream. */
 VVH_API int vvh_attention_paged(const vvh_paged_cache* cache, void* out, const void* q, const int32_t* lens,
                                 size_t max_len, size_t num_heads, float scale, void* stream);
 /* Linear of 4-bit weights: out[M,N] = inp[M,K] . W[N,K]^T + bias[N] (+
@@ -596,10 +601,15 @@ VVH_API int vvh_attention_paged(const vvh_paged_cache* cache, void* out, const v
  * the code c of 4 bits and its group's zero point z.  dev_weight: rows of K / 2
  * bytes, code k in the low (k even) or high (k odd) half of byte k / 2;
  * dev_scales: [N, K / group] fp16 bits; dev_zeros: [N, K / group] bytes, or
- * NULL for 8 everywhere.  group 32, 64 or 128, K a multiple of it; inp and
- * dev_weight 16-byte aligned.  Activations are used as given, products summed in
- * fp32, the epilogue rounds once (as vvh_linear_q8).  Made for the few rows of a decode
- * step; more than 64 are taken 64 at a time, each pass reading the weights again. */
+ * NULL for 8 everywhere.  group 32, 64 or 128, K a multiple of it (at most
+ * 2^24); inp and dev_weight 16-byte aligned, out not inp.  Codes less zero points
+ * are exact; fp16 activations are used as given, fp32 ones to 22 bits of the
+ * largest of 256 neighbours in their row; products are summed in fp32 and the
+ * epilogue rounds once (as vvh_linear_q8).  Made for the few rows of a decode step:
+ * rows are taken 16 at a time, each 16 reading the weights again.  Rows of inp too
+ * long for a block's shared memory (at 16 rows past 4096 fp16 or 1024 fp32
+ * activations) share out k, whose sums use the stream's workspace (splits * M * N
+ * floats): make one such call before capturing on the stream. */
 VVH_API int vvh_linear_q4(void* out, const void* inp, const uint8_t* dev_weight, const uint16_t* dev_scales,
                           const uint8_t* dev_zeros, const float* dev_bias, const void* residual, size_t M, size_t N,
                           size_t K, size_t group, int act_dtype, int out_dtype, void* stream);
@@ -608,7 +618,7 @@ VVH_API int vvh_linear_q4(void* out, const void* inp, const uint8_t* dev_weight,
  * device memory and may be NULL where the rule is not wanted. */
 typedef struct vvh_logits_spec {
     const int32_t* tokens;        /* row r's tokens so far: tokens[r * token_stride ..] */
-    uint64_t token_stride;
+    uint64_t token_stride;        /* at most 2^30 */
     const int32_t* token_counts;  /* [rows] (clamped to token_stride); needed with tokens */
     const int32_t* prompt_counts; /* [rows]: how many of them are the prompt's; NULL: none */
     const float* repetition;      /* [rows]: logit > 0 ? logit / r : logit * r for tokens among them (r > 0) */
@@ -623,8 +633,8 @@ typedef struct vvh_logits_spec {
 } vvh_logits_spec;
 /* out[rows, n] = logits[rows, n] under the rules, in the order repetition,
  * frequency, presence, bias, mask, in fp32 and rounded once to dtype; out may be
- * logits itself (then only what a rule changes is written).  Tokens and ids outside [0, n) are ignored.
- * vvh_argmax or vvh_sample then choose a row's token. */
+ * logits itself, but not overlap it otherwise.  Tokens and ids outside [0, n) are
+ * ignored.  vvh_argmax or vvh_sample then choose a row's token. */
 VVH_API int vvh_logits_rules(void* out, const void* logits, const vvh_logits_spec* rules, size_t rows, size_t n,
                              int dtype, void* stream);
 

@@ -155,6 +155,19 @@ def test_activations_of_any_size(gpu, M):
         assert np.isnan(c.got()[2]).all() and not np.isfinite(c.got()[1]).any()
 
 
+@pytest.mark.parametrize("M", [1, 20])
+def test_an_infinity_next_to_large_values(gpu, M):
+    """Infinite outputs where one activation is infinite, finite ones of the other sign next to it or not."""
+    c = Case(M, 50, 512, 64, F32, F32)
+    c.codes[:] = 0xCC  # every weight above 0
+    c.x[:, 3::2] = -1e30
+    c.x[:, 2] = np.inf
+    c.x[:, 300] = 2e38
+    c.d["x"], c.d["codes"] = capi.DevBuf.from_array(c.x), capi.DevBuf.from_array(c.codes)
+    c.run()
+    assert (c.got() == np.inf).all()
+
+
 @pytest.mark.parametrize("act", [F16, F32])
 def test_rows_of_a_large_call_are_the_small_calls(gpu, act):
     """Outputs next to the last row and channel stay as they were."""

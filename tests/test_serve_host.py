@@ -22,7 +22,7 @@ def append(c, q_out=P, q=P, k=P, v=P, seqs=P, pos=P, tokens=4, heads=14, rope=P,
     return capi.status_of("vvh_rope_append_paged", c, q_out, q, k, v, seqs, pos, tokens, heads, rope, positions, None)
 
 
-def attention(c, out=P, q=P, lens=P, max_len=0, heads=14):
+def attention(c, out=P, q=2 * P, lens=P, max_len=0, heads=14):
     return capi.status_of("vvh_attention_paged", c, out, q, lens, max_len, heads, 0.125, None)
 
 
@@ -63,6 +63,7 @@ def test_attention_arguments():
     for name in ("out", "q", "lens"):
         assert attention(cache(), **{name: None}) == INVALID
         assert attention(cache(), **{name: P + 1}) == INVALID
+    assert attention(cache(), out=2 * P) == INVALID               # out is q
     assert attention(cache(), heads=15) == INVALID                # two kv heads
     assert attention(cache(), heads=65536) == UNSUPPORTED
     assert attention(cache(), heads=0) == 0
@@ -81,7 +82,7 @@ def test_rope_table_arguments():
     assert st("vvh_rope_table", P, 10, 64, 1e4, None) == NOT_INIT
 
 
-def linear(out=P, inp=P, w=P, s=P, z=None, b=None, r=None, M=1, N=16, K=128, group=64, act=F16, outd=F16):
+def linear(out=P, inp=2 * P, w=P, s=P, z=None, b=None, r=None, M=1, N=16, K=128, group=64, act=F16, outd=F16):
     return capi.status_of("vvh_linear_q4", out, inp, w, s, z, b, r, M, N, K, group, act, outd, None)
 
 
@@ -93,7 +94,9 @@ def test_linear_q4_arguments():
                dict(K=96), dict(K=160, group=128), dict(N=1 << 40, K=1 << 40)):
         assert linear(**kw) == INVALID, kw
     assert linear(N=1 << 31) == UNSUPPORTED
-    assert linear(K=1 << 31) == UNSUPPORTED
+    assert linear(out=2 * P) == INVALID                           # out is inp
+    assert linear(K=1 << 31) == UNSUPPORTED and linear(K=(1 << 24) + 64) == UNSUPPORTED
+    assert linear(M=1 << 19, N=1 << 22, K=64) == UNSUPPORTED
     assert linear(M=1 << 21) == UNSUPPORTED
     assert linear(M=0, out=None) == 0 and linear(N=0, out=None) == 0
     assert linear() == NOT_INIT and linear(z=P + 1, b=P, r=P) == NOT_INIT
@@ -118,7 +121,7 @@ def test_logits_rules_arguments():
     assert rules(mask=P, mask_stride=3) == INVALID                # 100 logits take 4 words
     assert rules(n=1 << 31) == UNSUPPORTED
     assert rules(rows=65536) == UNSUPPORTED
-    assert rules(token_stride=1 << 31) == UNSUPPORTED
+    assert rules(token_stride=(1 << 30) + 1) == UNSUPPORTED
     assert rules(rows=0, out=None) == 0 and rules(n=0, out=None) == 0
     assert rules() == NOT_INIT and rules(mask=P, mask_stride=0) == NOT_INIT and rules(bias_offsets=P) == NOT_INIT
 

@@ -167,16 +167,16 @@ __global__ __launch_bounds__(512) void k_linear_q4(Q4Args a, Q4Launch L)
             } else {
                 const f4 v = __builtin_bit_cast(f4, xr[j]);
                 const float most = group_max(fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))), 64);
-                // 2^(14 - x) for most in [2^x, 2^(x + 1)), at most 2^126; 1 with an infinity or NaN
-                const int b = (int)(__builtin_bit_cast(uint32_t, most) >> 23), e = b < 15 ? 15 : b;
-                const float up = e == 255 ? 1.0f : __builtin_bit_cast(float, (uint32_t)(268 - e) << 23);
+                // 2^(14 - x) for most in [2^x, 2^(x + 1)), at most 2^126; with an infinity that of the largest finite ones
+                const int b = (int)(__builtin_bit_cast(uint32_t, most) >> 23), e = b < 15 ? 15 : b > 254 ? 254 : b;
+                const float up = __builtin_bit_cast(float, (uint32_t)(268 - e) << 23);
                 uint32_t hi[2], lo[2];
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
                     const float p = v[2 * c] * up, q = v[2 * c + 1] * up;
                     const h2 h = {(f16)p, (f16)q};
                     h2 l = {(f16)(p - (float)h[0]), (f16)(q - (float)h[1])};
-                    if (e == 255) l = h2{};  // an infinity or NaN is all in its high part
+                    if (b == 255) l = h2{};  // an infinity is all in its high part
                     hi[c] = __builtin_bit_cast(uint32_t, h);
                     lo[c] = __builtin_bit_cast(uint32_t, l);
                 }
@@ -188,7 +188,7 @@ __global__ __launch_bounds__(512) void k_linear_q4(Q4Args a, Q4Launch L)
                 const u4 o = order(odd ? u4{r0, r1, lo[0], lo[1]} : u4{hi[0], hi[1], r0, r1});
                 *reinterpret_cast<u4*>(xs + (odd ? plane : 0) + m * pitch + k + (lane >> 1) * 8) = o;
                 if (lane == 0)
-                    xinv[k / kQ4Step * kQ4Rows + m] = e == 255 ? 1.0f : __builtin_bit_cast(float, (uint32_t)(e - 14) << 23);
+                    xinv[k / kQ4Step * kQ4Rows + m] = __builtin_bit_cast(float, (uint32_t)(e - 14) << 23);
             }
         }
     };

@@ -13,6 +13,7 @@
 #include <cstdio>
 #include <cstring>
 #include <mutex>
+#include <new>
 #include <string>
 #include <unordered_map>
 #include <vector>
@@ -140,10 +141,11 @@ std::unordered_map<void*, Workspace> g_ws;
 // mode, which forbids hipMalloc to every thread but those in the relaxed mode and
 // fails the capture where one is made (calls that needed no workspace once).
 int workspace_for(void* stream, std::size_t bytes, float** out, bool relaxed = false)
-{
+try {
     std::lock_guard<std::mutex> lock(g_wsmu);
     Workspace& w = g_ws[stream];
     if (w.bytes < bytes) {
+        w.retired.reserve(w.retired.size() + 1);
         const std::size_t nb = std::max({bytes, 2 * w.bytes, std::size_t(1) << 20});
         void* p = nullptr;
         hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
@@ -160,6 +162,8 @@ int workspace_for(void* stream, std::size_t bytes, float** out, bool relaxed = f
     }
     *out = static_cast<float*>(w.p);
     return VVH_OK;
+} catch (const std::bad_alloc&) {
+    return fail(VVH_ERR_OUT_OF_MEMORY, "workspace bookkeeping");
 }
 
 // The stream's workspace of `bytes`, for calls that can do without: false
@@ -2403,6 +2407,7 @@ VVH_API int vvh_attention_paged(const vvh_paged_cache* cache, void* out, const v
                     (unsigned long long)cache->num_kv_heads);
     if (cache->num_seqs == 0 || num_heads == 0) return VVH_OK;
     if (!out || !q || !lens) return fail(VVH_ERR_INVALID_ARG, "null pointer");
+    if (out == q) return fail(VVH_ERR_INVALID_ARG, "out is q");
     if (num_heads > 65535) return fail(VVH_ERR_UNSUPPORTED, "%zu heads", num_heads);
     const uintptr_t e = cache->dtype == VVH_F32 ? 3 : 1;
     if ((((uintptr_t)q | (uintptr_t)out) & e) || ((uintptr_t)lens & 3)) return fail(VVH_ERR_INVALID_ARG, "misaligned pointer");
@@ -2429,10 +2434,13 @@ VVH_API int vvh_linear_q4(void* out, const void* inp, const uint8_t* dev_weight,
     if (!mul_ok(M, N, &t) || !mul_ok(N, K, &t) || !mul_ok(M, K, &t)) return fail(VVH_ERR_INVALID_ARG, "size overflow");
     if (M == 0 || N == 0) return VVH_OK;
     if (!out || (K > 0 && (!inp || !dev_weight || !dev_scales))) return fail(VVH_ERR_INVALID_ARG, "null pointer");
+    if (out == inp) return fail(VVH_ERR_INVALID_ARG, "out is inp");
     if (!aligned16(inp) || !aligned16(dev_weight) || ((uintptr_t)dev_scales & 1) || ((uintptr_t)dev_bias & 3) ||
         (((uintptr_t)out | (uintptr_t)residual) & (dsize(out_dtype) - 1)))
         return fail(VVH_ERR_INVALID_ARG, "misaligned pointer");
-    if (N > INT32_MAX || K > INT32_MAX / 2 || M > 65535 * 16) return fail(VVH_ERR_UNSUPPORTED, "M %zu, N %zu, K %zu", M, N, K);
+    // K: 2^16 steps, so at most 2^15 splits of them and 65535 in a grid; M * N: the splits' sums in 64 bits
+    if (N > INT32_MAX || K > (size_t(1) << 24) || M > 65535 * 16 || M * N > (size_t(1) << 40))
+        return fail(VVH_ERR_UNSUPPORTED, "M %zu, N %zu, K %zu", M, N, K);
     REQUIRE_INIT();
     const Q4Args a{out, inp, residual, dev_weight, dev_scales, dev_zeros, dev_bias, (int64_t)M, (int64_t)N, (int64_t)K,
                    (int32_t)group};
@@ -2460,7 +2468,7 @@ VVH_API int vvh_logits_rules(void* out, const void* logits, const vvh_logits_spe
         return fail(VVH_ERR_INVALID_ARG, "mask_stride %llu is short of %zu logits", (unsigned long long)r.mask_stride, n);
     if (rows == 0 || n == 0) return VVH_OK;
     if (!out || !logits) return fail(VVH_ERR_INVALID_ARG, "null pointer");
-    if (n > INT32_MAX || rows > 65535 || r.token_stride > INT32_MAX || r.bias_count > INT32_MAX || r.mask_stride > INT32_MAX)
+    if (n > INT32_MAX || rows > 65535 || r.token_stride > (uint64_t(1) << 30) || r.bias_count > INT32_MAX || r.mask_stride > INT32_MAX)
         return fail(VVH_ERR_UNSUPPORTED, "%zu rows of %zu logits", rows, n);
     if ((((uintptr_t)out | (uintptr_t)logits) & (dsize(dtype) - 1)) ||
         (((uintptr_t)r.tokens | (uintptr_t)r.token_counts | (uintptr_t)r.prompt_counts | (uintptr_t)r.repetition |
