@@ -28,14 +28,15 @@ namespace {
 // nibble 1024 + 16 c); one packed subtraction (or multiply-add by 1 / 16) leaves c - z, exactly.
 // The dword of 8 codes gives them in the order 0 4 1 5 2 6 3 7, and x is staged in that order.
 // fp32 rows of x are staged as two fp16 planes, high and low parts of x times a power of two that
-// puts the step's largest |x| into [2^14, 2^15) (22 bits; the sum of a step is multiplied back).
+// puts the step's largest |x| into [2^14, 2^15) (22 bits; the sum of a step is multiplied back).  Up to 8 such
+// rows make 16 rows of the operand (FOLD): one instruction then takes both parts.
 // ---------------------------------------------------------------------------
 constexpr int kQ4Step = 256;     // codes of a row a step
 constexpr int kQ4WPitch = 144;   // bytes between rows of the LDS weight tile
 constexpr int kQ4SPitch = 12;    // dwords between rows of its scales
 constexpr int kQ4Tile = 16 * kQ4WPitch + 16 * kQ4SPitch * 4;
 constexpr int kQ4Rows = 16;
-constexpr int kQ4Batch = 4;      // pieces of x a wave loads at a time
+constexpr int kQ4Batch = 8;      // pieces of x a wave loads at a time
 
 // How a launch's blocks share out the work: block (slot, pass, split) takes the groups slot, slot +
 // slots, ... of `tiles` tiles, 16 rows, and the steps [split * seg, + seg).  Blocks go to the 8 XCDs in
@@ -76,12 +77,13 @@ __device__ __forceinline__ h8 q4_codes(uint32_t w, h2 zl, h2 zh, const Q4Masks& 
     return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-template <typename AT, int G, bool ZP, int DEPTH>
+template <typename AT, int G, bool ZP, int DEPTH, bool FOLD>
 __global__ __launch_bounds__(512) void k_linear_q4(Q4Args a, Q4Launch L)
 {
     constexpr bool F32 = sizeof(AT) == 4;
     constexpr int PG = kQ4Step / G;                 // groups a step
     constexpr int NS = PG > 4 ? 2 : 1;              // scales a lane loads a step
+    constexpr int OUT = FOLD ? 2 : 4;               // rows of a lane's sums
     constexpr int DW = G / 32;                      // dwords of codes a lane reads a group
     extern __shared__ __align__(16) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g4 = lane >> 4;
@@ -134,7 +136,7 @@ __global__ __launch_bounds__(512) void k_linear_q4(Q4Args a, Q4Launch L)
     };
 
     // ---- x ----
-    const int32_t row = n < rows ? n : rows - 1;    // rows of the operand past the last are computed and dropped
+    const int32_t arow = FOLD ? n >> 1 : n, row = arow < rows ? arow : rows - 1;  // past the last: computed and dropped
     auto order = [](u4 v) {                         // 0 1 2 3 4 5 6 7 -> 0 4 1 5 2 6 3 7
         return u4{__builtin_amdgcn_perm(v[2], v[0], 0x05040100u), __builtin_amdgcn_perm(v[2], v[0], 0x07060302u),
                   __builtin_amdgcn_perm(v[3], v[1], 0x05040100u), __builtin_amdgcn_perm(v[3], v[1], 0x07060302u)};
@@ -208,7 +210,7 @@ __global__ __launch_bounds__(512) void k_linear_q4(Q4Args a, Q4Launch L)
         uint32_t sv[PG];
 #pragma unroll
         for (int g = 0; g < PG; g++) sv[g] = stile[n * kQ4SPitch + g];
-        const f16* xk = xs + row * pitch + st * kQ4Step;
+        const f16* xk = xs + (FOLD && n & 1 ? plane : 0) + row * pitch + st * kQ4Step;
         f4 part = {};
 #pragma unroll
         for (int g = 0; g < PG; g++) {
@@ -227,14 +229,18 @@ __global__ __launch_bounds__(512) void k_linear_q4(Q4Args a, Q4Launch L)
             for (int j = 0; j < DW; j++) {
                 const h8 b = q4_codes(w[j], zl, zh, masks);
                 const f16* xp = xk + g * G + (g4 * DW + j) * 8;
-                if (F32) d = __builtin_amdgcn_mfma_f32_16x16x32_f16(*reinterpret_cast<const h8*>(xp + plane), b, d, 0, 0, 0);
+                if (F32 && !FOLD) d = __builtin_amdgcn_mfma_f32_16x16x32_f16(*reinterpret_cast<const h8*>(xp + plane), b, d, 0, 0, 0);
                 d = __builtin_amdgcn_mfma_f32_16x16x32_f16(*reinterpret_cast<const h8*>(xp), b, d, 0, 0, 0);
             }
             const float s = (float)q4_h2(sv[g])[0];
 #pragma unroll
             for (int i = 0; i < 4; i++) part[i] = __builtin_fmaf(s, d[i], part[i]);
         }
-        if constexpr (F32) {
+        if constexpr (FOLD) {
+            const float* inv = xinv + st * kQ4Rows + 2 * g4;
+#pragma unroll
+            for (int i = 0; i < 2; i++) acc[i] = __builtin_fmaf(part[2 * i] + part[2 * i + 1], inv[i], acc[i]);
+        } else if constexpr (F32) {
             const f4 inv = *reinterpret_cast<const f4*>(xinv + st * kQ4Rows + 4 * g4);  // rows past the last: dropped
 #pragma unroll
             for (int i = 0; i < 4; i++) acc[i] = __builtin_fmaf(part[i], inv[i], acc[i]);
@@ -295,9 +301,9 @@ __global__ __launch_bounds__(512) void k_linear_q4(Q4Args a, Q4Launch L)
         if (n1 >= a.N) continue;
         const float bias = a.bias ? a.bias[n1] : 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if (4 * g4 + i >= rows) break;
-            const int64_t o = (m0 + 4 * g4 + i) * a.N + n1;
+        for (int i = 0; i < OUT; i++) {
+            if (OUT * g4 + i >= rows) break;
+            const int64_t o = (m0 + OUT * g4 + i) * a.N + n1;
             if (L.splits > 1) {
                 L.ws[(int64_t)split * a.M * a.N + o] = acc[i];
                 continue;
@@ -371,7 +377,7 @@ int launch_linear_q4(const Q4Plan& p, const Q4Args& a, int act, int out, float* 
         const int64_t tpb = p.waves / p.ks, groups = (tiles + tpb - 1) / tpb;
         // Blocks of a group are enough where x costs little to stage; else a block takes several groups with the
         // x it has, while the blocks still fill the device
-        const int64_t fit = std::max<int64_t>(1, std::min(kQ4Lds / lds, 16 / p.waves));
+        const int64_t fit = std::max<int64_t>(1, std::min(kQ4Lds / lds, 32 / p.waves));
         const int64_t worth = (rows * (f32 ? 4 : 2) + tpb - 1) / tpb, full = groups * passes * p.splits / (fit * cus);
         const int64_t turns = std::max<int64_t>(1, std::min(worth, full)), slots = (groups + turns - 1) / turns;
         const dim3 grid((unsigned)((slots + 7) / 8 * 8), (unsigned)passes, (unsigned)p.splits);
@@ -382,13 +388,22 @@ int launch_linear_q4(const Q4Plan& p, const Q4Args& a, int act, int out, float* 
         auto go = [&](auto kern) {
             hipLaunchKernelGGL(kern, grid, dim3((unsigned)(64 * p.waves)), (size_t)lds, st, a, L);
         };
-        auto go_group = [&](auto* t, auto z) {
+        auto go_fold = [&](auto* t, auto z, auto g, auto depth) {
             using AT = std::remove_pointer_t<decltype(t)>;
             constexpr bool ZP = decltype(z)::value;
-            if (one)
-                a.group == 32 ? go(k_linear_q4<AT, 32, ZP, 1>) : a.group == 64 ? go(k_linear_q4<AT, 64, ZP, 1>) : go(k_linear_q4<AT, 128, ZP, 1>);
-            else
-                a.group == 32 ? go(k_linear_q4<AT, 32, ZP, 2>) : a.group == 64 ? go(k_linear_q4<AT, 64, ZP, 2>) : go(k_linear_q4<AT, 128, ZP, 2>);
+            constexpr int G = decltype(g)::value, DEPTH = decltype(depth)::value;
+            if constexpr (sizeof(AT) == 4) {
+                if (rows <= 8) return go(k_linear_q4<AT, G, ZP, DEPTH, true>);
+            }
+            go(k_linear_q4<AT, G, ZP, DEPTH, false>);
+        };
+        auto go_depth = [&](auto* t, auto z, auto g) {
+            one ? go_fold(t, z, g, std::integral_constant<int, 1>{}) : go_fold(t, z, g, std::integral_constant<int, 2>{});
+        };
+        auto go_group = [&](auto* t, auto z) {
+            if (a.group == 32) go_depth(t, z, std::integral_constant<int, 32>{});
+            else if (a.group == 64) go_depth(t, z, std::integral_constant<int, 64>{});
+            else go_depth(t, z, std::integral_constant<int, 128>{});
         };
         auto go_type = [&](auto* t) { a.zeros ? go_group(t, std::true_type{}) : go_group(t, std::false_type{}); };
         f32 ? go_type((float*)nullptr) : go_type((f16*)nullptr);
