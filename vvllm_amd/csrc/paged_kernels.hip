@@ -288,16 +288,17 @@ __device__ __forceinline__ void paged_chunks(const PagedArgs& c, const T* kh, co
     const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<T*>(vh), 0, BIG ? 0 : (int)(uint32_t)((pool - (uint64_t)(vh - (const T*)c.vp)) * sizeof(T)), 0x00020000);
     const uint32_t stride = (uint32_t)kvs * (uint32_t)sizeof(T);
-    // The page of key at + lane and its row there, looked up a chunk ahead and turned into a row of the
-    // pages (-1: no key, or no page) only when it is used, so that nothing waits for it.
+    // The page of key at + lane and its row there, looked up a chunk ahead (the first one without waiting for the
+    // length) and turned into a row of the pages (-1: no key, or no page) only when it is used, so that nothing
+    // waits for it.
+    const uint32_t cap = (uint32_t)c.max_pages * (uint32_t)c.P;
     struct Spot {
         int32_t page, in;
     };
     auto look = [&](int32_t at) {
-        const uint32_t key = (uint32_t)(at + lane < ke ? at + lane : ke - 1), pg = key / (uint32_t)c.P;
+        const uint32_t want = (uint32_t)(at + lane), key = want < cap ? want : cap - 1, pg = key / (uint32_t)c.P;
         return Spot{table[pg], (int32_t)(key - pg * (uint32_t)c.P)};
     };
-    if (c0 >= ke) return;
     Spot spot = look(c0);
     for (; c0 < ke; c0 += cstep) {
         const int32_t row = lane < CH && c0 + lane < ke && spot.page >= 0 && spot.page < c.pages ? spot.page * c.P + spot.in : -1;
