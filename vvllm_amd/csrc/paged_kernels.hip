@@ -525,6 +525,10 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v)
     return v;
 }
 __device__ __forceinline__ uint32_t lane_of(uint32_t v, int l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); }
+__device__ __forceinline__ int64_t lane_of64(uint64_t v, int l)
+{
+    return (int64_t)((uint64_t)lane_of((uint32_t)(v >> 32), l) << 32 | lane_of((uint32_t)v, l));
+}
 
 // a b / c and a / c, in 32 bits where they fit (a 64-bit division is 100 instructions)
 __device__ __forceinline__ uint64_t muldiv(uint64_t a, uint64_t b, uint64_t c)
@@ -533,17 +537,12 @@ __device__ __forceinline__ uint64_t muldiv(uint64_t a, uint64_t b, uint64_t c)
     return (p | c) >> 32 ? p / c : (uint32_t)p / (uint32_t)c;
 }
 
-__device__ __forceinline__ int64_t uniform(uint64_t v)
-{
-    return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 |
-                     (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
-}
-
 // All chunks of all tiles of all sequences in one row (sequence by sequence, tile by
 // tile): wave w of W (all waves, or T) takes units [T w / W, T (w + 1) / W) of its T, so
 // every wave has the same work however ragged the batch.  The part of a tile that a wave has goes
 // straight to out if it is the whole tile, else to the wave's slot 1 (a tile that
-// begins in its range) or 0, a row per head: O, m, l.  k_attention_paged_merge joins them.
+// begins in its range) or 0, a row per head: O, m, l.  Where all four waves of a block are in one tile,
+// their parts are added through LDS and go to the first one's slot.  k_attention_paged_merge joins what there is.
 template <typename T, int D, bool BIG>
 __global__ __launch_bounds__(256, 2) void k_attention_paged_split(PagedArgs c, T* __restrict__ out, const T* __restrict__ q,
                                                                const int32_t* __restrict__ lens, PagedHeads hd, int32_t H,
@@ -551,8 +550,9 @@ __global__ __launch_bounds__(256, 2) void k_attention_paged_split(PagedArgs c, T
                                                                   int32_t VH)
 {
     constexpr int CH = PagedTile<T>::template CH<D>;
-    constexpr int VB = PagedTile<T>::template lds<D>;
-    __shared__ __align__(16) f16 vs[VB ? 4 * VB : 4];
+    constexpr int VB = PagedTile<T>::template lds<D> * 2, OP = D + 4, OB = 16 * OP * 4;  // bytes a wave
+    __shared__ __align__(16) char smem[4 * (VB > OB ? VB : OB)];
+    __shared__ float wm[4][16], wl[4][16];
     const int lane = threadIdx.x & 63, r = lane & 15, gr = lane >> 4;
     const int wb = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t w = (int64_t)blockIdx.x * 4 + wb;
@@ -567,7 +567,10 @@ __global__ __launch_bounds__(256, 2) void k_attention_paged_split(PagedArgs c, T
     total *= VH;
     const int64_t W = total < (int64_t)gridDim.x * 4 ? total : (int64_t)gridDim.x * 4;  // no wave without a unit
     if (w >= W) return;
-    const int64_t u0 = uniform(muldiv(total, w, W)), u1 = uniform(muldiv(total, w + 1, W));
+    // lane l: where wave l of the block begins, and the next block (l = 4)
+    const uint64_t begin = muldiv(total, w - wb + (lane < 4 ? lane : 4), W);
+    auto begin_of = [&](int l) { return lane_of64(begin, l); };
+    const int64_t u0 = begin_of(wb), u1 = begin_of(wb + 1);
     // the window of sequences that holds unit u0
     int32_t s0 = 0, n = paged_window(c, lens, 0, lane, CH);
     int64_t before = 0;
@@ -583,6 +586,9 @@ __global__ __launch_bounds__(256, 2) void k_attention_paged_split(PagedArgs c, T
     const int64_t rest = u0 - (before + lane_of(upto, sl) - ns) * VH;  // units before u0 in the sequence
     int32_t v = __builtin_amdgcn_readfirstlane((int32_t)muldiv(rest, 1, ns));
     int32_t ci = __builtin_amdgcn_readfirstlane((int32_t)(rest - (int64_t)v * ns));
+    // the block's range within this wave's first tile
+    const int64_t b0 = begin_of(0), b1 = begin_of(4);
+    const bool inside = w - wb + 4 <= W && u0 - b0 <= ci && b1 - u0 <= ns - ci;
     for (int64_t u = u0; u < u1;) {
         const int32_t s = s0 + sl, cnt = (int32_t)(ns - ci < u1 - u ? ns - ci : u1 - u);
         int32_t g, h0, nh;
@@ -595,7 +601,39 @@ __global__ __launch_bounds__(256, 2) void k_attention_paged_split(PagedArgs c, T
         const int32_t len = __builtin_amdgcn_readfirstlane(paged_len(c, lens, s));
         const int64_t end = (int64_t)(ci + cnt) * CH;
         paged_chunks<T, D, BIG>(c, (const T*)c.kp + g * D, (const T*)c.vp + g * D, s, x, ci * CH, CH,
-                           end < len ? (int32_t)end : len, scale_log2, vs + wb * VB, lane, acc);
+                           end < len ? (int32_t)end : len, scale_log2, reinterpret_cast<f16*>(smem + wb * VB), lane, acc);
+        if (inside) {
+            __syncthreads();
+            float* os = reinterpret_cast<float*>(smem);
+            if (gr == 0) {
+                wm[wb][r] = acc.m;
+                wl[wb][r] = acc.l;
+            }
+#pragma unroll
+            for (int e = 0; e < D / 16; e++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) os[(wb * 16 + r) * OP + paged_dim<T, D>(e, gr, i)] = acc.o[e][i];
+            __syncthreads();
+            const bool whole = b1 - b0 == ns;
+            float* part = ws + ((w - wb) * 2 + (u0 - b0 == ci)) * hd.GT * (D + 4);
+            for (int idx = threadIdx.x; idx < nh * D; idx += 256) {
+                const int h = idx / D, d = idx - h * D;
+                const float M = fmaxf(fmaxf(wm[0][h], wm[1][h]), fmaxf(wm[2][h], wm[3][h])), Mb = M == -INFINITY ? 0.0f : M;
+                float num = 0.0f, den = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; i++) attn_merge_add(num, den, wm[i][h], Mb, os[(i * 16 + h) * OP + d], wl[i][h]);
+                if (whole) {
+                    out[row0 * D + idx] = (T)(den == 0.0f ? 0.0f : num / den);
+                    continue;
+                }
+                part[h * (D + 4) + d] = num;
+                if (d == 0) {
+                    part[h * (D + 4) + D] = M;
+                    part[h * (D + 4) + D + 1] = den;
+                }
+            }
+            return;
+        }
         if (r < nh) {
             if (cnt == ns) {
                 const float inv = acc.l == 0.0f ? 0.0f : 1.0f / acc.l;
@@ -662,8 +700,16 @@ __global__ __launch_bounds__(1024) void k_attention_paged_merge(int32_t B, T* __
     }
     const int64_t a = first * VH + (g * hd.tiles + t) * ns, b = a + ns - 1;  // first and last unit
     const int64_t W = total < waves ? total : waves;
-    const int64_t w0 = last_wave(a, W, total), w1 = last_wave(b, W, total);
-    if (w0 == w1) return;  // one wave had it all
+    // lanes 0 and 1: the waves of units a and b; then where their blocks and the ones after them begin
+    const int64_t wl2 = last_wave(lane & 1 ? b : a, W, total), w0 = lane_of64(wl2, 0), w1 = lane_of64(wl2, 1), k0 = w0 / 4, k1 = w1 / 4;
+    const uint64_t at = muldiv(total, 4 * ((lane & 1 ? k1 : k0) + (lane >> 1 & 1)), W);
+    // its parts: those of the first block's waves (if it is not all in the tile), of the blocks that are, of the last
+    // one's waves
+    auto inside = [&](int64_t blk, int l) { return 4 * blk + 4 <= W && lane_of64(at, l) >= a && lane_of64(at, l + 2) <= b + 1; };
+    const bool in0 = inside(k0, 0), in1 = inside(k1, 1);
+    const int64_t lead = in0 ? 0 : (w1 < 4 * k0 + 3 ? w1 : 4 * k0 + 3) - w0 + 1, f0 = k0 + !in0;
+    const int64_t full = k1 + in1 > f0 ? k1 + in1 - f0 : 0, parts = lead + full + (k1 == k0 || in1 ? 0 : w1 - 4 * k1 + 1);
+    if (parts == 1) return;  // one wave or block had it all
     float M = -INFINITY, den = 0.0f;
     f4 num = {};
     auto join = [&](float m, float l, f4 o) {
@@ -675,7 +721,8 @@ __global__ __launch_bounds__(1024) void k_attention_paged_merge(int32_t B, T* __
     };
     if (grp < GW) {
 #pragma unroll 4
-        for (int64_t w = w0 + wv * GW + grp; w <= w1; w += NW * GW) {
+        for (int64_t i = wv * GW + grp; i < parts; i += NW * GW) {
+            const int64_t w = i < lead ? w0 + i : i < lead + full ? 4 * (f0 + i - lead) : 4 * k1 + i - lead - full;
             const float* p = ws + ((w * 2 + (w == w0)) * hd.GT + hr) * (D + 4);
             join(p[D], p[D + 1], *reinterpret_cast<const f4*>(p + 4 * d));
         }
@@ -771,10 +818,13 @@ AttnPagedPlan attention_paged_plan(const PagedArgs& c, const void* out, const vo
     const int64_t chunks = (len + 63) / 64;
     p.waves = chunks > 4 ? 8 : 4;
     if (chunks > kPagedOneChunks) {
-        const int64_t units = chunks * c.B * c.KVH * p.tiles;
-        // two blocks a CU; fp16 with few tiles one, whose waves have longer runs and fewer parts (32 contexts of
-        // 4096 keys of 8 heads of 128 107.0 -> 104.8 us; 96 ragged ones 84.5 -> 93; three of fp32 44.0 -> 51.3)
-        p.blocks = std::min<int64_t>((units + 3) / 4, (dtype == VVH_F16 && c.B * c.KVH * p.tiles <= cus ? 1 : 2) * cus);
+        // a chunk a wave at least (one context of 3000 keys, fp32 heads of 128, a wave every 4 chunks 17.9 us, every 2 14.9,
+        // every one 12.4), and two blocks a CU; fp16 of one sequence one, whose waves then have longer runs (30000 keys
+        // 18.9 -> 17.0 us, but 8 ragged contexts of up to 8000 keys 12.4 -> 13.5, 96 84.5 -> 92)
+        const int64_t ch = dtype == VVH_F16 ? (c.D == 64 ? PagedTile<f16>::CH<64> : PagedTile<f16>::CH<128>)
+                                            : (c.D == 128 ? PagedTile<float>::CH<128> : PagedTile<float>::CH<64>);
+        const int64_t units = (len + ch - 1) / ch * c.B * c.KVH * p.tiles;
+        p.blocks = std::min<int64_t>((units + 3) / 4, (dtype == VVH_F16 && c.B == 1 ? 1 : 2) * cus);
     }
     if (p.blocks > 0) p.ws_floats = paged_before_floats(c.B) + p.blocks * 4 * 2 * p.GT * (c.D + 4);
     return p;
@@ -801,7 +851,7 @@ static void paged_go(const AttnPagedPlan& p, const PagedArgs& c, T* out, const T
     // waves of a merge block: about 4 parts a group of lanes if the sequences are alike
     const int64_t W = p.blocks * 4;
     int64_t nw = 1;
-    while (nw < 16 && nw * (256 / D) * 4 < W / ((int64_t)VH * c.B)) nw *= 2;
+    while (nw < 16 && nw * (256 / D) * 4 < p.blocks / ((int64_t)VH * c.B)) nw *= 2;
     hipLaunchKernelGGL((k_attention_paged_merge<T, D>), dim3((unsigned)H, (unsigned)c.B), dim3((unsigned)(64 * nw)), 0, s,
                        (int32_t)c.B, out, hd, (int32_t)H, before, parts, VH, (int32_t)W);
 }
