@@ -791,7 +791,8 @@ int launch_rope_append_paged(const PagedArgs& c, void* q_out, const void* q, con
 }
 
 
-// Chunks of a context from which its tiles are split over waves.
+// A block takes up to two chunks a wave of a context by itself (400 fp16 keys of 128, 8 contexts, 8.9 us, split 11.2), more
+// are split (three a wave: 400 fp32 keys of 128 13.6 -> 11.4; four: 32 contexts of up to 1000 fp16 keys 15.5 -> 11.9).
 constexpr int64_t kPagedOneChunks = 16;
 
 // Floats of the chunk sums ahead of the parts in the workspace.
@@ -815,16 +816,15 @@ AttnPagedPlan attention_paged_plan(const PagedArgs& c, const void* out, const vo
     if (!p.tiled) return p;
     const int64_t cap = (int64_t)c.max_pages * c.P;
     const int64_t len = max_len > 0 && max_len < cap ? max_len : cap;
-    const int64_t chunks = (len + 63) / 64;
+    const int64_t ch = dtype == VVH_F16 ? (c.D == 64 ? PagedTile<f16>::CH<64> : PagedTile<f16>::CH<128>)
+                                        : (c.D == 128 ? PagedTile<float>::CH<128> : PagedTile<float>::CH<64>);
+    const int64_t chunks = (len + ch - 1) / ch;
     p.waves = chunks > 4 ? 8 : 4;
     if (chunks > kPagedOneChunks) {
         // a chunk a wave at least (one context of 3000 keys, fp32 heads of 128, a wave every 4 chunks 17.9 us, every 2 14.9,
         // every one 12.4), and two blocks a CU; fp16 of one sequence one, whose waves then have longer runs (30000 keys
         // 18.9 -> 17.0 us, but 8 ragged contexts of up to 8000 keys 12.4 -> 13.5, 96 84.5 -> 92)
-        const int64_t ch = dtype == VVH_F16 ? (c.D == 64 ? PagedTile<f16>::CH<64> : PagedTile<f16>::CH<128>)
-                                            : (c.D == 128 ? PagedTile<float>::CH<128> : PagedTile<float>::CH<64>);
-        const int64_t units = (len + ch - 1) / ch * c.B * c.KVH * p.tiles;
-        p.blocks = std::min<int64_t>((units + 3) / 4, (dtype == VVH_F16 && c.B == 1 ? 1 : 2) * cus);
+        p.blocks = std::min<int64_t>((chunks * c.B * c.KVH * p.tiles + 3) / 4, (dtype == VVH_F16 && c.B == 1 ? 1 : 2) * cus);
     }
     if (p.blocks > 0) p.ws_floats = paged_before_floats(c.B) + p.blocks * 4 * 2 * p.GT * (c.D + 4);
     return p;
