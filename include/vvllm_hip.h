@@ -606,10 +606,11 @@ VVH_API int vvh_attention_paged(const vvh_paged_cache* cache, void* out, const v
  * are exact; fp16 activations are used as given, fp32 ones to 22 bits of the
  * largest of 256 neighbours in their row; products are summed in fp32 and the
  * epilogue rounds once (as vvh_linear_q8).  Made for the few rows of a decode step:
- * rows are taken 16 at a time, each 16 reading the weights again.  Rows of inp too
- * long for a block's shared memory (at 16 rows past 4096 fp16 or 1024 fp32
- * activations) share out k, whose sums use the stream's workspace (splits * M * N
- * floats): make one such call before capturing on the stream. */
+ * rows are taken 16 or 32 at a time, each time reading the weights again.  Rows of
+ * inp too long for a block's shared memory (16 rows over few channels: past 4096
+ * fp16 or 1024 fp32 activations) share out k, whose sums use the stream's
+ * workspace (splits * M * N floats): make one such call before capturing on the
+ * stream. */
 VVH_API int vvh_linear_q4(void* out, const void* inp, const uint8_t* dev_weight, const uint16_t* dev_scales,
                           const uint8_t* dev_zeros, const float* dev_bias, const void* residual, size_t M, size_t N,
                           size_t K, size_t group, int act_dtype, int out_dtype, void* stream);

@@ -99,6 +99,34 @@ def test_many_channels(gpu, act, M, N):
     Case(M, N, 96, 32, act, act, bias=True).check()
 
 
+@pytest.mark.parametrize("act", [F16, F32])
+@pytest.mark.parametrize("group,K", [(32, 32), (32, 224), (64, 256), (64, 448), (32, 512), (128, 640), (64, 960), (128, 1024)])
+@pytest.mark.parametrize("M,N", [(5, 16390), (9, 16390), (16, 16300), (17, 8200), (23, 8200), (40, 16500), (65, 4100), (130, 2000)])
+def test_many_rows_and_channels(gpu, act, group, K, M, N):
+    """Steps of x in turn: one, even and odd numbers of them, rows that end inside one; passes of up to 16 and 32 rows."""
+    Case(M, N, K, group, act, act, zeros=K % 3 == 1, bias=M % 2 == 1, residual=M % 3 == 1).check()
+
+
+@pytest.mark.parametrize("act,outd", [(F16, F32), (F32, F16)])
+def test_many_rows_and_channels_of_mixed_types(gpu, act, outd):
+    Case(20, 8200, 512, 64, act, outd, zeros=True, bias=True, residual=True).check()
+
+
+@pytest.mark.parametrize("act", [F16, F32])
+def test_many_rows_in_place(gpu, act):
+    """The residual's place for the output, row by row; rows with infinities and NaN leave the others alone."""
+    c = Case(37, 8200, 320, 64, act, act, residual=True)
+    c.x[3, 7], c.x[20, 300], c.x[36, 0] = np.inf, np.nan, -np.inf
+    c.d["x"] = capi.DevBuf.from_array(c.x)
+    with np.errstate(invalid="ignore", over="ignore"):
+        y, tol = c.want()
+    c.run(out=c.d["res"])
+    got = c.got(c.d["res"]).astype(np.float64)
+    rows = [m for m in range(37) if m not in (3, 20, 36)]
+    assert (np.abs(got - y)[rows] <= tol[rows]).all()
+    assert np.isnan(got[20]).all() and not np.isfinite(got[[3, 36]]).any()
+
+
 @pytest.mark.parametrize("act,outd", [(F16, F32), (F32, F16)])
 @pytest.mark.parametrize("M", [1, 4, 16, 40])
 def test_mixed_types(gpu, act, outd, M):
@@ -182,7 +210,7 @@ def test_rows_of_a_large_call_are_the_small_calls(gpu, act):
 def test_captured(gpu):
     st = Stream()
     cs = [Case(1, 896, 896, 64, F16, F16), Case(8, 500, 4864, 128, F16, F16, zeros=True), Case(3, 300, 640, 32, F32, F32),
-          Case(40, 300, 640, 32, F32, F32), Case(40, 200, 4864, 64, F16, F16)]
+          Case(40, 300, 640, 32, F32, F32), Case(40, 200, 4864, 64, F16, F16), Case(20, 8200, 320, 64, F16, F16)]
     for c in cs:
         c.run()
     eager = [c.got() for c in cs]

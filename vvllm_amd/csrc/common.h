@@ -447,6 +447,7 @@ struct Q4Args {
 // LDS; splits > 1 blocks share a tile's k (ws_floats floats of workspace and a
 // second launch), 0: no k.
 struct Q4Plan {
+    int64_t rows;  // > 0: k_linear_q4_rows, of that many a pass; else
     int64_t waves, ks, seg, splits, ws_floats;
 };
 Q4Plan linear_q4_plan(const Q4Args& a, int act, int64_t cus);

@@ -77,14 +77,155 @@ __device__ __forceinline__ h8 q4_codes(uint32_t w, h2 zl, h2 zh, const Q4Masks& 
     return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+// A wave's stream of a tile's weights: 16 channels from n0 on, a step at a time from memory to registers (issue),
+// to its LDS tile (put) and through the matrix instruction (step).
+template <int G, bool ZP>
+struct Q4Stream {
+    static constexpr int PG = kQ4Step / G;          // groups a step
+    static constexpr int NS = PG > 4 ? 2 : 1;       // scales a lane loads a step
+    static constexpr int DW = G / 32;               // dwords of codes a lane reads a group
+    struct Slot {
+        u4 a, b;
+        uint16_t s[NS];
+        uint8_t z[NS];
+    };
+    const uint8_t *wa, *wb, *zp;
+    const uint16_t* sc;
+    int32_t K, steps, groups;
+    int lane, n, g4;
+    char* tile;
+    uint32_t* stile;
+    Q4Masks masks;
+
+    __device__ __forceinline__ Q4Stream(const Q4Args& a, char* lds, int l)
+        : zp(nullptr), K((int32_t)a.K), steps((K + kQ4Step - 1) / kQ4Step), groups(K / G), lane(l), n(l & 15), g4(l >> 4),
+          tile(lds), stile(reinterpret_cast<uint32_t*>(lds + 16 * kQ4WPitch)), masks(q4_masks())
+    {
+    }
+    // rows past N are row N - 1, pieces past K the last one (met by zeros in x)
+    __device__ __forceinline__ void point(const Q4Args& a, int64_t n0)
+    {
+        const int64_t last = a.N - 1, ra = n0 + (lane >> 3), rb = ra + 8, rn = n0 + n;
+        wa = a.w + (ra < last ? ra : last) * (K / 2);
+        wb = a.w + (rb < last ? rb : last) * (K / 2);
+        sc = a.scales + (rn < last ? rn : last) * groups;
+        if (ZP) zp = a.zeros + (rn < last ? rn : last) * groups;
+    }
+    __device__ __forceinline__ void issue(Slot& r, int32_t want) const
+    {
+        const int32_t st = want < steps ? want : steps - 1;  // past the end: never used
+        const int32_t at = st * (kQ4Step / 2) + (lane & 7) * 16, last = K / 2 - 16;
+        r.a = *reinterpret_cast<const u4*>(wa + (at < last ? at : last));
+        r.b = *reinterpret_cast<const u4*>(wb + (at < last ? at : last));
+#pragma unroll
+        for (int i = 0; i < NS; i++) {
+            const int32_t h = st * PG + (g4 * NS + i) % PG, g = h < groups ? h : groups - 1;
+            r.s[i] = sc[g];
+            if (ZP) r.z[i] = zp[g];
+        }
+    }
+    __device__ __forceinline__ void put(const Slot& r) const
+    {
+        *reinterpret_cast<u4*>(tile + (lane >> 3) * kQ4WPitch + (lane & 7) * 16) = r.a;
+        *reinterpret_cast<u4*>(tile + (8 + (lane >> 3)) * kQ4WPitch + (lane & 7) * 16) = r.b;
+#pragma unroll
+        for (int i = 0; i < NS; i++) {
+            uint32_t v = r.s[i];
+            if (ZP) v |= (uint32_t)__builtin_bit_cast(uint16_t, (f16)(float)r.z[i]) << 16;
+            if (g4 * NS + i < PG) stile[n * kQ4SPitch + g4 * NS + i] = v;
+        }
+        // one wave's LDS accesses complete in order
+    }
+    // part[r] += the step's sums; xk: the step's x, whose operand rows are at row[r], TWO: and row[r] + plane
+    template <int RT, bool TWO>
+    __device__ __forceinline__ void step(f4 (&part)[RT], const f16* xk, const int32_t (&row)[RT], int32_t plane) const
+    {
+        uint32_t sv[PG];
+#pragma unroll
+        for (int g = 0; g < PG; g++) sv[g] = stile[n * kQ4SPitch + g];
+#pragma unroll
+        for (int g = 0; g < PG; g++) {
+            uint32_t w[DW];
+            const uint32_t* wr = reinterpret_cast<const uint32_t*>(tile + n * kQ4WPitch) + g * (G / 8) + g4 * DW;
+#pragma unroll
+            for (int j = 0; j < DW; j++) w[j] = wr[j];
+            h2 zl = {(f16)1032.0f, (f16)1032.0f}, zh = {(f16)72.0f, (f16)72.0f};
+            if (ZP) {
+                const f16 z = q4_h2(sv[g])[1];
+                zl = h2{z, z} + h2{(f16)1024.0f, (f16)1024.0f};
+                zh = h2{z, z} + h2{(f16)64.0f, (f16)64.0f};
+            }
+            f4 d[RT] = {};
+#pragma unroll
+            for (int j = 0; j < DW; j++) {
+                const h8 b = q4_codes(w[j], zl, zh, masks);
+#pragma unroll
+                for (int r = 0; r < RT; r++) {
+                    const f16* xp = xk + row[r] + g * G + (g4 * DW + j) * 8;
+                    if (TWO) d[r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(*reinterpret_cast<const h8*>(xp + plane), b, d[r], 0, 0, 0);
+                    d[r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(*reinterpret_cast<const h8*>(xp), b, d[r], 0, 0, 0);
+                }
+            }
+            const float s = (float)q4_h2(sv[g])[0];
+#pragma unroll
+            for (int r = 0; r < RT; r++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) part[r][i] = __builtin_fmaf(s, d[r][i], part[r][i]);
+        }
+    }
+};
+
+// bias, residual and rounding of one output
+__device__ __forceinline__ void q4_store(const Q4Args& a, bool out_f16, int64_t o, float y)
+{
+    if (out_f16) {
+        if (a.res) y += (float)((const f16*)a.res)[o];
+        ((f16*)a.out)[o] = (f16)y;
+    } else {
+        if (a.res) y += ((const float*)a.res)[o];
+        ((float*)a.out)[o] = y;
+    }
+}
+
+// 8 values in the order of the codes: 0 1 2 3 4 5 6 7 -> 0 4 1 5 2 6 3 7
+__device__ __forceinline__ u4 q4_order(u4 v)
+{
+    return u4{__builtin_amdgcn_perm(v[2], v[0], 0x05040100u), __builtin_amdgcn_perm(v[2], v[0], 0x07060302u),
+              __builtin_amdgcn_perm(v[3], v[1], 0x05040100u), __builtin_amdgcn_perm(v[3], v[1], 0x07060302u)};
+}
+
+// A wave's 256 values of a row, 4 a lane, as their fp16 parts, in the order of the codes, and their inverse scale.
+__device__ __forceinline__ void q4_split(f4 v, int lane, f16* hi_row, f16* lo_row, float* inv)
+{
+    const float most = group_max(fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))), 64);
+    // 2^(14 - x) for most in [2^x, 2^(x + 1)), at most 2^126; with an infinity that of the largest finite ones
+    const int b = (int)(__builtin_bit_cast(uint32_t, most) >> 23), e = b < 15 ? 15 : b > 254 ? 254 : b;
+    const float up = __builtin_bit_cast(float, (uint32_t)(268 - e) << 23);
+    uint32_t hi[2], lo[2];
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+        const float p = v[2 * c] * up, q = v[2 * c + 1] * up;
+        const h2 h = {(f16)p, (f16)q};
+        h2 l = {(f16)(p - (float)h[0]), (f16)(q - (float)h[1])};
+        if (b == 255) l = h2{};  // an infinity is all in its high part
+        hi[c] = __builtin_bit_cast(uint32_t, h);
+        lo[c] = __builtin_bit_cast(uint32_t, l);
+    }
+    // lanes of a pair hold values 0-3 and 4-7: the even one stores the high parts, the odd one the low
+    const bool odd = lane & 1;
+    const uint32_t s0 = odd ? hi[0] : lo[0], s1 = odd ? hi[1] : lo[1];
+    const uint32_t r0 = __builtin_amdgcn_mov_dpp((int)s0, 0xB1, 0xF, 0xF, false);
+    const uint32_t r1 = __builtin_amdgcn_mov_dpp((int)s1, 0xB1, 0xF, 0xF, false);
+    const u4 o = q4_order(odd ? u4{r0, r1, lo[0], lo[1]} : u4{hi[0], hi[1], r0, r1});
+    *reinterpret_cast<u4*>((odd ? lo_row : hi_row) + (lane >> 1) * 8) = o;
+    if (lane == 0) *inv = __builtin_bit_cast(float, (uint32_t)(e - 14) << 23);
+}
+
 template <typename AT, int G, bool ZP, int DEPTH, bool FOLD>
 __global__ __launch_bounds__(512) void k_linear_q4(Q4Args a, Q4Launch L)
 {
     constexpr bool F32 = sizeof(AT) == 4;
-    constexpr int PG = kQ4Step / G;                 // groups a step
-    constexpr int NS = PG > 4 ? 2 : 1;              // scales a lane loads a step
     constexpr int OUT = FOLD ? 2 : 4;               // rows of a lane's sums
-    constexpr int DW = G / 32;                      // dwords of codes a lane reads a group
     extern __shared__ __align__(16) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g4 = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), threads = L.waves * 64;
@@ -93,7 +234,7 @@ __global__ __launch_bounds__(512) void k_linear_q4(Q4Args a, Q4Launch L)
     const int32_t KS = 1 << L.log_ks, ks = wave & (KS - 1), mytile = wave >> L.log_ks;
     const int64_t m0 = (int64_t)pass * kQ4Rows;
     const int32_t rows = (int32_t)(a.M - m0 < kQ4Rows ? a.M - m0 : kQ4Rows);
-    const int32_t K = (int32_t)a.K, steps = (K + kQ4Step - 1) / kQ4Step, groups = K / G;
+    const int32_t K = (int32_t)a.K, steps = (K + kQ4Step - 1) / kQ4Step;
     const int32_t s0 = split * L.seg, s1 = s0 + L.seg < steps ? s0 + L.seg : steps;
     const int32_t mine = (s1 - s0 - ks + KS - 1) >> L.log_ks;   // steps s0 + ks + KS i of every tile are the wave's
     const int32_t turns = (mine + DEPTH - 1) / DEPTH * DEPTH;   // whole rings
@@ -102,45 +243,15 @@ __global__ __launch_bounds__(512) void k_linear_q4(Q4Args a, Q4Launch L)
     const int32_t plane = L.rows * pitch;           // F32: the low parts' plane is at +plane
     float* xinv = reinterpret_cast<float*>(xs + (F32 ? 2 : 1) * plane);  // F32: [seg][16] inverse scales
     char* tile = reinterpret_cast<char*>(xinv + (F32 ? L.seg * kQ4Rows : 0)) + wave * kQ4Tile;
-    uint32_t* stile = reinterpret_cast<uint32_t*>(tile + 16 * kQ4WPitch);
     const AT* x = (const AT*)a.inp + m0 * a.K;
 
-    // the weights of a group's tile: rows past N are row N - 1, pieces past K the last one (met by zeros in x)
-    const uint8_t *wa, *wb, *zp = nullptr;
-    const uint16_t* sc;
+    Q4Stream<G, ZP> ws(a, tile, lane);
+    typename Q4Stream<G, ZP>::Slot ring[DEPTH];
     auto first_channel = [&](int32_t grp) { return ((int64_t)grp * L.tiles + mytile) * 16; };
-    auto point = [&](int32_t grp) {
-        const int64_t n0 = first_channel(grp), last = a.N - 1;
-        const int64_t ra = n0 + (lane >> 3), rb = ra + 8, rn = n0 + n;
-        wa = a.w + (ra < last ? ra : last) * (K / 2);
-        wb = a.w + (rb < last ? rb : last) * (K / 2);
-        sc = a.scales + (rn < last ? rn : last) * groups;
-        if (ZP) zp = a.zeros + (rn < last ? rn : last) * groups;
-    };
-    struct Slot {
-        u4 a, b;
-        uint16_t s[NS];
-        uint8_t z[NS];
-    } ring[DEPTH];
-    auto issue = [&](int u, int32_t i) {
-        const int32_t at_step = s0 + ks + (i << L.log_ks), st = at_step < steps ? at_step : steps - 1;  // past the end: never used
-        const int32_t at = st * (kQ4Step / 2) + (lane & 7) * 16, last = K / 2 - 16;
-        ring[u].a = *reinterpret_cast<const u4*>(wa + (at < last ? at : last));
-        ring[u].b = *reinterpret_cast<const u4*>(wb + (at < last ? at : last));
-#pragma unroll
-        for (int i = 0; i < NS; i++) {
-            const int32_t h = st * PG + (g4 * NS + i) % PG, g = h < groups ? h : groups - 1;
-            ring[u].s[i] = sc[g];
-            if (ZP) ring[u].z[i] = zp[g];
-        }
-    };
+    auto issue = [&](int u, int32_t i) { ws.issue(ring[u], s0 + ks + (i << L.log_ks)); };
 
     // ---- x ----
     const int32_t arow = FOLD ? n >> 1 : n, row = arow < rows ? arow : rows - 1;  // past the last: computed and dropped
-    auto order = [](u4 v) {                         // 0 1 2 3 4 5 6 7 -> 0 4 1 5 2 6 3 7
-        return u4{__builtin_amdgcn_perm(v[2], v[0], 0x05040100u), __builtin_amdgcn_perm(v[2], v[0], 0x07060302u),
-                  __builtin_amdgcn_perm(v[3], v[1], 0x05040100u), __builtin_amdgcn_perm(v[3], v[1], 0x07060302u)};
-    };
     // x to LDS.  A unit is 16 bytes of a row: unit i is piece i % per of row i / per (fp32: a wave's unit, 256
     // values of a row, 4 a lane, whose largest the lanes share).  kQ4Batch of them are loaded together; the
     // first batch ahead of the weight ring, whose loads it then does not wait for.
@@ -165,77 +276,21 @@ __global__ __launch_bounds__(512) void k_linear_q4(Q4Args a, Q4Launch L)
             if ((F32 ? i : i - first) >= rows * per) break;
             const int32_t m = (int32_t)__umulhi((uint32_t)i, L.inv_per), k = (i - m * per) * PIECE;
             if constexpr (!F32) {
-                if (m < rows) *reinterpret_cast<u4*>(xs + m * pitch + k) = order(xr[j]);
+                if (m < rows) *reinterpret_cast<u4*>(xs + m * pitch + k) = q4_order(xr[j]);
             } else {
-                const f4 v = __builtin_bit_cast(f4, xr[j]);
-                const float most = group_max(fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))), 64);
-                // 2^(14 - x) for most in [2^x, 2^(x + 1)), at most 2^126; with an infinity that of the largest finite ones
-                const int b = (int)(__builtin_bit_cast(uint32_t, most) >> 23), e = b < 15 ? 15 : b > 254 ? 254 : b;
-                const float up = __builtin_bit_cast(float, (uint32_t)(268 - e) << 23);
-                uint32_t hi[2], lo[2];
-#pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    const float p = v[2 * c] * up, q = v[2 * c + 1] * up;
-                    const h2 h = {(f16)p, (f16)q};
-                    h2 l = {(f16)(p - (float)h[0]), (f16)(q - (float)h[1])};
-                    if (b == 255) l = h2{};  // an infinity is all in its high part
-                    hi[c] = __builtin_bit_cast(uint32_t, h);
-                    lo[c] = __builtin_bit_cast(uint32_t, l);
-                }
-                // lanes of a pair hold values 0-3 and 4-7: the even one stores the high parts, the odd one the low
-                const bool odd = lane & 1;
-                const uint32_t s0 = odd ? hi[0] : lo[0], s1 = odd ? hi[1] : lo[1];
-                const uint32_t r0 = __builtin_amdgcn_mov_dpp((int)s0, 0xB1, 0xF, 0xF, false);
-                const uint32_t r1 = __builtin_amdgcn_mov_dpp((int)s1, 0xB1, 0xF, 0xF, false);
-                const u4 o = order(odd ? u4{r0, r1, lo[0], lo[1]} : u4{hi[0], hi[1], r0, r1});
-                *reinterpret_cast<u4*>(xs + (odd ? plane : 0) + m * pitch + k + (lane >> 1) * 8) = o;
-                if (lane == 0)
-                    xinv[k / kQ4Step * kQ4Rows + m] = __builtin_bit_cast(float, (uint32_t)(e - 14) << 23);
+                f16* to = xs + m * pitch + k;
+                q4_split(__builtin_bit_cast(f4, xr[j]), lane, to, to + plane, xinv + k / kQ4Step * kQ4Rows + m);
             }
         }
     };
-    const Q4Masks masks = q4_masks();
     f4 acc;
     auto consume = [&](int u, int32_t i) {
         const int32_t st = ks + (i << L.log_ks);           // within x in LDS
-        *reinterpret_cast<u4*>(tile + (lane >> 3) * kQ4WPitch + (lane & 7) * 16) = ring[u].a;
-        *reinterpret_cast<u4*>(tile + (8 + (lane >> 3)) * kQ4WPitch + (lane & 7) * 16) = ring[u].b;
-#pragma unroll
-        for (int i = 0; i < NS; i++) {
-            uint32_t v = ring[u].s[i];
-            if (ZP) v |= (uint32_t)__builtin_bit_cast(uint16_t, (f16)(float)ring[u].z[i]) << 16;
-            if (g4 * NS + i < PG) stile[n * kQ4SPitch + g4 * NS + i] = v;
-        }
-        // one wave's LDS accesses complete in order
-        uint32_t sv[PG];
-#pragma unroll
-        for (int g = 0; g < PG; g++) sv[g] = stile[n * kQ4SPitch + g];
-        const f16* xk = xs + (FOLD && n & 1 ? plane : 0) + row * pitch + st * kQ4Step;
-        f4 part = {};
-#pragma unroll
-        for (int g = 0; g < PG; g++) {
-            uint32_t w[DW];
-            const uint32_t* wr = reinterpret_cast<const uint32_t*>(tile + n * kQ4WPitch) + g * (G / 8) + g4 * DW;
-#pragma unroll
-            for (int j = 0; j < DW; j++) w[j] = wr[j];
-            h2 zl = {(f16)1032.0f, (f16)1032.0f}, zh = {(f16)72.0f, (f16)72.0f};
-            if (ZP) {
-                const f16 z = q4_h2(sv[g])[1];
-                zl = h2{z, z} + h2{(f16)1024.0f, (f16)1024.0f};
-                zh = h2{z, z} + h2{(f16)64.0f, (f16)64.0f};
-            }
-            f4 d = {};
-#pragma unroll
-            for (int j = 0; j < DW; j++) {
-                const h8 b = q4_codes(w[j], zl, zh, masks);
-                const f16* xp = xk + g * G + (g4 * DW + j) * 8;
-                if (F32 && !FOLD) d = __builtin_amdgcn_mfma_f32_16x16x32_f16(*reinterpret_cast<const h8*>(xp + plane), b, d, 0, 0, 0);
-                d = __builtin_amdgcn_mfma_f32_16x16x32_f16(*reinterpret_cast<const h8*>(xp), b, d, 0, 0, 0);
-            }
-            const float s = (float)q4_h2(sv[g])[0];
-#pragma unroll
-            for (int i = 0; i < 4; i++) part[i] = __builtin_fmaf(s, d[i], part[i]);
-        }
+        ws.put(ring[u]);
+        f4 parts[1] = {};
+        const int32_t at[1] = {(FOLD && n & 1 ? plane : 0) + row * pitch};
+        ws.template step<1, F32 && !FOLD>(parts, xs + st * kQ4Step, at, plane);
+        const f4 part = parts[0];
         if constexpr (FOLD) {
             const float* inv = xinv + st * kQ4Rows + 2 * g4;
 #pragma unroll
@@ -250,7 +305,7 @@ __global__ __launch_bounds__(512) void k_linear_q4(Q4Args a, Q4Launch L)
     };
 
     load_x(first);
-    point(slot);
+    ws.point(a, first_channel(slot));
 #pragma unroll
     for (int u = 0; u < DEPTH; u++) issue(u, u);
     store_x(first);
@@ -273,7 +328,7 @@ __global__ __launch_bounds__(512) void k_linear_q4(Q4Args a, Q4Launch L)
                     issue(u, i + u + DEPTH);
                 }
             } else if (next) {
-                point(grp + L.slots);
+                ws.point(a, first_channel(grp + L.slots));
 #pragma unroll
                 for (int u = 0; u < DEPTH; u++) {
                     if (i + u < mine) consume(u, i + u);
@@ -308,15 +363,99 @@ __global__ __launch_bounds__(512) void k_linear_q4(Q4Args a, Q4Launch L)
                 L.ws[(int64_t)split * a.M * a.N + o] = acc[i];
                 continue;
             }
-            float y = acc[i] + bias;
-            if (L.out_f16) {
-                if (a.res) y += (float)((const f16*)a.res)[o];
-                ((f16*)a.out)[o] = (f16)y;
+            q4_store(a, L.out_f16, o, acc[i] + bias);
+        }
+    }
+}
+
+// Many rows over many channels: a block takes 8 tiles, a wave each, and up to 16 RT rows, and x goes through LDS a step
+// at a time: two buffers, the next step's x on its way from memory while the waves work on this one, a barrier a step.
+// A wave's codes meet RT operands of x.  Against the kernel above, which needs all of x before it begins: 13 rows of 17920 x
+// 1536 9.0 -> 8.1 us, 32 13.2 -> 10.0, 64 18.2 -> 14.6 (fp32 32.7 -> 25.9), 64 rows of 151936 x 896 69.9 -> 53.9; up to 4 rows
+// it is slower (1 of 28672 x 8192 31.1 -> 38.5), and with few blocks (76: 8 rows of 9728 x 896 5.0 -> 5.6).
+template <typename AT, int G, bool ZP, int RT>
+__global__ __launch_bounds__(512) void k_linear_q4_rows(Q4Args a, int32_t pass_rows, int32_t groups_n, int32_t out_f16)
+{
+    constexpr bool F32 = sizeof(AT) == 4;
+    constexpr int R = 16 * RT, PITCH = kQ4Step + 8, NX = F32 ? 2 * RT : RT, PLANE = R * PITCH, BUF = (F32 ? 2 : 1) * PLANE;
+    extern __shared__ __align__(16) char smem[];
+    const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g4 = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int32_t grp = blockIdx.x;
+    if (grp >= groups_n) return;
+    const int64_t m0 = (int64_t)blockIdx.y * pass_rows, n0 = ((int64_t)grp * 8 + wave) * 16;
+    const int32_t rows = (int32_t)(a.M - m0 < pass_rows ? a.M - m0 : pass_rows), K = (int32_t)a.K;
+    f16* xs = reinterpret_cast<f16*>(smem);                        // [2][planes][R][PITCH]
+    float* xinv = reinterpret_cast<float*>(xs + 2 * BUF);          // F32: [2][R]
+    Q4Stream<G, ZP> ws(a, reinterpret_cast<char*>(xinv + (F32 ? 2 * R : 0)) + wave * kQ4Tile, lane);
+    typename Q4Stream<G, ZP>::Slot ring[2];
+    const AT* x = (const AT*)a.inp + m0 * a.K;
+    const int32_t xrow = F32 ? wave : tid >> 5, xat = F32 ? lane * 4 : (tid & 31) * 8;
+    constexpr int XROWS = F32 ? 8 : 16;  // rows the block loads at a time
+    u4 xr[NX];
+    auto load_x = [&](int32_t st) {
+#pragma unroll
+        for (int j = 0; j < NX; j++) {
+            const int32_t m = xrow + XROWS * j, at = st * kQ4Step + xat;
+            xr[j] = u4{};
+            if (m < rows && at < K) xr[j] = *reinterpret_cast<const u4*>(x + (int64_t)m * K + at);
+        }
+    };
+    auto store_x = [&](int buf) {
+#pragma unroll
+        for (int j = 0; j < NX; j++) {
+            const int32_t m = xrow + XROWS * j;
+            if (m >= rows) break;
+            f16* to = xs + buf * BUF + m * PITCH;
+            if constexpr (F32) q4_split(__builtin_bit_cast(f4, xr[j]), lane, to, to + PLANE, xinv + buf * R + m);
+            else *reinterpret_cast<u4*>(to + xat) = q4_order(xr[j]);
+        }
+    };
+    int32_t row[RT];                                // rows of the operand past the last are computed and dropped
+#pragma unroll
+    for (int r = 0; r < RT; r++) row[r] = (r * 16 + n < rows ? r * 16 + n : rows - 1) * PITCH;
+
+    load_x(0);
+    ws.point(a, n0);
+    ws.issue(ring[0], 0);
+    ws.issue(ring[1], 1);
+    store_x(0);
+    load_x(1);
+    lds_barrier();
+    f4 acc[RT] = {};
+    for (int32_t st = 0; st < ws.steps; st += 2) {
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            if (u == 1 && st + 1 >= ws.steps) break;
+            ws.put(ring[u]);
+            if constexpr (F32) {
+                f4 part[RT] = {};
+                ws.template step<RT, true>(part, xs + u * BUF, row, PLANE);
+#pragma unroll
+                for (int r = 0; r < RT; r++) {
+                    const f4 inv = *reinterpret_cast<const f4*>(xinv + u * R + r * 16 + 4 * g4);  // rows past the last: dropped
+#pragma unroll
+                    for (int i = 0; i < 4; i++) acc[r][i] = __builtin_fmaf(part[r][i], inv[i], acc[r][i]);
+                }
             } else {
-                if (a.res) y += ((const float*)a.res)[o];
-                ((float*)a.out)[o] = y;
+                ws.template step<RT, false>(acc, xs + u * BUF, row, PLANE);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (st + u + 1 < ws.steps) {
+                ws.issue(ring[u], st + u + 2);
+                store_x(u ^ 1);
+                load_x(st + u + 2);
+                lds_barrier();
             }
         }
+    }
+    if (n0 + n >= a.N) return;
+    const float bias = a.bias ? a.bias[n0 + n] : 0.0f;
+#pragma unroll
+    for (int e = 0; e < 4 * RT; e++) {
+        const int m = e / 4 * 16 + 4 * g4 + e % 4;
+        if (m >= rows) break;
+        q4_store(a, out_f16, (m0 + m) * a.N + n0 + n, acc[e / 4][e % 4] + bias);
     }
 }
 
@@ -351,6 +490,16 @@ Q4Plan linear_q4_plan(const Q4Args& a, int act, int64_t cus)
                   rows = std::min<int64_t>(a.M, kQ4Rows);
     Q4Plan p{};
     if (steps == 0) return p;
+    // x a step at a time, where the blocks of 8 tiles fill half the device and there are rows to share the codes
+    const int64_t groups = (a.N + 127) / 128;
+    if (a.M > (f32 ? 8 : 4) && groups * ((a.M + 15) / 16) >= cus / 2) {
+        // passes of 16 or 32 rows, by the blocks a CU takes and what these cost (17920 x 1536: 1, 2, 3 of 16 rows 8.0, 11.7,
+        // 15.5 us; 1, 2 of 32 rows 9.3, 14.7); fp32 x of 32 rows leaves a CU one block (19.6 us, of 16 18.6)
+        const int64_t c16 = (groups * ((a.M + 15) / 16) + cus - 1) / cus, c32 = (groups * ((a.M + 31) / 32) + cus - 1) / cus;
+        const int64_t most = !f32 && 7 * c32 < 5 * c16 ? 32 : 16, n = (a.M + most - 1) / most;
+        p.rows = (a.M + n - 1) / n;
+        return p;
+    }
     p.splits = 1;
     p.ks = 1;
     p.waves = 8;
@@ -371,6 +520,31 @@ int launch_linear_q4(const Q4Plan& p, const Q4Args& a, int act, int out, float* 
 {
     hipStream_t st = static_cast<hipStream_t>(stream);
     const bool f32 = act == VVH_F32;
+    if (p.rows > 0) {
+        const int64_t groups = (a.N + 127) / 128, rt = (p.rows + 15) / 16, planes = f32 ? 2 : 1;
+        const int64_t lds = 2 * planes * rt * 16 * (kQ4Step + 8) * 2 + (f32 ? 2 * rt * 16 * 4 : 0) + 8 * kQ4Tile;
+        const dim3 grid((unsigned)((groups + 7) / 8 * 8), (unsigned)((a.M + p.rows - 1) / p.rows));
+        auto go = [&](auto kern) {
+            hipLaunchKernelGGL(kern, grid, dim3(512), (size_t)lds, st, a, (int32_t)p.rows, (int32_t)groups, (int32_t)(out == VVH_F16));
+        };
+        auto go_rt = [&](auto* t, auto z, auto g) {
+            using AT = std::remove_pointer_t<decltype(t)>;
+            constexpr bool ZP = decltype(z)::value;
+            constexpr int G = decltype(g)::value;
+            if constexpr (sizeof(AT) == 2) {
+                if (rt == 2) return go(k_linear_q4_rows<AT, G, ZP, 2>);
+            }
+            go(k_linear_q4_rows<AT, G, ZP, 1>);
+        };
+        auto go_group = [&](auto* t, auto z) {
+            if (a.group == 32) go_rt(t, z, std::integral_constant<int, 32>{});
+            else if (a.group == 64) go_rt(t, z, std::integral_constant<int, 64>{});
+            else go_rt(t, z, std::integral_constant<int, 128>{});
+        };
+        auto go_type = [&](auto* t) { a.zeros ? go_group(t, std::true_type{}) : go_group(t, std::false_type{}); };
+        f32 ? go_type((float*)nullptr) : go_type((f16*)nullptr);
+        return (int)hipGetLastError();
+    }
     if (p.splits > 0) {
         const int64_t tiles = (a.N + 15) / 16, passes = (a.M + kQ4Rows - 1) / kQ4Rows, rows = std::min<int64_t>(a.M, kQ4Rows);
         const int64_t per = p.seg * (f32 ? 1 : kQ4Step / 8), lds = q4_lds(p, rows, f32);
