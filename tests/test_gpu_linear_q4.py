@@ -86,7 +86,8 @@ def test_short_and_odd_rows(gpu, act, K, group, M):
 
 
 @pytest.mark.parametrize("act", [F16, F32])
-@pytest.mark.parametrize("M,N,K", [(1, 40, 90112), (2, 33, 45056), (16, 130, 8960), (40, 100, 8960), (9, 1, 20480)])
+@pytest.mark.parametrize("M,N,K", [(1, 40, 90112), (2, 33, 45056), (16, 130, 8960), (40, 100, 8960), (9, 1, 20480),
+                                   (5, 200, 33280), (6, 17, 99968), (17, 130, 2176), (33, 260, 5120), (64, 40, 16640), (64, 4000, 3200)])
 def test_rows_of_x_past_the_lds(gpu, act, M, N, K):
     """k shared by several blocks, whose sums a second launch adds."""
     Case(M, N, K, 128, act, act, zeros=True, bias=True, residual=True).check()

@@ -374,7 +374,8 @@ __global__ __launch_bounds__(512) void k_linear_q4(Q4Args a, Q4Launch L)
 // 1536 9.0 -> 8.1 us, 32 13.2 -> 10.0, 64 18.2 -> 14.6 (fp32 32.7 -> 25.9), 64 rows of 151936 x 896 69.9 -> 53.9; up to 4 rows
 // it is slower (1 of 28672 x 8192 31.1 -> 38.5), and with few blocks (76: 8 rows of 9728 x 896 5.0 -> 5.6).
 template <typename AT, int G, bool ZP, int RT>
-__global__ __launch_bounds__(512) void k_linear_q4_rows(Q4Args a, int32_t pass_rows, int32_t groups_n, int32_t out_f16)
+__global__ __launch_bounds__(512) void k_linear_q4_rows(Q4Args a, int32_t pass_rows, int32_t groups_n, int32_t out_f16, int32_t seg,
+                                                        float* __restrict__ parts)
 {
     constexpr bool F32 = sizeof(AT) == 4;
     constexpr int R = 16 * RT, PITCH = kQ4Step + 8, NX = F32 ? 2 * RT : RT, PLANE = R * PITCH, BUF = (F32 ? 2 : 1) * PLANE;
@@ -389,6 +390,7 @@ __global__ __launch_bounds__(512) void k_linear_q4_rows(Q4Args a, int32_t pass_r
     float* xinv = reinterpret_cast<float*>(xs + 2 * BUF);          // F32: [2][R]
     Q4Stream<G, ZP> ws(a, reinterpret_cast<char*>(xinv + (F32 ? 2 * R : 0)) + wave * kQ4Tile, lane);
     typename Q4Stream<G, ZP>::Slot ring[2];
+    const int32_t s0 = blockIdx.z * seg, s1 = s0 + seg < ws.steps ? s0 + seg : ws.steps;  // the split's steps
     const AT* x = (const AT*)a.inp + m0 * a.K;
     const int32_t xrow = F32 ? wave : tid >> 5, xat = F32 ? lane * 4 : (tid & 31) * 8;
     constexpr int XROWS = F32 ? 8 : 16;  // rows the block loads at a time
@@ -415,18 +417,18 @@ __global__ __launch_bounds__(512) void k_linear_q4_rows(Q4Args a, int32_t pass_r
 #pragma unroll
     for (int r = 0; r < RT; r++) row[r] = (r * 16 + n < rows ? r * 16 + n : rows - 1) * PITCH;
 
-    load_x(0);
+    load_x(s0);
     ws.point(a, n0);
-    ws.issue(ring[0], 0);
-    ws.issue(ring[1], 1);
+    ws.issue(ring[0], s0);
+    ws.issue(ring[1], s0 + 1);
     store_x(0);
-    load_x(1);
+    load_x(s0 + 1);
     lds_barrier();
     f4 acc[RT] = {};
-    for (int32_t st = 0; st < ws.steps; st += 2) {
+    for (int32_t st = s0; st < s1; st += 2) {
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            if (u == 1 && st + 1 >= ws.steps) break;
+            if (u == 1 && st + 1 >= s1) break;
             ws.put(ring[u]);
             if constexpr (F32) {
                 f4 part[RT] = {};
@@ -441,7 +443,7 @@ __global__ __launch_bounds__(512) void k_linear_q4_rows(Q4Args a, int32_t pass_r
                 ws.template step<RT, false>(acc, xs + u * BUF, row, PLANE);
             }
             __builtin_amdgcn_sched_barrier(0);
-            if (st + u + 1 < ws.steps) {
+            if (st + u + 1 < s1) {
                 ws.issue(ring[u], st + u + 2);
                 store_x(u ^ 1);
                 load_x(st + u + 2);
@@ -455,7 +457,9 @@ __global__ __launch_bounds__(512) void k_linear_q4_rows(Q4Args a, int32_t pass_r
     for (int e = 0; e < 4 * RT; e++) {
         const int m = e / 4 * 16 + 4 * g4 + e % 4;
         if (m >= rows) break;
-        q4_store(a, out_f16, (m0 + m) * a.N + n0 + n, acc[e / 4][e % 4] + bias);
+        const int64_t o = (m0 + m) * a.N + n0 + n;
+        if (parts) parts[blockIdx.z * a.M * a.N + o] = acc[e / 4][e % 4];  // for k_linear_q4_join
+        else q4_store(a, out_f16, o, acc[e / 4][e % 4] + bias);
     }
 }
 
@@ -490,15 +494,25 @@ Q4Plan linear_q4_plan(const Q4Args& a, int act, int64_t cus)
                   rows = std::min<int64_t>(a.M, kQ4Rows);
     Q4Plan p{};
     if (steps == 0) return p;
-    // x a step at a time, where the blocks of 8 tiles fill half the device and there are rows to share the codes
-    const int64_t groups = (a.N + 127) / 128;
-    if (a.M > (f32 ? 8 : 4) && groups * ((a.M + 15) / 16) >= cus / 2) {
+    // x a step at a time, passes of `most` rows, `parts` shares of k
+    const int64_t groups = (a.N + 127) / 128, n16 = (a.M + 15) / 16, n32 = (a.M + 31) / 32;
+    auto stepwise = [&](int64_t most, int64_t parts) {
+        const int64_t n = (a.M + most - 1) / most;
+        p.rows = (a.M + n - 1) / n;
+        p.seg = (steps + parts - 1) / parts;
+        p.splits = (steps + p.seg - 1) / p.seg;
+        p.ws_floats = p.splits > 1 ? p.splits * a.M * a.N : 0;
+        return p;
+    };
+    // 5 / 8 of a device of blocks, and at most 12 parts to join
+    const int64_t parts = std::min<int64_t>({(cus * 5 / 8 + groups * n16 - 1) / (groups * n16), 12, steps});
+    // where the blocks of 8 tiles fill half the device and there are rows to share the codes
+    if (a.M > (f32 ? 8 : 4) && groups * n16 >= cus / 2) {
+        if (parts > 1 && steps >= 12) return stepwise(16, parts);  // 64 rows of 4000 x 4096 16.7 -> 13.1 us
         // passes of 16 or 32 rows, by the blocks a CU takes and what these cost (17920 x 1536: 1, 2, 3 of 16 rows 8.0, 11.7,
         // 15.5 us; 1, 2 of 32 rows 9.3, 14.7); fp32 x of 32 rows leaves a CU one block (19.6 us, of 16 18.6)
-        const int64_t c16 = (groups * ((a.M + 15) / 16) + cus - 1) / cus, c32 = (groups * ((a.M + 31) / 32) + cus - 1) / cus;
-        const int64_t most = !f32 && 7 * c32 < 5 * c16 ? 32 : 16, n = (a.M + most - 1) / most;
-        p.rows = (a.M + n - 1) / n;
-        return p;
+        const int64_t c16 = (groups * n16 + cus - 1) / cus, c32 = (groups * n32 + cus - 1) / cus;
+        return stepwise(!f32 && 7 * c32 < 5 * c16 ? 32 : 16, 1);
     }
     p.splits = 1;
     p.ks = 1;
@@ -509,6 +523,9 @@ Q4Plan linear_q4_plan(const Q4Args& a, int act, int64_t cus)
         p.splits++;
         p.seg = std::max<int64_t>(2, (steps + p.splits - 1) / p.splits);
     }
+    // where x does not fit (16 rows of 1536 x 8960 10.7 -> 8.7 us, 64 18.1 -> 13.7; fp32 17 rows of 1536 x 1536 8.6 -> 7.0); x that
+    // fits stays whole (17 rows of 4000 x 4096 9.0, in 3 shares 10.7)
+    if (a.M > 4 && p.splits > 1) return stepwise(16, parts);
     while (p.ks < 8 && p.ks < p.seg && tiles * passes * p.splits * p.ks < (rows > 4 ? 4 : 8) * cus) p.ks *= 2;
     p.waves = rows > 4 ? 8 : std::max<int64_t>(4, p.ks);
     p.splits = (steps + p.seg - 1) / p.seg;
@@ -523,9 +540,10 @@ int launch_linear_q4(const Q4Plan& p, const Q4Args& a, int act, int out, float* 
     if (p.rows > 0) {
         const int64_t groups = (a.N + 127) / 128, rt = (p.rows + 15) / 16, planes = f32 ? 2 : 1;
         const int64_t lds = 2 * planes * rt * 16 * (kQ4Step + 8) * 2 + (f32 ? 2 * rt * 16 * 4 : 0) + 8 * kQ4Tile;
-        const dim3 grid((unsigned)((groups + 7) / 8 * 8), (unsigned)((a.M + p.rows - 1) / p.rows));
+        const dim3 grid((unsigned)((groups + 7) / 8 * 8), (unsigned)((a.M + p.rows - 1) / p.rows), (unsigned)p.splits);
         auto go = [&](auto kern) {
-            hipLaunchKernelGGL(kern, grid, dim3(512), (size_t)lds, st, a, (int32_t)p.rows, (int32_t)groups, (int32_t)(out == VVH_F16));
+            hipLaunchKernelGGL(kern, grid, dim3(512), (size_t)lds, st, a, (int32_t)p.rows, (int32_t)groups, (int32_t)(out == VVH_F16),
+                               (int32_t)p.seg, p.splits > 1 ? ws : nullptr);
         };
         auto go_rt = [&](auto* t, auto z, auto g) {
             using AT = std::remove_pointer_t<decltype(t)>;
@@ -543,9 +561,7 @@ int launch_linear_q4(const Q4Plan& p, const Q4Args& a, int act, int out, float* 
         };
         auto go_type = [&](auto* t) { a.zeros ? go_group(t, std::true_type{}) : go_group(t, std::false_type{}); };
         f32 ? go_type((float*)nullptr) : go_type((f16*)nullptr);
-        return (int)hipGetLastError();
-    }
-    if (p.splits > 0) {
+    } else if (p.splits > 0) {
         const int64_t tiles = (a.N + 15) / 16, passes = (a.M + kQ4Rows - 1) / kQ4Rows, rows = std::min<int64_t>(a.M, kQ4Rows);
         const int64_t per = p.seg * (f32 ? 1 : kQ4Step / 8), lds = q4_lds(p, rows, f32);
         const int64_t tpb = p.waves / p.ks, groups = (tiles + tpb - 1) / tpb;
