@@ -183,6 +183,15 @@ def test_ragged_batches(gpu, dtype, lens, H, KVH, D):
 
 
 @pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("lens,H,KVH,D", [([9000], 4, 2, 80), ([20001, 3, 0, 700], 2, 1, 256), ([1] * 300, 4, 2, 40), ([0, 5000] * 4, 3, 3, 112),
+                                          ([64, 65, 63, 128, 4], 8, 2, 256), ([3000] * 3, 2, 1, 7)])
+@pytest.mark.parametrize("max_len", [0, 64, 100])
+def test_ragged_batches_of_other_head_dims(gpu, dtype, lens, H, KVH, D, max_len):
+    rng = np.random.default_rng(len(lens) + D)
+    check_attention(rng, lens, 24, H, KVH, D, dtype, max_len)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
 @pytest.mark.parametrize("D", [64, 128, 40])
 def test_pages_that_are_gone(gpu, dtype, D):
     """Entries below 0 and past the pool: their positions are left out, at the start, inside, everywhere."""

@@ -426,7 +426,7 @@ struct AttnPagedPlan {
     bool tiled;
     int64_t GT, tiles, waves, blocks, ws_floats;
 };
-AttnPagedPlan attention_paged_plan(const PagedArgs& c, const void* out, const void* q, int64_t max_len, int64_t H, int dtype,
+AttnPagedPlan attention_paged_plan(const PagedArgs& c, const void* q, int64_t max_len, int64_t H, int dtype,
                                    int64_t cus);
 int launch_attention_paged(const AttnPagedPlan& p, const PagedArgs& c, void* out, const void* q, const int32_t* lens, int64_t H,
                            float scale, float* ws, int dtype, void* stream);

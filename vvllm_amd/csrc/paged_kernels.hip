@@ -117,40 +117,67 @@ __global__ __launch_bounds__(512) void k_rope_append_paged_vec(PagedArgs c, T* q
     }
 }
 
-// softmax(scale q K^T) V of one query and head over the pages, any head_dim up to
-// 256: a block per (head, sequence), its 4 waves each every fourth position, lane
-// l the dims l, l + 64, ...; per position the dot product is summed over the wave
-// and joins a running maximum m, sum l and numerator o (o and l rescaled by
-// e^(m_old - m)).  The waves' three merge through LDS.
-template <typename T>
-__global__ __launch_bounds__(256) void k_attention_paged(PagedArgs c, T* __restrict__ out, const T* __restrict__ q,
-                                                         const int32_t* __restrict__ lens, int32_t H, float scale)
+// softmax(scale q K^T) V of one query and head over the pages, any head_dim up to 256 and any alignment: a block per
+// (head, sequence, share of its keys), its 4 waves each every fourth 8 keys, lane l the dims l, l + 64, ... (ND of them).
+// The 8 keys' loads are in flight together; a dot product is summed over the wave; they join a running maximum m, sum l
+// and numerator o (rescaled by e^(m_old - m)).  The waves' three merge through LDS, the shares' through the
+// workspace (a row of D + 2 floats each) in k_attention_paged_any_merge.  8 contexts of 1000 fp16 keys, 16 heads on 8, of 256:
+// 66 us (a key at a time, in one block a row: 646), of 80: 25 (385); bound by the 2-byte loads.
+template <typename T, int ND>
+__global__ __launch_bounds__(256) void k_attention_paged_any(PagedArgs c, T* __restrict__ out, const T* __restrict__ q,
+                                                             const int32_t* __restrict__ lens, int32_t H, float scale,
+                                                             float* __restrict__ parts)
 {
-    __shared__ float wm[4], wl[4], wo[4][256];
-    const int32_t h = blockIdx.x, s = blockIdx.y, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    constexpr int KU = 8;
+    __shared__ float wm[4], wl[4], wo[4][64 * ND];
+    const int32_t h = blockIdx.x, s = blockIdx.y, lane = threadIdx.x & 63, w = threadIdx.x >> 6, S = gridDim.z;
     const int32_t D = c.D, g = h / (H / c.KVH);
     const int64_t cap = (int64_t)c.max_pages * c.P;
-    const int64_t len = lens[s] < cap ? lens[s] : cap;
+    const int64_t len = lens[s] < 0 ? 0 : lens[s] < cap ? lens[s] : cap;
+    const int32_t p0 = (int32_t)(len * blockIdx.z / S), p1 = (int32_t)(len * (blockIdx.z + 1) / S);
     const T* qr = q + ((int64_t)s * H + h) * D;
-    float x[4], o[4] = {}, m = -INFINITY, l = 0.0f;
+    bool on[ND];
+    float x[ND], o[ND] = {}, m = -INFINITY, l = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; i++) x[i] = lane + 64 * i < D ? (float)qr[lane + 64 * i] * scale : 0.0f;
-    for (int64_t p = w; p < len; p += 4) {
-        const int64_t row = paged_row(c, s, (int32_t)p);
-        if (row < 0) continue;
-        const int64_t at = (row * c.KVH + g) * D + lane;
-        float d = 0.0f, vv[4];
+    for (int i = 0; i < ND; i++) {
+        on[i] = lane + 64 * i < D;
+        x[i] = on[i] ? (float)qr[lane + 64 * i] * scale : 0.0f;
+    }
+    for (int32_t p = p0 + w * KU; p < p1; p += 4 * KU) {
+        const int64_t mine = lane < KU && p + lane < p1 ? paged_row(c, s, p + lane) : -1;
+        bool live[KU];
+        float k[KU][ND], v[KU][ND], d[KU];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const bool on = lane + 64 * i < D;
-            d = __builtin_fmaf(x[i], on ? (float)((const T*)c.kp)[at + 64 * i] : 0.0f, d);
-            vv[i] = on ? (float)((const T*)c.vp)[at + 64 * i] : 0.0f;
+        for (int j = 0; j < KU; j++) {
+            const int32_t row = __builtin_amdgcn_readlane((int)mine, j);
+            live[j] = row >= 0;
+            const int64_t at = ((int64_t)(row < 0 ? 0 : row) * c.KVH + g) * D + lane;  // no key: row 0, whatever it holds
+#pragma unroll
+            for (int i = 0; i < ND; i++) {
+                k[j][i] = on[i] ? (float)((const T*)c.kp)[at + 64 * i] : 0.0f;
+                v[j][i] = on[i] ? (float)((const T*)c.vp)[at + 64 * i] : 0.0f;
+            }
         }
-        d = wave_sum_xor(d);
-        const float mn = fmaxf(m, d), f = m == -INFINITY ? 0.0f : expf(m - mn), e = d == -INFINITY ? 0.0f : expf(d - mn);
-        l = __builtin_fmaf(l, f, e);
+        float mn = m;
 #pragma unroll
-        for (int i = 0; i < 4; i++) o[i] = __builtin_fmaf(o[i], f, e * vv[i]);
+        for (int j = 0; j < KU; j++) {
+            d[j] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < ND; i++) d[j] = __builtin_fmaf(x[i], k[j][i], d[j]);
+            d[j] = live[j] ? wave_sum_xor(d[j]) : -INFINITY;
+            mn = fmaxf(mn, d[j]);
+        }
+        const float f = m == -INFINITY ? 0.0f : expf(m - mn);
+        l *= f;
+#pragma unroll
+        for (int i = 0; i < ND; i++) o[i] *= f;
+#pragma unroll
+        for (int j = 0; j < KU; j++) {
+            const float e = d[j] == -INFINITY ? 0.0f : expf(d[j] - mn);
+            l += e;
+#pragma unroll
+            for (int i = 0; i < ND; i++) o[i] = __builtin_fmaf(e, live[j] ? v[j][i] : 0.0f, o[i]);
+        }
         m = mn;
     }
     if (lane == 0) {
@@ -158,19 +185,63 @@ __global__ __launch_bounds__(256) void k_attention_paged(PagedArgs c, T* __restr
         wl[w] = l;
     }
 #pragma unroll
-    for (int i = 0; i < 4; i++) wo[w][lane + 64 * i] = o[i];
+    for (int i = 0; i < ND; i++) wo[w][lane + 64 * i] = o[i];
     __syncthreads();
     const float M = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
+    const int32_t d = threadIdx.x;
+    if (d >= D) return;
     float num = 0.0f, den = 0.0f;
     for (int i = 0; i < 4; i++) {
         const float f = wm[i] == -INFINITY ? 0.0f : expf(wm[i] - M);
-        num = __builtin_fmaf(f, wo[i][threadIdx.x], num);
+        num = __builtin_fmaf(f, wo[i][d], num);
         den = __builtin_fmaf(f, wl[i], den);
     }
-    if ((int)threadIdx.x < D)
-        out[((int64_t)s * H + h) * D + threadIdx.x] = (T)(M == -INFINITY && den == 0.0f ? 0.0f : num / den);
+    const int64_t row = (int64_t)s * H + h;
+    if (S == 1) {
+        out[row * D + d] = (T)(M == -INFINITY && den == 0.0f ? 0.0f : num / den);
+        return;
+    }
+    float* part = parts + (row * S + blockIdx.z) * (D + 2);
+    part[d] = num;
+    if (d == 0) {
+        part[D] = M;
+        part[D + 1] = den;
+    }
 }
-
+// Block r: row r's S shares, 16 / ND groups of 64 ND threads each every 16 / ND-th, then the groups through LDS.
+template <typename T, int ND>
+__global__ __launch_bounds__(1024) void k_attention_paged_any_merge(T* __restrict__ out, const float* __restrict__ parts, int32_t D, int32_t S)
+{
+    constexpr int G = 16 / ND;
+    __shared__ float wm[G], wl[G], wo[G][64 * ND];
+    const int64_t row = blockIdx.x;
+    const int32_t d = threadIdx.x % (64 * ND), gr = threadIdx.x / (64 * ND);
+    const float* p = parts + row * S * (D + 2);
+    float M = -INFINITY, num = 0.0f, den = 0.0f;
+#pragma unroll 4
+    for (int32_t i = gr; i < S; i += G) {
+        const float *part = p + (int64_t)i * (D + 2), m = part[D], l = part[D + 1], o = part[d < D ? d : 0];
+        const float mn = fmaxf(M, m), f = M == -INFINITY ? 0.0f : expf(M - mn), e = m == -INFINITY ? 0.0f : expf(m - mn);
+        num = __builtin_fmaf(num, f, e * o);
+        den = __builtin_fmaf(den, f, e * l);
+        M = mn;
+    }
+    wo[gr][d] = num;
+    if (d == 0) {
+        wm[gr] = M;
+        wl[gr] = den;
+    }
+    __syncthreads();
+    if (gr > 0 || d >= D) return;
+    for (int i = 1; i < G; i++) M = fmaxf(M, wm[i]);
+    num = den = 0.0f;
+    for (int i = 0; i < G; i++) {
+        const float f = wm[i] == -INFINITY ? 0.0f : expf(wm[i] - M);
+        num = __builtin_fmaf(f, wo[i][d], num);
+        den = __builtin_fmaf(f, wl[i], den);
+    }
+    out[row * D + d] = (T)(M == -INFINITY && den == 0.0f ? 0.0f : num / den);
+}
 
 // ---------------------------------------------------------------------------
 // The matrix-core form: head_dim 64, 96 or 128, aligned arrays.
@@ -798,24 +869,27 @@ constexpr int64_t kPagedOneChunks = 16;
 // Floats of the chunk sums ahead of the parts in the workspace.
 static int64_t paged_before_floats(int64_t B) { return (2 * (B + 1) + 3) / 4 * 4; }
 
-bool attention_paged_tiled(const PagedArgs& c, const void* out, const void* q, int dtype)
+static bool attention_paged_tiled(const PagedArgs& c, const void* q, int dtype)
 {
     const uintptr_t all = (uintptr_t)c.kp | (uintptr_t)c.vp | (uintptr_t)q;
-    (void)out;
     return (c.D == 64 || c.D == 96 || c.D == 128) && all % 16 == 0 && (dtype == VVH_F16 || dtype == VVH_F32);
 }
 
-AttnPagedPlan attention_paged_plan(const PagedArgs& c, const void* out, const void* q, int64_t max_len, int64_t H, int dtype,
+AttnPagedPlan attention_paged_plan(const PagedArgs& c, const void* q, int64_t max_len, int64_t H, int dtype,
                                    int64_t cus)
 {
     AttnPagedPlan p{};
     const int64_t G = H / c.KVH;
-    p.tiled = attention_paged_tiled(c, out, q, dtype);
+    p.tiled = attention_paged_tiled(c, q, dtype);
     p.tiles = (G + 15) / 16;
     p.GT = (G + p.tiles - 1) / p.tiles;
-    if (!p.tiled) return p;
     const int64_t cap = (int64_t)c.max_pages * c.P;
     const int64_t len = max_len > 0 && max_len < cap ? max_len : cap;
+    if (!p.tiled) {  // shares of at least 64 keys, to about 8 blocks a CU (8 contexts of 1000 keys of 80 24.8 us, to 4 a CU 34.3, to 2 57)
+        p.blocks = std::max<int64_t>(1, std::min<int64_t>({(len + 63) / 64, (8 * cus + c.B * H - 1) / (c.B * H), 256}));
+        p.ws_floats = p.blocks > 1 ? c.B * H * p.blocks * (c.D + 2) : 0;
+        return p;
+    }
     const int64_t ch = dtype == VVH_F16 ? (c.D == 64 ? PagedTile<f16>::CH<64> : PagedTile<f16>::CH<128>)
                                         : (c.D == 128 ? PagedTile<float>::CH<128> : PagedTile<float>::CH<64>);
     const int64_t chunks = (len + ch - 1) / ch;
@@ -872,8 +946,16 @@ int launch_attention_paged(const AttnPagedPlan& p, const PagedArgs& c, void* out
             };
             c.D == 64 ? run(std::integral_constant<int, 64>{}) : c.D == 96 ? run(std::integral_constant<int, 96>{}) : run(std::integral_constant<int, 128>{});
         } else {
-            hipLaunchKernelGGL(k_attention_paged<T>, dim3((unsigned)H, (unsigned)c.B), dim3(256), 0, st, c, (T*)out,
-                               (const T*)q, lens, (int32_t)H, scale);
+            auto any = [&](auto nd) {
+                constexpr int ND = decltype(nd)::value;
+                hipLaunchKernelGGL((k_attention_paged_any<T, ND>), dim3((unsigned)H, (unsigned)c.B, (unsigned)p.blocks), dim3(256), 0, st, c,
+                                   (T*)out, (const T*)q, lens, (int32_t)H, scale, ws);
+                if (p.blocks > 1)
+                    hipLaunchKernelGGL((k_attention_paged_any_merge<T, ND>), dim3((unsigned)(c.B * H)), dim3(1024), 0, st, (T*)out,
+                                       (const float*)ws, c.D, (int32_t)p.blocks);
+            };
+            c.D <= 64 ? any(std::integral_constant<int, 1>{})
+            : c.D <= 128 ? any(std::integral_constant<int, 2>{}) : any(std::integral_constant<int, 4>{});
         }
     };
     dtype == VVH_F16 ? go((f16*)nullptr) : go((float*)nullptr);

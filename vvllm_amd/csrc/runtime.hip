@@ -2412,7 +2412,7 @@ VVH_API int vvh_attention_paged(const vvh_paged_cache* cache, void* out, const v
     const uintptr_t e = cache->dtype == VVH_F32 ? 3 : 1;
     if ((((uintptr_t)q | (uintptr_t)out) & e) || ((uintptr_t)lens & 3)) return fail(VVH_ERR_INVALID_ARG, "misaligned pointer");
     REQUIRE_INIT();
-    const AttnPagedPlan p = attention_paged_plan(a, out, q, (int64_t)std::min(max_len, (size_t)INT32_MAX), (int64_t)num_heads,
+    const AttnPagedPlan p = attention_paged_plan(a, q, (int64_t)std::min(max_len, (size_t)INT32_MAX), (int64_t)num_heads,
                                                  cache->dtype, g_cu_count > 0 ? g_cu_count : 256);
     float* ws = nullptr;
     if (p.ws_floats > 0) {
