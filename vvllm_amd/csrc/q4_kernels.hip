@@ -30,6 +30,11 @@ namespace {
 // fp32 rows of x are staged as two fp16 planes, high and low parts of x times a power of two that
 // puts the step's largest |x| into [2^14, 2^15) (22 bits; the sum of a step is multiplied back).  Up to 8 such
 // rows make 16 rows of the operand (FOLD): one instruction then takes both parts.
+//
+// One fp32 row of 151936 x 896 in groups of 32, 78 MB: 23.7 us, 3.3 TB/s (from weights that the last level cache still holds in
+// part 21); fp16 in groups of 128, 70 MB, 20; one fp16 row of 28672 x 8192, 121 MB, 31 us, 3.9 TB/s: bound by
+// HBM.  One fp16 row of 896 x 896: 3.1 us, a launch and two round trips.  Loading the codes straight into the instruction's
+// layout (16 pieces of 64 bytes a load, dwords exchanged between lanes) instead of through LDS: 24 -> 29 us on the first.
 // ---------------------------------------------------------------------------
 constexpr int kQ4Step = 256;     // codes of a row a step
 constexpr int kQ4WPitch = 144;   // bytes between rows of the LDS weight tile
@@ -372,7 +377,8 @@ __global__ __launch_bounds__(512) void k_linear_q4(Q4Args a, Q4Launch L)
 // at a time: two buffers, the next step's x on its way from memory while the waves work on this one, a barrier a step.
 // A wave's codes meet RT operands of x.  Against the kernel above, which needs all of x before it begins: 13 rows of 17920 x
 // 1536 9.0 -> 8.1 us, 32 13.2 -> 10.0, 64 18.2 -> 14.6 (fp32 32.7 -> 25.9), 64 rows of 151936 x 896 69.9 -> 53.9; up to 4 rows
-// it is slower (1 of 28672 x 8192 31.1 -> 38.5), and with few blocks (76: 8 rows of 9728 x 896 5.0 -> 5.6).
+// it is slower (1 of 28672 x 8192 31.1 -> 38.5), and with few blocks (76: 8 rows of 9728 x 896 5.0 -> 5.6).  The steps' latency
+// bounds it (13 rows: 14.9 MB, 1.8 TB/s), and from 32 rows on the LDS reads of x, 8 KB for 16 rows and a step of a wave.
 template <typename AT, int G, bool ZP, int RT>
 __global__ __launch_bounds__(512) void k_linear_q4_rows(Q4Args a, int32_t pass_rows, int32_t groups_n, int32_t out_f16, int32_t seg,
                                                         float* __restrict__ parts)
