@@ -555,7 +555,7 @@ typedef struct vvh_paged_cache {
     uint64_t num_pages;
     uint64_t page_size;        /* any size >= 1 (num_pages * page_size < 2^31) */
     uint64_t num_seqs;         /* < 65536 */
-    uint64_t max_pages;        /* max_pages * page_size <= 2^30 */
+    uint64_t max_pages;        /* max_pages * page_size <= 2^29 */
     uint64_t num_kv_heads;
     uint64_t head_dim;         /* <= 256 */
     int32_t dtype;             /* VVH_F32 or VVH_F16: pages, queries and outputs */

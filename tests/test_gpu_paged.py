@@ -425,3 +425,33 @@ def test_two_streams_at_once(gpu):
     for pg, q, dq, do, st, want in sets:
         np.testing.assert_array_equal(do.to_array(np.float16, q.shape).astype(np.float64), want)
         st.close()
+
+
+def test_two_graphs_of_one_stream(gpu):
+    """Two captured batches that share the stream's workspace, replayed in turn, and after a larger call has outgrown the
+    workspace that they hold."""
+    rng = np.random.default_rng(11)
+    st, sets = Stream(), []
+    for lens, H, KVH, D in (([2500, 50], 12, 2, 128), ([1900, 700, 1], 14, 2, 64), ([4000], 4, 2, 80)):
+        pg = Pages(rng, lens, 16, KVH, D, F16)
+        q = rng.normal(0, 2, (len(lens), H, D)).astype(np.float16)
+        dq, do = capi.DevBuf.from_array(q), capi.DevBuf(q.nbytes)
+
+        def issue(s, pg=pg, dq=dq, do=do, H=H):
+            capi.call("vvh_attention_paged", pg.cache(), do.ptr, dq.ptr, pg.d_n.ptr, 0, H, 0.1, s)
+
+        issue(st.s)
+        st.sync()
+        sets.append((do, q.shape, do.to_array(np.float16, q.shape), issue))
+    graphs = [st.capture(x[3]) for x in sets]
+    big = Pages(rng, [3000] * 40, 64, 8, 128, F16)
+    for step in range(3):
+        for (do, shape, want, _), replay in zip(sets, graphs):
+            capi.call("vvh_fill_normal", do.ptr, F16, want.size, 1, 0.0, 1.0, None)
+            capi.sync()
+            replay()
+            np.testing.assert_array_equal(do.to_array(np.float16, shape), want)
+        if step == 0:
+            q = rng.normal(0, 2, (40, 128, 128)).astype(np.float16)
+            run_attention(big, q, stream=st.s)
+    st.close()

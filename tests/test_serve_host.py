@@ -32,7 +32,7 @@ def attention(c, out=P, q=2 * P, lens=P, max_len=0, heads=14):
     (dict(num_kv_heads=0), INVALID), (dict(head_dim=0), INVALID), (dict(head_dim=258), INVALID), (dict(dtype=2), INVALID),
     (dict(k_pages=P + 1), INVALID), (dict(dtype=F32, v_pages=P + 2), INVALID), (dict(page_table=P + 2), INVALID),
     (dict(num_pages=1 << 27, page_size=16), UNSUPPORTED), (dict(num_pages=1 << 40), UNSUPPORTED),
-    (dict(page_size=(1 << 64) - 1), UNSUPPORTED), (dict(max_pages=(1 << 26) + 1), UNSUPPORTED),
+    (dict(page_size=(1 << 64) - 1), UNSUPPORTED), (dict(max_pages=(1 << 25) + 1), UNSUPPORTED),
     (dict(num_seqs=65536), UNSUPPORTED), (dict(num_kv_heads=65536), UNSUPPORTED)])
 def test_bad_caches(kw, status):
     heads = 14 if kw.get("num_kv_heads") != 65536 else 65536

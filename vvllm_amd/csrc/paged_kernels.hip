@@ -636,7 +636,7 @@ __global__ __launch_bounds__(256, 2) void k_attention_paged_split(PagedArgs c, T
     // the sums of the chunks before each sequence, and of all: the first wave keeps them for the merge
     int64_t total = 0;
     for (int32_t s0 = 0; s0 < c.B; s0 += 64) {
-        const uint32_t upto = wave_scan((uint32_t)paged_window(c, lens, s0, lane, CH));  // at most 64 * 2^26
+        const uint32_t upto = wave_scan((uint32_t)paged_window(c, lens, s0, lane, CH));  // at most 64 * 2^25
         if (w == 0 && s0 + lane < c.B) before_out[s0 + lane + 1] = total + upto;
         total += lane_of(upto, 63);
     }

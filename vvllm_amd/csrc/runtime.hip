@@ -2350,8 +2350,8 @@ static int paged_args(const vvh_paged_cache* c, PagedArgs* a)
         return fail(VVH_ERR_INVALID_ARG, "%llu kv heads, head_dim %llu outside 1..256", (unsigned long long)c->num_kv_heads,
                     (unsigned long long)c->head_dim);
     if (c->num_pages > INT32_MAX || c->page_size > INT32_MAX / c->num_pages ||
-        c->max_pages > (uint64_t(1) << 30) / c->page_size || c->num_seqs > 65535 || c->num_kv_heads > 65535)
-        return fail(VVH_ERR_UNSUPPORTED, "a cache of 2^31 rows, 2^30 positions a sequence, 65536 sequences or kv heads");
+        c->max_pages > (uint64_t(1) << 29) / c->page_size || c->num_seqs > 65535 || c->num_kv_heads > 65535)
+        return fail(VVH_ERR_UNSUPPORTED, "a cache of 2^31 rows, more than 2^29 positions a sequence, 65536 sequences or kv heads");
     const uintptr_t e = c->dtype == VVH_F32 ? 3 : 1;
     if (((uintptr_t)c->k_pages & e) || ((uintptr_t)c->v_pages & e) || ((uintptr_t)c->page_table & 3))
         return fail(VVH_ERR_INVALID_ARG, "misaligned pointer");
