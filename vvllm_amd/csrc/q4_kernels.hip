@@ -31,9 +31,9 @@ namespace {
 // puts the step's largest |x| into [2^14, 2^15) (22 bits; the sum of a step is multiplied back).  Up to 8 such
 // rows make 16 rows of the operand (FOLD): one instruction then takes both parts.
 //
-// One fp32 row of 151936 x 896 in groups of 32, 78 MB: 23.7 us, 3.3 TB/s (from weights that the last level cache still holds in
-// part 21); fp16 in groups of 128, 70 MB, 20; one fp16 row of 28672 x 8192, 121 MB, 31 us, 3.9 TB/s: bound by
-// HBM.  One fp16 row of 896 x 896: 3.1 us, a launch and two round trips.  Loading the codes straight into the instruction's
+// One fp32 row of 151936 x 896 in groups of 32, 78 MB: 22 us, 3.5 TB/s; fp16 in groups of 128, 70 MB, 19, 3.7 TB/s; one
+// fp16 row of 28672 x 8192, 121 MB, 29.6 us, 4.1 TB/s: bound by HBM and, beside it, the LDS round trips of the codes.  One fp16
+// row of 896 x 896: 3.0 us, a launch and two round trips.  Loading the codes straight into the instruction's
 // layout (16 pieces of 64 bytes a load, dwords exchanged between lanes) instead of through LDS: 24 -> 29 us on the first.
 // ---------------------------------------------------------------------------
 constexpr int kQ4Step = 256;     // codes of a row a step
@@ -82,6 +82,14 @@ __device__ __forceinline__ h8 q4_codes(uint32_t w, h2 zl, h2 zh, const Q4Masks& 
     return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+// Waits until at most N loads are in flight.
+template <int N>
+__device__ __forceinline__ void wait_loads()
+{
+    static_assert(N < 64, "vmcnt");
+    __builtin_amdgcn_s_waitcnt((N & 15) | 7 << 4 | 15 << 8 | (N >> 4) << 14);
+}
+
 // A wave's stream of a tile's weights: 16 channels from n0 on, a step at a time from memory to registers (issue),
 // to its LDS tile (put) and through the matrix instruction (step).
 template <int G, bool ZP>
@@ -89,6 +97,7 @@ struct Q4Stream {
     static constexpr int PG = kQ4Step / G;          // groups a step
     static constexpr int NS = PG > 4 ? 2 : 1;       // scales a lane loads a step
     static constexpr int DW = G / 32;               // dwords of codes a lane reads a group
+    static constexpr int loads = 2 + NS * (ZP ? 2 : 1);  // of a step
     struct Slot {
         u4 a, b;
         uint16_t s[NS];
@@ -137,7 +146,7 @@ struct Q4Stream {
         for (int i = 0; i < NS; i++) {
             uint32_t v = r.s[i];
             if (ZP) v |= (uint32_t)__builtin_bit_cast(uint16_t, (f16)(float)r.z[i]) << 16;
-            if (g4 * NS + i < PG) stile[n * kQ4SPitch + g4 * NS + i] = v;
+            stile[n * kQ4SPitch + (g4 * NS + i) % PG] = v;  // two lanes the same where there are fewer groups
         }
         // one wave's LDS accesses complete in order
     }
@@ -176,6 +185,8 @@ struct Q4Stream {
             for (int r = 0; r < RT; r++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) part[r][i] = __builtin_fmaf(s, d[r][i], part[r][i]);
+            // not all of a step's reads at once: registers
+            if ((g + 1) % (PG / 2) == 0) __builtin_amdgcn_sched_barrier(0);
         }
     }
 };
@@ -190,6 +201,14 @@ __device__ __forceinline__ void q4_store(const Q4Args& a, bool out_f16, int64_t 
         if (a.res) y += ((const float*)a.res)[o];
         ((float*)a.out)[o] = y;
     }
+}
+
+// Channel n's bias, 0 without one: no branch, so that the loads in flight around it are still counted.  (x is 16-byte
+// aligned and has a group of 32 values at least.)
+__device__ __forceinline__ float q4_bias(const Q4Args& a, int64_t n)
+{
+    const float b = *(a.bias ? a.bias + (n < a.N ? n : a.N - 1) : (const float*)a.inp);
+    return a.bias ? b : 0.0f;
 }
 
 // 8 values in the order of the codes: 0 1 2 3 4 5 6 7 -> 0 4 1 5 2 6 3 7
@@ -223,7 +242,7 @@ __device__ __forceinline__ void q4_split(f4 v, int lane, f16* hi_row, f16* lo_ro
     const uint32_t r1 = __builtin_amdgcn_mov_dpp((int)s1, 0xB1, 0xF, 0xF, false);
     const u4 o = q4_order(odd ? u4{r0, r1, lo[0], lo[1]} : u4{hi[0], hi[1], r0, r1});
     *reinterpret_cast<u4*>((odd ? lo_row : hi_row) + (lane >> 1) * 8) = o;
-    if (lane == 0) *inv = __builtin_bit_cast(float, (uint32_t)(e - 14) << 23);
+    *inv = __builtin_bit_cast(float, (uint32_t)(e - 14) << 23);  // every lane the same: no branch
 }
 
 template <typename AT, int G, bool ZP, int DEPTH, bool FOLD>
@@ -242,7 +261,7 @@ __global__ __launch_bounds__(512) void k_linear_q4(Q4Args a, Q4Launch L)
     const int32_t K = (int32_t)a.K, steps = (K + kQ4Step - 1) / kQ4Step;
     const int32_t s0 = split * L.seg, s1 = s0 + L.seg < steps ? s0 + L.seg : steps;
     const int32_t mine = (s1 - s0 - ks + KS - 1) >> L.log_ks;   // steps s0 + ks + KS i of every tile are the wave's
-    const int32_t turns = (mine + DEPTH - 1) / DEPTH * DEPTH;   // whole rings
+    const int32_t turns = mine > DEPTH ? (mine + DEPTH - 1) / DEPTH * DEPTH : DEPTH;  // whole rings, one at least
     const int32_t pitch = L.seg * kQ4Step + 8;      // halves between rows of x in LDS
     f16* xs = reinterpret_cast<f16*>(smem);
     const int32_t plane = L.rows * pitch;           // F32: the low parts' plane is at +plane
@@ -289,63 +308,74 @@ __global__ __launch_bounds__(512) void k_linear_q4(Q4Args a, Q4Launch L)
         }
     };
     f4 acc;
-    auto consume = [&](int u, int32_t i) {
-        const int32_t st = ks + (i << L.log_ks);           // within x in LDS
+    // step i of the wave (last: of the last ring, which may be past its end and then adds nothing)
+    auto consume = [&](int u, int32_t i, bool last) {
+        const bool is = !last || i < mine;
+        const int32_t st = is ? ks + (i << L.log_ks) : 0;  // within x in LDS
         ws.put(ring[u]);
         f4 parts[1] = {};
         const int32_t at[1] = {(FOLD && n & 1 ? plane : 0) + row * pitch};
         ws.template step<1, F32 && !FOLD>(parts, xs + st * kQ4Step, at, plane);
         const f4 part = parts[0];
+        f4 to = acc;
         if constexpr (FOLD) {
             const float* inv = xinv + st * kQ4Rows + 2 * g4;
 #pragma unroll
-            for (int i = 0; i < 2; i++) acc[i] = __builtin_fmaf(part[2 * i] + part[2 * i + 1], inv[i], acc[i]);
+            for (int j = 0; j < 2; j++) to[j] = __builtin_fmaf(part[2 * j] + part[2 * j + 1], inv[j], acc[j]);
         } else if constexpr (F32) {
             const f4 inv = *reinterpret_cast<const f4*>(xinv + st * kQ4Rows + 4 * g4);  // rows past the last: dropped
 #pragma unroll
-            for (int i = 0; i < 4; i++) acc[i] = __builtin_fmaf(part[i], inv[i], acc[i]);
+            for (int j = 0; j < 4; j++) to[j] = __builtin_fmaf(part[j], inv[j], acc[j]);
         } else {
-            acc += part;
+            to = acc + part;
         }
+#pragma unroll
+        for (int j = 0; j < 4; j++) acc[j] = is ? to[j] : acc[j];
     };
 
     load_x(first);
+    float bias = q4_bias(a, first_channel(slot) + n), bias_next = 0.0f;
     ws.point(a, first_channel(slot));
 #pragma unroll
     for (int u = 0; u < DEPTH; u++) issue(u, u);
     store_x(first);
+    // Waits that are there anyway, said once more where every path has had them: x's registers are free, the ring still on
+    // its way
+    wait_loads<DEPTH * Q4Stream<G, ZP>::loads>();
     for (int32_t i = kQ4Batch * stride; i < rows * per; i += kQ4Batch * stride) {
         load_x(first + i);
         store_x(first + i);
+        wait_loads<0>();
     }
     lds_barrier();
-    for (int32_t grp = slot; grp < L.groups_n; grp += L.slots) {
+    for (int32_t grp = slot;; grp += L.slots) {
         const bool next = grp + L.slots < L.groups_n;
         acc = f4{};
-        for (int32_t i = 0; i < turns; i += DEPTH) {
-            // the ring is refilled with this tile's steps, at their end with the next tile's first ones
-            // (no work of a step ahead of the one before it: registers)
-            if (i + DEPTH < turns) {
+        // The ring is refilled with this tile's steps, at their end with the next tile's first ones (no work of a step ahead
+        // of the one before it: registers).  No branch around its loads but the last: waits count what is in flight.
+        int32_t i = 0;
+        for (; i + DEPTH < turns; i += DEPTH)
 #pragma unroll
-                for (int u = 0; u < DEPTH; u++) {
-                    consume(u, i + u);
-                    __builtin_amdgcn_sched_barrier(0);
-                    issue(u, i + u + DEPTH);
-                }
-            } else if (next) {
-                ws.point(a, first_channel(grp + L.slots));
+            for (int u = 0; u < DEPTH; u++) {
+                consume(u, i + u, false);
+                __builtin_amdgcn_sched_barrier(0);
+                issue(u, i + u + DEPTH);
+            }
+        if (next) {
+            bias_next = q4_bias(a, first_channel(grp + L.slots) + n);
+            ws.point(a, first_channel(grp + L.slots));
 #pragma unroll
-                for (int u = 0; u < DEPTH; u++) {
-                    if (i + u < mine) consume(u, i + u);
-                    __builtin_amdgcn_sched_barrier(0);
-                    issue(u, u);
-                }
-            } else {
+            for (int u = 0; u < DEPTH; u++) {
+                consume(u, i + u, true);
+                __builtin_amdgcn_sched_barrier(0);
+                issue(u, u);
+            }
+        } else {
 #pragma unroll
-                for (int u = 0; u < DEPTH; u++) {
-                    if (i + u < mine) consume(u, i + u);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
+            for (int u = 0; u < DEPTH; u++) {
+                if (u > 0 && i + u >= mine) break;  // no loads follow
+                consume(u, i + u, u == 0);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
         // the sums of the tile's waves, through their weight tiles
@@ -355,36 +385,36 @@ __global__ __launch_bounds__(512) void k_linear_q4(Q4Args a, Q4Launch L)
             if (ks == 0)
                 for (int i = 1; i < KS; i++) acc += *reinterpret_cast<const f4*>(tile + i * kQ4Tile + lane * 16);
             if (next) lds_barrier();  // read before the next tile's weights
-            if (ks != 0) continue;
         }
         const int64_t n1 = first_channel(grp) + n;
-        if (n1 >= a.N) continue;
-        const float bias = a.bias ? a.bias[n1] : 0.0f;
+        if (ks == 0 && n1 < a.N) {
 #pragma unroll
-        for (int i = 0; i < OUT; i++) {
-            if (OUT * g4 + i >= rows) break;
-            const int64_t o = (m0 + OUT * g4 + i) * a.N + n1;
-            if (L.splits > 1) {
-                L.ws[(int64_t)split * a.M * a.N + o] = acc[i];
-                continue;
+            for (int i = 0; i < OUT; i++) {
+                if (OUT * g4 + i >= rows) break;
+                const int64_t o = (m0 + OUT * g4 + i) * a.N + n1;
+                if (L.splits > 1) L.ws[(int64_t)split * a.M * a.N + o] = acc[i];
+                else q4_store(a, L.out_f16, o, acc[i] + bias);
             }
-            q4_store(a, L.out_f16, o, acc[i] + bias);
         }
+        if (!next) break;
+        bias = bias_next;
     }
 }
 
 // Many rows over many channels: a block takes 8 tiles, a wave each, and up to 16 RT rows, and x goes through LDS a step
 // at a time: two buffers, the next step's x on its way from memory while the waves work on this one, a barrier a step.
 // A wave's codes meet RT operands of x.  Against the kernel above, which needs all of x before it begins: 13 rows of 17920 x
-// 1536 9.0 -> 8.1 us, 32 13.2 -> 10.0, 64 18.2 -> 14.6 (fp32 32.7 -> 25.9), 64 rows of 151936 x 896 69.9 -> 53.9; up to 4 rows
-// it is slower (1 of 28672 x 8192 31.1 -> 38.5), and with few blocks (76: 8 rows of 9728 x 896 5.0 -> 5.6).  The steps' latency
-// bounds it (13 rows: 14.9 MB, 1.8 TB/s), and from 32 rows on the LDS reads of x, 8 KB for 16 rows and a step of a wave.
+// 1536 9.0 -> 8.0 us, 32 13.2 -> 10.0, 64 18.2 -> 14.8 (fp32 32.7 -> 26.5), 64 rows of 151936 x 896 69.9 -> 52; up to 4 rows
+// it is slower (1 of 28672 x 8192 31 -> 38), and with few blocks (76: 8 rows of 9728 x 896 4.7 -> 5.6).  The steps' latency
+// bounds it (13 rows: 14.9 MB, 1.9 TB/s), and from 32 rows on the LDS reads of x, 8 KB for 16 rows and a step of a wave.
+// Nothing in the loop branches on a lane: a branch costs 50 registers here, and waits past it take every load for pending.
 template <typename AT, int G, bool ZP, int RT>
 __global__ __launch_bounds__(512) void k_linear_q4_rows(Q4Args a, int32_t pass_rows, int32_t groups_n, int32_t out_f16, int32_t seg,
                                                         float* __restrict__ parts)
 {
     constexpr bool F32 = sizeof(AT) == 4;
     constexpr int R = 16 * RT, PITCH = kQ4Step + 8, NX = F32 ? 2 * RT : RT, PLANE = R * PITCH, BUF = (F32 ? 2 : 1) * PLANE;
+    constexpr int DEPTH = 2;
     extern __shared__ __align__(16) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g4 = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -395,70 +425,85 @@ __global__ __launch_bounds__(512) void k_linear_q4_rows(Q4Args a, int32_t pass_r
     f16* xs = reinterpret_cast<f16*>(smem);                        // [2][planes][R][PITCH]
     float* xinv = reinterpret_cast<float*>(xs + 2 * BUF);          // F32: [2][R]
     Q4Stream<G, ZP> ws(a, reinterpret_cast<char*>(xinv + (F32 ? 2 * R : 0)) + wave * kQ4Tile, lane);
-    typename Q4Stream<G, ZP>::Slot ring[2];
+    typename Q4Stream<G, ZP>::Slot ring[DEPTH];
     const int32_t s0 = blockIdx.z * seg, s1 = s0 + seg < ws.steps ? s0 + seg : ws.steps;  // the split's steps
     const AT* x = (const AT*)a.inp + m0 * a.K;
     const int32_t xrow = F32 ? wave : tid >> 5, xat = F32 ? lane * 4 : (tid & 31) * 8;
     constexpr int XROWS = F32 ? 8 : 16;  // rows the block loads at a time
-    u4 xr[NX];
+    u4 xr[NX];  // x of the next step
+    // rows past the last are the last, values past K the row's last ones, stored as 0 (no branch around the loads, so that
+    // waits count what is in flight)
+    constexpr int XV = 16 / (int)sizeof(AT);  // values a load
     auto load_x = [&](int32_t st) {
-#pragma unroll
-        for (int j = 0; j < NX; j++) {
-            const int32_t m = xrow + XROWS * j, at = st * kQ4Step + xat;
-            xr[j] = u4{};
-            if (m < rows && at < K) xr[j] = *reinterpret_cast<const u4*>(x + (int64_t)m * K + at);
-        }
-    };
-    auto store_x = [&](int buf) {
+        const int32_t at = st * kQ4Step + xat;
 #pragma unroll
         for (int j = 0; j < NX; j++) {
             const int32_t m = xrow + XROWS * j;
-            if (m >= rows) break;
+            xr[j] = *reinterpret_cast<const u4*>(x + (int64_t)(m < rows ? m : rows - 1) * K + (at < K ? at : K - XV));
+        }
+    };
+    auto store_x = [&](int32_t st, int buf) {
+        const bool is = st * kQ4Step + xat < K;
+#pragma unroll
+        for (int j = 0; j < NX; j++) {
+            const int32_t m = xrow + XROWS * j;
             f16* to = xs + buf * BUF + m * PITCH;
-            if constexpr (F32) q4_split(__builtin_bit_cast(f4, xr[j]), lane, to, to + PLANE, xinv + buf * R + m);
-            else *reinterpret_cast<u4*>(to + xat) = q4_order(xr[j]);
+            const u4 v = is ? xr[j] : u4{};
+            if constexpr (F32) q4_split(__builtin_bit_cast(f4, v), lane, to, to + PLANE, xinv + buf * R + m);
+            else *reinterpret_cast<u4*>(to + xat) = q4_order(v);
         }
     };
     int32_t row[RT];                                // rows of the operand past the last are computed and dropped
 #pragma unroll
     for (int r = 0; r < RT; r++) row[r] = (r * 16 + n < rows ? r * 16 + n : rows - 1) * PITCH;
 
+    f4 acc[RT] = {};
+    auto consume = [&](int u) {
+        const int buf = u & 1;
+        ws.put(ring[u]);
+        if constexpr (F32) {
+            f4 part[RT] = {};
+            ws.template step<RT, true>(part, xs + buf * BUF, row, PLANE);
+#pragma unroll
+            for (int r = 0; r < RT; r++) {
+                const f4 inv = *reinterpret_cast<const f4*>(xinv + buf * R + r * 16 + 4 * g4);  // rows past the last: dropped
+#pragma unroll
+                for (int i = 0; i < 4; i++) acc[r][i] = __builtin_fmaf(part[r][i], inv[i], acc[r][i]);
+            }
+        } else {
+            ws.template step<RT, false>(acc, xs + buf * BUF, row, PLANE);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+
     load_x(s0);
+    const float bias = q4_bias(a, n0 + n);
     ws.point(a, n0);
     ws.issue(ring[0], s0);
-    ws.issue(ring[1], s0 + 1);
-    store_x(0);
+    store_x(s0, 0);
     load_x(s0 + 1);
+    ws.issue(ring[1], s0 + 1);
     lds_barrier();
-    f4 acc[RT] = {};
-    for (int32_t st = s0; st < s1; st += 2) {
+    int32_t st = s0;
+    for (; st + DEPTH < s1; st += DEPTH)
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
-            if (u == 1 && st + 1 >= s1) break;
-            ws.put(ring[u]);
-            if constexpr (F32) {
-                f4 part[RT] = {};
-                ws.template step<RT, true>(part, xs + u * BUF, row, PLANE);
+        for (int u = 0; u < DEPTH; u++) {
+            consume(u);
+            ws.issue(ring[u], st + u + DEPTH);
+            store_x(st + u + 1, (u + 1) & 1);
+            load_x(st + u + 2);
+            lds_barrier();
+        }
 #pragma unroll
-                for (int r = 0; r < RT; r++) {
-                    const f4 inv = *reinterpret_cast<const f4*>(xinv + u * R + r * 16 + 4 * g4);  // rows past the last: dropped
-#pragma unroll
-                    for (int i = 0; i < 4; i++) acc[r][i] = __builtin_fmaf(part[r][i], inv[i], acc[r][i]);
-                }
-            } else {
-                ws.template step<RT, false>(acc, xs + u * BUF, row, PLANE);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-            if (st + u + 1 < s1) {
-                ws.issue(ring[u], st + u + 2);
-                store_x(u ^ 1);
-                load_x(st + u + 2);
-                lds_barrier();
-            }
+    for (int u = 0; u < DEPTH; u++) {
+        if (st + u >= s1) break;
+        consume(u);
+        if (st + u + 1 < s1) {
+            store_x(st + u + 1, (u + 1) & 1);
+            lds_barrier();
         }
     }
     if (n0 + n >= a.N) return;
-    const float bias = a.bias ? a.bias[n0 + n] : 0.0f;
 #pragma unroll
     for (int e = 0; e < 4 * RT; e++) {
         const int m = e / 4 * 16 + 4 * g4 + e % 4;
