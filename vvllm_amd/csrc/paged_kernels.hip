@@ -421,6 +421,9 @@ __device__ __forceinline__ void paged_chunks(const PagedArgs& c, const T* kh, co
                 }
         }
         spot = look(c0 + cstep);
+        // all of the chunk's loads before its first product: fp32 heads of 96 30.0 -> 28.0 us (4 contexts of 8000 keys); the others are
+        // as fast either way, or slower for it (fp16 heads of 64, 1000 keys, 8.3 -> 8.9)
+        if constexpr (!H16 && D == 96) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             sc[t] = f4{};
