@@ -198,6 +198,20 @@ def test_an_infinity_next_to_large_values(gpu, M):
 
 
 @pytest.mark.parametrize("act", [F16, F32])
+@pytest.mark.parametrize("M,N,K,group", [(1, 50, 96, 32), (3, 50, 640, 64), (20, 8200, 352, 32), (2, 50, 384, 128)])
+def test_an_infinite_scale_in_the_last_group(gpu, act, M, N, K, group):
+    """Rows that end inside a step: the infinity is met by its own group's sum, not by what is past the row."""
+    c = Case(M, N, K, group, act, F32)
+    c.codes[:] = 0xCC  # every weight above 0
+    c.x = np.abs(c.x) + NP[act](0.1)
+    c.scales[1::2, -1] = np.inf
+    c.d = {n: capi.DevBuf.from_array(a) for n, a in vars(c).items() if isinstance(a, np.ndarray)}
+    c.run()
+    got = c.got()
+    assert (got[:, 1::2] == np.inf).all() and np.isfinite(got[:, ::2]).all()
+
+
+@pytest.mark.parametrize("act", [F16, F32])
 def test_rows_of_a_large_call_are_the_small_calls(gpu, act):
     """Outputs next to the last row and channel stay as they were."""
     c = Case(5, 77, 320, 64, act, act)

@@ -138,20 +138,23 @@ struct Q4Stream {
             if (ZP) r.z[i] = zp[g];
         }
     }
-    __device__ __forceinline__ void put(const Slot& r) const
+    // st: the step in the slot (a group past the row's end has no sum; its scale, the last group's, may be infinite)
+    __device__ __forceinline__ void put(const Slot& r, int32_t st) const
     {
         *reinterpret_cast<u4*>(tile + (lane >> 3) * kQ4WPitch + (lane & 7) * 16) = r.a;
         *reinterpret_cast<u4*>(tile + (8 + (lane >> 3)) * kQ4WPitch + (lane & 7) * 16) = r.b;
 #pragma unroll
         for (int i = 0; i < NS; i++) {
-            uint32_t v = r.s[i];
+            const int g = (g4 * NS + i) % PG;  // two lanes the same where there are fewer groups
+            uint32_t v = st * PG + g < groups ? r.s[i] : 0;
             if (ZP) v |= (uint32_t)__builtin_bit_cast(uint16_t, (f16)(float)r.z[i]) << 16;
-            stile[n * kQ4SPitch + (g4 * NS + i) % PG] = v;  // two lanes the same where there are fewer groups
+            stile[n * kQ4SPitch + g] = v;
         }
         // one wave's LDS accesses complete in order
     }
-    // part[r] += the step's sums; xk: the step's x, whose operand rows are at row[r], TWO: and row[r] + plane
-    template <int RT, bool TWO>
+    // part[r] += the step's sums; xk: the step's x, whose operand rows are at row[r], TWO: and row[r] + plane; FOLD: the two
+    // parts of a row are neighbouring rows of the operand, added before the scale
+    template <int RT, bool TWO, bool FOLD>
     __device__ __forceinline__ void step(f4 (&part)[RT], const f16* xk, const int32_t (&row)[RT], int32_t plane) const
     {
         uint32_t sv[PG];
@@ -184,7 +187,8 @@ struct Q4Stream {
 #pragma unroll
             for (int r = 0; r < RT; r++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) part[r][i] = __builtin_fmaf(s, d[r][i], part[r][i]);
+                for (int i = 0; i < (FOLD ? 2 : 4); i++)
+                    part[r][i] = __builtin_fmaf(s, FOLD ? d[r][2 * i] + d[r][2 * i + 1] : d[r][i], part[r][i]);
             // not all of a step's reads at once: registers
             if ((g + 1) % (PG / 2) == 0) __builtin_amdgcn_sched_barrier(0);
         }
@@ -312,16 +316,16 @@ __global__ __launch_bounds__(512) void k_linear_q4(Q4Args a, Q4Launch L)
     auto consume = [&](int u, int32_t i, bool last) {
         const bool is = !last || i < mine;
         const int32_t st = is ? ks + (i << L.log_ks) : 0;  // within x in LDS
-        ws.put(ring[u]);
+        ws.put(ring[u], s0 + st);
         f4 parts[1] = {};
         const int32_t at[1] = {(FOLD && n & 1 ? plane : 0) + row * pitch};
-        ws.template step<1, F32 && !FOLD>(parts, xs + st * kQ4Step, at, plane);
+        ws.template step<1, F32 && !FOLD, FOLD>(parts, xs + st * kQ4Step, at, plane);
         const f4 part = parts[0];
         f4 to = acc;
         if constexpr (FOLD) {
             const float* inv = xinv + st * kQ4Rows + 2 * g4;
 #pragma unroll
-            for (int j = 0; j < 2; j++) to[j] = __builtin_fmaf(part[2 * j] + part[2 * j + 1], inv[j], acc[j]);
+            for (int j = 0; j < 2; j++) to[j] = __builtin_fmaf(part[j], inv[j], acc[j]);
         } else if constexpr (F32) {
             const f4 inv = *reinterpret_cast<const f4*>(xinv + st * kQ4Rows + 4 * g4);  // rows past the last: dropped
 #pragma unroll
@@ -458,12 +462,12 @@ __global__ __launch_bounds__(512) void k_linear_q4_rows(Q4Args a, int32_t pass_r
     for (int r = 0; r < RT; r++) row[r] = (r * 16 + n < rows ? r * 16 + n : rows - 1) * PITCH;
 
     f4 acc[RT] = {};
-    auto consume = [&](int u) {
+    auto consume = [&](int u, int32_t st) {
         const int buf = u & 1;
-        ws.put(ring[u]);
+        ws.put(ring[u], st);
         if constexpr (F32) {
             f4 part[RT] = {};
-            ws.template step<RT, true>(part, xs + buf * BUF, row, PLANE);
+            ws.template step<RT, true, false>(part, xs + buf * BUF, row, PLANE);
 #pragma unroll
             for (int r = 0; r < RT; r++) {
                 const f4 inv = *reinterpret_cast<const f4*>(xinv + buf * R + r * 16 + 4 * g4);  // rows past the last: dropped
@@ -471,7 +475,7 @@ __global__ __launch_bounds__(512) void k_linear_q4_rows(Q4Args a, int32_t pass_r
                 for (int i = 0; i < 4; i++) acc[r][i] = __builtin_fmaf(part[r][i], inv[i], acc[r][i]);
             }
         } else {
-            ws.template step<RT, false>(acc, xs + buf * BUF, row, PLANE);
+            ws.template step<RT, false, false>(acc, xs + buf * BUF, row, PLANE);
         }
         __builtin_amdgcn_sched_barrier(0);
     };
@@ -488,7 +492,7 @@ __global__ __launch_bounds__(512) void k_linear_q4_rows(Q4Args a, int32_t pass_r
     for (; st + DEPTH < s1; st += DEPTH)
 #pragma unroll
         for (int u = 0; u < DEPTH; u++) {
-            consume(u);
+            consume(u, st + u);
             ws.issue(ring[u], st + u + DEPTH);
             store_x(st + u + 1, (u + 1) & 1);
             load_x(st + u + 2);
@@ -497,7 +501,7 @@ __global__ __launch_bounds__(512) void k_linear_q4_rows(Q4Args a, int32_t pass_r
 #pragma unroll
     for (int u = 0; u < DEPTH; u++) {
         if (st + u >= s1) break;
-        consume(u);
+        consume(u, st + u);
         if (st + u + 1 < s1) {
             store_x(st + u + 1, (u + 1) & 1);
             lds_barrier();
