@@ -254,3 +254,25 @@ def test_quantized_weights(gpu):
     y = c.x.astype(np.float64) @ w.astype(np.float64).T
     # half a step (absmax / 14, at most 0.1 / 14 here) per weight, each of its own sign
     assert np.abs(c.got() - y).max() <= 0.1 / 14 * 6 * np.sqrt(896 / 3)
+
+
+def test_two_streams_at_once(gpu):
+    """Calls that share out k, on two streams without waiting: each stream has a workspace of its own."""
+    cs = [Case(16, 130, 8960, 128, F16, F16), Case(40, 100, 8960, 64, F16, F16, zeros=True), Case(2, 33, 45056, 128, F16, F16)]
+    for c in cs:
+        c.run()
+    want = [c.got() for c in cs]
+    streams = [Stream(), Stream()]
+    outs = [[capi.DevBuf(c.M * c.N * 4) for c in cs] for _ in streams]
+    for st, bufs in zip(streams, outs):  # the streams' workspaces
+        for c, b in zip(cs, bufs):
+            c.run(out=b, stream=st.s)
+    for _ in range(10):
+        for st, bufs in zip(streams, outs):
+            for c, b in zip(cs, bufs):
+                c.run(out=b, stream=st.s)
+    for st, bufs in zip(streams, outs):
+        st.sync()
+        for c, b, w in zip(cs, bufs, want):
+            np.testing.assert_array_equal(c.got(b), w)
+        st.close()
