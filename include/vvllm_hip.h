@@ -587,8 +587,9 @@ VVH_API int vvh_rope_append_paged(const vvh_paged_cache* cache, void* q_out, con
  * entries that are no page are left out; a row without any position gives
  * zeros.  Cache rows that no sequence has reached may hold anything.  Sums and
  * weights are fp32 (products of fp16 values exact), rounded once to the output;
- * an infinite value among the rows attended to gives NaN in its dim.  max_len:
- * the longest length to expect, 0 for unknown (the page table's capacity); it
+ * an infinite value among the rows attended to gives its infinity in its dim, NaN
+ * where it meets one of the other sign or a NaN (also where its weight is below
+ * fp32's range, 2^-126 of the row's largest).  max_len: the longest length to expect, 0 for unknown (the page table's capacity); it
  * steers how the work is split, longer rows are attended in full all the same.
  * Made for head_dim 64, 96 and 128 and 16-byte aligned arrays; others take a
  * slower kernel.  A split's partial sums use the stream's workspace, whose size

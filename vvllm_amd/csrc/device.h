@@ -75,6 +75,14 @@ __device__ __forceinline__ void attn_merge_add(float& num, float& den, float mi,
     den = __builtin_fmaf(f, li, den);
 }
 
+// Waits until at most N loads are in flight.
+template <int N>
+__device__ __forceinline__ void wait_loads()
+{
+    static_assert(N < 64, "vmcnt");
+    __builtin_amdgcn_s_waitcnt((N & 15) | 7 << 4 | 15 << 8 | (N >> 4) << 14);
+}
+
 // LDS reads done (lgkmcnt(0)), then s_barrier, without waiting on vector
 // memory loads.  Written with builtins so the compiler's wait-count tracking
 // sees the lgkmcnt(0); the empty asm with a memory clobber keeps the

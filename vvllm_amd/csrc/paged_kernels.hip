@@ -266,6 +266,11 @@ __global__ __launch_bounds__(1024) void k_attention_paged_any_merge(T* __restric
 // A lane finds the row of key c0 + lane in the page table and hands it to the lanes that
 // load it.  A key past the end or on no page loads row 0 instead; its score becomes
 // -infinity and its value 0, whatever that row holds.
+//
+// Infinite values: inf w is the infinity for a weight above 0 (fp32), but the low part of an fp16 pair is 0 or below it
+// and makes a NaN of it.  A wave whose fp16 sums are not finite therefore looks its values over once more
+// (paged_infinities); all others pay one test of their sums at the end (16 contexts of 4000 keys, 12 heads on 2
+// of 96, 16.8 -> 17.0 us; 96 contexts from 1 to 8192 keys even).
 // ---------------------------------------------------------------------------
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 
@@ -424,6 +429,13 @@ __device__ __forceinline__ void paged_chunks(const PagedArgs& c, const T* kh, co
         // all of the chunk's loads before its first product: fp32 heads of 96 30.0 -> 28.0 us (4 contexts of 8000 keys); the others are
         // as fast either way, or slower for it (fp16 heads of 64, 1000 keys, 8.3 -> 8.9)
         if constexpr (!H16 && D == 96) __builtin_amdgcn_sched_barrier(0);
+        // there the page lookup is on its way first and one wait takes all of K: V and the lookup stay in flight (left to the
+        // scheduler, which now waits fragment by fragment, 8.75 us, so 8.25)
+        if constexpr (H16 && D == 64) {
+            __builtin_amdgcn_sched_barrier(0);
+            wait_loads<CH * D / 512 + 1>();
+            __builtin_amdgcn_sched_barrier(0);
+        }
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             sc[t] = f4{};
@@ -518,6 +530,57 @@ __device__ __forceinline__ void paged_chunks(const PagedArgs& c, const T* kh, co
     }
 }
 
+// The sums of fp16 values that are not finite: each dim's infinities and NaN, whose weights only have to be told from 0
+// (2^-126 of the wave's largest, the exponential's range in fp32); finite sums stay as they are.  qh: the tile's n queries;
+// the rest as paged_chunks.
+template <int D>
+__device__ __forceinline__ void paged_infinities(PagedArgs c, const f16* kh, const f16* vh, int32_t s, const f16* qh, int n,
+                                                 int32_t c0, int32_t cstep, int32_t ke, float scale_log2, PagedAcc<D>& acc)
+{
+    float z = 0.0f;
+#pragma unroll
+    for (int e = 0; e < D / 16; e++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) z = __builtin_fmaf(acc.o[e][i], 0.0f, z);  // 0, or NaN
+    if (__builtin_expect(!__any(z != 0.0f), 1)) return;
+    asm volatile("" : "+s"(c.P), "+s"(c.KVH), "+s"(c.max_pages));  // nothing of this is worked out before the loop above
+    const int lane = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0));
+    constexpr int CH = PagedTile<f16>::CH<D>;
+    const int r = (lane & 15) < n ? lane & 15 : n - 1, gr = lane >> 4;
+    const int64_t kvs = (int64_t)c.KVH * D;
+    f4 sum[D / 16] = {};
+    for (; c0 < ke; c0 += cstep)
+        for (int32_t p = c0; p < c0 + CH && p < ke; p++) {
+            const int64_t row = paged_row(c, s, p);
+            if (row < 0) continue;
+            f4 v[D / 16];  // the lane's values that are not finite, 0 for the others
+            float some = 0.0f;
+#pragma unroll
+            for (int e = 0; e < D / 16; e++) {
+                const h4 a = *reinterpret_cast<const h4*>(vh + row * kvs + 16 * e + 4 * gr);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float b = (float)a[i];
+                    v[e][i] = __builtin_fabsf(b) <= 65504.0f ? 0.0f : b;
+                    some = __builtin_fmaf(v[e][i], 0.0f, some);
+                }
+            }
+            if (!__any(some != 0.0f)) continue;
+            float x = 0.0f;  // the score
+#pragma unroll 4
+            for (int d = gr; d < D; d += 4) x = __builtin_fmaf((float)kh[row * kvs + d], (float)qh[r * D + d], x);
+            const float w = sum_x32(sum_x16(x)) * scale_log2 - acc.m > -126.0f ? 1.0f : 0.0f;
+#pragma unroll
+            for (int e = 0; e < D / 16; e++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) sum[e][i] = __builtin_fmaf(w, v[e][i], sum[e][i]);
+        }
+#pragma unroll
+    for (int e = 0; e < D / 16; e++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc.o[e][i] = sum[e][i] != 0.0f ? sum[e][i] : acc.o[e][i];
+}
+
 // Sequence s's length, as the kernels take it
 __device__ __forceinline__ int32_t paged_len(const PagedArgs& c, const int32_t* lens, int32_t s)
 {
@@ -561,6 +624,8 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attention_paged_one(PagedArgs c,
     acc.clear();
     paged_chunks<T, D, BIG>(c, (const T*)c.kp + g * D, (const T*)c.vp + g * D, s, x, w * CH, NW * CH, len, scale_log2,
                        reinterpret_cast<f16*>(smem + w * VB), lane, acc);
+    if constexpr (sizeof(T) == 2)
+        paged_infinities<D>(c, (const T*)c.kp + g * D, (const T*)c.vp + g * D, s, q + row0 * D, n, w * CH, NW * CH, len, scale_log2, acc);
     __syncthreads();
     float* os = reinterpret_cast<float*>(smem);
     if (gr == 0) {
@@ -682,6 +747,9 @@ __global__ __launch_bounds__(256, 2) void k_attention_paged_split(PagedArgs c, T
         const int64_t end = (int64_t)(ci + cnt) * CH;
         paged_chunks<T, D, BIG>(c, (const T*)c.kp + g * D, (const T*)c.vp + g * D, s, x, ci * CH, CH,
                            end < len ? (int32_t)end : len, scale_log2, reinterpret_cast<f16*>(smem + wb * VB), lane, acc);
+        if constexpr (sizeof(T) == 2)
+            paged_infinities<D>(c, (const T*)c.kp + g * D, (const T*)c.vp + g * D, s, q + row0 * D, nh, ci * CH, CH,
+                                end < len ? (int32_t)end : len, scale_log2, acc);
         if (inside) {
             __syncthreads();
             float* os = reinterpret_cast<float*>(smem);

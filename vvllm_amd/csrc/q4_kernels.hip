@@ -82,14 +82,6 @@ __device__ __forceinline__ h8 q4_codes(uint32_t w, h2 zl, h2 zh, const Q4Masks& 
     return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// Waits until at most N loads are in flight.
-template <int N>
-__device__ __forceinline__ void wait_loads()
-{
-    static_assert(N < 64, "vmcnt");
-    __builtin_amdgcn_s_waitcnt((N & 15) | 7 << 4 | 15 << 8 | (N >> 4) << 14);
-}
-
 // A wave's stream of a tile's weights: 16 channels from n0 on, a step at a time from memory to registers (issue),
 // to its LDS tile (put) and through the matrix instruction (step).
 template <int G, bool ZP>
