@@ -83,6 +83,16 @@ __device__ __forceinline__ void wait_loads()
     __builtin_amdgcn_s_waitcnt((N & 15) | 7 << 4 | 15 << 8 | (N >> 4) << 14);
 }
 
+// Between a wave's writes to LDS and its other lanes' reads of them, and between those reads and the next writes.  The
+// hardware completes one wave's LDS accesses in order; this tells the compiler, which sees no dependence between lanes,
+// to keep them so.  No instruction comes of it.
+__device__ __forceinline__ void wave_lds_order()
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+}
+
 // LDS reads done (lgkmcnt(0)), then s_barrier, without waiting on vector
 // memory loads.  Written with builtins so the compiler's wait-count tracking
 // sees the lgkmcnt(0); the empty asm with a memory clobber keeps the

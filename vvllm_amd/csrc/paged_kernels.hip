@@ -484,14 +484,15 @@ __device__ __forceinline__ void paged_chunks(const PagedArgs& c, const T* kh, co
                 for (int i = 0; i < CH * D / 512; i++)
                     if (!(live >> ((i * 64 + lane) / (D / 8)) & 1)) vr[i] = h8{};
             }
-            // one wave's LDS accesses complete in order: the reads below see these rows,
-            // and the next chunk's writes come after them
+            // the reads below see these rows, and the next chunk's writes come after them
+            wave_lds_order();
 #pragma unroll
             for (int i = 0; i < CH * D / 512; i++) {
                 const int p = i * 64 + lane, j = p / (D / 8), col = p % (D / 8) * 8;
                 *reinterpret_cast<h4*>(vw + j * VP + col) = h4{vr[i][0], vr[i][1], vr[i][2], vr[i][3]};
                 *reinterpret_cast<h4*>(vw + j * VP + col + 4) = h4{vr[i][4], vr[i][5], vr[i][6], vr[i][7]};
             }
+            wave_lds_order();
 #pragma unroll
             for (int u = 0; u < NT / 2; u++) {
                 h8 hi, lo;

@@ -133,6 +133,7 @@ struct Q4Stream {
     // st: the step in the slot (a group past the row's end has no sum; its scale, the last group's, may be infinite)
     __device__ __forceinline__ void put(const Slot& r, int32_t st) const
     {
+        wave_lds_order();  // after the reads of the step before
         *reinterpret_cast<u4*>(tile + (lane >> 3) * kQ4WPitch + (lane & 7) * 16) = r.a;
         *reinterpret_cast<u4*>(tile + (8 + (lane >> 3)) * kQ4WPitch + (lane & 7) * 16) = r.b;
 #pragma unroll
@@ -142,7 +143,7 @@ struct Q4Stream {
             if (ZP) v |= (uint32_t)__builtin_bit_cast(uint16_t, (f16)(float)r.z[i]) << 16;
             stile[n * kQ4SPitch + g] = v;
         }
-        // one wave's LDS accesses complete in order
+        wave_lds_order();
     }
     // part[r] += the step's sums; xk: the step's x, whose operand rows are at row[r], TWO: and row[r] + plane; FOLD: the two
     // parts of a row are neighbouring rows of the operand, added before the scale
@@ -376,6 +377,7 @@ __global__ __launch_bounds__(512) void k_linear_q4(Q4Args a, Q4Launch L)
         }
         // the sums of the tile's waves, through their weight tiles
         if (KS > 1) {
+            wave_lds_order();
             *reinterpret_cast<f4*>(tile + lane * 16) = acc;
             lds_barrier();
             if (ks == 0)
