@@ -607,11 +607,13 @@ VVH_API int vvh_attention_paged(const vvh_paged_cache* cache, void* out, const v
  * are exact; fp16 activations are used as given, fp32 ones to 22 bits of the
  * largest of 256 neighbours in their row; products are summed in fp32 and the
  * epilogue rounds once (as vvh_linear_q8).  Made for the few rows of a decode step:
- * rows are taken 16 or 32 at a time, each time reading the weights again.  Rows of
- * inp too long for a block's shared memory (16 rows over few channels: past 4096
- * fp16 or 1024 fp32 activations) share out k, whose sums use the stream's
- * workspace (splits * M * N floats): make one such call before capturing on the
- * stream. */
+ * rows are taken 16 or 32 at a time, each time reading the weights again.  Where
+ * rows of inp are too long for a block's shared memory, or too few blocks come of
+ * the channels and rows to fill the device, blocks share out k, and their sums use
+ * the stream's workspace (splits * M * N floats, from 5 rows on at most 12 splits).
+ * M, N, K and act_dtype alone decide it: make one call of such sizes before
+ * capturing on the stream.  None is needed for K up to 2816 (fp16 activations;
+ * fp32 1024), and with up to 4 rows for K up to 17152 (fp32 8448). */
 VVH_API int vvh_linear_q4(void* out, const void* inp, const uint8_t* dev_weight, const uint16_t* dev_scales,
                           const uint8_t* dev_zeros, const float* dev_bias, const void* residual, size_t M, size_t N,
                           size_t K, size_t group, int act_dtype, int out_dtype, void* stream);
