@@ -574,7 +574,7 @@ VVH_API int vvh_rope_table(float* table, size_t positions, size_t head_dim, floa
  * even); rope_table NULL stores k as it is, for num_heads = 0 only.  A token whose sequence, position
  * or page is out of range (-1 by convention: the padding of a captured batch)
  * is left out: nothing is read or written for it.  No two tokens of a call
- * may be one row of the cache. */
+ * may be one row of the cache.  Fewer than 2^31 tokens and 2^16 heads. */
 VVH_API int vvh_rope_append_paged(const vvh_paged_cache* cache, void* q_out, const void* q, const void* k,
                                   const void* v, const int32_t* seqs, const int32_t* positions, size_t tokens,
                                   size_t num_heads, const float* rope_table, size_t rope_positions, void* stream);

@@ -910,9 +910,12 @@ int launch_rope_table_theta(float* out, int64_t positions, int64_t D, float thet
     return (int)hipGetLastError();
 }
 
-int launch_rope_append_paged(const PagedArgs& c, void* q_out, const void* q, const void* k, const void* v,
-                             const int32_t* seqs, const int32_t* positions, int64_t tokens, int64_t H,
-                             const float* rope, int64_t rope_positions, int dtype, void* stream)
+// A launch holds fewer than 2^32 threads: at most 2^22 tokens each (of up to 512).
+constexpr int64_t kAppendTokens = int64_t(1) << 22;
+
+static int launch_append_part(const PagedArgs& c, void* q_out, const void* q, const void* k, const void* v,
+                              const int32_t* seqs, const int32_t* positions, int64_t tokens, int64_t H,
+                              const float* rope, int64_t rope_positions, int dtype, void* stream)
 {
     const uintptr_t all = (uintptr_t)q_out | (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)c.kp | (uintptr_t)c.vp | (uintptr_t)rope;
     if (rope && c.D % 16 == 0 && all % 16 == 0) {
@@ -937,6 +940,21 @@ int launch_rope_append_paged(const PagedArgs& c, void* q_out, const void* q, con
     };
     dtype == VVH_F16 ? go(k_rope_append_paged<f16>, (f16*)nullptr) : go(k_rope_append_paged<float>, (float*)nullptr);
     return (int)hipGetLastError();
+}
+
+int launch_rope_append_paged(const PagedArgs& c, void* q_out, const void* q, const void* k, const void* v,
+                             const int32_t* seqs, const int32_t* positions, int64_t tokens, int64_t H,
+                             const float* rope, int64_t rope_positions, int dtype, void* stream)
+{
+    // without seqs token t is sequence t, of fewer than 2^16: one launch
+    const int64_t e = dtype == VVH_F16 ? 2 : 4, qb = H * c.D * e, kvb = (int64_t)c.KVH * c.D * e;
+    for (int64_t t = 0; t < tokens; t += kAppendTokens) {
+        auto at = [&](const void* p, int64_t row) { return p ? (const char*)p + t * row : nullptr; };
+        const int st = launch_append_part(c, (void*)at(q_out, qb), at(q, qb), at(k, kvb), at(v, kvb), seqs ? seqs + t : nullptr,
+                                          positions + t, std::min(tokens - t, kAppendTokens), H, rope, rope_positions, dtype, stream);
+        if (st != 0) return st;
+    }
+    return 0;
 }
 
 
