@@ -603,7 +603,7 @@ VVH_API int vvh_attention_paged(const vvh_paged_cache* cache, void* out, const v
  * bytes, code k in the low (k even) or high (k odd) half of byte k / 2;
  * dev_scales: [N, K / group] fp16 bits; dev_zeros: [N, K / group] bytes, or
  * NULL for 8 everywhere.  group 32, 64 or 128, K a multiple of it (at most
- * 2^24); inp and dev_weight 16-byte aligned, out not inp.  Codes less zero points
+ * 2^24; N at most 2^30 - 1024, M 65535 * 16, M * N 2^40); inp and dev_weight 16-byte aligned, out not inp.  Codes less zero points
  * are exact; fp16 activations are used as given, fp32 ones to 22 bits of the
  * largest of 256 neighbours in their row; products are summed in fp32 and the
  * epilogue rounds once (as vvh_linear_q8).  Made for the few rows of a decode step:

@@ -2439,7 +2439,8 @@ VVH_API int vvh_linear_q4(void* out, const void* inp, const uint8_t* dev_weight,
         (((uintptr_t)out | (uintptr_t)residual) & (dsize(out_dtype) - 1)))
         return fail(VVH_ERR_INVALID_ARG, "misaligned pointer");
     // K: 2^16 steps, so at most 2^15 splits of them and 65535 in a grid; M * N: the splits' sums in 64 bits
-    if (N > INT32_MAX || K > (size_t(1) << 24) || M > 65535 * 16 || M * N > (size_t(1) << 40))
+    // N: 4 threads a channel, fewer than 2^32 in a launch
+    if (N > (size_t(1) << 30) - 1024 || K > (size_t(1) << 24) || M > 65535 * 16 || M * N > (size_t(1) << 40))
         return fail(VVH_ERR_UNSUPPORTED, "M %zu, N %zu, K %zu", M, N, K);
     REQUIRE_INIT();
     const Q4Args a{out, inp, residual, dev_weight, dev_scales, dev_zeros, dev_bias, (int64_t)M, (int64_t)N, (int64_t)K,
