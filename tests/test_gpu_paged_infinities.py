@@ -128,3 +128,26 @@ def test_infinite_values_come_and_go_in_a_graph(gpu):
         else:
             np.testing.assert_array_equal(got, plain)
     st.close()
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("H,KVH,D", [(14, 2, 64), (6, 2, 96), (12, 2, 128), (4, 2, 80)])
+@pytest.mark.parametrize("lens", [[130, 64, 90], [3000, 1500, 700]])
+def test_dims_and_rows_that_overflowed(gpu, dtype, H, KVH, D, lens):
+    """A dim infinite for every key, one of NaN, a sequence whose keys are NaN next to them."""
+    print("[case] overflowed", dtype, H, KVH, D, lens, flush=True)
+    rng = np.random.default_rng(H * D)
+    pg = Pages(rng, lens, 16, KVH, D, dtype)
+    pages = lambda s: pg.table[s, :-(-lens[s] // 16)]  # noqa: E731
+    pg.vp[pages(0), :, 0, 4] = -np.inf
+    pg.vp[pages(0), :, KVH - 1, 9] = np.nan
+    pg.vp[pages(1), ::2, 0, 6] = np.inf
+    pg.kp[pages(2)] = np.nan
+    pg.upload()
+    q = rng.normal(0, 1, (3, H, D)).astype(NP[dtype])
+    scale = float(np.float32(1 / np.sqrt(D)))
+    pg.lens[2] = 0
+    ref, tol = want(pg, q, scale)
+    pg.lens[2] = lens[2]
+    ref[2] = np.nan
+    check(attend(pg, q, scale), ref, tol)

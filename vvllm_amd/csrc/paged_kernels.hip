@@ -268,9 +268,10 @@ __global__ __launch_bounds__(1024) void k_attention_paged_any_merge(T* __restric
 // -infinity and its value 0, whatever that row holds.
 //
 // Infinite values: inf w is the infinity for a weight above 0 (fp32), but the low part of an fp16 pair is 0 or below it
-// and makes a NaN of it.  A wave whose fp16 sums are not finite therefore looks its values over once more
-// (paged_infinities); all others pay one test of their sums at the end (16 contexts of 4000 keys, 12 heads on 2
-// of 96, 16.8 -> 17.0 us; 96 contexts from 1 to 8192 keys even).
+// and makes a NaN of it.  A wave whose fp16 sums are not finite therefore takes its chunks once more (INF), the infinities
+// apart from the pairs, against 1 where the weight is above 0; all others pay one test of their sums at the end (16 contexts of
+// 4000 keys, 12 heads on 2 of 96, 16.7 -> 16.9 us; 96 contexts from 1 to 8192 keys 84.5 -> 85.2).  The second pass costs what
+// the first does (one of 30000 keys 29 -> 47).  A head whose weights' sum is not finite gives NaN without it.
 // ---------------------------------------------------------------------------
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 
@@ -346,8 +347,9 @@ __device__ __forceinline__ constexpr int paged_dim(int e, int gr, int i)
 
 // The chunks c0, c0 + cstep, ... below ke of sequence s.  kh, vh: the kv head's column
 // in the pages; vw: the wave's LDS region (fp16).  BIG: the pages of K or V pass 4 GB, the reach of a
-// buffer load's 32-bit offset, and take 64-bit addresses (16 clocks of multiplication a load).
-template <typename T, int D, bool BIG>
+// buffer load's 32-bit offset, and take 64-bit addresses (16 clocks of multiplication a load).  INF (fp16): infinite values
+// apart.
+template <typename T, int D, bool BIG, bool INF>
 __device__ __forceinline__ void paged_chunks(const PagedArgs& c, const T* kh, const T* vh, int32_t s,
                                              const typename PagedTile<T>::template Q<D>& q, int32_t c0, int32_t cstep,
                                              int32_t ke, float scale_log2, f16* vw, int lane, PagedAcc<D>& acc)
@@ -429,9 +431,9 @@ __device__ __forceinline__ void paged_chunks(const PagedArgs& c, const T* kh, co
         // all of the chunk's loads before its first product: fp32 heads of 96 30.0 -> 28.0 us (4 contexts of 8000 keys); the others are
         // as fast either way, or slower for it (fp16 heads of 64, 1000 keys, 8.3 -> 8.9)
         if constexpr (!H16 && D == 96) __builtin_amdgcn_sched_barrier(0);
-        // there the page lookup is on its way first and one wait takes all of K: V and the lookup stay in flight (left to the
-        // scheduler, which now waits fragment by fragment, 8.75 us, so 8.25)
-        if constexpr (H16 && D == 64) {
+        // the page lookup on its way first and one wait for all of K, while V and the lookup stay in flight: fp16 heads of 64, 1000
+        // keys, 8.3 us, left to the scheduler 8.8
+        if constexpr (H16 && !INF && D == 64) {
             __builtin_amdgcn_sched_barrier(0);
             wait_loads<CH * D / 512 + 1>();
             __builtin_amdgcn_sched_barrier(0);
@@ -495,12 +497,13 @@ __device__ __forceinline__ void paged_chunks(const PagedArgs& c, const T* kh, co
             wave_lds_order();
 #pragma unroll
             for (int u = 0; u < NT / 2; u++) {
-                h8 hi, lo;
+                h8 hi, lo, on;
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     const float w = sc[2 * u + j / 4][j % 4];
                     hi[j] = (f16)w;
                     lo[j] = (f16)(w - (float)hi[j]);
+                    if constexpr (INF) on[j] = (f16)(w > 0.0f ? 1.0f : 0.0f);
                 }
                 // lane (r, gr): V[32 u + 4 gr + j][16 e + r] and the same 16 keys on, j < 4: in each
                 // group of 16 lanes the transposing read gives lane i element i % 4 of lane 4 j + i / 4's
@@ -509,7 +512,17 @@ __device__ __forceinline__ void paged_chunks(const PagedArgs& c, const T* kh, co
                 for (int e = 0; e < DE; e++) {
                     const f16* src = vw + (32 * u + 4 * gr + (r >> 2)) * VP + 16 * e + 4 * (r & 3);
                     const h4 a = lds_tr16(src), b = lds_tr16(src + 16 * VP);
-                    const h8 va = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+                    h8 va = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+                    if constexpr (INF) {
+                        h8 vi;
+#pragma unroll
+                        for (int j = 0; j < 8; j++) {
+                            const bool is = __builtin_fabsf((float)va[j]) == INFINITY;
+                            vi[j] = is ? va[j] : (f16)0.0f;
+                            va[j] = is ? (f16)0.0f : va[j];
+                        }
+                        acc.o[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vi, on, acc.o[e], 0, 0, 0);
+                    }
                     acc.o[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, hi, acc.o[e], 0, 0, 0);
                     acc.o[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, lo, acc.o[e], 0, 0, 0);
                 }
@@ -531,55 +544,28 @@ __device__ __forceinline__ void paged_chunks(const PagedArgs& c, const T* kh, co
     }
 }
 
-// The sums of fp16 values that are not finite: each dim's infinities and NaN, whose weights only have to be told from 0
-// (2^-126 of the wave's largest, the exponential's range in fp32); finite sums stay as they are.  qh: the tile's n queries;
-// the rest as paged_chunks.
-template <int D>
-__device__ __forceinline__ void paged_infinities(PagedArgs c, const f16* kh, const f16* vh, int32_t s, const f16* qh, int n,
-                                                 int32_t c0, int32_t cstep, int32_t ke, float scale_log2, PagedAcc<D>& acc)
+// The chunks, and once more where a sum of the wave is not finite although its weights' sum is
+template <typename T, int D, bool BIG>
+__device__ __forceinline__ void paged_tile(const PagedArgs& c, const T* kh, const T* vh, int32_t s,
+                                           const typename PagedTile<T>::template Q<D>& q, int32_t c0, int32_t cstep,
+                                           int32_t ke, float scale_log2, f16* vw, int lane, PagedAcc<D>& acc)
 {
-    float z = 0.0f;
+    acc.clear();
+    paged_chunks<T, D, BIG, false>(c, kh, vh, s, q, c0, cstep, ke, scale_log2, vw, lane, acc);
+    if constexpr (sizeof(T) == 2) {
+        f4 z = {};  // 0, or NaN; four chains
 #pragma unroll
-    for (int e = 0; e < D / 16; e++)
+        for (int e = 0; e < D / 16; e++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) z = __builtin_fmaf(acc.o[e][i], 0.0f, z);  // 0, or NaN
-    if (__builtin_expect(!__any(z != 0.0f), 1)) return;
-    asm volatile("" : "+s"(c.P), "+s"(c.KVH), "+s"(c.max_pages));  // nothing of this is worked out before the loop above
-    const int lane = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0));
-    constexpr int CH = PagedTile<f16>::CH<D>;
-    const int r = (lane & 15) < n ? lane & 15 : n - 1, gr = lane >> 4;
-    const int64_t kvs = (int64_t)c.KVH * D;
-    f4 sum[D / 16] = {};
-    for (; c0 < ke; c0 += cstep)
-        for (int32_t p = c0; p < c0 + CH && p < ke; p++) {
-            const int64_t row = paged_row(c, s, p);
-            if (row < 0) continue;
-            f4 v[D / 16];  // the lane's values that are not finite, 0 for the others
-            float some = 0.0f;
-#pragma unroll
-            for (int e = 0; e < D / 16; e++) {
-                const h4 a = *reinterpret_cast<const h4*>(vh + row * kvs + 16 * e + 4 * gr);
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float b = (float)a[i];
-                    v[e][i] = __builtin_fabsf(b) <= 65504.0f ? 0.0f : b;
-                    some = __builtin_fmaf(v[e][i], 0.0f, some);
-                }
-            }
-            if (!__any(some != 0.0f)) continue;
-            float x = 0.0f;  // the score
-#pragma unroll 4
-            for (int d = gr; d < D; d += 4) x = __builtin_fmaf((float)kh[row * kvs + d], (float)qh[r * D + d], x);
-            const float w = sum_x32(sum_x16(x)) * scale_log2 - acc.m > -126.0f ? 1.0f : 0.0f;
-#pragma unroll
-            for (int e = 0; e < D / 16; e++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) sum[e][i] = __builtin_fmaf(w, v[e][i], sum[e][i]);
-        }
-#pragma unroll
-    for (int e = 0; e < D / 16; e++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) acc.o[e][i] = sum[e][i] != 0.0f ? sum[e][i] : acc.o[e][i];
+            for (int i = 0; i < 4; i++) z[i] = __builtin_fmaf(acc.o[e][i], 0.0f, z[i]);
+        if (__builtin_expect(!__any((z[0] + z[1]) + (z[2] + z[3]) != 0.0f && acc.l - acc.l == 0.0f), 1)) return;
+        // nothing of this pass is worked out ahead of the first one (16 contexts of 4000 keys of 96 17.1 -> 16.9 us)
+        PagedArgs c2 = c;
+        asm volatile("" : "+s"(c2.P), "+s"(c2.KVH), "+s"(c2.max_pages), "+s"(c2.pages), "+s"(c2.table));
+        const int lane2 = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0));
+        acc.clear();
+        paged_chunks<T, D, BIG, true>(c2, kh, vh, s, q, c0, cstep, ke, scale_log2, vw, lane2, acc);
+    }
 }
 
 // Sequence s's length, as the kernels take it
@@ -622,11 +608,8 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attention_paged_one(PagedArgs c,
     typename PagedTile<T>::template Q<D> x;
     paged_load_q<D>(q + row0 * D, n, lane, x);
     PagedAcc<D> acc;
-    acc.clear();
-    paged_chunks<T, D, BIG>(c, (const T*)c.kp + g * D, (const T*)c.vp + g * D, s, x, w * CH, NW * CH, len, scale_log2,
-                       reinterpret_cast<f16*>(smem + w * VB), lane, acc);
-    if constexpr (sizeof(T) == 2)
-        paged_infinities<D>(c, (const T*)c.kp + g * D, (const T*)c.vp + g * D, s, q + row0 * D, n, w * CH, NW * CH, len, scale_log2, acc);
+    paged_tile<T, D, BIG>(c, (const T*)c.kp + g * D, (const T*)c.vp + g * D, s, x, w * CH, NW * CH, len, scale_log2,
+                          reinterpret_cast<f16*>(smem + w * VB), lane, acc);
     __syncthreads();
     float* os = reinterpret_cast<float*>(smem);
     if (gr == 0) {
@@ -743,14 +726,10 @@ __global__ __launch_bounds__(256, 2) void k_attention_paged_split(PagedArgs c, T
         typename PagedTile<T>::template Q<D> x;
         paged_load_q<D>(q + row0 * D, nh, lane, x);
         PagedAcc<D> acc;
-        acc.clear();
         const int32_t len = __builtin_amdgcn_readfirstlane(paged_len(c, lens, s));
         const int64_t end = (int64_t)(ci + cnt) * CH;
-        paged_chunks<T, D, BIG>(c, (const T*)c.kp + g * D, (const T*)c.vp + g * D, s, x, ci * CH, CH,
-                           end < len ? (int32_t)end : len, scale_log2, reinterpret_cast<f16*>(smem + wb * VB), lane, acc);
-        if constexpr (sizeof(T) == 2)
-            paged_infinities<D>(c, (const T*)c.kp + g * D, (const T*)c.vp + g * D, s, q + row0 * D, nh, ci * CH, CH,
-                                end < len ? (int32_t)end : len, scale_log2, acc);
+        paged_tile<T, D, BIG>(c, (const T*)c.kp + g * D, (const T*)c.vp + g * D, s, x, ci * CH, CH,
+                              end < len ? (int32_t)end : len, scale_log2, reinterpret_cast<f16*>(smem + wb * VB), lane, acc);
         if (inside) {
             __syncthreads();
             float* os = reinterpret_cast<float*>(smem);
