@@ -593,8 +593,8 @@ VVH_API int vvh_rope_append_paged(const vvh_paged_cache* cache, void* q_out, con
  * steers how the work is split, longer rows are attended in full all the same.
  * Made for head_dim 64, 96 and 128 and 16-byte aligned arrays; others take a
  * slower kernel.  A split's partial sums use the stream's workspace, whose size
- * depends only on the cache's sizes, num_heads and max_len: make one such call
- * before capturing on the stream. */
+ * depends only on the cache's sizes and type, num_heads, max_len and whether the
+ * arrays are aligned: make one such call before capturing on the stream. */
 VVH_API int vvh_attention_paged(const vvh_paged_cache* cache, void* out, const void* q, const int32_t* lens,
                                 size_t max_len, size_t num_heads, float scale, void* stream);
 /* Linear of 4-bit weights: out[M,N] = inp[M,K] . W[N,K]^T + bias[N] (+

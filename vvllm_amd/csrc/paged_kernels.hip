@@ -589,7 +589,7 @@ struct PagedHeads {
 };
 
 // One tile of one sequence by one block, its NW waves each every NW-th chunk, merged
-// through LDS: short contexts, in one launch.  4 chats of up to 512 fp16 keys, 14 heads on 2 of 64: 5.6 us, of which a launch
+// through LDS: short contexts, in one launch.  4 chats of up to 512 fp16 keys, 14 heads on 2 of 64: 5.8 us, of which a launch
 // and the round trips for lengths and pages, rows, and the merge; 1.1 MB is not what bounds it.
 template <typename T, int D, int NW, bool BIG>
 __global__ __launch_bounds__(64 * NW, 2) void k_attention_paged_one(PagedArgs c, T* __restrict__ out, const T* __restrict__ q,
@@ -669,8 +669,8 @@ __device__ __forceinline__ uint64_t muldiv(uint64_t a, uint64_t b, uint64_t c)
 // straight to out if it is the whole tile, else to the wave's slot 1 (a tile that
 // begins in its range) or 0, a row per head: O, m, l.  Where all four waves of a block are in one tile,
 // their parts are added through LDS and go to the first one's slot.  k_attention_paged_merge joins what there is.
-// With the merge: 96 contexts from 1 to 8192 fp16 keys, 32 heads on 8 of 128, 373 MB in 84 us, 4.4 TB/s; 32 of 4096, 8 heads on
-// 8, 537 MB in 105 us, 5.1 TB/s; 3 of up to 30001 fp32 keys, 12 heads on 2, 153 MB in 41 us, 3.7 TB/s.  Bound by HBM; about 7
+// With the merge: 96 contexts from 1 to 8192 fp16 keys, 32 heads on 8 of 128, 373 MB in 85 us, 4.4 TB/s; 32 of 4096, 8 heads on
+// 8, 537 MB in 101 us, 5.3 TB/s; 3 of up to 30001 fp32 keys, 12 heads on 2, 153 MB in 41 us, 3.7 TB/s.  Bound by HBM; about 7
 // us of the first and last are the merge's launch and round trips.
 template <typename T, int D, bool BIG>
 __global__ __launch_bounds__(256, 2) void k_attention_paged_split(PagedArgs c, T* __restrict__ out, const T* __restrict__ q,

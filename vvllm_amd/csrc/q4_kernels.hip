@@ -31,9 +31,11 @@ namespace {
 // puts the step's largest |x| into [2^14, 2^15) (22 bits; the sum of a step is multiplied back).  Up to 8 such
 // rows make 16 rows of the operand (FOLD): one instruction then takes both parts.
 //
-// One fp32 row of 151936 x 896 in groups of 32, 78 MB: 22 us, 3.5 TB/s; fp16 in groups of 128, 70 MB, 19, 3.7 TB/s; one
-// fp16 row of 28672 x 8192, 121 MB, 29.6 us, 4.1 TB/s: bound by HBM and, beside it, the LDS round trips of the codes.  One fp16
-// row of 896 x 896: 3.0 us, a launch and two round trips.  Loading the codes straight into the instruction's
+// One fp32 row of 151936 x 896 in groups of 32, 78 MB: 21.3 us, 3.65 TB/s; fp16 in groups of 128, 70 MB, 17.3, 4.1 TB/s; one
+// fp16 row of 28672 x 8192, 121 MB, 29.4 us, 4.1 TB/s: bound by HBM and, beside it, the LDS round trips of the codes.  One fp16
+// row of 896 x 896: 3.0 us, a launch and two round trips, which one of 17920 x 1536, 14.3 MB, has before and behind its stream:
+// 6.3 us.  Rings of 3 and 4 steps: 24.2 and 25.9 us on the first, 28.7 and 28.1 on the third, 8 rows of 9728 x 896 4.8 -> 5.1 and
+// 5.4.  Loading the codes straight into the instruction's
 // layout (16 pieces of 64 bytes a load, dwords exchanged between lanes) instead of through LDS: 24 -> 29 us on the first.
 // ---------------------------------------------------------------------------
 constexpr int kQ4Step = 256;     // codes of a row a step
@@ -557,7 +559,10 @@ Q4Plan linear_q4_plan(const Q4Args& a, int act, int64_t cus)
     const int64_t parts = std::min<int64_t>({(cus * 5 / 8 + groups * n16 - 1) / (groups * n16), 12, steps});
     // where the blocks of 8 tiles fill half the device and there are rows to share the codes
     if (a.M > (f32 ? 8 : 4) && groups * n16 >= cus / 2) {
-        if (parts > 1 && steps >= 12) return stepwise(16, parts);  // 64 rows of 4000 x 4096 16.7 -> 13.1 us
+        // k in two from 12 steps on, where the second launch is made up for: 16 rows of 16384 channels, whole and shared, 6 steps 7.5
+        // and 8.9 us, 11 steps 11.15 and 11.27, 14 steps 13.1 and 11.9, 20 steps 17.6 and 14.1; 64 rows of 4000 the same but 11 steps
+        // 11.0 and 10.7
+        if (parts > 1 && steps >= 12) return stepwise(16, parts);
         // passes of 16 or 32 rows, by the blocks a CU takes and what these cost (17920 x 1536: 1, 2, 3 of 16 rows 8.0, 11.7,
         // 15.5 us; 1, 2 of 32 rows 9.3, 14.7); fp32 x of 32 rows leaves a CU one block (19.6 us, of 16 18.6)
         const int64_t c16 = (groups * n16 + cus - 1) / cus, c32 = (groups * n32 + cus - 1) / cus;
@@ -567,6 +572,9 @@ Q4Plan linear_q4_plan(const Q4Args& a, int act, int64_t cus)
     p.ks = 1;
     p.waves = 8;
     p.seg = std::max<int64_t>(2, steps);
+    // 5 to 16 fp32 rows up to 96 KB: a block that needs more has a CU for itself (16 rows of 1536 x 1536, 121 KB, 9.1 us, a step at a
+    // time 6.8); below it whole is faster or even (6 rows of 1536 x 1792, 67 KB, 5.7 and 6.8; 16 of 1536 x 768, 73 KB, 6.3 and 6.7;
+    // 16 of 1536 x 1024, 89 KB, 7.0 and 6.2)
     const int64_t most = f32 && rows > 4 ? 96 * 1024 : kQ4Lds;
     while (q4_lds(p, rows, f32) > most) {
         p.splits++;
