@@ -589,8 +589,9 @@ VVH_API int vvh_rope_append_paged(const vvh_paged_cache* cache, void* q_out, con
  * weights are fp32 (products of fp16 values exact), rounded once to the output;
  * an infinite value among the rows attended to gives its infinity in its dim, NaN
  * where it meets one of the other sign or a NaN (also where its weight is below
- * fp32's range, 2^-126 of the row's largest).  max_len: the longest length to expect, 0 for unknown (the page table's capacity); it
- * steers how the work is split, longer rows are attended in full all the same.
+ * fp32's range, 2^-126 of the row's largest).  max_len: the longest length to
+ * expect, 0 for unknown (the page table's capacity); it steers how the work is
+ * split, longer rows are attended in full all the same.
  * Made for head_dim 64, 96 and 128 and 16-byte aligned arrays; others take a
  * slower kernel.  A split's partial sums use the stream's workspace, whose size
  * depends only on the cache's sizes and type, num_heads, max_len and whether the
@@ -603,11 +604,12 @@ VVH_API int vvh_attention_paged(const vvh_paged_cache* cache, void* out, const v
  * bytes, code k in the low (k even) or high (k odd) half of byte k / 2;
  * dev_scales: [N, K / group] fp16 bits; dev_zeros: [N, K / group] bytes, or
  * NULL for 8 everywhere.  group 32, 64 or 128, K a multiple of it (at most
- * 2^24; N at most 2^30 - 1024, M 65535 * 16, M * N 2^40); inp and dev_weight 16-byte aligned, out not inp.  Codes less zero points
- * are exact; fp16 activations are used as given, fp32 ones to 22 bits of the
- * largest of 256 neighbours in their row; products are summed in fp32 and the
- * epilogue rounds once (as vvh_linear_q8).  Made for the few rows of a decode step:
- * rows are taken 16 or 32 at a time, each time reading the weights again.  Where
+ * 2^24; N at most 2^30 - 1024, M 65535 * 16, M * N 2^40); inp and dev_weight
+ * 16-byte aligned, out not inp.  Codes less zero points are exact; fp16
+ * activations are used as given, fp32 ones to 22 bits of the largest of 256
+ * neighbours in their row; products are summed in fp32 and the epilogue rounds
+ * once (as vvh_linear_q8).  Made for the few rows of a decode step: rows are
+ * taken 16 or 32 at a time, each time reading the weights again.  Where
  * rows of inp are too long for a block's shared memory, or too few blocks come of
  * the channels and rows to fill the device, blocks share out k, and their sums use
  * the stream's workspace (splits * M * N floats, from 5 rows on at most 12 splits).

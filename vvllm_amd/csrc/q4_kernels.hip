@@ -573,7 +573,7 @@ Q4Plan linear_q4_plan(const Q4Args& a, int act, int64_t cus)
     p.waves = 8;
     p.seg = std::max<int64_t>(2, steps);
     // 5 to 16 fp32 rows up to 96 KB: a block that needs more has a CU for itself (16 rows of 1536 x 1536, 121 KB, 9.1 us, a step at a
-    // time 6.8); below it whole is faster or even (6 rows of 1536 x 1792, 67 KB, 5.7 and 6.8; 16 of 1536 x 768, 73 KB, 6.3 and 6.7;
+    // time 6.8); below it whole is faster for most (6 rows of 1536 x 1792, 67 KB, 5.7 and 6.8; 16 of 1536 x 768, 73 KB, 6.3 and 6.7;
     // 16 of 1536 x 1024, 89 KB, 7.0 and 6.2)
     const int64_t most = f32 && rows > 4 ? 96 * 1024 : kQ4Lds;
     while (q4_lds(p, rows, f32) > most) {
