@@ -598,6 +598,54 @@ VVH_API int vvh_rope_append_paged(const vvh_paged_cache* cache, void* q_out, con
  * arrays are aligned: make one such call before capturing on the stream. */
 VVH_API int vvh_attention_paged(const vvh_paged_cache* cache, void* out, const void* q, const int32_t* lens,
                                 size_t max_len, size_t num_heads, float scale, void* stream);
+/* A paged cache held in 8 or 4 bits a value, keys and values apart (no counterpart in the reference).  Positions and
+ * pages are those of vvh_paged_cache, but a kv head's rows of a page lie together.  Each group of `group` dims of a row
+ * keeps a minimum m and a scale s in fp16, and its values as codes c of `bits` bits that stand for m + s c:
+ *   m = fp16(min x), s = fp16(fp32((max x - m) / (2^bits - 1))), both within +-65504,
+ *   c = the nearest whole number to (x - m) / s (the even one of two) within 0 .. 2^bits - 1, 0 where s is 0.
+ * A value within fp16's range is off by at most s / 2 and what the roundings of m and s leave out.  A group that has a NaN
+ * or an infinity is stored as NaN in all its dims (scale and minimum NaN).
+ * Rows of codes: 4-bit code d of values is in the low (d even) or high (d odd) half of byte d / 2, 8-bit code d byte d.
+ * Keys' rows have their units of 8 dims in another order, unit 4 j + i (dims 32 j + 8 i on) at place i * (head_dim / 32) +
+ * j, so that a lane group of the attention kernel loads its dims of all 32-dim steps as one piece.
+ * (vvllm_amd.capi: pack_paged_q and unpack_paged_q on the host.) */
+typedef struct vvh_paged_cache_q {
+    void* k_pages;             /* device, [num_pages, num_kv_heads, page_size, head_dim * k_bits / 8] bytes */
+    void* v_pages;             /* device, [num_pages, num_kv_heads, page_size, head_dim * v_bits / 8] bytes */
+    void* k_scales;            /* device, [num_pages, num_kv_heads, page_size, head_dim / group] of {s, m}, fp16 each */
+    void* v_scales;            /* the same */
+    const int32_t* page_table; /* device, [num_seqs, max_pages], as in vvh_paged_cache */
+    uint64_t num_pages;
+    uint64_t page_size;        /* a multiple of 16 (num_pages * page_size < 2^31) */
+    uint64_t num_seqs;         /* < 65536 */
+    uint64_t max_pages;        /* max_pages * page_size <= 2^29 */
+    uint64_t num_kv_heads;
+    uint64_t head_dim;         /* 64, 96 or 128 */
+    uint64_t group;            /* 32, 64 or 128, head_dim a multiple of it */
+    int32_t k_bits, v_bits;    /* 4 or 8; k_bits >= v_bits (keys suffer more from few bits) */
+    int32_t dtype;             /* VVH_F32 or VVH_F16: queries, keys and values given, and outputs */
+} vvh_paged_cache_q;
+/* Arrays of the three calls below are 16-byte aligned, but for page tables, sequences, positions and lengths. */
+
+/* vvh_rope_append_paged into a cache of codes: the same tokens, rotation of q, and tokens left out.  A key is rotated with
+ * one rounding to fp32 (x0 cos - x1 sin and x1 cos + x0 sin), and its groups' codes are worked out from that; a value's
+ * from the value given.  Both are exact: equal to the formulas above in 64 bits.  rope_table NULL, for num_heads = 0 only,
+ * takes k as it is.  No two tokens of a call may be one row of the cache. */
+VVH_API int vvh_rope_append_paged_q(const vvh_paged_cache_q* cache, void* q_out, const void* q, const void* k,
+                                    const void* v, const int32_t* seqs, const int32_t* positions, size_t tokens,
+                                    size_t num_heads, const float* rope_table, size_t rope_positions, void* stream);
+/* Rows of the cache as the values that they stand for: row t of k_out and v_out [tokens, num_kv_heads, head_dim] (either
+ * may be NULL) from position positions[t] of sequence seqs[t] (seqs NULL: sequence t); m + s c in fp32, rounded to dtype.
+ * A token whose sequence, position or page is out of range leaves its rows as they are.  With the positions of a
+ * sequence in order, vvh_attention then takes the rows: several queries, such as a prompt's next part. */
+VVH_API int vvh_read_paged_q(const vvh_paged_cache_q* cache, void* k_out, void* v_out, const int32_t* seqs,
+                             const int32_t* positions, size_t tokens, void* stream);
+/* vvh_attention_paged over a cache of codes: one query per sequence, lengths, positions without a page, rows without a
+ * position and max_len as there.  Queries are used as given (fp32 ones to 22 bits of their row's largest), products
+ * with codes are exact, sums and weights fp32, rounded once to the output.  Rows of the cache that no sequence has reached
+ * may hold anything.  A NaN group of a key makes its heads' rows NaN, one of a value its dims. */
+VVH_API int vvh_attention_paged_q(const vvh_paged_cache_q* cache, void* out, const void* q, const int32_t* lens,
+                                  size_t max_len, size_t num_heads, float scale, void* stream);
 /* Linear of 4-bit weights: out[M,N] = inp[M,K] . W[N,K]^T + bias[N] (+
  * residual[M,N], may alias out), W[n][k] = (c - z) * scales[n][k / group] with
  * the code c of 4 bits and its group's zero point z.  dev_weight: rows of K / 2

@@ -30,8 +30,8 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 CXX = os.environ.get("CXX", "g++")
 
 HIP_SOURCES = ["runtime.hip", "linear_kernels.hip", "gemv_kernels.hip", "gemm_kernels.hip", "model_kernels.hip",
-               "attention_kernels.hip", "dense_kernels.hip", "paged_kernels.hip", "q4_kernels.hip", "logits_kernels.hip",
-               "aux_kernels.hip"]
+               "attention_kernels.hip", "dense_kernels.hip", "paged_kernels.hip", "paged_q_kernels.hip",
+               "q4_kernels.hip", "logits_kernels.hip", "aux_kernels.hip"]
 HIP_FLAGS = [
     "--offload-arch=gfx950",
     "-O3",

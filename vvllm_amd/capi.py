@@ -41,6 +41,13 @@ class PagedCache(ctypes.Structure):
                 ("head_dim", c_uint64), ("dtype", ctypes.c_int32)]
 
 
+class PagedCacheQ(ctypes.Structure):
+    _fields_ = [("k_pages", c_void_p), ("v_pages", c_void_p), ("k_scales", c_void_p), ("v_scales", c_void_p),
+                ("page_table", c_void_p), ("num_pages", c_uint64), ("page_size", c_uint64), ("num_seqs", c_uint64),
+                ("max_pages", c_uint64), ("num_kv_heads", c_uint64), ("head_dim", c_uint64), ("group", c_uint64),
+                ("k_bits", ctypes.c_int32), ("v_bits", ctypes.c_int32), ("dtype", ctypes.c_int32)]
+
+
 class LogitsRules(ctypes.Structure):
     _fields_ = [("tokens", c_void_p), ("token_stride", c_uint64), ("token_counts", c_void_p),
                 ("prompt_counts", c_void_p), ("repetition", c_void_p), ("frequency", c_void_p), ("presence", c_void_p),
@@ -129,6 +136,11 @@ SIGNATURES = {
                                       c_size_t, c_size_t, c_void_p, c_size_t, c_void_p]),
     "vvh_attention_paged": (c_int, [POINTER(PagedCache), c_void_p, c_void_p, c_void_p, c_size_t, c_size_t, c_float,
                                     c_void_p]),
+    "vvh_rope_append_paged_q": (c_int, [POINTER(PagedCacheQ), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                        c_size_t, c_size_t, c_void_p, c_size_t, c_void_p]),
+    "vvh_read_paged_q": (c_int, [POINTER(PagedCacheQ), c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "vvh_attention_paged_q": (c_int, [POINTER(PagedCacheQ), c_void_p, c_void_p, c_void_p, c_size_t, c_size_t, c_float,
+                                      c_void_p]),
     "vvh_linear_q4": (c_int, [c_void_p] * 7 + [c_size_t] * 4 + [c_int, c_int, c_void_p]),
     "vvh_logits_rules": (c_int, [c_void_p, c_void_p, POINTER(LogitsRules), c_size_t, c_size_t, c_int, c_void_p]),
 }
@@ -273,6 +285,40 @@ def quantize_q4(w: np.ndarray, group: int) -> tuple[np.ndarray, np.ndarray]:
     q = np.divide(g, s, out=np.zeros_like(g), where=s > 0)
     c = (8 + np.clip(np.rint(q), -8, 7)).astype(np.uint8).reshape(n, k)
     return c[:, 0::2] | c[:, 1::2] << 4, scales
+
+
+def _unit_order(codes: np.ndarray, keys: bool, back: bool = False) -> np.ndarray:
+    """Codes [..., head_dim] in the order of a page row: keys' units of 8 dims by (unit of a 32-dim step, step)."""
+    if not keys:
+        return codes
+    steps = codes.shape[-1] // 32
+    shape = (4, steps, 8) if back else (steps, 4, 8)
+    return codes.reshape(codes.shape[:-1] + shape).swapaxes(-3, -2).reshape(codes.shape)
+
+
+def pack_paged_q(x: np.ndarray, bits: int, group: int, keys: bool) -> tuple[np.ndarray, np.ndarray]:
+    """Rows x [..., head_dim] of keys (rotated) or values as a vvh_paged_cache_q holds them, with the codes that
+    vvh_rope_append_paged_q gives them: (page rows [..., head_dim * bits / 8] uint8, {scale, minimum} [..., head_dim /
+    group, 2] fp16)."""
+    top = 2 ** bits - 1
+    with np.errstate(over="ignore", invalid="ignore", divide="ignore"):
+        g = np.asarray(x, np.float32).reshape(x.shape[:-1] + (x.shape[-1] // group, group)).astype(np.float64)
+        fine = np.isfinite(g).all(-1)
+        m = np.clip(g.min(-1), -65504, 65504).astype(np.float32).astype(np.float16)
+        s = np.clip((g.max(-1) - m) / top, -65504, 65504).astype(np.float32).astype(np.float16)
+        m, s = (np.where(fine, a, np.float16(np.nan)) for a in (m, s))
+        level = (g - m[..., None].astype(np.float64)) / s[..., None].astype(np.float64)
+    c = np.where(fine[..., None] & (s != 0)[..., None], np.clip(np.rint(level), 0, top), 0).astype(np.uint8).reshape(x.shape)
+    c = _unit_order(c, keys)
+    return (c if bits == 8 else c[..., 0::2] | c[..., 1::2] << 4), np.stack([s, m], -1)
+
+
+def unpack_paged_q(held: np.ndarray, scales: np.ndarray, bits: int, keys: bool) -> np.ndarray:
+    """What page rows [..., bytes] with scales [..., groups, 2] stand for, minimum + scale * code, in 64 bits."""
+    c = held if bits == 8 else np.stack([held & 15, held >> 4], -1).reshape(held.shape[:-1] + (2 * held.shape[-1],))
+    c = _unit_order(c, keys, back=True).astype(np.float64)
+    s = np.repeat(scales.astype(np.float64), c.shape[-1] // scales.shape[-2], axis=-2)
+    return s[..., 1] + s[..., 0] * c
 
 
 def plan_kernel(plan: int) -> str:

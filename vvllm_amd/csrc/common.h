@@ -431,6 +431,24 @@ AttnPagedPlan attention_paged_plan(const PagedArgs& c, const void* q, int64_t ma
 int launch_attention_paged(const AttnPagedPlan& p, const PagedArgs& c, void* out, const void* q, const int32_t* lens, int64_t H,
                            float scale, float* ws, int dtype, void* stream);
 
+// Paged cache of 8- and 4-bit codes (paged_q_kernels.hip): pages [pages, KVH, P] of rows of D kb / 8 (vb / 8) bytes, and
+// their groups' {scale, minimum}, fp16 each, [pages, KVH, P, D / group]
+struct PagedQArgs {
+    uint8_t* kp;
+    uint8_t* vp;
+    uint32_t* ks;
+    uint32_t* vs;
+    const int32_t* table;  // [B, max_pages]
+    int32_t pages, P, B, max_pages, KVH, D, group, kb, vb;
+};
+int launch_rope_append_paged_q(const PagedQArgs& c, void* q_out, const void* q, const void* k, const void* v,
+                               const int32_t* seqs, const int32_t* positions, int64_t tokens, int64_t H, const float* rope,
+                               int64_t rope_positions, int dtype, void* stream);
+int launch_read_paged_q(const PagedQArgs& c, void* k_out, void* v_out, const int32_t* seqs, const int32_t* positions,
+                        int64_t tokens, int dtype, void* stream);
+int launch_attention_paged_q(const PagedQArgs& c, void* out, const void* q, const int32_t* lens, int64_t H, float scale,
+                             int dtype, void* stream);
+
 // 4-bit linear (q4_kernels.hip)
 struct Q4Args {
     void* out;

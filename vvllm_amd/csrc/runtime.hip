@@ -2423,6 +2423,96 @@ VVH_API int vvh_attention_paged(const vvh_paged_cache* cache, void* out, const v
                       "paged attention launch");
 }
 
+// The checks of a paged cache of codes, and its form for the launchers.
+static int paged_q_args(const vvh_paged_cache_q* c, PagedQArgs* a)
+{
+    if (!c) return fail(VVH_ERR_INVALID_ARG, "cache is null");
+    if (!act_ok(c->dtype)) return fail(VVH_ERR_INVALID_ARG, "bad dtype");
+    if (!c->k_pages || !c->v_pages || !c->k_scales || !c->v_scales || !c->page_table)
+        return fail(VVH_ERR_INVALID_ARG, "null pointer");
+    if ((c->k_bits != 4 && c->k_bits != 8) || (c->v_bits != 4 && c->v_bits != 8))
+        return fail(VVH_ERR_INVALID_ARG, "keys of %d and values of %d bits, not 4 or 8", c->k_bits, c->v_bits);
+    if (c->k_bits < c->v_bits) return fail(VVH_ERR_UNSUPPORTED, "keys in fewer bits than values");
+    if (c->page_size == 0 || c->num_pages == 0 || c->max_pages == 0 || c->page_size % 16 != 0)
+        return fail(VVH_ERR_INVALID_ARG, "a cache of codes has pages of whole 16 rows");
+    if (c->num_kv_heads == 0 || c->head_dim == 0) return fail(VVH_ERR_INVALID_ARG, "no kv heads or head_dim 0");
+    if (c->head_dim != 64 && c->head_dim != 96 && c->head_dim != 128)
+        return fail(VVH_ERR_UNSUPPORTED, "codes of head_dim %llu, not 64, 96 or 128", (unsigned long long)c->head_dim);
+    if ((c->group != 32 && c->group != 64 && c->group != 128) || c->head_dim % c->group != 0)
+        return fail(VVH_ERR_INVALID_ARG, "groups of %llu of head_dim %llu", (unsigned long long)c->group,
+                    (unsigned long long)c->head_dim);
+    if (c->num_pages > INT32_MAX || c->page_size > INT32_MAX / c->num_pages ||
+        c->max_pages > (uint64_t(1) << 29) / c->page_size || c->num_seqs > 65535 || c->num_kv_heads > 65535)
+        return fail(VVH_ERR_UNSUPPORTED, "a cache of 2^31 rows, more than 2^29 positions a sequence, 65536 sequences or kv heads");
+    if (!aligned16(c->k_pages) || !aligned16(c->v_pages) || !aligned16(c->k_scales) || !aligned16(c->v_scales) ||
+        ((uintptr_t)c->page_table & 3))
+        return fail(VVH_ERR_INVALID_ARG, "misaligned pointer");
+    *a = PagedQArgs{(uint8_t*)c->k_pages, (uint8_t*)c->v_pages, (uint32_t*)c->k_scales, (uint32_t*)c->v_scales, c->page_table,
+                    (int32_t)c->num_pages, (int32_t)c->page_size, (int32_t)c->num_seqs, (int32_t)c->max_pages,
+                    (int32_t)c->num_kv_heads, (int32_t)c->head_dim, (int32_t)c->group, c->k_bits, c->v_bits};
+    return VVH_OK;
+}
+
+VVH_API int vvh_rope_append_paged_q(const vvh_paged_cache_q* cache, void* q_out, const void* q, const void* k, const void* v,
+                                    const int32_t* seqs, const int32_t* positions, size_t tokens, size_t num_heads,
+                                    const float* rope_table, size_t rope_positions, void* stream)
+{
+    PagedQArgs a;
+    const int st = paged_q_args(cache, &a);
+    if (st != VVH_OK || tokens == 0) return st;
+    if (!k || !v || !positions || (num_heads && (!q || !q_out))) return fail(VVH_ERR_INVALID_ARG, "null pointer");
+    if (!seqs && tokens > cache->num_seqs)
+        return fail(VVH_ERR_INVALID_ARG, "%zu tokens of %llu sequences without seqs", tokens, (unsigned long long)cache->num_seqs);
+    if (!rope_table && num_heads != 0) return fail(VVH_ERR_INVALID_ARG, "queries without a rope table");
+    if (tokens > INT32_MAX || num_heads > 65535) return fail(VVH_ERR_UNSUPPORTED, "%zu tokens, %zu heads", tokens, num_heads);
+    if (!aligned16(q) || !aligned16(q_out) || !aligned16(k) || !aligned16(v) || !aligned16(rope_table) ||
+        (((uintptr_t)seqs | (uintptr_t)positions) & 3))
+        return fail(VVH_ERR_INVALID_ARG, "misaligned pointer");
+    REQUIRE_INIT();
+    return ret_launch(launch_rope_append_paged_q(a, q_out, q, k, v, seqs, positions, (int64_t)tokens, (int64_t)num_heads,
+                                                 rope_table, (int64_t)std::min(rope_positions, (size_t)INT32_MAX),
+                                                 cache->dtype, stream),
+                      "append to a paged cache of codes");
+}
+
+VVH_API int vvh_read_paged_q(const vvh_paged_cache_q* cache, void* k_out, void* v_out, const int32_t* seqs,
+                             const int32_t* positions, size_t tokens, void* stream)
+{
+    PagedQArgs a;
+    const int st = paged_q_args(cache, &a);
+    if (st != VVH_OK || tokens == 0) return st;
+    if ((!k_out && !v_out) || !positions) return fail(VVH_ERR_INVALID_ARG, "null pointer");
+    if (k_out == v_out) return fail(VVH_ERR_INVALID_ARG, "k_out is v_out");
+    if (!seqs && tokens > cache->num_seqs)
+        return fail(VVH_ERR_INVALID_ARG, "%zu tokens of %llu sequences without seqs", tokens, (unsigned long long)cache->num_seqs);
+    if (tokens > INT32_MAX) return fail(VVH_ERR_UNSUPPORTED, "%zu tokens", tokens);
+    if (!aligned16(k_out) || !aligned16(v_out) || (((uintptr_t)seqs | (uintptr_t)positions) & 3))
+        return fail(VVH_ERR_INVALID_ARG, "misaligned pointer");
+    REQUIRE_INIT();
+    return ret_launch(launch_read_paged_q(a, k_out, v_out, seqs, positions, (int64_t)tokens, cache->dtype, stream),
+                      "read of a paged cache of codes");
+}
+
+VVH_API int vvh_attention_paged_q(const vvh_paged_cache_q* cache, void* out, const void* q, const int32_t* lens,
+                                  size_t max_len, size_t num_heads, float scale, void* stream)
+{
+    PagedQArgs a;
+    const int st = paged_q_args(cache, &a);
+    if (st != VVH_OK) return st;
+    if (num_heads % cache->num_kv_heads != 0)
+        return fail(VVH_ERR_INVALID_ARG, "num_heads %zu not a multiple of num_kv_heads %llu", num_heads,
+                    (unsigned long long)cache->num_kv_heads);
+    if (cache->num_seqs == 0 || num_heads == 0) return VVH_OK;
+    if (!out || !q || !lens) return fail(VVH_ERR_INVALID_ARG, "null pointer");
+    if (out == q) return fail(VVH_ERR_INVALID_ARG, "out is q");
+    if (num_heads > 65535) return fail(VVH_ERR_UNSUPPORTED, "%zu heads", num_heads);
+    if (!aligned16(q) || !aligned16(out) || ((uintptr_t)lens & 3)) return fail(VVH_ERR_INVALID_ARG, "misaligned pointer");
+    REQUIRE_INIT();
+    (void)max_len;
+    return ret_launch(launch_attention_paged_q(a, out, q, lens, (int64_t)num_heads, scale, cache->dtype, stream),
+                      "attention over a paged cache of codes");
+}
+
 VVH_API int vvh_linear_q4(void* out, const void* inp, const uint8_t* dev_weight, const uint16_t* dev_scales,
                           const uint8_t* dev_zeros, const float* dev_bias, const void* residual, size_t M, size_t N,
                           size_t K, size_t group, int act_dtype, int out_dtype, void* stream)
