@@ -446,8 +446,9 @@ int launch_rope_append_paged_q(const PagedQArgs& c, void* q_out, const void* q, 
                                int64_t rope_positions, int dtype, void* stream);
 int launch_read_paged_q(const PagedQArgs& c, void* k_out, void* v_out, const int32_t* seqs, const int32_t* positions,
                         int64_t tokens, int dtype, void* stream);
-int launch_attention_paged_q(const PagedQArgs& c, void* out, const void* q, const int32_t* lens, int64_t H, float scale,
-                             int dtype, void* stream);
+AttnPagedPlan attention_paged_q_plan(const PagedQArgs& c, int64_t max_len, int64_t H, int64_t cus);
+int launch_attention_paged_q(const AttnPagedPlan& p, const PagedQArgs& c, void* out, const void* q, const int32_t* lens, int64_t H,
+                             float scale, float* ws, int dtype, void* stream);
 
 // 4-bit linear (q4_kernels.hip)
 struct Q4Args {

@@ -9,6 +9,7 @@
 
 #include "common.h"
 #include "device.h"
+#include "paged_split.h"
 
 namespace vvh {
 
@@ -168,60 +169,335 @@ __global__ __launch_bounds__(256) void k_read_paged_q(PagedQArgs c, T* __restric
     }
 }
 
-__device__ __forceinline__ float code_of(const uint8_t* row, int32_t d, int bits, bool key, int32_t D)
+// ---------------------------------------------------------------------------
+// Attention on the matrix cores, a tile of up to 16 query heads of one kv head (paged_split.h says how tiles and chunks of keys
+// are shared out).  A wave takes CH keys at a time, in tiles of 16 that lie together in a page:
+//   S^T = K . q^T   A = K's codes as they are: a 4-bit code in the low bits of an fp16 is the subnormal c 2^-24 (the instruction
+//                   takes subnormals, exact), an 8-bit one too; (w & 0x00f000f0) gives 16 c, whose q is 1 / 16.  The four
+//                   sums of each group (part) are scaled in fp32:
+//                     score = sum_g s_g part_g + m_g Q_g,   Q_g the sum of the group's q.
+//                   The minima's share is one more instruction: A = the minima (fp16), B = Q_g in three fp16 parts.
+//                   q is scaled by a power of two to a largest of 2^10 .. 2^11 in its row (fp32: high and low part, 22 bits).
+//   softmax         online, in log2 units; maximum rounded up to an integer.
+//   O^T += V^T P^T  V's codes go through the wave's LDS region and its transposing reads of 4 and 8 bits, which give a lane the
+//                   codes of 16 (8) keys of one dim; taken as subnormals again.  B = p s_g, the weights times their keys'
+//                   scales, per group, as fp16 pairs high + low; the minima's share sum_k p m_g is added up in fp32 beside.
+//                   Weights are times 2^14 over 2^es, a power of two above every scale so far, so that p s_g has fp16's range.
+// Loads of the next chunk are in flight while a chunk is worked on: V and the scales are free once they are in LDS, K once
+// the scores are there.  A tile past the end or on no page loads the first rows of page 0 instead; its scores
+// become -infinity and its scales 0, whatever they hold.
+// ---------------------------------------------------------------------------
+template <int N>
+struct __attribute__((packed, aligned(4))) Words {
+    uint32_t w[N];
+};
+
+// {a's high half, b's high half}
+__device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+
+// 8 codes as an operand of subnormals.  4 bits: code pairs (0, 4), (1, 5), (2, 6), (3, 7) of a word, odd ones times 16; 8 bits:
+// in order.
+__device__ __forceinline__ h8 codes4(uint32_t w)
 {
-    if (key) d = key_unit(d / 8, D) * 8 + d % 8;
-    return (float)(bits == 8 ? row[d] : row[d / 2] >> (d % 2 * 4) & 15);
+    const uint32_t v = w >> 8;
+    return __builtin_bit_cast(h8, u4{w & 0x000f000fu, w & 0x00f000f0u, v & 0x000f000fu, v & 0x00f000f0u});
+}
+__device__ __forceinline__ h8 codes8(uint32_t w0, uint32_t w1)
+{
+    return __builtin_bit_cast(h8, u4{__builtin_amdgcn_perm(0, w0, 0x0c010c00u), __builtin_amdgcn_perm(0, w0, 0x0c030c02u),
+                                     __builtin_amdgcn_perm(0, w1, 0x0c010c00u), __builtin_amdgcn_perm(0, w1, 0x0c030c02u)});
+}
+// high and low fp16 part of a pair of weights
+__device__ __forceinline__ void weight_parts(float a, float b, uint32_t& hi, uint32_t& lo)
+{
+    const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
+    hi = __builtin_bit_cast(uint32_t, h);
+    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a - (float)h[0], b - (float)h[1]));
 }
 
-// softmax(scale q K^T) V of one query head: a block per (head, sequence), its 4 waves each every fourth key, lane l the
-// dims l and l + 64; a running maximum m, sum l and numerator o, merged through LDS.
-template <typename T>
-__global__ __launch_bounds__(256) void k_attention_paged_q(PagedQArgs c, T* __restrict__ out, const T* __restrict__ q,
-                                                           const int32_t* __restrict__ lens, int32_t H, float scale)
-{
-    __shared__ float wm[4], wl[4], wo[4][128];
-    const int32_t h = blockIdx.x, s = blockIdx.y, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int32_t D = c.D, NG = D / c.group, g = h / (H / c.KVH);
-    const int64_t cap = (int64_t)c.max_pages * c.P;
-    const int32_t len = lens[s] < 0 ? 0 : lens[s] < cap ? lens[s] : (int32_t)cap;
-    const T* qr = q + ((int64_t)s * H + h) * D;
-    float x[2], o[2] = {}, m = -INFINITY, l = 0.0f;
-    for (int i = 0; i < 2; i++) x[i] = lane + 64 * i < D ? (float)qr[lane + 64 * i] * scale : 0.0f;
-    for (int32_t p = w; p < len; p += 4) {
-        const int64_t row0 = paged_q_row(c, s, p);
-        if (row0 < 0) continue;
-        const int64_t row = row0 + (int64_t)g * c.P;
-        float d = 0.0f, v[2] = {};
-        for (int i = 0; i < 2; i++) {
-            const int32_t dim = lane + 64 * i;
-            if (dim >= D) continue;
-            const uint32_t ks = c.ks[row * NG + dim / c.group], vs = c.vs[row * NG + dim / c.group];
-            d += x[i] * __builtin_fmaf(pair_scale(ks), code_of(c.kp + row * (D * c.kb / 8), dim, c.kb, true, D), pair_min(ks));
-            v[i] = __builtin_fmaf(pair_scale(vs), code_of(c.vp + row * (D * c.vb / 8), dim, c.vb, false, D), pair_min(vs));
+template <typename T_, int D_, int NG, int KB, int VBITS>
+struct PagedQTiles {
+    typedef PagedQArgs Args;
+    typedef T_ T;
+    static constexpr int D = D_, CH = VBITS == 4 ? 64 : 32;
+    static constexpr int NT = CH / 16, DS = D / 32, GS = DS / NG;           // tiles, steps of 32 dims, steps of a group
+    static constexpr int KRB = D * KB / 8, VRB = D * VBITS / 8;             // bytes of a row
+    static constexpr int KW = KRB / 16, VW = VRB / 16;                      // words of a lane's piece of a tile
+    // bytes between V's rows in LDS: 16 (8 bits: 8) of them on distinct banks
+    static constexpr int VP = VRB == 32 ? 40 : VRB == 48 ? 48 : VRB + 16;
+    static constexpr int SW = CH * NG;                                       // words of a chunk's scales
+    static constexpr int VB = CH * VP + 2 * SW * 4;
+    static constexpr bool TWO = sizeof(T) == 4;
+    struct Q {
+        h8 hi[DS], lo[TWO ? DS : 1], sums;
+        int e;
+    };
+
+    // Lane (r, gr): dims 32 s + 8 gr .. + 7 of head r, in the order of the codes.
+    static __device__ __forceinline__ void load_q(const T* q, int heads, int lane, Q& x)
+    {
+        const int r = lane & 15, gr = lane >> 4;
+        float v[DS][8], mx = 0.0f;
+#pragma unroll
+        for (int s = 0; s < DS; s++) {
+            Eight<T> a = {};
+            if (r < heads) a = *reinterpret_cast<const Eight<T>*>(q + r * D + 32 * s + 8 * gr);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                v[s][j] = (float)a.v[j];
+                mx = fmaxf(mx, __builtin_fabsf(v[s][j]));
+            }
         }
-        d = wave_sum_xor(d);
-        const float mn = fmaxf(m, d), f = m == -INFINITY ? 0.0f : expf(m - mn), e = expf(d - mn);
-        l = l * f + e;
-        for (int i = 0; i < 2; i++) o[i] = o[i] * f + e * v[i];
-        m = mn;
+        mx = max_x32(max_x16(mx));
+        x.e = mx == 0.0f ? 0 : 137 - (int)(__builtin_bit_cast(uint32_t, mx) >> 23);
+        float sum[NG] = {};
+#pragma unroll
+        for (int s = 0; s < DS; s++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int o = KB == 4 ? j / 2 + 4 * (j % 2) : j;
+                const float y = __builtin_ldexpf(v[s][o], x.e), z = KB == 4 && o % 2 ? y * 0.0625f : y;
+                sum[s / GS] += y;
+                x.hi[s][j] = (f16)z;
+                if constexpr (TWO) x.lo[s][j] = (f16)(z - (float)x.hi[s][j]);
+            }
+        x.sums = h8{};
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+            const float y = sum_x32(sum_x16(sum[g])) * 0x1p-8f;
+            const f16 a = (f16)y, b = (f16)(y - (float)a), c = (f16)(y - (float)a - (float)b);
+            x.sums[g] = gr == 0 ? a : gr == 1 ? b : gr == 2 ? c : (f16)0.0f;
+        }
     }
-    if (lane == 0) {
-        wm[w] = m;
-        wl[w] = l;
+
+    struct Spot {
+        int32_t page, in;
+    };
+    // Page of the tile of lane's keys in the chunk at c0, and the tile's place in it.
+    static __device__ __forceinline__ Spot look(const PagedQArgs& c, int32_t s, int32_t c0, int lane)
+    {
+        const uint32_t per = (uint32_t)c.P / 16, cap = (uint32_t)c.max_pages * per;
+        const uint32_t want = (uint32_t)c0 / 16 + (lane >> 4) % NT, t = want < cap ? want : cap - 1, pg = t / per;
+        return Spot{c.table[(int64_t)s * c.max_pages + pg], (int32_t)(t - pg * per)};
     }
-    for (int i = 0; i < 2; i++) wo[w][lane + 64 * i] = o[i];
-    __syncthreads();
-    const float M = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
-    const int32_t d = threadIdx.x;
-    if (d >= D) return;
-    float num = 0.0f, den = 0.0f;
-    for (int i = 0; i < 4; i++) {
-        const float f = wm[i] == -INFINITY && wl[i] == 0.0f ? 0.0f : expf(wm[i] - M);
-        num = __builtin_fmaf(f, wo[i][d], num);
-        den = __builtin_fmaf(f, wl[i], den);
+
+    static __device__ __forceinline__ void tile(const PagedQArgs& c, int32_t g, int32_t s, const Q& q, int32_t c0, int32_t cstep,
+                                                int32_t ke, float scale_log2, char* lds, int lane, PagedAcc<D>& acc)
+    {
+        const int r = lane & 15, gr = lane >> 4;
+        uint32_t* const lk = reinterpret_cast<uint32_t*>(lds + CH * VP);
+        uint32_t* const lv = lk + SW;
+        const float kl = __builtin_ldexpf(scale_log2, 24 - q.e);
+        acc.clear();
+        float om[NG] = {}, omo[NG] = {}, m = -INFINITY, l = 0.0f, l_odd = 0.0f, ref = 0x1p-30f;
+        int es = -30;
+
+        Words<KW> K[NT];
+        Words<VW> V[NT];
+        Words<NG> S[CH == 64 ? 2 : 1];  // lane = key (32 keys: K's in lanes 0 .. 31, V's in the others)
+        int64_t rows[NT];
+        bool on;                        // lane's key is one
+        auto locate = [&](const Spot& p, int32_t at) {
+            const int32_t first = at + 16 * ((lane >> 4) % NT);
+            const bool has = p.page >= 0 && p.page < c.pages && first < ke;
+            on = has && first + r < ke;
+            const int64_t row = has ? ((int64_t)p.page * c.KVH + g) * c.P + p.in * 16 : (int64_t)g * c.P;
+#pragma unroll
+            for (int t = 0; t < NT; t++) rows[t] = lane_of64((uint64_t)row, 16 * t);
+            return row + r;
+        };
+        auto load_v = [&](int64_t row) {
+#pragma unroll
+            for (int t = 0; t < NT; t++) V[t] = *reinterpret_cast<const Words<VW>*>(c.vp + rows[t] * VRB + lane * (VW * 4));
+            if constexpr (CH == 64) {
+                S[0] = *reinterpret_cast<const Words<NG>*>(c.ks + row * NG);
+                S[1] = *reinterpret_cast<const Words<NG>*>(c.vs + row * NG);
+            } else {
+                S[0] = *reinterpret_cast<const Words<NG>*>((lane < 32 ? c.ks : c.vs) + row * NG);
+            }
+        };
+        auto load_k = [&]() {
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+                K[t] = *reinterpret_cast<const Words<KW>*>(c.kp + rows[t] * KRB + (r * KRB + gr * (KRB / 4)));
+        };
+        Spot spot = look(c, s, c0, lane);
+        load_v(locate(spot, c0));
+        load_k();
+        spot = look(c, s, c0 + cstep, lane);
+        for (; c0 < ke; c0 += cstep) {
+            const uint64_t live = __ballot(on);
+            const bool all = CH == 64 ? live == ~0ull : (uint32_t)live == ~0u;
+            // ---- V and the scales to LDS
+            wave_lds_order();  // after the reads of the chunk before
+            float smax = 0.0f;
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                uint32_t* to = reinterpret_cast<uint32_t*>(lds + (NT * (lane >> 2) + t) * VP + (lane & 3) * (VRB / 4));
+#pragma unroll
+                for (int i = 0; i < VW; i++) to[i] = V[t].w[i];
+            }
+#pragma unroll
+            for (int i = 0; i < NG; i++) {
+                const uint32_t a = on ? S[0].w[i] : 0u, b = CH == 64 ? (on ? S[CH / 64].w[i] : 0u) : a;
+                lk[lane * NG + i] = a;  // 32 keys: V's are in the upper half
+                if (CH == 64) lv[lane * NG + i] = b;
+                smax = fmaxf(smax, __builtin_fabsf(pair_scale(b)));
+            }
+            if (CH == 32 && lane < 32) smax = 0.0f;
+            wave_lds_order();
+            // ---- the next chunk's V and scales
+            load_v(locate(spot, c0 + cstep));
+            spot = look(c, s, c0 + 2 * cstep, lane);
+            // ---- scores
+            f4 sc[NT];
+            float cm = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                uint32_t sw[4][NG];
+#pragma unroll
+                for (int i = 0; i < 4 * NG; i++) sw[i / NG][i % NG] = lk[(16 * t + 4 * gr) * NG + i];
+                uint32_t mine[NG];
+#pragma unroll
+                for (int i = 0; i < NG; i++) mine[i] = lk[(16 * t + r) * NG + i];
+                u4 mins = {};
+#pragma unroll
+                for (int i = 0; i < NG; i += 2) mins[i / 2] = high_halves(mine[i], i + 1 < NG ? mine[i + 1] : 0u);
+                sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, mins), q.sums, f4{}, 0, 0, 0) * 0x1p-16f;
+#pragma unroll
+                for (int gq = 0; gq < NG; gq++) {
+                    f4 part = {};
+#pragma unroll
+                    for (int x = gq * GS; x < gq * GS + GS; x++) {
+                        const h8 a = KB == 4 ? codes4(K[t].w[x]) : codes8(K[t].w[2 * x % KW], K[t].w[(2 * x + 1) % KW]);
+                        if constexpr (TWO) part = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q.lo[x], part, 0, 0, 0);
+                        part = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q.hi[x], part, 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; i++) sc[t][i] = __builtin_fmaf(pair_scale(sw[i][gq]), part[i], sc[t][i]);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    float x = sc[t][i] * kl;
+                    if (!all && !(live >> (16 * t + 4 * gr + i) & 1)) x = -INFINITY;
+                    sc[t][i] = x;
+                    cm = fmaxf(cm, x);
+                }
+            }
+            load_k();
+            cm = max_x32(max_x16(cm));
+            if (__any(cm > m || smax > ref)) {  // a new maximum for some head, or a new largest scale
+                const float mn = __builtin_ceilf(fmaxf(m, cm));
+                int en = es;
+                if (__any(smax > ref)) {
+                    en = (int)(__builtin_bit_cast(uint32_t, group_max(smax, 64)) >> 23) - 126;
+                    en = __builtin_amdgcn_readfirstlane(en < 16 ? en : 16);
+                    ref = __builtin_ldexpf(1.0f, en);
+                }
+                const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn + (float)(es - en));
+                m = mn;
+                es = en;
+                l *= f;
+                l_odd *= f;
+#pragma unroll
+                for (int i = 0; i < NG; i++) {
+                    om[i] *= f;
+                    omo[i] *= f;
+                }
+#pragma unroll
+                for (int e = 0; e < D / 16; e++) acc.o[e] *= f;
+            }
+            const float mb = m == -INFINITY ? 0.0f : m - 14.0f + (float)es;  // no key yet: every weight below is 0
+            // 4 bits: odd keys' weights are over 16, as their codes are times 16
+            const float mo = VBITS == 4 ? mb + 4.0f : mb;
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    sc[t][i] = __builtin_amdgcn_exp2f(sc[t][i] - (i % 2 ? mo : mb));
+                    (i % 2 ? l_odd : l) += sc[t][i];
+                }
+            // ---- values, group by group
+            uint32_t sw[NT][4][NG];
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int i = 0; i < 4 * NG; i++) sw[t][i / NG][i % NG] = lv[(16 * t + 4 * gr) * NG + i];
+#pragma unroll
+            for (int gq = 0; gq < NG; gq++) {
+                u4 hi[NT / 2], lo[NT / 2];
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        (i % 2 ? omo : om)[gq] = __builtin_fmaf(sc[t][i], pair_min(sw[t][i][gq]), (i % 2 ? omo : om)[gq]);
+                auto w = [&](int t, int i) { return sc[t][i] * pair_scale(sw[t][i][gq]); };
+#pragma unroll
+                for (int u = 0; u < NT / 2; u++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        uint32_t h, o;
+                        if (VBITS == 4) weight_parts(w(2 * u, i), w(2 * u + 1, i), h, o);
+                        else weight_parts(w(i / 2, 2 * (i % 2)), w(i / 2, 2 * (i % 2) + 1), h, o);
+                        hi[u][i] = h;
+                        lo[u][i] = o;
+                    }
+#pragma unroll
+                for (int e = gq * GS * 2; e < (gq + 1) * GS * 2; e++) {
+                    h8 a[NT / 2];
+                    typedef int i2 __attribute__((ext_vector_type(2)));
+                    if constexpr (VBITS == 4) {
+                        // nibble n of a lane: key 4 gr + n % 4 of tile n / 4
+                        const char* src = lds + (16 * gr + 4 * (r & 3) + (r >> 2)) * VP + 8 * e;
+                        const i2 w2 = __builtin_amdgcn_ds_read_tr4_b64_v2i32((__attribute__((address_space(3))) i2*)(src));
+                        a[0] = codes4((uint32_t)w2[0]);
+                        a[1] = codes4((uint32_t)w2[1]);
+                    } else {
+                        // byte n of a lane: key 4 gr + n % 4 of tile n / 4
+                        const char* src = lds + (8 * gr + 2 * (r >> 1 & 3) + (r >> 3)) * VP + 16 * e + 8 * (r & 1);
+                        const i2 w2 = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i2*)(src));
+                        a[0] = codes8((uint32_t)w2[0], (uint32_t)w2[1]);
+                    }
+#pragma unroll
+                    for (int u = 0; u < NT / 2; u++) {
+                        acc.o[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[u], __builtin_bit_cast(h8, lo[u]), acc.o[e], 0, 0, 0);
+                        acc.o[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[u], __builtin_bit_cast(h8, hi[u]), acc.o[e], 0, 0, 0);
+                    }
+                }
+            }
+        }
+        const float odd = VBITS == 4 ? 16.0f : 1.0f;
+        acc.l = sum_x32(sum_x16(__builtin_fmaf(l_odd, odd, l)));
+        acc.m = m == -INFINITY ? m : m + (float)es;
+#pragma unroll
+        for (int gq = 0; gq < NG; gq++) {
+            const float y = sum_x32(sum_x16(__builtin_fmaf(omo[gq], odd, om[gq])));
+#pragma unroll
+            for (int e = gq * GS * 2; e < (gq + 1) * GS * 2; e++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) acc.o[e][i] = __builtin_fmaf(acc.o[e][i], 0x1p24f, y);
+        }
     }
-    out[((int64_t)s * H + h) * D + d] = (T)(den == 0.0f ? 0.0f : num / den);
+
+    static __device__ __forceinline__ constexpr int dim(int e, int gr, int i) { return 16 * e + 4 * gr + i; }
+};
+
+template <typename TL>
+__global__ __launch_bounds__(512, 2) void k_attention_paged_q_one(PagedQArgs c, typename TL::T* __restrict__ out,
+                                                                  const typename TL::T* __restrict__ q,
+                                                                  const int32_t* __restrict__ lens, PagedHeads hd, int32_t H,
+                                                                  float scale_log2)
+{
+    paged_one<TL, 8>(c, out, q, lens, hd, H, scale_log2);
+}
+template <typename TL>
+__global__ __launch_bounds__(256, 2) void k_attention_paged_q_split(PagedQArgs c, typename TL::T* __restrict__ out,
+                                                                    const typename TL::T* __restrict__ q,
+                                                                    const int32_t* __restrict__ lens, PagedHeads hd, int32_t H,
+                                                                    float scale_log2, int64_t* __restrict__ before_out,
+                                                                    float* __restrict__ ws, int32_t VH)
+{
+    paged_split<TL>(c, out, q, lens, hd, H, scale_log2, before_out, ws, VH);
 }
 
 // A launch holds fewer than 2^32 threads: at most 2^22 tokens each (of up to 512).
@@ -266,15 +542,74 @@ int launch_read_paged_q(const PagedQArgs& c, void* k_out, void* v_out, const int
     return (int)hipGetLastError();
 }
 
-int launch_attention_paged_q(const PagedQArgs& c, void* out, const void* q, const int32_t* lens, int64_t H, float scale,
-                             int dtype, void* stream)
+// Chunks that a block takes by itself, as in paged_kernels.hip
+constexpr int64_t kQOneChunks = 16;
+
+AttnPagedPlan attention_paged_q_plan(const PagedQArgs& c, int64_t max_len, int64_t H, int64_t cus)
 {
-    auto go = [&](auto kern, auto* type) {
-        using T = std::remove_pointer_t<decltype(type)>;
-        hipLaunchKernelGGL(kern, dim3((unsigned)H, (unsigned)c.B), dim3(256), 0, static_cast<hipStream_t>(stream), c, (T*)out,
-                           (const T*)q, lens, (int32_t)H, scale);
+    AttnPagedPlan p{};
+    const int64_t G = H / c.KVH;
+    p.tiled = true;
+    p.tiles = (G + 15) / 16;
+    p.GT = (G + p.tiles - 1) / p.tiles;
+    p.waves = 8;
+    const int64_t cap = (int64_t)c.max_pages * c.P, ch = c.vb == 4 ? 64 : 32;
+    const int64_t chunks = ((max_len > 0 && max_len < cap ? max_len : cap) + ch - 1) / ch;
+    if (chunks > kQOneChunks) p.blocks = std::min<int64_t>((chunks * c.B * c.KVH * p.tiles + 3) / 4, 2 * cus);
+    if (p.blocks > 0) p.ws_floats = paged_before_floats(c.B) + p.blocks * 4 * 2 * p.GT * (c.D + 4);
+    return p;
+}
+
+template <typename TL>
+static void paged_q_go(const AttnPagedPlan& p, const PagedQArgs& c, typename TL::T* out, const typename TL::T* q, const int32_t* lens,
+                       int64_t H, float scale_log2, float* ws, hipStream_t s)
+{
+    const PagedHeads hd{(int32_t)(H / c.KVH), (int32_t)p.GT, (int32_t)p.tiles};
+    const int32_t VH = (int32_t)(c.KVH * p.tiles);
+    if (p.blocks == 0) {
+        hipLaunchKernelGGL((k_attention_paged_q_one<TL>), dim3((unsigned)VH, (unsigned)c.B), dim3(512), 0, s, c, out, q, lens, hd,
+                           (int32_t)H, scale_log2);
+        return;
+    }
+    int64_t* before = reinterpret_cast<int64_t*>(ws);
+    float* parts = ws + paged_before_floats(c.B);
+    hipLaunchKernelGGL((k_attention_paged_q_split<TL>), dim3((unsigned)p.blocks), dim3(256), 0, s, c, out, q, lens, hd, (int32_t)H,
+                       scale_log2, before, parts, VH);
+    const int64_t W = p.blocks * 4;
+    int64_t nw = 1;  // waves of a merge block: about 4 parts a group of lanes if the sequences are alike
+    while (nw < 16 && nw * (256 / TL::D) * 4 < p.blocks / ((int64_t)VH * c.B)) nw *= 2;
+    hipLaunchKernelGGL((k_attention_paged_merge<typename TL::T, TL::D>), dim3((unsigned)H, (unsigned)c.B), dim3((unsigned)(64 * nw)), 0,
+                       s, (int32_t)c.B, out, hd, (int32_t)H, before, parts, VH, (int32_t)W);
+}
+
+int launch_attention_paged_q(const AttnPagedPlan& p, const PagedQArgs& c, void* out, const void* q, const int32_t* lens, int64_t H,
+                             float scale, float* ws, int dtype, void* stream)
+{
+    const float sl = (float)((double)scale * 1.4426950408889634);  // scores in log2 units
+    auto run = [&](auto* t, auto d, auto ng, auto kb, auto vb) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        paged_q_go<PagedQTiles<T, decltype(d)::value, decltype(ng)::value, decltype(kb)::value, decltype(vb)::value>>(
+            p, c, (T*)out, (const T*)q, lens, H, sl, ws, static_cast<hipStream_t>(stream));
     };
-    dtype == VVH_F16 ? go(k_attention_paged_q<f16>, (f16*)nullptr) : go(k_attention_paged_q<float>, (float*)nullptr);
+    auto bits = [&](auto* t, auto d, auto ng) {
+        constexpr std::integral_constant<int, 4> four{};
+        constexpr std::integral_constant<int, 8> eight{};
+        c.kb == 4 ? run(t, d, ng, four, four) : c.vb == 4 ? run(t, d, ng, eight, four) : run(t, d, ng, eight, eight);
+    };
+    auto shape = [&](auto* t) {
+        constexpr std::integral_constant<int, 1> g1{};
+        constexpr std::integral_constant<int, 2> g2{};
+        constexpr std::integral_constant<int, 3> g3{};
+        constexpr std::integral_constant<int, 4> g4{};
+        constexpr std::integral_constant<int, 64> d64{};
+        constexpr std::integral_constant<int, 96> d96{};
+        constexpr std::integral_constant<int, 128> d128{};
+        const int ng = c.D / c.group;
+        if (c.D == 64) ng == 1 ? bits(t, d64, g1) : bits(t, d64, g2);
+        else if (c.D == 96) bits(t, d96, g3);
+        else ng == 1 ? bits(t, d128, g1) : ng == 2 ? bits(t, d128, g2) : bits(t, d128, g4);
+    };
+    dtype == VVH_F16 ? shape((f16*)nullptr) : shape((float*)nullptr);
     return (int)hipGetLastError();
 }
 

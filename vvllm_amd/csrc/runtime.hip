@@ -2508,8 +2508,14 @@ VVH_API int vvh_attention_paged_q(const vvh_paged_cache_q* cache, void* out, con
     if (num_heads > 65535) return fail(VVH_ERR_UNSUPPORTED, "%zu heads", num_heads);
     if (!aligned16(q) || !aligned16(out) || ((uintptr_t)lens & 3)) return fail(VVH_ERR_INVALID_ARG, "misaligned pointer");
     REQUIRE_INIT();
-    (void)max_len;
-    return ret_launch(launch_attention_paged_q(a, out, q, lens, (int64_t)num_heads, scale, cache->dtype, stream),
+    const AttnPagedPlan p = attention_paged_q_plan(a, (int64_t)std::min(max_len, (size_t)INT32_MAX), (int64_t)num_heads,
+                                                   g_cu_count > 0 ? g_cu_count : 256);
+    float* ws = nullptr;
+    if (p.ws_floats > 0) {
+        const int ws_st = workspace_for(stream, (std::size_t)p.ws_floats * 4, &ws);
+        if (ws_st != VVH_OK) return ws_st;
+    }
+    return ret_launch(launch_attention_paged_q(p, a, out, q, lens, (int64_t)num_heads, scale, ws, cache->dtype, stream),
                       "attention over a paged cache of codes");
 }
 
