@@ -422,9 +422,10 @@ int launch_rope_append_paged(const PagedArgs& c, void* q_out, const void* q, con
 // How a call is run: tiled on the matrix cores or by the form for any shape; tiled
 // with blocks > 0 split over 4 * blocks waves (ws_floats floats of workspace, a
 // merge launch), else one block of `waves` waves per tile of GT heads (`tiles` of a kv head).
+// columns: of a head in the products with codes.
 struct AttnPagedPlan {
     bool tiled;
-    int64_t GT, tiles, waves, blocks, ws_floats;
+    int64_t GT, tiles, waves, blocks, ws_floats, columns;
 };
 AttnPagedPlan attention_paged_plan(const PagedArgs& c, const void* q, int64_t max_len, int64_t H, int dtype,
                                    int64_t cus);

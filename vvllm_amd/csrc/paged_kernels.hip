@@ -560,7 +560,7 @@ template <typename T_, int D_, bool BIG>
 struct PagedTiles {
     typedef PagedArgs Args;
     typedef T_ T;
-    static constexpr int D = D_, CH = PagedTile<T>::template CH<D>, VB = PagedTile<T>::template lds<D> * 2;
+    static constexpr int D = D_, CH = PagedTile<T>::template CH<D>, HEAD = 0, VB = PagedTile<T>::template lds<D> * 2;
     typedef typename PagedTile<T>::template Q<D> Q;
     static __device__ __forceinline__ void load_q(const T* q, int heads, int lane, Q& x) { paged_load_q<D>(q, heads, lane, x); }
     static __device__ __forceinline__ void tile(const PagedArgs& c, int32_t g, int32_t s, const Q& x, int32_t c0, int32_t cstep, int32_t ke,

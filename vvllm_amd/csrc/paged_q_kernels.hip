@@ -11,6 +11,12 @@
 #include "device.h"
 #include "paged_split.h"
 
+#ifndef QWAVES
+#define QWAVES 2
+#endif
+#ifndef QHEAD
+#define QHEAD 2
+#endif
 namespace vvh {
 
 namespace {
@@ -173,16 +179,18 @@ __global__ __launch_bounds__(256) void k_read_paged_q(PagedQArgs c, T* __restric
 // Attention on the matrix cores, a tile of up to 16 query heads of one kv head (paged_split.h says how tiles and chunks of keys
 // are shared out).  A wave takes CH keys at a time, in tiles of 16 that lie together in a page:
 //   S^T = K . q^T   A = K's codes as they are: a 4-bit code in the low bits of an fp16 is the subnormal c 2^-24 (the instruction
-//                   takes subnormals, exact), an 8-bit one too; (w & 0x00f000f0) gives 16 c, whose q is 1 / 16.  The four
-//                   sums of each group (part) are scaled in fp32:
-//                     score = sum_g s_g part_g + m_g Q_g,   Q_g the sum of the group's q.
-//                   The minima's share is one more instruction: A = the minima (fp16), B = Q_g in three fp16 parts.
+//                   takes subnormals, exact), an 8-bit one too; (w & 0x00f000f0) gives 16 c, whose q is 1 / 16.  A group's
+//                   sum is scaled in fp32: score = sum_g s_g part_g + m_g Q_g, Q_g the sum of the group's q.
 //                   q is scaled by a power of two to a largest of 2^10 .. 2^11 in its row (fp32: high and low part, 22 bits).
 //   softmax         online, in log2 units; maximum rounded up to an integer.
 //   O^T += V^T P^T  V's codes go through the wave's LDS region and its transposing reads of 4 and 8 bits, which give a lane the
 //                   codes of 16 (8) keys of one dim; taken as subnormals again.  B = p s_g, the weights times their keys'
-//                   scales, per group, as fp16 pairs high + low; the minima's share sum_k p m_g is added up in fp32 beside.
+//                   scales, as fp16 pairs high + low; the minima's share sum_k p m_g is added up in fp32 beside.
 //                   Weights are times 2^14 over 2^es, a power of two above every scale so far, so that p s_g has fp16's range.
+// Column r of the products is head r / NGS and, of its groups, every NGS-th from r % NGS on: few heads leave columns free,
+// and scaling scores and weights is most of what a chunk costs (96 ragged contexts of 4 heads a kv head and 4 groups 116 us with a
+// column a head, which scales everything 4 times).  A column's q is 0 outside of the group, so that an instruction sums
+// each column's own; the scores of a head's columns are then added.  Of the output's columns those of a dim's group count.
 // Loads of the next chunk are in flight while a chunk is worked on: V and the scales are free once they are in LDS, K once
 // the scores are there.  A tile past the end or on no page loads the first rows of page 0 instead; its scores
 // become -infinity and its scales 0, whatever they hold.
@@ -191,9 +199,6 @@ template <int N>
 struct __attribute__((packed, aligned(4))) Words {
     uint32_t w[N];
 };
-
-// {a's high half, b's high half}
-__device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 
 // 8 codes as an operand of subnormals.  4 bits: code pairs (0, 4), (1, 5), (2, 6), (3, 7) of a word, odd ones times 16; 8 bits:
 // in order.
@@ -207,41 +212,56 @@ __device__ __forceinline__ h8 codes8(uint32_t w0, uint32_t w1)
     return __builtin_bit_cast(h8, u4{__builtin_amdgcn_perm(0, w0, 0x0c010c00u), __builtin_amdgcn_perm(0, w0, 0x0c030c02u),
                                      __builtin_amdgcn_perm(0, w1, 0x0c010c00u), __builtin_amdgcn_perm(0, w1, 0x0c030c02u)});
 }
-// high and low fp16 part of a pair of weights
-__device__ __forceinline__ void weight_parts(float a, float b, uint32_t& hi, uint32_t& lo)
+// High and low fp16 part of a pair of weights; minus: -1, in a register that the compiler knows nothing of, so that a
+// difference is one instruction that takes the fp16 as it is.
+__device__ __forceinline__ void weight_parts(float a, float b, float minus, uint32_t& hi, uint32_t& lo)
 {
     const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
     hi = __builtin_bit_cast(uint32_t, h);
-    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a - (float)h[0], b - (float)h[1]));
+    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)h[0], minus, a), __builtin_fmaf((float)h[1], minus, b)));
+}
+// v of the lane that the quad permutation names, as an operand of the instruction that takes it
+template <int CTRL>
+__device__ __forceinline__ float quad(float v)
+{
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
 }
 
-template <typename T_, int D_, int NG, int KB, int VBITS>
+template <typename T_, int D_, int NG, int NGS, int KB, int VBITS>
 struct PagedQTiles {
     typedef PagedQArgs Args;
     typedef T_ T;
-    static constexpr int D = D_, CH = VBITS == 4 ? 64 : 32;
+    static constexpr int D = D_, CH = VBITS == 4 ? 64 : 32, HEAD = QHEAD;
     static constexpr int NT = CH / 16, DS = D / 32, GS = DS / NG;           // tiles, steps of 32 dims, steps of a group
     static constexpr int KRB = D * KB / 8, VRB = D * VBITS / 8;             // bytes of a row
     static constexpr int KW = KRB / 16, VW = VRB / 16;                      // words of a lane's piece of a tile
     // bytes between V's rows in LDS: 16 (8 bits: 8) of them on distinct banks
     static constexpr int VP = VRB == 32 ? 40 : VRB == 48 ? 48 : VRB + 16;
-    static constexpr int SW = CH * NG;                                       // words of a chunk's scales
+    static constexpr int NP = (NG + NGS - 1) / NGS;                          // groups of a column
+    static constexpr int SR = CH + 16, SW = NG * SR;                         // words of a group's scales in LDS, of a chunk's
     static constexpr int VB = CH * VP + 2 * SW * 4;
     static constexpr bool TWO = sizeof(T) == 4;
     struct Q {
-        h8 hi[DS], lo[TWO ? DS : 1], sums;
+        h8 hi[DS], lo[TWO ? DS : 1];
+        float sum[NP];  // of the column's groups, times 2^-24
         int e;
     };
+    // group `p` of column r; where NG is no multiple of NGS, a column without one takes the last again, with a q of 0
+    static __device__ __forceinline__ int group_of(int r, int p)
+    {
+        const int g = p * NGS + r % NGS;
+        return NG % NGS == 0 || g < NG ? g : NG - 1;
+    }
 
-    // Lane (r, gr): dims 32 s + 8 gr .. + 7 of head r, in the order of the codes.
+    // Lane (r, gr): dims 32 s + 8 gr .. + 7 of head r / NGS, in the order of the codes.
     static __device__ __forceinline__ void load_q(const T* q, int heads, int lane, Q& x)
     {
-        const int r = lane & 15, gr = lane >> 4;
+        const int r = lane & 15, gr = lane >> 4, h = r / NGS;
         float v[DS][8], mx = 0.0f;
 #pragma unroll
         for (int s = 0; s < DS; s++) {
             Eight<T> a = {};
-            if (r < heads) a = *reinterpret_cast<const Eight<T>*>(q + r * D + 32 * s + 8 * gr);
+            if (h < heads) a = *reinterpret_cast<const Eight<T>*>(q + h * D + 32 * s + 8 * gr);
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 v[s][j] = (float)a.v[j];
@@ -250,24 +270,22 @@ struct PagedQTiles {
         }
         mx = max_x32(max_x16(mx));
         x.e = mx == 0.0f ? 0 : 137 - (int)(__builtin_bit_cast(uint32_t, mx) >> 23);
-        float sum[NG] = {};
 #pragma unroll
-        for (int s = 0; s < DS; s++)
+        for (int p = 0; p < NP; p++) x.sum[p] = 0.0f;
+#pragma unroll
+        for (int s = 0; s < DS; s++) {
+            const bool mine = s / GS % NGS == r % NGS;
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const int o = KB == 4 ? j / 2 + 4 * (j % 2) : j;
-                const float y = __builtin_ldexpf(v[s][o], x.e), z = KB == 4 && o % 2 ? y * 0.0625f : y;
-                sum[s / GS] += y;
+                const float y = mine ? __builtin_ldexpf(v[s][o], x.e) : 0.0f, z = KB == 4 && o % 2 ? y * 0.0625f : y;
+                x.sum[s / GS / NGS] += y;
                 x.hi[s][j] = (f16)z;
                 if constexpr (TWO) x.lo[s][j] = (f16)(z - (float)x.hi[s][j]);
             }
-        x.sums = h8{};
-#pragma unroll
-        for (int g = 0; g < NG; g++) {
-            const float y = sum_x32(sum_x16(sum[g])) * 0x1p-8f;
-            const f16 a = (f16)y, b = (f16)(y - (float)a), c = (f16)(y - (float)a - (float)b);
-            x.sums[g] = gr == 0 ? a : gr == 1 ? b : gr == 2 ? c : (f16)0.0f;
         }
+#pragma unroll
+        for (int p = 0; p < NP; p++) x.sum[p] = sum_x32(sum_x16(x.sum[p])) * 0x1p-24f;
     }
 
     struct Spot {
@@ -281,15 +299,29 @@ struct PagedQTiles {
         return Spot{c.table[(int64_t)s * c.max_pages + pg], (int32_t)(t - pg * per)};
     }
 
-    static __device__ __forceinline__ void tile(const PagedQArgs& c, int32_t g, int32_t s, const Q& q, int32_t c0, int32_t cstep,
+    static __device__ __forceinline__ void tile(const PagedQArgs& c, int32_t g, int32_t s, const Q& q0, int32_t c0, int32_t cstep,
                                                 int32_t ke, float scale_log2, char* lds, int lane, PagedAcc<D>& acc)
     {
         const int r = lane & 15, gr = lane >> 4;
         uint32_t* const lk = reinterpret_cast<uint32_t*>(lds + CH * VP);
         uint32_t* const lv = lk + SW;
-        const float kl = __builtin_ldexpf(scale_log2, 24 - q.e);
+        // scores to log2 units: positive (a negative scale turns q's sign), never 0, so that the maximum of the scores is
+        // that of the products and -infinity stays (2^-100 times any score is 0 for the exponential)
+        const float kl = fmaxf(__builtin_fabsf(__builtin_ldexpf(scale_log2, 24 - q0.e)), 0x1p-100f);
+        Q q = q0;
+        if (scale_log2 < 0.0f) {
+#pragma unroll
+            for (int x = 0; x < DS; x++) {
+                q.hi[x] = -q.hi[x];
+                if constexpr (TWO) q.lo[x] = -q.lo[x];
+            }
+#pragma unroll
+            for (int p = 0; p < NP; p++) q.sum[p] = -q.sum[p];
+        }
+        float minus = -1.0f;
+        asm("" : "+s"(minus));
         acc.clear();
-        float om[NG] = {}, omo[NG] = {}, m = -INFINITY, l = 0.0f, l_odd = 0.0f, ref = 0x1p-30f;
+        float om[NP] = {}, om_odd[NP] = {}, m = -INFINITY, l = 0.0f, l_odd = 0.0f, ref = 0x1p-30f;
         int es = -30;
 
         Words<KW> K[NT];
@@ -321,6 +353,10 @@ struct PagedQTiles {
             for (int t = 0; t < NT; t++)
                 K[t] = *reinterpret_cast<const Words<KW>*>(c.kp + rows[t] * KRB + (r * KRB + gr * (KRB / 4)));
         };
+        if (c0 >= ke) {
+            acc.l = 0.0f;
+            return;
+        }
         Spot spot = look(c, s, c0, lane);
         load_v(locate(spot, c0));
         load_k();
@@ -340,8 +376,12 @@ struct PagedQTiles {
 #pragma unroll
             for (int i = 0; i < NG; i++) {
                 const uint32_t a = on ? S[0].w[i] : 0u, b = CH == 64 ? (on ? S[CH / 64].w[i] : 0u) : a;
-                lk[lane * NG + i] = a;  // 32 keys: V's are in the upper half
-                if (CH == 64) lv[lane * NG + i] = b;
+                if constexpr (CH == 64) {
+                    lk[i * SR + lane] = a;
+                    lv[i * SR + lane] = b;
+                } else {
+                    (lane < 32 ? lk : lv)[i * SR + lane % 32] = a;
+                }
                 smax = fmaxf(smax, __builtin_fabsf(pair_scale(b)));
             }
             if (CH == 32 && lane < 32) smax = 0.0f;
@@ -354,38 +394,43 @@ struct PagedQTiles {
             float cm = -INFINITY;
 #pragma unroll
             for (int t = 0; t < NT; t++) {
-                uint32_t sw[4][NG];
 #pragma unroll
-                for (int i = 0; i < 4 * NG; i++) sw[i / NG][i % NG] = lk[(16 * t + 4 * gr) * NG + i];
-                uint32_t mine[NG];
-#pragma unroll
-                for (int i = 0; i < NG; i++) mine[i] = lk[(16 * t + r) * NG + i];
-                u4 mins = {};
-#pragma unroll
-                for (int i = 0; i < NG; i += 2) mins[i / 2] = high_halves(mine[i], i + 1 < NG ? mine[i + 1] : 0u);
-                sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, mins), q.sums, f4{}, 0, 0, 0) * 0x1p-16f;
-#pragma unroll
-                for (int gq = 0; gq < NG; gq++) {
+                for (int p = 0; p < NP; p++) {
+                    const u4 sm = *reinterpret_cast<const u4*>(lk + group_of(r, p) * SR + 16 * t + 4 * gr);
                     f4 part = {};
 #pragma unroll
-                    for (int x = gq * GS; x < gq * GS + GS; x++) {
+                    for (int x = p * NGS * GS; x < (p + 1) * NGS * GS && x < DS; x++) {
                         const h8 a = KB == 4 ? codes4(K[t].w[x]) : codes8(K[t].w[2 * x % KW], K[t].w[(2 * x + 1) % KW]);
                         if constexpr (TWO) part = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q.lo[x], part, 0, 0, 0);
                         part = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q.hi[x], part, 0, 0, 0);
                     }
 #pragma unroll
-                    for (int i = 0; i < 4; i++) sc[t][i] = __builtin_fmaf(pair_scale(sw[i][gq]), part[i], sc[t][i]);
+                    for (int i = 0; i < 4; i++) {
+                        const float y = __builtin_fmaf(pair_min(sm[i]), q.sum[p], p ? sc[t][i] : 0.0f);
+                        sc[t][i] = __builtin_fmaf(pair_scale(sm[i]), part[i], y);
+                    }
                 }
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    float x = sc[t][i] * kl;
-                    if (!all && !(live >> (16 * t + 4 * gr + i) & 1)) x = -INFINITY;
-                    sc[t][i] = x;
-                    cm = fmaxf(cm, x);
+                    if (NGS >= 2) sc[t][i] += quad<0xB1>(sc[t][i]);
+                    if (NGS >= 4) sc[t][i] += quad<0x4E>(sc[t][i]);
                 }
             }
+            if (!all) {
+                uint64_t bits = live;
+                asm volatile("" : "+s"(bits));  // a branch, not 16 selects in every chunk
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (!(bits >> (16 * t + 4 * gr + i) & 1)) sc[t][i] = -INFINITY;
+            }
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) cm = fmaxf(cm, sc[t][i]);
             load_k();
-            cm = max_x32(max_x16(cm));
+            cm = max_x32(max_x16(cm)) * kl;
             if (__any(cm > m || smax > ref)) {  // a new maximum for some head, or a new largest scale
                 const float mn = __builtin_ceilf(fmaxf(m, cm));
                 int en = es;
@@ -400,9 +445,9 @@ struct PagedQTiles {
                 l *= f;
                 l_odd *= f;
 #pragma unroll
-                for (int i = 0; i < NG; i++) {
-                    om[i] *= f;
-                    omo[i] *= f;
+                for (int p = 0; p < NP; p++) {
+                    om[p] *= f;
+                    om_odd[p] *= f;
                 }
 #pragma unroll
                 for (int e = 0; e < D / 16; e++) acc.o[e] *= f;
@@ -414,36 +459,34 @@ struct PagedQTiles {
             for (int t = 0; t < NT; t++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    sc[t][i] = __builtin_amdgcn_exp2f(sc[t][i] - (i % 2 ? mo : mb));
+                    sc[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][i], kl, i % 2 ? -mo : -mb));
                     (i % 2 ? l_odd : l) += sc[t][i];
                 }
-            // ---- values, group by group
-            uint32_t sw[NT][4][NG];
+            // ---- values
 #pragma unroll
-            for (int t = 0; t < NT; t++)
+            for (int p = 0; p < NP; p++) {
+                u4 sm[NT], hi[NT / 2], lo[NT / 2];
 #pragma unroll
-                for (int i = 0; i < 4 * NG; i++) sw[t][i / NG][i % NG] = lv[(16 * t + 4 * gr) * NG + i];
-#pragma unroll
-            for (int gq = 0; gq < NG; gq++) {
-                u4 hi[NT / 2], lo[NT / 2];
+                for (int t = 0; t < NT; t++) sm[t] = *reinterpret_cast<const u4*>(lv + group_of(r, p) * SR + 16 * t + 4 * gr);
 #pragma unroll
                 for (int t = 0; t < NT; t++)
 #pragma unroll
                     for (int i = 0; i < 4; i++)
-                        (i % 2 ? omo : om)[gq] = __builtin_fmaf(sc[t][i], pair_min(sw[t][i][gq]), (i % 2 ? omo : om)[gq]);
-                auto w = [&](int t, int i) { return sc[t][i] * pair_scale(sw[t][i][gq]); };
+                        (i % 2 ? om_odd : om)[p] = __builtin_fmaf(sc[t][i], pair_min(sm[t][i]), (i % 2 ? om_odd : om)[p]);
+                // + 0: one instruction that takes the scale as it is
+                auto w = [&](int t, int i) { return __builtin_fmaf(sc[t][i], pair_scale(sm[t][i]), 0.0f); };
 #pragma unroll
                 for (int u = 0; u < NT / 2; u++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         uint32_t h, o;
-                        if (VBITS == 4) weight_parts(w(2 * u, i), w(2 * u + 1, i), h, o);
-                        else weight_parts(w(i / 2, 2 * (i % 2)), w(i / 2, 2 * (i % 2) + 1), h, o);
+                        if (VBITS == 4) weight_parts(w(2 * u, i), w(2 * u + 1, i), minus, h, o);
+                        else weight_parts(w(i / 2, 2 * (i % 2)), w(i / 2, 2 * (i % 2) + 1), minus, h, o);
                         hi[u][i] = h;
                         lo[u][i] = o;
                     }
 #pragma unroll
-                for (int e = gq * GS * 2; e < (gq + 1) * GS * 2; e++) {
+                for (int e = p * NGS * GS * 2; e < (p + 1) * NGS * GS * 2 && e < D / 16; e++) {
                     h8 a[NT / 2];
                     typedef int i2 __attribute__((ext_vector_type(2)));
                     if constexpr (VBITS == 4) {
@@ -467,31 +510,106 @@ struct PagedQTiles {
             }
         }
         const float odd = VBITS == 4 ? 16.0f : 1.0f;
-        acc.l = sum_x32(sum_x16(__builtin_fmaf(l_odd, odd, l)));
-        acc.m = m == -INFINITY ? m : m + (float)es;
+        float ms[NP];
 #pragma unroll
-        for (int gq = 0; gq < NG; gq++) {
-            const float y = sum_x32(sum_x16(__builtin_fmaf(omo[gq], odd, om[gq])));
+        for (int p = 0; p < NP; p++) ms[p] = sum_x32(sum_x16(__builtin_fmaf(om_odd[p], odd, om[p])));
+        // to lane r what is head r's
+        auto from = [&](float v, int col) { return NGS == 1 ? v : __shfl(v, (lane & 48) + (r * NGS + col) % 16); };
 #pragma unroll
-            for (int e = gq * GS * 2; e < (gq + 1) * GS * 2; e++)
+        for (int e = 0; e < D / 16; e++) {
+            const int gq = e / (2 * GS);
 #pragma unroll
-                for (int i = 0; i < 4; i++) acc.o[e][i] = __builtin_fmaf(acc.o[e][i], 0x1p24f, y);
+            for (int i = 0; i < 4; i++) acc.o[e][i] = from(__builtin_fmaf(acc.o[e][i], 0x1p24f, ms[gq / NGS]), gq % NGS);
         }
+        acc.l = from(sum_x32(sum_x16(__builtin_fmaf(l_odd, odd, l))), 0);
+        acc.m = from(m == -INFINITY ? m : m + (float)es, 0);
     }
 
     static __device__ __forceinline__ constexpr int dim(int e, int gr, int i) { return 16 * e + 4 * gr + i; }
 };
 
+// Bytes of LDS a wave: its chunk, then its sums
+template <typename TL>
+constexpr int kQWaveBytes = TL::VB > 16 * (TL::D + 4) * 4 ? TL::VB : 16 * (TL::D + 4) * 4;
+
+// The block's output from its NW waves' sums: wm, wl [.][16] and os [16 NW][D + 4]; n heads, 4 dims a thread.
+template <typename TL, int NW>
+__device__ __forceinline__ void paged_q_join(typename TL::T* __restrict__ out, const float (*wm)[16], const float (*wl)[16],
+                                             const float* os, int32_t n)
+{
+    constexpr int D = TL::D, OP = D + 4;
+    for (int idx = threadIdx.x; idx < n * (D / 4); idx += 64 * NW) {
+        const int h = idx / (D / 4), d = (idx - h * (D / 4)) * 4;
+        float m[NW], M = -INFINITY, den = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NW; i++) {
+            m[i] = wm[i][h];
+            M = fmaxf(M, m[i]);
+        }
+        const float Mb = M == -INFINITY ? 0.0f : M;
+        f4 num = {};
+#pragma unroll
+        for (int i = 0; i < NW; i++) {
+            const float f = __builtin_amdgcn_exp2f(m[i] - Mb);
+            num += *reinterpret_cast<const f4*>(os + (i * 16 + h) * OP + d) * f;
+            den = __builtin_fmaf(f, wl[i][h], den);
+        }
+        const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+#pragma unroll
+        for (int i = 0; i < 4; i++) out[h * D + d + i] = (typename TL::T)(num[i] * inv);
+    }
+}
+
+// One tile of one sequence by one block of 1, 2, 4 or 8 waves, each every so many-th chunk, merged through LDS (a wave by itself
+// has its sums in registers).
 template <typename TL>
 __global__ __launch_bounds__(512, 2) void k_attention_paged_q_one(PagedQArgs c, typename TL::T* __restrict__ out,
                                                                   const typename TL::T* __restrict__ q,
                                                                   const int32_t* __restrict__ lens, PagedHeads hd, int32_t H,
                                                                   float scale_log2)
 {
-    paged_one<TL, 8>(c, out, q, lens, hd, H, scale_log2);
+    constexpr int D = TL::D, CH = TL::CH, OP = D + 4;
+    extern __shared__ __align__(16) char smem[];
+    __shared__ float wm[8][16], wl[8][16];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, gr = lane >> 4;
+    const int NW = blockDim.x >> 6;
+    const int32_t s = blockIdx.y, len = paged_len(c, lens, s);
+    int32_t g, h0, n;
+    hd.at(blockIdx.x, g, h0, n);
+    const int64_t row0 = (int64_t)s * H + h0;
+    typename TL::Q x;
+    TL::load_q(q + row0 * D, n, lane, x);
+    PagedAcc<D> acc;
+    TL::tile(c, g, s, x, w * CH, NW * CH, len, scale_log2, smem + w * kQWaveBytes<TL>, lane, acc);
+    if (len <= CH) {  // all of it is the first wave's
+        const float inv = acc.l == 0.0f ? 0.0f : 1.0f / acc.l;
+        if (w == 0 && r < n) {
+#pragma unroll
+            for (int e = 0; e < D / 16; e++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) out[(row0 + r) * D + TL::dim(e, gr, i)] = (typename TL::T)(acc.o[e][i] * inv);
+        }
+        return;
+    }
+    if (NW > 1) __syncthreads();
+    float* os = reinterpret_cast<float*>(smem);
+    if (gr == 0) {
+        wm[w][r] = acc.m;
+        wl[w][r] = acc.l;
+    }
+    if (r < n) {
+#pragma unroll
+        for (int e = 0; e < D / 16; e++) *reinterpret_cast<f4*>(os + (w * 16 + r) * OP + TL::dim(e, gr, 0)) = acc.o[e];
+    }
+    __syncthreads();
+    typename TL::T* to = out + row0 * D;
+    if (NW == 8) paged_q_join<TL, 8>(to, wm, wl, os, n);
+    else if (NW == 4) paged_q_join<TL, 4>(to, wm, wl, os, n);
+    else if (NW == 2) paged_q_join<TL, 2>(to, wm, wl, os, n);
+    else paged_q_join<TL, 1>(to, wm, wl, os, n);
 }
 template <typename TL>
-__global__ __launch_bounds__(256, 2) void k_attention_paged_q_split(PagedQArgs c, typename TL::T* __restrict__ out,
+__global__ __launch_bounds__(256, QWAVES) void k_attention_paged_q_split(PagedQArgs c, typename TL::T* __restrict__ out,
                                                                     const typename TL::T* __restrict__ q,
                                                                     const int32_t* __restrict__ lens, PagedHeads hd, int32_t H,
                                                                     float scale_log2, int64_t* __restrict__ before_out,
@@ -552,9 +670,14 @@ AttnPagedPlan attention_paged_q_plan(const PagedQArgs& c, int64_t max_len, int64
     p.tiled = true;
     p.tiles = (G + 15) / 16;
     p.GT = (G + p.tiles - 1) / p.tiles;
-    p.waves = 8;
+    // columns of a head: as many of its groups as 16 columns hold
+    p.columns = 1;
+    while (p.columns * 2 < 2 * (c.D / c.group) && p.GT * p.columns * 2 <= 16) p.columns *= 2;
     const int64_t cap = (int64_t)c.max_pages * c.P, ch = c.vb == 4 ? 64 : 32;
     const int64_t chunks = ((max_len > 0 && max_len < cap ? max_len : cap) + ch - 1) / ch;
+    // a wave for each chunk, but no more than the device holds at a time
+    p.waves = 1;
+    while (p.waves < 8 && p.waves < chunks && p.waves * 2 * c.B * c.KVH * p.tiles <= 8 * cus) p.waves *= 2;
     if (chunks > kQOneChunks) p.blocks = std::min<int64_t>((chunks * c.B * c.KVH * p.tiles + 3) / 4, 2 * cus);
     if (p.blocks > 0) p.ws_floats = paged_before_floats(c.B) + p.blocks * 4 * 2 * p.GT * (c.D + 4);
     return p;
@@ -567,8 +690,8 @@ static void paged_q_go(const AttnPagedPlan& p, const PagedQArgs& c, typename TL:
     const PagedHeads hd{(int32_t)(H / c.KVH), (int32_t)p.GT, (int32_t)p.tiles};
     const int32_t VH = (int32_t)(c.KVH * p.tiles);
     if (p.blocks == 0) {
-        hipLaunchKernelGGL((k_attention_paged_q_one<TL>), dim3((unsigned)VH, (unsigned)c.B), dim3(512), 0, s, c, out, q, lens, hd,
-                           (int32_t)H, scale_log2);
+        hipLaunchKernelGGL((k_attention_paged_q_one<TL>), dim3((unsigned)VH, (unsigned)c.B), dim3((unsigned)(64 * p.waves)),
+                           (unsigned)(p.waves * kQWaveBytes<TL>), s, c, out, q, lens, hd, (int32_t)H, scale_log2);
         return;
     }
     int64_t* before = reinterpret_cast<int64_t*>(ws);
@@ -586,28 +709,30 @@ int launch_attention_paged_q(const AttnPagedPlan& p, const PagedQArgs& c, void* 
                              float scale, float* ws, int dtype, void* stream)
 {
     const float sl = (float)((double)scale * 1.4426950408889634);  // scores in log2 units
-    auto run = [&](auto* t, auto d, auto ng, auto kb, auto vb) {
+    auto run = [&](auto* t, auto d, auto ng, auto ngs) {
         using T = std::remove_pointer_t<decltype(t)>;
-        paged_q_go<PagedQTiles<T, decltype(d)::value, decltype(ng)::value, decltype(kb)::value, decltype(vb)::value>>(
-            p, c, (T*)out, (const T*)q, lens, H, sl, ws, static_cast<hipStream_t>(stream));
+        constexpr int D = decltype(d)::value, NG = decltype(ng)::value, NGS = decltype(ngs)::value;
+        auto go = [&](auto tl) {
+            paged_q_go<decltype(tl)>(p, c, (T*)out, (const T*)q, lens, H, sl, ws, static_cast<hipStream_t>(stream));
+        };
+        c.kb == 4   ? go(PagedQTiles<T, D, NG, NGS, 4, 4>{})
+        : c.vb == 4 ? go(PagedQTiles<T, D, NG, NGS, 8, 4>{})
+                    : go(PagedQTiles<T, D, NG, NGS, 8, 8>{});
     };
-    auto bits = [&](auto* t, auto d, auto ng) {
-        constexpr std::integral_constant<int, 4> four{};
-        constexpr std::integral_constant<int, 8> eight{};
-        c.kb == 4 ? run(t, d, ng, four, four) : c.vb == 4 ? run(t, d, ng, eight, four) : run(t, d, ng, eight, eight);
-    };
+    constexpr std::integral_constant<int, 1> n1{};
+    constexpr std::integral_constant<int, 2> n2{};
+    constexpr std::integral_constant<int, 3> n3{};
+    constexpr std::integral_constant<int, 4> n4{};
+    constexpr std::integral_constant<int, 64> d64{};
+    constexpr std::integral_constant<int, 96> d96{};
+    constexpr std::integral_constant<int, 128> d128{};
+    auto columns2 = [&](auto* t, auto d, auto ng) { p.columns == 1 ? run(t, d, ng, n1) : run(t, d, ng, n2); };
+    auto columns4 = [&](auto* t, auto d, auto ng) { p.columns == 4 ? run(t, d, ng, n4) : columns2(t, d, ng); };
     auto shape = [&](auto* t) {
-        constexpr std::integral_constant<int, 1> g1{};
-        constexpr std::integral_constant<int, 2> g2{};
-        constexpr std::integral_constant<int, 3> g3{};
-        constexpr std::integral_constant<int, 4> g4{};
-        constexpr std::integral_constant<int, 64> d64{};
-        constexpr std::integral_constant<int, 96> d96{};
-        constexpr std::integral_constant<int, 128> d128{};
         const int ng = c.D / c.group;
-        if (c.D == 64) ng == 1 ? bits(t, d64, g1) : bits(t, d64, g2);
-        else if (c.D == 96) bits(t, d96, g3);
-        else ng == 1 ? bits(t, d128, g1) : ng == 2 ? bits(t, d128, g2) : bits(t, d128, g4);
+        if (c.D == 64) ng == 1 ? run(t, d64, n1, n1) : columns2(t, d64, n2);
+        else if (c.D == 96) columns4(t, d96, n3);
+        else ng == 1 ? run(t, d128, n1, n1) : ng == 2 ? columns2(t, d128, n2) : columns4(t, d128, n4);
     };
     dtype == VVH_F16 ? shape((f16*)nullptr) : shape((float*)nullptr);
     return (int)hipGetLastError();

@@ -1,6 +1,7 @@
 // Attention of one query per sequence over a paged cache, whatever its rows hold: a tile of up to 16 query heads of one kv
 // head is a wave's work on a chunk of keys, and here is how a batch's tiles and chunks are shared out and joined.  A class TL
-// of static members says the rest: Args (the cache; B, P, max_pages), T (queries and outputs), D, CH (keys of a chunk), VB
+// of static members says the rest: Args (the cache; B, P, max_pages), T (queries and outputs), D, CH (keys of a chunk), HEAD
+// (chunks that the beginning of a tile is as long as: what comes before the first chunk's products counts in a batch of short contexts), VB
 // (bytes of LDS a wave), Q (a tile's queries in registers), load_q, tile (the chunks c0, c0 + cstep, ... below ke of sequence s
 // and kv head g), dim (of accumulator element (e, lane group, i)).
 #pragma once
@@ -93,11 +94,13 @@ __device__ __forceinline__ void paged_one(const typename TL::Args& c, typename T
     }
 }
 
-// Chunks of the 64 sequences from s0 on, one a lane, and their sums up to each lane.
-template <typename Args>
-__device__ __forceinline__ int32_t paged_window(const Args& c, const int32_t* lens, int32_t s0, int lane, int ch)
+// Units of the 64 sequences from s0 on, one a lane, and their sums up to each lane: a sequence's chunks, and TL::HEAD for
+// the beginning of a tile, where there is any.
+template <typename TL>
+__device__ __forceinline__ int32_t paged_window(const typename TL::Args& c, const int32_t* lens, int32_t s0, int lane)
 {
-    return s0 + lane < c.B ? (paged_len(c, lens, s0 + lane) + ch - 1) / ch : 0;
+    const int32_t n = s0 + lane < c.B ? (paged_len(c, lens, s0 + lane) + TL::CH - 1) / TL::CH : 0;
+    return n > 0 ? n + TL::HEAD : 0;
 }
 // Sums over lanes 0 .. l in lane l (shifts within rows of 16, then the rows' last lanes broadcast).
 __device__ __forceinline__ uint32_t wave_scan(uint32_t v)
@@ -145,7 +148,7 @@ __device__ __forceinline__ void paged_split(const typename TL::Args& c, typename
     // the sums of the chunks before each sequence, and of all: the first wave keeps them for the merge
     int64_t total = 0;
     for (int32_t s0 = 0; s0 < c.B; s0 += 64) {
-        const uint32_t upto = wave_scan((uint32_t)paged_window(c, lens, s0, lane, CH));  // at most 64 * 2^25
+        const uint32_t upto = wave_scan((uint32_t)paged_window<TL>(c, lens, s0, lane));  // at most 64 * 2^25
         if (w == 0 && s0 + lane < c.B) before_out[s0 + lane + 1] = total + upto;
         total += lane_of(upto, 63);
     }
@@ -158,13 +161,13 @@ __device__ __forceinline__ void paged_split(const typename TL::Args& c, typename
     auto begin_of = [&](int l) { return lane_of64(begin, l); };
     const int64_t u0 = begin_of(wb), u1 = begin_of(wb + 1);
     // the window of sequences that holds unit u0
-    int32_t s0 = 0, n = paged_window(c, lens, 0, lane, CH);
+    int32_t s0 = 0, n = paged_window<TL>(c, lens, 0, lane);
     int64_t before = 0;
     uint32_t upto = wave_scan((uint32_t)n);
     while ((before + lane_of(upto, 63)) * VH <= u0) {
         before += lane_of(upto, 63);
         s0 += 64;
-        n = paged_window(c, lens, s0, lane, CH);
+        n = paged_window<TL>(c, lens, s0, lane);
         upto = wave_scan((uint32_t)n);
     }
     int sl = __builtin_ctzll(__ballot((before + upto) * VH > u0));  // the sequence's lane
@@ -184,8 +187,9 @@ __device__ __forceinline__ void paged_split(const typename TL::Args& c, typename
         TL::load_q(q + row0 * D, nh, lane, x);
         PagedAcc<D> acc;
         const int32_t len = __builtin_amdgcn_readfirstlane(paged_len(c, lens, s));
-        const int64_t end = (int64_t)(ci + cnt) * CH;
-        TL::tile(c, g, s, x, ci * CH, CH, end < len ? (int32_t)end : len, scale_log2, smem + wb * VB, lane, acc);
+        const int32_t first = ci > TL::HEAD ? ci - TL::HEAD : 0;  // chunk; a range of the tile's head alone has none
+        const int64_t end = (int64_t)(ci + cnt - TL::HEAD) * CH;
+        TL::tile(c, g, s, x, first * CH, CH, end < len ? (int32_t)end : len, scale_log2, smem + wb * VB, lane, acc);
         if (inside) {
             __syncthreads();
             float* os = reinterpret_cast<float*>(smem);
@@ -245,7 +249,7 @@ __device__ __forceinline__ void paged_split(const typename TL::Args& c, typename
             uint64_t more = __ballot(n > 0) & (sl == 63 ? 0 : ~0ull << (sl + 1));
             while (!more) {
                 s0 += 64;
-                n = paged_window(c, lens, s0, lane, CH);
+                n = paged_window<TL>(c, lens, s0, lane);
                 more = __ballot(n > 0);
             }
             sl = __builtin_ctzll(more);
