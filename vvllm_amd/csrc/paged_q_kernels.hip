@@ -45,7 +45,9 @@ __device__ __forceinline__ float pair_scale(uint32_t x) { return (float)__builti
 __device__ __forceinline__ float pair_min(uint32_t x) { return (float)__builtin_bit_cast(h2, x)[1]; }
 
 // Codes of a lane's 8 values, whose group is the `lanes` lanes around it, to `to`; the group's first lane writes {s, m}.
-// In 64 bits: a code is a choice between two neighbours, and half of them would be another one where a last bit differs.
+// A code is a choice between two neighbours, and the formula's in 64 bits.  In 32 bits the level (x - m) / s is off by at most
+// 2^-22 of itself (a difference, a reciprocal of one step, a product): where it is further than that from the middle of
+// two levels its nearest is the exact one's, else (4 bits: one value in 65536, and real ties) the lane takes 64 bits.
 __device__ __forceinline__ void quantise8(const float (&x)[8], int bits, int lanes, uint8_t* to, uint32_t* sm, bool first)
 {
     float lo = x[0], hi = x[0], z = 0.0f;
@@ -59,32 +61,48 @@ __device__ __forceinline__ void quantise8(const float (&x)[8], int bits, int lan
     hi = group_max(hi, lanes);
     const bool fine = group_max(z == 0.0f ? 0.0f : 1.0f, lanes) == 0.0f;
     const float top = bits == 8 ? 255.0f : 15.0f;
-    const f16 m = (f16)fminf(fmaxf(lo, -65504.0f), 65504.0f);
-    const f16 s = (f16)fminf(fmaxf((float)(((double)hi - (double)m) / (double)top), -65504.0f), 65504.0f);
+    const f16 m = (f16)__builtin_amdgcn_fmed3f(lo, -65504.0f, 65504.0f);
+    // (hi - m) / top in 64 bits: by the reciprocal and its remainder, which is the quotient rounded once
+    const double r = bits == 8 ? 1.0 / 255.0 : 1.0 / 15.0, range = (double)hi - (double)m, q0 = range * r;
+    const double quot = __builtin_fma(__builtin_fma(-(double)top, q0, range), r, q0);
+    const f16 s = (f16)__builtin_amdgcn_fmed3f((float)quot, -65504.0f, 65504.0f);
     if (first) *sm = fine ? scale_pair((float)s, (float)m) : 0x7e007e00u;
     uint32_t w[2] = {0, 0};
     if (fine && s != (f16)0.0f) {
+        const float rs = __builtin_amdgcn_rcpf((float)s);
+        float c[8], far = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const double level = __builtin_rint(((double)x[i] - (double)m) / (double)s);
-            const uint32_t c = (uint32_t)fminf(fmaxf((float)level, 0.0f), top);
-            if (bits == 8) w[i / 4] |= c << (8 * (i % 4));
-            else w[0] |= c << (4 * i);
+            const float level = (x[i] - (float)m) * rs;
+            c[i] = __builtin_rintf(level);
+            far = fmaxf(far, __builtin_fabsf(level - c[i]));
+        }
+        if (far > 0.5f - (bits == 8 ? 0x1p-13f : 0x1p-17f)) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) c[i] = (float)__builtin_rint(((double)x[i] - (double)m) / (double)s);
+        }
+        // bytes, within 0 .. 255 by the conversion; 4 bits: those of even and of odd codes, then as halves of bytes
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int word = bits == 8 ? i / 4 : i % 2, byte = bits == 8 ? i % 4 : i / 2;
+            w[word] = __builtin_amdgcn_cvt_pk_u8_f32(fminf(c[i], top), byte, w[word]);
         }
     }
     if (bits == 8) *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
-    else *reinterpret_cast<uint32_t*>(to) = w[0];
+    else *reinterpret_cast<uint32_t*>(to) = w[0] | w[1] << 4;
 }
 
 // A block a token.  Items: 8 dims of a key (its own 8 values and the 8 that the rotation pairs them with), 8 of a value,
-// or 8 pairs of a query head.  A group is 4, 8 or 16 lanes in a row of one wave.
-template <typename T>
+// or 8 pairs of a query head.  A group is 4, 8 or 16 lanes in a row of one wave.  4001 tokens of 32 query and 8 kv heads of
+// 128 in fp16 to 4 bits, 88 MB: APPEND_US.
+template <typename T, int D>
 __global__ __launch_bounds__(512) void k_rope_append_paged_q(PagedQArgs c, T* q_out, const T* q, const T* __restrict__ k,
                                                              const T* __restrict__ v, const int32_t* __restrict__ seqs,
                                                              const int32_t* __restrict__ positions, int32_t H,
                                                              const float* __restrict__ rope, int32_t rope_positions)
 {
-    const int32_t D = c.D, half = D / 2, per = D / 8, kvu = c.KVH * per, items = 2 * kvu + H * (half / 8);
+    constexpr int half = D / 2, per = D / 8;
+    const int32_t kvu = c.KVH * per, items = 2 * kvu + H * (half / 8);
     const int64_t t = blockIdx.x;
     const int32_t s = seqs ? seqs[t] : (int32_t)t, p = positions[t];
     if (rope && p >= rope_positions) return;
@@ -94,7 +112,7 @@ __global__ __launch_bounds__(512) void k_rope_append_paged_q(PagedQArgs c, T* q_
     for (int32_t i = threadIdx.x; i < items; i += blockDim.x) {
         if (i < 2 * kvu) {
             const bool key = i < kvu;
-            const int32_t h = (key ? i : i - kvu) / per, u = (key ? i : i - kvu) - h * per;
+            const int32_t j = key ? i : i - kvu, h = j / per, u = j - h * per;
             const T* src = (key ? k : v) + (t * c.KVH + h) * D;
             const Eight<T> a = *reinterpret_cast<const Eight<T>*>(src + 8 * u);
             float x[8];
@@ -137,41 +155,73 @@ __global__ __launch_bounds__(512) void k_rope_append_paged_q(PagedQArgs c, T* q_
     }
 }
 
-// A thread 8 dims of a key or a value: a unit of codes, its group's {s, m}, 8 values.  A block a token after another.
-template <typename T>
+// A block takes up to 32 tokens: their rows are looked up first, then a wave takes the keys or the values of one kv head at a
+// time (gridDim.y blocks share them), 64 pieces of its tokens' rows together, which lie in a row where the tokens do.  A piece
+// is 16 bytes of output; UN of them a lane are on their way at a time (a token left out loads row 0).  READ_US
+constexpr int kReadTokens = 32;
+template <typename T, int D, int UN>
 __global__ __launch_bounds__(256) void k_read_paged_q(PagedQArgs c, T* __restrict__ k_out, T* __restrict__ v_out,
                                                       const int32_t* __restrict__ seqs, const int32_t* __restrict__ positions,
-                                                      int64_t tokens)
+                                                      int64_t tokens, int32_t each)
 {
-    const int32_t D = c.D, per = D / 8, kvu = c.KVH * per, lanes = c.group / 8;
-    const int32_t mine = (256 + 2 * kvu - 1) / (2 * kvu);  // tokens of a block
-    const int64_t t0 = (int64_t)blockIdx.x * mine;
-    const int32_t n = tokens - t0 < mine ? (int32_t)(tokens - t0) : mine;
-    for (int32_t i = threadIdx.x; i < n * 2 * kvu; i += 256) {
-        const int32_t tt = i / (2 * kvu), j = i - tt * 2 * kvu;
-        const bool key = j < kvu;
+    constexpr int V = 16 / sizeof(T), per = D / V;
+    struct __attribute__((aligned(16))) Out {
+        T v[V];
+    };
+    __shared__ int64_t rows[kReadTokens];
+    const int64_t t0 = (int64_t)blockIdx.x * each;
+    const int32_t n = tokens - t0 < each ? (int32_t)(tokens - t0) : each, lane = threadIdx.x & 63;
+    if ((int32_t)threadIdx.x < n) {
+        const int64_t t = t0 + threadIdx.x;
+        rows[threadIdx.x] = paged_q_row(c, seqs ? seqs[t] : (int32_t)t, positions[t]);
+    }
+    __syncthreads();
+    const int32_t NG = D / c.group, glog = __builtin_ctz(c.group / V);
+    for (int32_t part = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); part < 2 * c.KVH; part += gridDim.y * 4) {
+        const bool key = part < c.KVH;
         T* out = key ? k_out : v_out;
         if (!out) continue;
-        const int64_t t = t0 + tt;
-        const int64_t row = paged_q_row(c, seqs ? seqs[t] : (int32_t)t, positions[t]);
-        if (row < 0) continue;
-        const int32_t h = (key ? j : j - kvu) / per, u = (key ? j : j - kvu) - h * per;
-        const int bits = key ? c.kb : c.vb;
-        const int64_t r = row + (int64_t)h * c.P;
-        const uint8_t* at = (key ? c.kp : c.vp) + r * (D * bits / 8) + (key ? key_unit(u, D) : u) * bits;
-        const uint32_t sm = (key ? c.ks : c.vs)[r * (D / c.group) + u / lanes];
-        const float s = pair_scale(sm), m = pair_min(sm);
-        Eight<T> y;
-        if (bits == 8) {
-            const uint2 w = *reinterpret_cast<const uint2*>(at);
+        const int32_t h = key ? part : part - c.KVH;
+        const uint8_t* held = key ? c.kp : c.vp;
+        const uint32_t* scales = key ? c.ks : c.vs;
+        auto some = [&](auto b) {
+            constexpr int B = decltype(b)::value;
+            typedef typename std::conditional<V * B == 16, uint16_t, typename std::conditional<V * B == 32, uint32_t, uint2>::type>::type Codes;
+            for (int32_t i0 = lane; i0 < n * per; i0 += 64 * UN) {
+                Codes w[UN];
+                uint32_t sm[UN];
+                int64_t to[UN];
 #pragma unroll
-            for (int e = 0; e < 8; e++) y.v[e] = (T)__builtin_fmaf(s, (float)((e < 4 ? w.x : w.y) >> (8 * (e % 4)) & 255), m);
-        } else {
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(at);
+                for (int j = 0; j < UN; j++) {
+                    const int32_t i = i0 + 64 * j < n * per ? i0 + 64 * j : 0, tt = i / per, u = i - tt * per;
+                    const int64_t row = rows[tt], r = (row < 0 ? 0 : row) + (int64_t)h * c.P;
+                    to[j] = row < 0 || i0 + 64 * j >= n * per ? -1 : ((t0 + tt) * c.KVH + h) * D + V * u;
+                    const int32_t place = key ? key_unit(V * u / 8, D) * 8 + V * u % 8 : V * u;  // of the piece's codes
+                    w[j] = *reinterpret_cast<const Codes*>(held + r * (D * B / 8) + place * B / 8);
+                    sm[j] = scales[r * NG + (u >> glog)];
+                }
 #pragma unroll
-            for (int e = 0; e < 8; e++) y.v[e] = (T)__builtin_fmaf(s, (float)(w >> (4 * e) & 15), m);
-        }
-        *reinterpret_cast<Eight<T>*>(out + (t * c.KVH + h) * D + 8 * u) = y;
+                for (int j = 0; j < UN; j++) {
+                    const float s = pair_scale(sm[j]), m = pair_min(sm[j]);
+                    uint32_t x[2];  // bytes: the codes in order, or of 4 bits the even and the odd ones
+                    if constexpr (V * B == 64) {
+                        x[0] = w[j].x;
+                        x[1] = w[j].y;
+                    } else {
+                        x[0] = B == 8 ? (uint32_t)w[j] : (uint32_t)w[j] & 0x0f0f0f0fu;
+                        x[1] = B == 8 ? 0 : (uint32_t)w[j] >> 4 & 0x0f0f0f0fu;
+                    }
+                    Out y;
+#pragma unroll
+                    for (int e = 0; e < V; e++) {
+                        const int word = B == 8 ? e / 4 : e % 2, byte = B == 8 ? e % 4 : e / 2;
+                        y.v[e] = (T)__builtin_fmaf(s, (float)(x[word] >> (8 * byte) & 255), m);
+                    }
+                    if (to[j] >= 0) *reinterpret_cast<Out*>(out + to[j]) = y;
+                }
+            }
+        };
+        (key ? c.kb : c.vb) == 8 ? some(std::integral_constant<int, 8>{}) : some(std::integral_constant<int, 4>{});
     }
 }
 
@@ -640,23 +690,39 @@ int launch_rope_append_paged_q(const PagedQArgs& c, void* q_out, const void* q, 
                                (int32_t)rope_positions);
         }
     };
-    dtype == VVH_F16 ? go(k_rope_append_paged_q<f16>, (f16*)nullptr) : go(k_rope_append_paged_q<float>, (float*)nullptr);
+    auto dims = [&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        c.D == 64 ? go(k_rope_append_paged_q<T, 64>, t) : c.D == 96 ? go(k_rope_append_paged_q<T, 96>, t) : go(k_rope_append_paged_q<T, 128>, t);
+    };
+    dtype == VVH_F16 ? dims((f16*)nullptr) : dims((float*)nullptr);
     return (int)hipGetLastError();
 }
 
 int launch_read_paged_q(const PagedQArgs& c, void* k_out, void* v_out, const int32_t* seqs, const int32_t* positions,
                         int64_t tokens, int dtype, void* stream)
 {
-    const int64_t kvu = (int64_t)c.KVH * (c.D / 8), mine = (256 + 2 * kvu - 1) / (2 * kvu);
+    // tokens of a block: as many as leave 1024 blocks of 4 parts (a head's keys or values)
+    const int64_t parts = (2 * (int64_t)c.KVH + 3) / 4;
+    int64_t each = kReadTokens;
+    while (each > 4 && (tokens + each - 1) / each * parts < 1024) each /= 2;
     auto go = [&](auto kern, auto* type) {
         using T = std::remove_pointer_t<decltype(type)>;
         for (int64_t t = 0; t < tokens; t += kQTokens) {  // as above
             const int64_t n = std::min(tokens - t, kQTokens), kd = t * c.KVH * c.D;
-            hipLaunchKernelGGL(kern, dim3((unsigned)((n + mine - 1) / mine)), dim3(256), 0, static_cast<hipStream_t>(stream), c,
-                               (T*)k_out + (k_out ? kd : 0), (T*)v_out + (v_out ? kd : 0), seqs ? seqs + t : nullptr, positions + t, n);
+            hipLaunchKernelGGL(kern, dim3((unsigned)((n + each - 1) / each), (unsigned)parts), dim3(256), 0,
+                               static_cast<hipStream_t>(stream), c, (T*)k_out + (k_out ? kd : 0), (T*)v_out + (v_out ? kd : 0),
+                               seqs ? seqs + t : nullptr, positions + t, n, (int32_t)each);
         }
     };
-    dtype == VVH_F16 ? go(k_read_paged_q<f16>, (f16*)nullptr) : go(k_read_paged_q<float>, (float*)nullptr);
+    // 8 pieces a lane at a time where a block has as many, else 2 (40 contexts of up to 2000 tokens, 8 heads of 128, 23.6 us, 2
+    // at a time 29.7; one of 1500, 2 heads of 64, with 8 4.1, with 2 3.1)
+    auto dims = [&](auto* t, auto un) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        constexpr int UN = decltype(un)::value;
+        c.D == 64 ? go(k_read_paged_q<T, 64, UN>, t) : c.D == 96 ? go(k_read_paged_q<T, 96, UN>, t) : go(k_read_paged_q<T, 128, UN>, t);
+    };
+    auto types = [&](auto un) { dtype == VVH_F16 ? dims((f16*)nullptr, un) : dims((float*)nullptr, un); };
+    each == kReadTokens ? types(std::integral_constant<int, 8>{}) : types(std::integral_constant<int, 2>{});
     return (int)hipGetLastError();
 }
 
