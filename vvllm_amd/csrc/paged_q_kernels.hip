@@ -14,6 +14,9 @@
 #ifndef QWAVES
 #define QWAVES 2
 #endif
+#ifndef QBLK
+#define QBLK 2
+#endif
 #ifndef QHEAD
 #define QHEAD 2
 #endif
@@ -291,7 +294,12 @@ struct PagedQTiles {
     static constexpr int SR = CH + 16, SW = NG * SR;                         // words of a group's scales in LDS, of a chunk's
     static constexpr int VB = CH * VP + 2 * SW * 4;
     static constexpr bool TWO = sizeof(T) == 4;
+    // Lane (r, gr): dims 32 s + 8 gr .. + 7 of head r / NGS
     struct Q {
+        Eight<T> v[DS];
+    };
+    // The same as an operand, in the order of the codes
+    struct Operand {
         h8 hi[DS], lo[TWO ? DS : 1];
         float sum[NP];  // of the column's groups, times 2^-24
         int e;
@@ -303,21 +311,23 @@ struct PagedQTiles {
         return NG % NGS == 0 || g < NG ? g : NG - 1;
     }
 
-    // Lane (r, gr): dims 32 s + 8 gr .. + 7 of head r / NGS, in the order of the codes.
     static __device__ __forceinline__ void load_q(const T* q, int heads, int lane, Q& x)
     {
-        const int r = lane & 15, gr = lane >> 4, h = r / NGS;
+        const int h = (lane & 15) / NGS, gr = lane >> 4;
+#pragma unroll
+        for (int s = 0; s < DS; s++) x.v[s] = h < heads ? *reinterpret_cast<const Eight<T>*>(q + h * D + 32 * s + 8 * gr) : Eight<T>{};
+    }
+    static __device__ __forceinline__ void prepare(const Q& q, int lane, Operand& x)
+    {
+        const int r = lane & 15;
         float v[DS][8], mx = 0.0f;
 #pragma unroll
-        for (int s = 0; s < DS; s++) {
-            Eight<T> a = {};
-            if (h < heads) a = *reinterpret_cast<const Eight<T>*>(q + h * D + 32 * s + 8 * gr);
+        for (int s = 0; s < DS; s++)
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                v[s][j] = (float)a.v[j];
+                v[s][j] = (float)q.v[s].v[j];
                 mx = fmaxf(mx, __builtin_fabsf(v[s][j]));
             }
-        }
         mx = max_x32(max_x16(mx));
         x.e = mx == 0.0f ? 0 : 137 - (int)(__builtin_bit_cast(uint32_t, mx) >> 23);
 #pragma unroll
@@ -355,19 +365,6 @@ struct PagedQTiles {
         const int r = lane & 15, gr = lane >> 4;
         uint32_t* const lk = reinterpret_cast<uint32_t*>(lds + CH * VP);
         uint32_t* const lv = lk + SW;
-        // scores to log2 units: positive (a negative scale turns q's sign), never 0, so that the maximum of the scores is
-        // that of the products and -infinity stays (2^-100 times any score is 0 for the exponential)
-        const float kl = fmaxf(__builtin_fabsf(__builtin_ldexpf(scale_log2, 24 - q0.e)), 0x1p-100f);
-        Q q = q0;
-        if (scale_log2 < 0.0f) {
-#pragma unroll
-            for (int x = 0; x < DS; x++) {
-                q.hi[x] = -q.hi[x];
-                if constexpr (TWO) q.lo[x] = -q.lo[x];
-            }
-#pragma unroll
-            for (int p = 0; p < NP; p++) q.sum[p] = -q.sum[p];
-        }
         float minus = -1.0f;
         asm("" : "+s"(minus));
         acc.clear();
@@ -411,6 +408,20 @@ struct PagedQTiles {
         load_v(locate(spot, c0));
         load_k();
         spot = look(c, s, c0 + cstep, lane);
+        Operand q;  // worked out while the first chunk is on its way
+        prepare(q0, lane, q);
+        // scores to log2 units: positive (a negative scale turns q's sign), never 0, so that the maximum of the scores is
+        // that of the products and -infinity stays (2^-100 times any score is 0 for the exponential)
+        const float kl = fmaxf(__builtin_fabsf(__builtin_ldexpf(scale_log2, 24 - q.e)), 0x1p-100f);
+        if (scale_log2 < 0.0f) {
+#pragma unroll
+            for (int x = 0; x < DS; x++) {
+                q.hi[x] = -q.hi[x];
+                if constexpr (TWO) q.lo[x] = -q.lo[x];
+            }
+#pragma unroll
+            for (int p = 0; p < NP; p++) q.sum[p] = -q.sum[p];
+        }
         for (; c0 < ke; c0 += cstep) {
             const uint64_t live = __ballot(on);
             const bool all = CH == 64 ? live == ~0ull : (uint32_t)live == ~0u;
@@ -744,7 +755,7 @@ AttnPagedPlan attention_paged_q_plan(const PagedQArgs& c, int64_t max_len, int64
     // a wave for each chunk, but no more than the device holds at a time
     p.waves = 1;
     while (p.waves < 8 && p.waves < chunks && p.waves * 2 * c.B * c.KVH * p.tiles <= 8 * cus) p.waves *= 2;
-    if (chunks > kQOneChunks) p.blocks = std::min<int64_t>((chunks * c.B * c.KVH * p.tiles + 3) / 4, 2 * cus);
+    if (chunks > kQOneChunks) p.blocks = std::min<int64_t>((chunks * c.B * c.KVH * p.tiles + 3) / 4, QBLK * cus);
     if (p.blocks > 0) p.ws_floats = paged_before_floats(c.B) + p.blocks * 4 * 2 * p.GT * (c.D + 4);
     return p;
 }

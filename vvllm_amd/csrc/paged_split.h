@@ -147,10 +147,17 @@ __device__ __forceinline__ void paged_split(const typename TL::Args& c, typename
     const int64_t w = (int64_t)blockIdx.x * 4 + wb;
     // the sums of the chunks before each sequence, and of all: the first wave keeps them for the merge
     int64_t total = 0;
+    int32_t n = 0;  // the first 64 sequences' units, and their sums
+    uint32_t upto = 0;
     for (int32_t s0 = 0; s0 < c.B; s0 += 64) {
-        const uint32_t upto = wave_scan((uint32_t)paged_window<TL>(c, lens, s0, lane));  // at most 64 * 2^25
-        if (w == 0 && s0 + lane < c.B) before_out[s0 + lane + 1] = total + upto;
-        total += lane_of(upto, 63);
+        const int32_t m = paged_window<TL>(c, lens, s0, lane);
+        const uint32_t sums = wave_scan((uint32_t)m);  // at most 64 * 2^25
+        if (s0 == 0) {
+            n = m;
+            upto = sums;
+        }
+        if (w == 0 && s0 + lane < c.B) before_out[s0 + lane + 1] = total + sums;
+        total += lane_of(sums, 63);
     }
     if (w == 0 && lane == 0) before_out[0] = 0;
     total *= VH;
@@ -161,9 +168,8 @@ __device__ __forceinline__ void paged_split(const typename TL::Args& c, typename
     auto begin_of = [&](int l) { return lane_of64(begin, l); };
     const int64_t u0 = begin_of(wb), u1 = begin_of(wb + 1);
     // the window of sequences that holds unit u0
-    int32_t s0 = 0, n = paged_window<TL>(c, lens, 0, lane);
+    int32_t s0 = 0;
     int64_t before = 0;
-    uint32_t upto = wave_scan((uint32_t)n);
     while ((before + lane_of(upto, 63)) * VH <= u0) {
         before += lane_of(upto, 63);
         s0 += 64;
