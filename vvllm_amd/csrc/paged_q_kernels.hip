@@ -11,15 +11,6 @@
 #include "device.h"
 #include "paged_split.h"
 
-#ifndef QWAVES
-#define QWAVES 2
-#endif
-#ifndef QBLK
-#define QBLK 2
-#endif
-#ifndef QHEAD
-#define QHEAD 2
-#endif
 namespace vvh {
 
 namespace {
@@ -284,7 +275,7 @@ template <typename T_, int D_, int NG, int NGS, int KB, int VBITS>
 struct PagedQTiles {
     typedef PagedQArgs Args;
     typedef T_ T;
-    static constexpr int D = D_, CH = VBITS == 4 ? 64 : 32, HEAD = QHEAD;
+    static constexpr int D = D_, CH = VBITS == 4 ? 64 : 32, HEAD = CH == 64 ? 2 : 3;
     static constexpr int NT = CH / 16, DS = D / 32, GS = DS / NG;           // tiles, steps of 32 dims, steps of a group
     static constexpr int KRB = D * KB / 8, VRB = D * VBITS / 8;             // bytes of a row
     static constexpr int KW = KRB / 16, VW = VRB / 16;                      // words of a lane's piece of a tile
@@ -454,29 +445,35 @@ struct PagedQTiles {
             f4 sc[NT];
             float cm = -INFINITY;
 #pragma unroll
-            for (int t = 0; t < NT; t++) {
+            for (int p = 0; p < NP; p++) {
+                f4 part[NT];
 #pragma unroll
-                for (int p = 0; p < NP; p++) {
-                    const u4 sm = *reinterpret_cast<const u4*>(lk + group_of(r, p) * SR + 16 * t + 4 * gr);
-                    f4 part = {};
+                for (int t = 0; t < NT; t++) {
+                    part[t] = f4{};
 #pragma unroll
                     for (int x = p * NGS * GS; x < (p + 1) * NGS * GS && x < DS; x++) {
                         const h8 a = KB == 4 ? codes4(K[t].w[x]) : codes8(K[t].w[2 * x % KW], K[t].w[(2 * x + 1) % KW]);
-                        if constexpr (TWO) part = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q.lo[x], part, 0, 0, 0);
-                        part = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q.hi[x], part, 0, 0, 0);
+                        if constexpr (TWO) part[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q.lo[x], part[t], 0, 0, 0);
+                        part[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q.hi[x], part[t], 0, 0, 0);
                     }
+                }
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    const u4 sm = *reinterpret_cast<const u4*>(lk + group_of(r, p) * SR + 16 * t + 4 * gr);
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const float y = __builtin_fmaf(pair_min(sm[i]), q.sum[p], p ? sc[t][i] : 0.0f);
-                        sc[t][i] = __builtin_fmaf(pair_scale(sm[i]), part[i], y);
+                        sc[t][i] = __builtin_fmaf(pair_scale(sm[i]), part[t][i], y);
                     }
                 }
+            }
+#pragma unroll
+            for (int t = 0; t < NT; t++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     if (NGS >= 2) sc[t][i] += quad<0xB1>(sc[t][i]);
                     if (NGS >= 4) sc[t][i] += quad<0x4E>(sc[t][i]);
                 }
-            }
             if (!all) {
                 uint64_t bits = live;
                 asm volatile("" : "+s"(bits));  // a branch, not 16 selects in every chunk
@@ -670,7 +667,7 @@ __global__ __launch_bounds__(512, 2) void k_attention_paged_q_one(PagedQArgs c, 
     else paged_q_join<TL, 1>(to, wm, wl, os, n);
 }
 template <typename TL>
-__global__ __launch_bounds__(256, QWAVES) void k_attention_paged_q_split(PagedQArgs c, typename TL::T* __restrict__ out,
+__global__ __launch_bounds__(256, 2) void k_attention_paged_q_split(PagedQArgs c, typename TL::T* __restrict__ out,
                                                                     const typename TL::T* __restrict__ q,
                                                                     const int32_t* __restrict__ lens, PagedHeads hd, int32_t H,
                                                                     float scale_log2, int64_t* __restrict__ before_out,
@@ -755,7 +752,7 @@ AttnPagedPlan attention_paged_q_plan(const PagedQArgs& c, int64_t max_len, int64
     // a wave for each chunk, but no more than the device holds at a time
     p.waves = 1;
     while (p.waves < 8 && p.waves < chunks && p.waves * 2 * c.B * c.KVH * p.tiles <= 8 * cus) p.waves *= 2;
-    if (chunks > kQOneChunks) p.blocks = std::min<int64_t>((chunks * c.B * c.KVH * p.tiles + 3) / 4, QBLK * cus);
+    if (chunks > kQOneChunks) p.blocks = std::min<int64_t>((chunks * c.B * c.KVH * p.tiles + 3) / 4, 2 * cus);
     if (p.blocks > 0) p.ws_floats = paged_before_floats(c.B) + p.blocks * 4 * 2 * p.GT * (c.D + 4);
     return p;
 }
