@@ -236,6 +236,49 @@ def test_attention_formats_long(gpu, dtype, D, group, kb, vb):
     check_attention(rng, [3000, 5, 0, 1999, 2500], 48, 6, 2, D, group, kb, vb, dtype)
 
 
+def attention_fp32(pages, q, scale):
+    """The cache's values in fp32, then products, exponentials and sums in fp32."""
+    out = np.zeros(q.shape, np.float32)
+    for s in range(len(q)):
+        k, v, _, _ = pages.rows(s)
+        for h in range(q.shape[1] if len(k) else 0):
+            g = h // (q.shape[1] // pages.KVH)
+            sc = (k[:, g].astype(np.float32) @ q[s, h].astype(np.float32)) * np.float32(scale)
+            p = np.exp(sc - sc.max())
+            out[s, h] = (p / p.sum()) @ v[:, g].astype(np.float32)
+    return out
+
+
+@pytest.mark.parametrize("D,group,kb,vb", FORMATS)
+@pytest.mark.parametrize("lens", [[1, 1, 1], [7, 60, 300], [2000, 3000]])
+def test_attention_is_as_exact_as_fp32(gpu, D, group, kb, vb, lens):
+    """fp32 rows: the error's norm is within three times that of fp32 arithmetic on the values, or 2^-20 of the output's
+    (weights and queries of 22 bits, whose errors are 2^-22 at most each, and sums with codes of up to twice the values'
+    size)."""
+    rng = np.random.default_rng(D + kb + len(lens))
+    pg = PagesQ(rng, lens, 16, 2, D, group, kb, vb, F32)
+    q = rng.normal(0, 2, (len(lens), 8, D)).astype(np.float32)
+    scale = float(np.float32(1 / np.sqrt(D)))
+    ref, _ = attention_q_ref(pg, q, scale, 0)
+    off = lambda y: np.linalg.norm(y - ref) / np.linalg.norm(ref)  # noqa: E731
+    own, plain = off(run_attention(pg, q)), off(attention_fp32(pg, q, scale))
+    case("errors", own, plain)
+    assert own <= max(3 * plain, 2.0 ** -20)
+
+
+@pytest.mark.parametrize("D,group,kb,vb", FORMATS)
+def test_attention_of_fp16_is_bound_by_its_rounding(gpu, D, group, kb, vb):
+    """fp16 rows: the error's norm is at most a tenth above that of the exact output rounded to fp16."""
+    rng = np.random.default_rng(D + kb)
+    pg = PagesQ(rng, [1, 40, 700, 2500], 16, 2, D, group, kb, vb, F16)
+    q = rng.normal(0, 2, (4, 8, D)).astype(np.float16)
+    scale = float(np.float32(1 / np.sqrt(D)))
+    ref, _ = attention_q_ref(pg, q, scale, 0)
+    own, best = (np.linalg.norm(y - ref) / np.linalg.norm(ref) for y in (run_attention(pg, q), ref.astype(np.float16)))
+    case("errors", own, best)
+    assert own <= 1.1 * best
+
+
 @pytest.mark.parametrize("dtype", [F16, F32])
 @pytest.mark.parametrize("H,KVH", [(1, 1), (2, 2), (8, 1), (5, 1), (16, 1), (17, 1), (20, 1), (33, 1), (34, 2), (32, 8), (24, 3)])
 def test_attention_heads(gpu, dtype, H, KVH):

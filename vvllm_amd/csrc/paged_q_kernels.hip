@@ -222,14 +222,15 @@ __global__ __launch_bounds__(256) void k_read_paged_q(PagedQArgs c, T* __restric
 // ---------------------------------------------------------------------------
 // Attention on the matrix cores, a tile of up to 16 query heads of one kv head (paged_split.h says how tiles and chunks of keys
 // are shared out).  A wave takes CH keys at a time, in tiles of 16 that lie together in a page:
-//   S^T = K . q^T   A = K's codes as they are: a 4-bit code in the low bits of an fp16 is the subnormal c 2^-24 (the instruction
-//                   takes subnormals, exact), an 8-bit one too; (w & 0x00f000f0) gives 16 c, whose q is 1 / 16.  A group's
-//                   sum is scaled in fp32: score = sum_g s_g part_g + m_g Q_g, Q_g the sum of the group's q.
+//   S^T = K . q^T   A = K's codes c + b for a bias b that makes them fp16 values in one or two instructions a pair (CodeBias),
+//                   exact.  A group's sum begins at -b Q_g, Q_g the sum of the group's q, and is scaled in fp32:
+//                     score = sum_g s_g part_g + m_g Q_g.
 //                   q is scaled by a power of two to a largest of 2^10 .. 2^11 in its row (fp32: high and low part, 22 bits).
 //   softmax         online, in log2 units; maximum rounded up to an integer.
 //   O^T += V^T P^T  V's codes go through the wave's LDS region and its transposing reads of 4 and 8 bits, which give a lane the
-//                   codes of 16 (8) keys of one dim; taken as subnormals again.  B = p s_g, the weights times their keys'
-//                   scales, as fp16 pairs high + low; the minima's share sum_k p m_g is added up in fp32 beside.
+//                   codes of 16 (8) keys of one dim; taken with a bias again.  B = p s_g, the weights times their keys'
+//                   scales, as fp16 pairs high + low.  What the minima give, sum_k p m_g, is added up in fp32 beside, and what
+//                   the bias gives, b sum_k p s_g, by one more row of the product, whose A is 1.
 //                   Weights are times 2^14 over 2^es, a power of two above every scale so far, so that p s_g has fp16's range.
 // Column r of the products is head r / NGS and, of its groups, every NGS-th from r % NGS on: few heads leave columns free,
 // and scaling scores and weights is most of what a chunk costs (96 ragged contexts of 4 heads a kv head and 4 groups 116 us with a
@@ -244,25 +245,57 @@ struct __attribute__((packed, aligned(4))) Words {
     uint32_t w[N];
 };
 
-// 8 codes as an operand of subnormals.  4 bits: code pairs (0, 4), (1, 5), (2, 6), (3, 7) of a word, odd ones times 16; 8 bits:
-// in order.
-__device__ __forceinline__ h8 codes4(uint32_t w)
+// What is added to a code of BITS bits to make an fp16 of it.  fp32 rows have the codes in the middle, and their minima moved by as
+// much (m - b s is the middle of the group's values, so that the two terms of a score are small).  fp16 rows take the cheapest,
+// 8 times as large, and its share out of the sums.  (The code's bits alone, an fp16 subnormal, would cost less yet, but the
+// matrix instruction keeps only about 17 bits of products of subnormals.)
+template <int BITS, bool TWO>
+constexpr float CodeBias = BITS == 8 ? (TWO ? -128.0f : 1024.0f) : (TWO ? -8.0f : 64.0f);
+
+// Masks that the compiler knows nothing of: one in a vector and one in a scalar register are what v_and_or_b32 takes.
+struct CodeMasks {
+    uint32_t mid, low, mid_one, low_one;
+};
+__device__ __forceinline__ CodeMasks code_masks()
 {
-    const uint32_t v = w >> 8;
-    return __builtin_bit_cast(h8, u4{w & 0x000f000fu, w & 0x00f000f0u, v & 0x000f000fu, v & 0x00f000f0u});
+    CodeMasks k{0x00f000f0u, 0x000f000fu, 0x54005400u, 0x64006400u};
+    asm("" : "+v"(k.mid), "+v"(k.low), "+s"(k.mid_one), "+s"(k.low_one));
+    return k;
 }
+
+// 8 codes as an operand.  4 bits: code pairs (0, 4), (1, 5), (2, 6), (3, 7) of a word, the code in the mantissa's bits 4 to 7 (64 +
+// c), for fp32 rows also 0 to 3 (1024 + c), then less 72 or 1032; 8 bits: in order, in the mantissa's low bits (1024 + c), for
+// fp32 rows less 1152.
+template <bool TWO>
+__device__ __forceinline__ h8 codes4(uint32_t w, const CodeMasks& k)
+{
+    if constexpr (TWO) {
+        const uint32_t v = w >> 8;
+        const h2 c72 = {(f16)72.0f, (f16)72.0f}, c1032 = {(f16)1032.0f, (f16)1032.0f};
+        const h2 a = __builtin_bit_cast(h2, (w & k.low) | k.low_one) - c1032, b = __builtin_bit_cast(h2, (w & k.mid) | k.mid_one) - c72;
+        const h2 c = __builtin_bit_cast(h2, (v & k.low) | k.low_one) - c1032, d = __builtin_bit_cast(h2, (v & k.mid) | k.mid_one) - c72;
+        return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+    }
+    return __builtin_bit_cast(h8, u4{(w << 4 & k.mid) | k.mid_one, (w & k.mid) | k.mid_one, (w >> 4 & k.mid) | k.mid_one,
+                                     (w >> 8 & k.mid) | k.mid_one});
+}
+template <bool TWO>
 __device__ __forceinline__ h8 codes8(uint32_t w0, uint32_t w1)
 {
-    return __builtin_bit_cast(h8, u4{__builtin_amdgcn_perm(0, w0, 0x0c010c00u), __builtin_amdgcn_perm(0, w0, 0x0c030c02u),
-                                     __builtin_amdgcn_perm(0, w1, 0x0c010c00u), __builtin_amdgcn_perm(0, w1, 0x0c030c02u)});
+    const u4 x = {__builtin_amdgcn_perm(0x64646464u, w0, 0x04010400u), __builtin_amdgcn_perm(0x64646464u, w0, 0x04030402u),
+                  __builtin_amdgcn_perm(0x64646464u, w1, 0x04010400u), __builtin_amdgcn_perm(0x64646464u, w1, 0x04030402u)};
+    h8 y = __builtin_bit_cast(h8, x);
+    if constexpr (TWO) y -= (f16)1152.0f;
+    return y;
 }
 // High and low fp16 part of a pair of weights; minus: -1, in a register that the compiler knows nothing of, so that a
 // difference is one instruction that takes the fp16 as it is.
 __device__ __forceinline__ void weight_parts(float a, float b, float minus, uint32_t& hi, uint32_t& lo)
 {
-    const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
+    const h2 h = {(f16)a, (f16)b};
+    const h2 o = {(f16)__builtin_fmaf((float)h[0], minus, a), (f16)__builtin_fmaf((float)h[1], minus, b)};
     hi = __builtin_bit_cast(uint32_t, h);
-    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)h[0], minus, a), __builtin_fmaf((float)h[1], minus, b)));
+    lo = __builtin_bit_cast(uint32_t, o);
 }
 // v of the lane that the quad permutation names, as an operand of the instruction that takes it
 template <int CTRL>
@@ -292,7 +325,7 @@ struct PagedQTiles {
     // The same as an operand, in the order of the codes
     struct Operand {
         h8 hi[DS], lo[TWO ? DS : 1];
-        float sum[NP];  // of the column's groups, times 2^-24
+        float sum[NP];  // of the column's groups
         int e;
     };
     // group `p` of column r; where NG is no multiple of NGS, a column without one takes the last again, with a q of 0
@@ -329,14 +362,21 @@ struct PagedQTiles {
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const int o = KB == 4 ? j / 2 + 4 * (j % 2) : j;
-                const float y = mine ? __builtin_ldexpf(v[s][o], x.e) : 0.0f, z = KB == 4 && o % 2 ? y * 0.0625f : y;
-                x.sum[s / GS / NGS] += y;
-                x.hi[s][j] = (f16)z;
-                if constexpr (TWO) x.lo[s][j] = (f16)(z - (float)x.hi[s][j]);
+                const float y = mine ? __builtin_ldexpf(v[s][o], x.e) : 0.0f;
+                x.hi[s][j] = (f16)y;
+                if constexpr (TWO) x.lo[s][j] = (f16)(y - (float)x.hi[s][j]);
+                x.sum[s / GS / NGS] += TWO ? (float)x.hi[s][j] + (float)x.lo[TWO ? s : 0][j] : y;
             }
         }
 #pragma unroll
-        for (int p = 0; p < NP; p++) x.sum[p] = sum_x32(sum_x16(x.sum[p])) * 0x1p-24f;
+        for (int p = 0; p < NP; p++) x.sum[p] = sum_x32(sum_x16(x.sum[p]));
+    }
+
+    // What a group's codes less their bias are added to: its minimum, for fp32 rows less the bias' share
+    template <int BITS>
+    static __device__ __forceinline__ float middle(uint32_t sm)
+    {
+        return TWO ? __builtin_fmaf(pair_scale(sm), -CodeBias<BITS, TWO>, pair_min(sm)) : pair_min(sm);
     }
 
     struct Spot {
@@ -358,8 +398,11 @@ struct PagedQTiles {
         uint32_t* const lv = lk + SW;
         float minus = -1.0f;
         asm("" : "+s"(minus));
+        const CodeMasks masks = code_masks();
         acc.clear();
-        float om[NP] = {}, om_odd[NP] = {}, m = -INFINITY, l = 0.0f, l_odd = 0.0f, ref = 0x1p-30f;
+        f4 ones = {};  // the row of ones
+        float ws[NP] = {};  // several groups a column: the sums of the weights themselves, in a register each
+        float om[NP] = {}, m = -INFINITY, l = 0.0f, ref = 0x1p-30f;
         int es = -30;
 
         Words<KW> K[NT];
@@ -403,7 +446,7 @@ struct PagedQTiles {
         prepare(q0, lane, q);
         // scores to log2 units: positive (a negative scale turns q's sign), never 0, so that the maximum of the scores is
         // that of the products and -infinity stays (2^-100 times any score is 0 for the exponential)
-        const float kl = fmaxf(__builtin_fabsf(__builtin_ldexpf(scale_log2, 24 - q.e)), 0x1p-100f);
+        const float kl = fmaxf(__builtin_fabsf(__builtin_ldexpf(scale_log2, -q.e)), 0x1p-100f);
         if (scale_log2 < 0.0f) {
 #pragma unroll
             for (int x = 0; x < DS; x++) {
@@ -449,10 +492,11 @@ struct PagedQTiles {
                 f4 part[NT];
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
-                    part[t] = f4{};
+                    const float first = TWO ? 0.0f : -CodeBias<KB, TWO> * q.sum[p];
+                    part[t] = f4{first, first, first, first};
 #pragma unroll
                     for (int x = p * NGS * GS; x < (p + 1) * NGS * GS && x < DS; x++) {
-                        const h8 a = KB == 4 ? codes4(K[t].w[x]) : codes8(K[t].w[2 * x % KW], K[t].w[(2 * x + 1) % KW]);
+                        const h8 a = KB == 4 ? codes4<TWO>(K[t].w[x], masks) : codes8<TWO>(K[t].w[2 * x % KW], K[t].w[(2 * x + 1) % KW]);
                         if constexpr (TWO) part[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q.lo[x], part[t], 0, 0, 0);
                         part[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q.hi[x], part[t], 0, 0, 0);
                     }
@@ -462,7 +506,7 @@ struct PagedQTiles {
                     const u4 sm = *reinterpret_cast<const u4*>(lk + group_of(r, p) * SR + 16 * t + 4 * gr);
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const float y = __builtin_fmaf(pair_min(sm[i]), q.sum[p], p ? sc[t][i] : 0.0f);
+                        const float y = __builtin_fmaf(middle<KB>(sm[i]), q.sum[p], p ? sc[t][i] : 0.0f);
                         sc[t][i] = __builtin_fmaf(pair_scale(sm[i]), part[t][i], y);
                     }
                 }
@@ -501,24 +545,22 @@ struct PagedQTiles {
                 m = mn;
                 es = en;
                 l *= f;
-                l_odd *= f;
+                ones *= f;
 #pragma unroll
                 for (int p = 0; p < NP; p++) {
                     om[p] *= f;
-                    om_odd[p] *= f;
+                    ws[p] *= f;
                 }
 #pragma unroll
                 for (int e = 0; e < D / 16; e++) acc.o[e] *= f;
             }
             const float mb = m == -INFINITY ? 0.0f : m - 14.0f + (float)es;  // no key yet: every weight below is 0
-            // 4 bits: odd keys' weights are over 16, as their codes are times 16
-            const float mo = VBITS == 4 ? mb + 4.0f : mb;
 #pragma unroll
             for (int t = 0; t < NT; t++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    sc[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][i], kl, i % 2 ? -mo : -mb));
-                    (i % 2 ? l_odd : l) += sc[t][i];
+                    sc[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][i], kl, -mb));
+                    l += sc[t][i];
                 }
             // ---- values
 #pragma unroll
@@ -530,9 +572,13 @@ struct PagedQTiles {
                 for (int t = 0; t < NT; t++)
 #pragma unroll
                     for (int i = 0; i < 4; i++)
-                        (i % 2 ? om_odd : om)[p] = __builtin_fmaf(sc[t][i], pair_min(sm[t][i]), (i % 2 ? om_odd : om)[p]);
+                        om[p] = __builtin_fmaf(sc[t][i], middle<VBITS>(sm[t][i]), om[p]);
                 // + 0: one instruction that takes the scale as it is
-                auto w = [&](int t, int i) { return __builtin_fmaf(sc[t][i], pair_scale(sm[t][i]), 0.0f); };
+                auto w = [&](int t, int i) {
+                    const float x = __builtin_fmaf(sc[t][i], pair_scale(sm[t][i]), 0.0f);
+                    if constexpr (!TWO && NP > 1) ws[p] += x;
+                    return x;
+                };
 #pragma unroll
                 for (int u = 0; u < NT / 2; u++)
 #pragma unroll
@@ -543,6 +589,15 @@ struct PagedQTiles {
                         hi[u][i] = h;
                         lo[u][i] = o;
                     }
+                if constexpr (!TWO && NP == 1) {
+                    const f16 one = (f16)1.0f;
+                    const h8 row = {one, one, one, one, one, one, one, one};
+#pragma unroll
+                    for (int u = 0; u < NT / 2; u++) {
+                        ones = __builtin_amdgcn_mfma_f32_16x16x32_f16(row, __builtin_bit_cast(h8, lo[u]), ones, 0, 0, 0);
+                        ones = __builtin_amdgcn_mfma_f32_16x16x32_f16(row, __builtin_bit_cast(h8, hi[u]), ones, 0, 0, 0);
+                    }
+                }
 #pragma unroll
                 for (int e = p * NGS * GS * 2; e < (p + 1) * NGS * GS * 2 && e < D / 16; e++) {
                     h8 a[NT / 2];
@@ -551,13 +606,13 @@ struct PagedQTiles {
                         // nibble n of a lane: key 4 gr + n % 4 of tile n / 4
                         const char* src = lds + (16 * gr + 4 * (r & 3) + (r >> 2)) * VP + 8 * e;
                         const i2 w2 = __builtin_amdgcn_ds_read_tr4_b64_v2i32((__attribute__((address_space(3))) i2*)(src));
-                        a[0] = codes4((uint32_t)w2[0]);
-                        a[1] = codes4((uint32_t)w2[1]);
+                        a[0] = codes4<TWO>((uint32_t)w2[0], masks);
+                        a[1] = codes4<TWO>((uint32_t)w2[1], masks);
                     } else {
                         // byte n of a lane: key 4 gr + n % 4 of tile n / 4
                         const char* src = lds + (8 * gr + 2 * (r >> 1 & 3) + (r >> 3)) * VP + 16 * e + 8 * (r & 1);
                         const i2 w2 = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i2*)(src));
-                        a[0] = codes8((uint32_t)w2[0], (uint32_t)w2[1]);
+                        a[0] = codes8<TWO>((uint32_t)w2[0], (uint32_t)w2[1]);
                     }
 #pragma unroll
                     for (int u = 0; u < NT / 2; u++) {
@@ -567,19 +622,21 @@ struct PagedQTiles {
                 }
             }
         }
-        const float odd = VBITS == 4 ? 16.0f : 1.0f;
         float ms[NP];
 #pragma unroll
-        for (int p = 0; p < NP; p++) ms[p] = sum_x32(sum_x16(__builtin_fmaf(om_odd[p], odd, om[p])));
+        for (int p = 0; p < NP; p++) {
+            ms[p] = sum_x32(sum_x16(om[p]));
+            if constexpr (!TWO) ms[p] = __builtin_fmaf(-CodeBias<VBITS, TWO>, NP == 1 ? ones[0] : sum_x32(sum_x16(ws[p])), ms[p]);
+        }
         // to lane r what is head r's
         auto from = [&](float v, int col) { return NGS == 1 ? v : __shfl(v, (lane & 48) + (r * NGS + col) % 16); };
 #pragma unroll
         for (int e = 0; e < D / 16; e++) {
             const int gq = e / (2 * GS);
 #pragma unroll
-            for (int i = 0; i < 4; i++) acc.o[e][i] = from(__builtin_fmaf(acc.o[e][i], 0x1p24f, ms[gq / NGS]), gq % NGS);
+            for (int i = 0; i < 4; i++) acc.o[e][i] = from(acc.o[e][i] + ms[gq / NGS], gq % NGS);
         }
-        acc.l = from(sum_x32(sum_x16(__builtin_fmaf(l_odd, odd, l))), 0);
+        acc.l = from(sum_x32(sum_x16(l)), 0);
         acc.m = from(m == -INFINITY ? m : m + (float)es, 0);
     }
 
