@@ -560,6 +560,7 @@ template <typename T_, int D_, bool BIG>
 struct PagedTiles {
     typedef PagedArgs Args;
     typedef T_ T;
+    static constexpr bool COLUMNS = false;
     static constexpr int D = D_, CH = PagedTile<T>::template CH<D>, HEAD = 0, VB = PagedTile<T>::template lds<D> * 2;
     typedef typename PagedTile<T>::template Q<D> Q;
     static __device__ __forceinline__ void load_q(const T* q, int heads, int lane, Q& x) { paged_load_q<D>(q, heads, lane, x); }
@@ -715,7 +716,7 @@ static void paged_go(const AttnPagedPlan& p, const PagedArgs& c, T* out, const T
     const int64_t W = p.blocks * 4;
     int64_t nw = 1;
     while (nw < 16 && nw * (256 / D) * 4 < p.blocks / ((int64_t)VH * c.B)) nw *= 2;
-    hipLaunchKernelGGL((k_attention_paged_merge<T, D>), dim3((unsigned)H, (unsigned)c.B), dim3((unsigned)(64 * nw)), 0, s,
+    hipLaunchKernelGGL((k_attention_paged_merge<T, D, false>), dim3((unsigned)H, (unsigned)c.B), dim3((unsigned)(64 * nw)), 0, s,
                        (int32_t)c.B, out, hd, (int32_t)H, before, parts, VH, (int32_t)W);
 }
 

@@ -308,6 +308,7 @@ template <typename T_, int D_, int NG, int NGS, int KB, int VBITS>
 struct PagedQTiles {
     typedef PagedQArgs Args;
     typedef T_ T;
+    static constexpr bool COLUMNS = true;
     static constexpr int D = D_, CH = VBITS == 4 ? 64 : 32, HEAD = CH == 64 ? 2 : 3;
     static constexpr int NT = CH / 16, DS = D / 32, GS = DS / NG;           // tiles, steps of 32 dims, steps of a group
     static constexpr int KRB = D * KB / 8, VRB = D * VBITS / 8;             // bytes of a row
@@ -628,52 +629,86 @@ struct PagedQTiles {
             ms[p] = sum_x32(sum_x16(om[p]));
             if constexpr (!TWO) ms[p] = __builtin_fmaf(-CodeBias<VBITS, TWO>, NP == 1 ? ones[0] : sum_x32(sum_x16(ws[p])), ms[p]);
         }
-        // to lane r what is head r's
-        auto from = [&](float v, int col) { return NGS == 1 ? v : __shfl(v, (lane & 48) + (r * NGS + col) % 16); };
 #pragma unroll
-        for (int e = 0; e < D / 16; e++) {
-            const int gq = e / (2 * GS);
-#pragma unroll
-            for (int i = 0; i < 4; i++) acc.o[e][i] = from(acc.o[e][i] + ms[gq / NGS], gq % NGS);
-        }
-        acc.l = from(sum_x32(sum_x16(l)), 0);
-        acc.m = from(m == -INFINITY ? m : m + (float)es, 0);
+        for (int e = 0; e < D / 16; e++) acc.o[e] += ms[e / (2 * GS) / NGS];
+        acc.l = sum_x32(sum_x16(l));
+        acc.m = m == -INFINITY ? m : m + (float)es;
     }
 
-    static __device__ __forceinline__ constexpr int dim(int e, int gr, int i) { return 16 * e + 4 * gr + i; }
+    // The n heads' sums, from the columns of each dim's group: rows of `pitch` floats and their maxima and sums, which without
+    // arrays of their own follow the rows
+    static __device__ __forceinline__ void put(const PagedAcc<D>& acc, int lane, int n, float* rows, int pitch, float* wm, float* wl)
+    {
+        const int r = lane & 15, gr = lane >> 4, h = r / NGS;
+        if (h >= n) return;
+        float* row = rows + h * pitch;
+#pragma unroll
+        for (int e = 0; e < D / 16; e++) {
+            f4 v = acc.o[e];
+            asm("" : "+v"(v));  // here, whatever the column: else the sums go to memory, to be read from there by column
+            if (e / (2 * GS) % NGS == r % NGS) *reinterpret_cast<f4*>(row + 16 * e + 4 * gr) = v;
+        }
+        if (lane % NGS == 0 && gr == 0) {
+            (wm ? wm[h] : row[D]) = acc.m;
+            (wl ? wl[h] : row[D + 1]) = acc.l;
+        }
+    }
+    // The n heads' outputs
+    static __device__ __forceinline__ void store(const PagedAcc<D>& acc, int lane, int n, T* __restrict__ out)
+    {
+        const int r = lane & 15, gr = lane >> 4, h = r / NGS;
+        if (h >= n) return;
+        const float inv = acc.l == 0.0f ? 0.0f : 1.0f / acc.l;
+#pragma unroll
+        for (int e = 0; e < D / 16; e++) {
+            f4 v = acc.o[e] * inv;
+            asm("" : "+v"(v));  // as above
+            if (e / (2 * GS) % NGS == r % NGS) store4(out + h * D + 16 * e + 4 * gr, v);
+        }
+    }
+    static __device__ __forceinline__ void store4(T* to, f4 v)
+    {
+        typedef T t4 __attribute__((ext_vector_type(4)));
+        *reinterpret_cast<t4*>(to) = t4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+    }
+    // A block's sums from its NW waves' (put's rows in os, 16 a wave, D + 4 apart), 4 dims a thread: outputs, or without them a part
+    template <int NW>
+    static __device__ __forceinline__ void join(T* __restrict__ out, float* __restrict__ part, const float (*wm)[16],
+                                                const float (*wl)[16], const float* os, int32_t n)
+    {
+        constexpr int OP = D + 4;
+        for (int idx = threadIdx.x; idx < n * (D / 4); idx += 64 * NW) {
+            const int h = idx / (D / 4), d = (idx - h * (D / 4)) * 4;
+            float m[NW], M = -INFINITY, den = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NW; i++) {
+                m[i] = wm[i][h];
+                M = fmaxf(M, m[i]);
+            }
+            const float Mb = M == -INFINITY ? 0.0f : M;
+            f4 num = {};
+#pragma unroll
+            for (int i = 0; i < NW; i++) {
+                const float f = __builtin_amdgcn_exp2f(m[i] - Mb);
+                num += *reinterpret_cast<const f4*>(os + (i * 16 + h) * OP + d) * f;
+                den = __builtin_fmaf(f, wl[i][h], den);
+            }
+            if (out) {
+                store4(out + h * D + d, num * (den == 0.0f ? 0.0f : 1.0f / den));
+                continue;
+            }
+            *reinterpret_cast<f4*>(part + h * (D + 4) + d) = num;
+            if (d == 0) {
+                part[h * (D + 4) + D] = M;
+                part[h * (D + 4) + D + 1] = den;
+            }
+        }
+    }
 };
 
 // Bytes of LDS a wave: its chunk, then its sums
 template <typename TL>
 constexpr int kQWaveBytes = TL::VB > 16 * (TL::D + 4) * 4 ? TL::VB : 16 * (TL::D + 4) * 4;
-
-// The block's output from its NW waves' sums: wm, wl [.][16] and os [16 NW][D + 4]; n heads, 4 dims a thread.
-template <typename TL, int NW>
-__device__ __forceinline__ void paged_q_join(typename TL::T* __restrict__ out, const float (*wm)[16], const float (*wl)[16],
-                                             const float* os, int32_t n)
-{
-    constexpr int D = TL::D, OP = D + 4;
-    for (int idx = threadIdx.x; idx < n * (D / 4); idx += 64 * NW) {
-        const int h = idx / (D / 4), d = (idx - h * (D / 4)) * 4;
-        float m[NW], M = -INFINITY, den = 0.0f;
-#pragma unroll
-        for (int i = 0; i < NW; i++) {
-            m[i] = wm[i][h];
-            M = fmaxf(M, m[i]);
-        }
-        const float Mb = M == -INFINITY ? 0.0f : M;
-        f4 num = {};
-#pragma unroll
-        for (int i = 0; i < NW; i++) {
-            const float f = __builtin_amdgcn_exp2f(m[i] - Mb);
-            num += *reinterpret_cast<const f4*>(os + (i * 16 + h) * OP + d) * f;
-            den = __builtin_fmaf(f, wl[i][h], den);
-        }
-        const float inv = den == 0.0f ? 0.0f : 1.0f / den;
-#pragma unroll
-        for (int i = 0; i < 4; i++) out[h * D + d + i] = (typename TL::T)(num[i] * inv);
-    }
-}
 
 // One tile of one sequence by one block of 1, 2, 4 or 8 waves, each every so many-th chunk, merged through LDS (a wave by itself
 // has its sums in registers).
@@ -686,7 +721,7 @@ __global__ __launch_bounds__(512, 2) void k_attention_paged_q_one(PagedQArgs c, 
     constexpr int D = TL::D, CH = TL::CH, OP = D + 4;
     extern __shared__ __align__(16) char smem[];
     __shared__ float wm[8][16], wl[8][16];
-    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, gr = lane >> 4;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int NW = blockDim.x >> 6;
     const int32_t s = blockIdx.y, len = paged_len(c, lens, s);
     int32_t g, h0, n;
@@ -696,32 +731,18 @@ __global__ __launch_bounds__(512, 2) void k_attention_paged_q_one(PagedQArgs c, 
     TL::load_q(q + row0 * D, n, lane, x);
     PagedAcc<D> acc;
     TL::tile(c, g, s, x, w * CH, NW * CH, len, scale_log2, smem + w * kQWaveBytes<TL>, lane, acc);
-    if (len <= CH) {  // all of it is the first wave's
-        const float inv = acc.l == 0.0f ? 0.0f : 1.0f / acc.l;
-        if (w == 0 && r < n) {
-#pragma unroll
-            for (int e = 0; e < D / 16; e++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) out[(row0 + r) * D + TL::dim(e, gr, i)] = (typename TL::T)(acc.o[e][i] * inv);
-        }
+    typename TL::T* to = out + row0 * D;
+    if (NW == 1 || len <= CH) {  // all of it is the first wave's
+        if (w == 0) TL::store(acc, lane, n, to);
         return;
     }
-    if (NW > 1) __syncthreads();
-    float* os = reinterpret_cast<float*>(smem);
-    if (gr == 0) {
-        wm[w][r] = acc.m;
-        wl[w][r] = acc.l;
-    }
-    if (r < n) {
-#pragma unroll
-        for (int e = 0; e < D / 16; e++) *reinterpret_cast<f4*>(os + (w * 16 + r) * OP + TL::dim(e, gr, 0)) = acc.o[e];
-    }
     __syncthreads();
-    typename TL::T* to = out + row0 * D;
-    if (NW == 8) paged_q_join<TL, 8>(to, wm, wl, os, n);
-    else if (NW == 4) paged_q_join<TL, 4>(to, wm, wl, os, n);
-    else if (NW == 2) paged_q_join<TL, 2>(to, wm, wl, os, n);
-    else paged_q_join<TL, 1>(to, wm, wl, os, n);
+    float* os = reinterpret_cast<float*>(smem);
+    TL::put(acc, lane, n, os + w * 16 * OP, OP, wm[w], wl[w]);
+    __syncthreads();
+    if (NW == 8) TL::template join<8>(to, nullptr, wm, wl, os, n);
+    else if (NW == 4) TL::template join<4>(to, nullptr, wm, wl, os, n);
+    else TL::template join<2>(to, nullptr, wm, wl, os, n);
 }
 template <typename TL>
 __global__ __launch_bounds__(256, 2) void k_attention_paged_q_split(PagedQArgs c, typename TL::T* __restrict__ out,
@@ -832,7 +853,7 @@ static void paged_q_go(const AttnPagedPlan& p, const PagedQArgs& c, typename TL:
     const int64_t W = p.blocks * 4;
     int64_t nw = 1;  // waves of a merge block: about 4 parts a group of lanes if the sequences are alike
     while (nw < 16 && nw * (256 / TL::D) * 4 < p.blocks / ((int64_t)VH * c.B)) nw *= 2;
-    hipLaunchKernelGGL((k_attention_paged_merge<typename TL::T, TL::D>), dim3((unsigned)H, (unsigned)c.B), dim3((unsigned)(64 * nw)), 0,
+    hipLaunchKernelGGL((k_attention_paged_merge<typename TL::T, TL::D, true>), dim3((unsigned)H, (unsigned)c.B), dim3((unsigned)(64 * nw)), 0,
                        s, (int32_t)c.B, out, hd, (int32_t)H, before, parts, VH, (int32_t)W);
 }
 

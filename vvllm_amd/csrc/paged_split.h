@@ -1,7 +1,7 @@
 // Attention of one query per sequence over a paged cache, whatever its rows hold: a tile of up to 16 query heads of one kv
 // head is a wave's work on a chunk of keys, and here is how a batch's tiles and chunks are shared out and joined.  A class TL
 // of static members says the rest: Args (the cache; B, P, max_pages), T (queries and outputs), D, CH (keys of a chunk), HEAD
-// (chunks that the beginning of a tile is as long as: what comes before the first chunk's products counts in a batch of short contexts), VB
+// COLUMNS (a head's sums may be in several columns: put, store and join write what this code writes for the others), HEAD (chunks that the beginning of a tile is as long as: what comes before the first chunk's products counts in a batch of short contexts), VB
 // (bytes of LDS a wave), Q (a tile's queries in registers), load_q, tile (the chunks c0, c0 + cstep, ... below ke of sequence s
 // and kv head g), dim (of accumulator element (e, lane group, i)).
 #pragma once
@@ -196,55 +196,70 @@ __device__ __forceinline__ void paged_split(const typename TL::Args& c, typename
         const int32_t first = ci > TL::HEAD ? ci - TL::HEAD : 0;  // chunk; a range of the tile's head alone has none
         const int64_t end = (int64_t)(ci + cnt - TL::HEAD) * CH;
         TL::tile(c, g, s, x, first * CH, CH, end < len ? (int32_t)end : len, scale_log2, smem + wb * VB, lane, acc);
-        if (inside) {
-            __syncthreads();
-            float* os = reinterpret_cast<float*>(smem);
-            if (gr == 0) {
-                wm[wb][r] = acc.m;
-                wl[wb][r] = acc.l;
+        if constexpr (TL::COLUMNS) {
+            const bool whole = inside ? b1 - b0 == ns : cnt == ns;
+            if (inside) {
+                __syncthreads();
+                float* os = reinterpret_cast<float*>(smem);
+                TL::put(acc, lane, nh, os + wb * 16 * OP, OP, wm[wb], wl[wb]);
+                __syncthreads();
+                float* part = ws + ((w - wb) * 2 + (u0 - b0 == ci)) * hd.GT * (D + 4);
+                TL::template join<4>(whole ? out + row0 * D : nullptr, part, wm, wl, os, nh);
+                return;
             }
-#pragma unroll
-            for (int e = 0; e < D / 16; e++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) os[(wb * 16 + r) * OP + TL::dim(e, gr, i)] = acc.o[e][i];
-            __syncthreads();
-            const bool whole = b1 - b0 == ns;
-            float* part = ws + ((w - wb) * 2 + (u0 - b0 == ci)) * hd.GT * (D + 4);
-            for (int idx = threadIdx.x; idx < nh * D; idx += 256) {
-                const int h = idx / D, d = idx - h * D;
-                const float M = fmaxf(fmaxf(wm[0][h], wm[1][h]), fmaxf(wm[2][h], wm[3][h])), Mb = M == -INFINITY ? 0.0f : M;
-                float num = 0.0f, den = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 4; i++) attn_merge_add(num, den, wm[i][h], Mb, os[(i * 16 + h) * OP + d], wl[i][h]);
-                if (whole) {
-                    out[row0 * D + idx] = (typename TL::T)(den == 0.0f ? 0.0f : num / den);
-                    continue;
-                }
-                part[h * (D + 4) + d] = num;
-                if (d == 0) {
-                    part[h * (D + 4) + D] = M;
-                    part[h * (D + 4) + D + 1] = den;
-                }
-            }
-            return;
-        }
-        if (r < nh) {
-            if (cnt == ns) {
-                const float inv = acc.l == 0.0f ? 0.0f : 1.0f / acc.l;
-#pragma unroll
-                for (int e = 0; e < D / 16; e++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        out[(row0 + r) * D + TL::dim(e, gr, i)] = (typename TL::T)(acc.o[e][i] * inv);
-            } else {
-                float* p = ws + ((w * 2 + (ci == 0)) * hd.GT + r) * (D + 4);
-#pragma unroll
-                for (int e = 0; e < D / 16; e++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) p[TL::dim(e, gr, i)] = acc.o[e][i];
+            if (whole) TL::store(acc, lane, nh, out + row0 * D);
+            else TL::put(acc, lane, nh, ws + (w * 2 + (ci == 0)) * hd.GT * (D + 4), D + 4, nullptr, nullptr);
+        } else {
+            if (inside) {
+                __syncthreads();
+                float* os = reinterpret_cast<float*>(smem);
                 if (gr == 0) {
-                    p[D] = acc.m;
-                    p[D + 1] = acc.l;
+                    wm[wb][r] = acc.m;
+                    wl[wb][r] = acc.l;
+                }
+#pragma unroll
+                for (int e = 0; e < D / 16; e++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) os[(wb * 16 + r) * OP + TL::dim(e, gr, i)] = acc.o[e][i];
+                __syncthreads();
+                const bool whole = b1 - b0 == ns;
+                float* part = ws + ((w - wb) * 2 + (u0 - b0 == ci)) * hd.GT * (D + 4);
+                for (int idx = threadIdx.x; idx < nh * D; idx += 256) {
+                    const int h = idx / D, d = idx - h * D;
+                    const float M = fmaxf(fmaxf(wm[0][h], wm[1][h]), fmaxf(wm[2][h], wm[3][h])), Mb = M == -INFINITY ? 0.0f : M;
+                    float num = 0.0f, den = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) attn_merge_add(num, den, wm[i][h], Mb, os[(i * 16 + h) * OP + d], wl[i][h]);
+                    if (whole) {
+                        out[row0 * D + idx] = (typename TL::T)(den == 0.0f ? 0.0f : num / den);
+                        continue;
+                    }
+                    part[h * (D + 4) + d] = num;
+                    if (d == 0) {
+                        part[h * (D + 4) + D] = M;
+                        part[h * (D + 4) + D + 1] = den;
+                    }
+                }
+                return;
+            }
+            if (r < nh) {
+                if (cnt == ns) {
+                    const float inv = acc.l == 0.0f ? 0.0f : 1.0f / acc.l;
+#pragma unroll
+                    for (int e = 0; e < D / 16; e++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            out[(row0 + r) * D + TL::dim(e, gr, i)] = (typename TL::T)(acc.o[e][i] * inv);
+                } else {
+                    float* p = ws + ((w * 2 + (ci == 0)) * hd.GT + r) * (D + 4);
+#pragma unroll
+                    for (int e = 0; e < D / 16; e++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) p[TL::dim(e, gr, i)] = acc.o[e][i];
+                    if (gr == 0) {
+                        p[D] = acc.m;
+                        p[D + 1] = acc.l;
+                    }
                 }
             }
         }
@@ -274,7 +289,8 @@ __device__ __forceinline__ int64_t last_wave(int64_t u, int64_t W, int64_t total
 // Block (h, s) joins the parts of head h of sequence s: D / 4 lanes a part, 4 dims a lane, each
 // group of lanes every S-th part into a running maximum and sums rescaled to it; then the groups of a
 // wave by lane shuffles, and the waves through LDS.
-template <typename T, int D>
+// FAST: exponentials as the hardware has them (of differences of at most 0), and all waves' sums at once.
+template <typename T, int D, bool FAST>
 __global__ __launch_bounds__(1024) void k_attention_paged_merge(int32_t B, T* __restrict__ out, PagedHeads hd, int32_t H,
                                                                 const int64_t* __restrict__ before, const float* __restrict__ ws,
                                                                 int32_t VH, int32_t waves)
@@ -308,7 +324,7 @@ __global__ __launch_bounds__(1024) void k_attention_paged_merge(int32_t B, T* __
     f4 num = {};
     auto join = [&](float m, float l, f4 o) {
         const float mn = fmaxf(M, m), mb = mn == -INFINITY ? 0.0f : mn;
-        const float f = exp2f(M - mb), e = exp2f(m - mb);
+        const float f = FAST ? __builtin_amdgcn_exp2f(M - mb) : exp2f(M - mb), e = FAST ? __builtin_amdgcn_exp2f(m - mb) : exp2f(m - mb);
         num = num * f + o * e;
         den = den * f + l * e;
         M = mn;
@@ -336,8 +352,26 @@ __global__ __launch_bounds__(1024) void k_attention_paged_merge(int32_t B, T* __
         }
         __syncthreads();
         if (wv > 0) return;
-        if (lane < L)
+        if (lane < L && !FAST)
             for (int i = 1; i < NW; i++) join(sm[i], sl[i], so[i][d]);
+        if (lane < L && FAST) {
+            float m[16];
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                m[i] = i < NW ? sm[i] : -INFINITY;
+                M = fmaxf(M, m[i]);
+            }
+            const float mb = M == -INFINITY ? 0.0f : M;
+            num = f4{};
+            den = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                if (i >= NW) break;
+                const float f = __builtin_amdgcn_exp2f(m[i] - mb);
+                num += so[i][d] * f;
+                den = __builtin_fmaf(sl[i], f, den);
+            }
+        }
     }
     if (lane < L)
 #pragma unroll
