@@ -23,8 +23,8 @@
  *   - A per-stream workspace that grows on demand (hipMalloc, to at least
  *     twice its size, never below 1 MiB) serves split-K GEMMs and
  *     fp32-activation GEMMs (M * K * 4 + M * 4 bytes for the split activations),
- *     single or in plans, multi-chunk decode attention, vvh_attention_paged and
- *     vvh_linear_q4 where they split a row, multi-block sampling,
+ *     single or in plans, multi-chunk decode attention, vvh_attention_paged,
+ *     vvh_attention_paged_q and vvh_linear_q4 where they split a row, multi-block sampling,
  *     and outside of captures vvh_dense of more than 4 rows and vvh_attention
  *     of several queries, where they split k or the keys.  Under HIP graph
  *     capture it cannot grow: run the same calls once on that stream before
@@ -643,7 +643,11 @@ VVH_API int vvh_read_paged_q(const vvh_paged_cache_q* cache, void* k_out, void* 
 /* vvh_attention_paged over a cache of codes: one query per sequence, lengths, positions without a page, rows without a
  * position and max_len as there.  Queries are used as given (fp32 ones to 22 bits of their row's largest), products
  * with codes are exact, sums and weights fp32, rounded once to the output.  Rows of the cache that no sequence has reached
- * may hold anything.  A NaN group of a key makes its heads' rows NaN, one of a value its dims. */
+ * may hold anything.  A NaN group of a key makes its heads' rows NaN, one of a value its dims (scales and minima that a
+ * program packs itself are finite, of either sign, or NaN).  At most 2^25 rows (num_seqs * num_heads).  Contexts over 1024 keys
+ * (512 of 8-bit values) may be split, as max_len or the page table's capacity says, and their partial sums then use the
+ * stream's workspace; its size depends only on the cache's sizes and bits, num_heads and max_len: make one such call
+ * before capturing on the stream. */
 VVH_API int vvh_attention_paged_q(const vvh_paged_cache_q* cache, void* out, const void* q, const int32_t* lens,
                                   size_t max_len, size_t num_heads, float scale, void* stream);
 /* Linear of 4-bit weights: out[M,N] = inp[M,K] . W[N,K]^T + bias[N] (+

@@ -365,6 +365,33 @@ def test_attention_values_of_very_different_scales(gpu, dtype, vb):
     check_attention(rng, [700, 700, 1500], 16, 4, 2, 128, 64, 8, vb, dtype, change=change)
 
 
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("kb,vb", [(4, 4), (8, 8)])
+def test_attention_over_negative_scales(gpu, dtype, kb, vb):
+    """Groups that a packer counted down from their largest value."""
+    def change(pg):
+        rng = np.random.default_rng(2)
+        for a, b in ((pg.ks, kb), (pg.vs, vb)):
+            down = rng.random(a.shape[:-1]) < 0.5
+            with np.errstate(invalid="ignore"):
+                a[..., 1] = np.where(down, a[..., 1] + a[..., 0] * (2 ** b - 1), a[..., 1])
+            a[..., 0] = np.where(down, -a[..., 0], a[..., 0])
+
+    rng = np.random.default_rng(26)
+    check_attention(rng, [300, 1500, 70], 16, 6, 2, 64, 32, kb, vb, dtype, change=change)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("scale", [-0.125, 0.0, -3e-5, 40.0])
+def test_attention_of_any_scale(gpu, dtype, scale):
+    rng = np.random.default_rng(27)
+    pg = PagesQ(rng, [300, 1500, 0, 7], 16, 2, 64, 32, 4, 4, dtype)
+    q = rng.normal(0, 1, (4, 6, 64)).astype(NP[dtype])
+    ref, tol = attention_q_ref(pg, q, float(np.float32(scale)), HALF[dtype])
+    got = run_attention(pg, q, scale=scale)
+    assert (np.abs(got - ref) <= tol).all() and (got[2] == 0).all()
+
+
 def test_attention_scores_that_differ_by_hundreds(gpu):
     rng = np.random.default_rng(18)
     check_attention(rng, [900, 2000], 16, 4, 2, 64, 32, 8, 4, F32, std=60.0)
@@ -463,6 +490,39 @@ def test_captured_step_replayed_with_new_values(gpu):
             for (n, h), e in zip(names, eager):
                 x = bufs[n].to_array(np.uint16, (4, h, D))
                 np.testing.assert_array_equal(x[live], e[live])
+    st.close()
+
+
+def test_two_graphs_of_one_stream(gpu):
+    """Two captured calls that split, and so share the stream's workspace, replayed in turn."""
+    rng = np.random.default_rng(28)
+    st = Stream()
+    pgs = [PagesQ(rng, lens, 16, 2, 128, 32, kb, 4, F16) for lens, kb in (([3000, 20, 2500], 4), ([1500] * 5, 8))]
+    qs = [rng.normal(0, 2, (len(pg.lens), 12, 128)).astype(np.float16) for pg in pgs]
+    dq, do = [capi.DevBuf.from_array(q) for q in qs], [capi.DevBuf(q.nbytes) for q in qs]
+
+    def call(i):
+        return lambda s: capi.call("vvh_attention_paged_q", pgs[i].cache(), do[i].ptr, dq[i].ptr, pgs[i].d_n.ptr, 0, 12,
+                                   float(1 / np.sqrt(128)), s)
+
+    out = lambda i: do[i].to_array(np.float16, qs[i].shape)  # noqa: E731
+    eager = []
+    for i in (0, 1):
+        call(i)(st.s)
+        st.sync()
+        eager.append(out(i))
+    replays = []
+    for i in (0, 1):
+        replays.append((st.capture(call(i)), st.keep))
+    for i in (0, 1, 1, 0, 1, 0):
+        capi.call("vvh_fill_normal", do[i].ptr, F16, qs[i].size, 1, 0.0, 1.0, None)
+        capi.sync()
+        replays[i][0]()
+        np.testing.assert_array_equal(out(i), eager[i])
+    for _, (g, e) in replays:
+        st.hip.hipGraphExecDestroy(e)
+        st.hip.hipGraphDestroy(g)
+    del st.keep
     st.close()
 
 

@@ -94,6 +94,7 @@ def test_attention_arguments():
     assert attention(cache(), out=2 * P) == INVALID               # out is q
     assert attention(cache(), heads=15) == INVALID                # two kv heads
     assert attention(cache(), heads=65536) == UNSUPPORTED
+    assert attention(cache(num_seqs=1025), heads=32768) == UNSUPPORTED and attention(cache(num_seqs=1024), heads=32768) == NOT_INIT
     assert attention(cache(), heads=0) == 0
     assert attention(cache(num_seqs=0), q=None) == 0
 

@@ -791,10 +791,11 @@ int launch_read_paged_q(const PagedQArgs& c, void* k_out, void* v_out, const int
     const int64_t parts = (2 * (int64_t)c.KVH + 3) / 4;
     int64_t each = kReadTokens;
     while (each > 4 && (tokens + each - 1) / each * parts < 1024) each /= 2;
+    const int64_t step = std::max<int64_t>(1, kQTokens / parts) * each;  // of a launch: at most 2^22 blocks
     auto go = [&](auto kern, auto* type) {
         using T = std::remove_pointer_t<decltype(type)>;
-        for (int64_t t = 0; t < tokens; t += kQTokens) {  // as above
-            const int64_t n = std::min(tokens - t, kQTokens), kd = t * c.KVH * c.D;
+        for (int64_t t = 0; t < tokens; t += step) {
+            const int64_t n = std::min(tokens - t, step), kd = t * c.KVH * c.D;
             hipLaunchKernelGGL(kern, dim3((unsigned)((n + each - 1) / each), (unsigned)parts), dim3(256), 0,
                                static_cast<hipStream_t>(stream), c, (T*)k_out + (k_out ? kd : 0), (T*)v_out + (v_out ? kd : 0),
                                seqs ? seqs + t : nullptr, positions + t, n, (int32_t)each);

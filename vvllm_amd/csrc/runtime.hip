@@ -2505,7 +2505,9 @@ VVH_API int vvh_attention_paged_q(const vvh_paged_cache_q* cache, void* out, con
     if (cache->num_seqs == 0 || num_heads == 0) return VVH_OK;
     if (!out || !q || !lens) return fail(VVH_ERR_INVALID_ARG, "null pointer");
     if (out == q) return fail(VVH_ERR_INVALID_ARG, "out is q");
-    if (num_heads > 65535) return fail(VVH_ERR_UNSUPPORTED, "%zu heads", num_heads);
+    // a launch of 2^32 threads would leave blocks out
+    if (num_heads > 65535 || cache->num_seqs * num_heads > (uint64_t(1) << 25))
+        return fail(VVH_ERR_UNSUPPORTED, "%zu heads of %llu sequences", num_heads, (unsigned long long)cache->num_seqs);
     if (!aligned16(q) || !aligned16(out) || ((uintptr_t)lens & 3)) return fail(VVH_ERR_INVALID_ARG, "misaligned pointer");
     REQUIRE_INIT();
     const AttnPagedPlan p = attention_paged_q_plan(a, (int64_t)std::min(max_len, (size_t)INT32_MAX), (int64_t)num_heads,
