@@ -197,6 +197,28 @@ def test_read_of_odd_scales(gpu, dtype):
                                           .astype(NP[dtype]))
 
 
+def test_read_of_many_heads_takes_several_launches(gpu):
+    """A launch of 65535 kv heads holds 4096 tokens: those after them are still their own sequences'."""
+    rng = np.random.default_rng(29)
+    KVH, D, T = 65535, 64, 4100
+    pg = PagesQ(rng, [16], 16, KVH, D, 64, 4, 4, F16, spare=0)
+    table = np.full((T, 1), int(pg.table[0, 0]), np.int32)
+    dt, dp = capi.DevBuf.from_array(table), capi.DevBuf.from_array((np.arange(T) % 16).astype(np.int32))
+    table[4097] = -1  # its row stays as it was
+    put(dt, table)
+    out = capi.DevBuf(T * KVH * D * 2)
+    row = KVH * D * 2
+    keep = rng.normal(0, 1, (KVH, D)).astype(np.float16)
+    capi.call("vvh_memcpy_h2d", out.addr(4097 * row), keep.ctypes.data, row)
+    capi.call("vvh_read_paged_q", pg.cache(page_table=dt.ptr, num_seqs=T), out.ptr, None, None, dp.ptr, T, None)
+    capi.sync()
+    for t in (0, 31, 4095, 4096, 4097, 4098, 4099):
+        got = np.empty((KVH, D), np.float16)
+        capi.call("vvh_memcpy_d2h", got.ctypes.data, out.addr(t * row), row)
+        w = pg.table[0, 0], slice(None), t % 16
+        bits_equal(got, keep if t == 4097 else capi.unpack_paged_q(pg.kp[w], pg.ks[w], 4, True).astype(np.float32).astype(np.float16))
+
+
 # ---- attention -------------------------------------------------------------------------
 def run_attention(pg, q, out=None, max_len=0, scale=None, stream=None):
     B, H, D = q.shape

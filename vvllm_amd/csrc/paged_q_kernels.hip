@@ -88,7 +88,8 @@ __device__ __forceinline__ void quantise8(const float (&x)[8], int bits, int lan
 
 // A block a token.  Items: 8 dims of a key (its own 8 values and the 8 that the rotation pairs them with), 8 of a value,
 // or 8 pairs of a query head.  A group is 4, 8 or 16 lanes in a row of one wave.  4001 tokens of 32 query and 8 kv heads of
-// 128 in fp16 to 4 bits, 88 MB: APPEND_US.
+// 128 in fp16 to 4 bits, 88 MB: 21.5 us, 4.1 TB/s, 0.86 of a large copy's rate (with 64-bit divisions for every code 25); 8 tokens of
+// 14 and 2 heads of 64: 3.1 us, a launch and its round trips.
 template <typename T, int D>
 __global__ __launch_bounds__(512) void k_rope_append_paged_q(PagedQArgs c, T* q_out, const T* q, const T* __restrict__ k,
                                                              const T* __restrict__ v, const int32_t* __restrict__ seqs,
@@ -151,12 +152,14 @@ __global__ __launch_bounds__(512) void k_rope_append_paged_q(PagedQArgs c, T* q_
 
 // A block takes up to 32 tokens: their rows are looked up first, then a wave takes the keys or the values of one kv head at a
 // time (gridDim.y blocks share them), 64 pieces of its tokens' rows together, which lie in a row where the tokens do.  A piece
-// is 16 bytes of output; UN of them a lane are on their way at a time (a token left out loads row 0).  READ_US
+// is 16 bytes of output; UN of them a lane are on their way at a time (a token left out loads row 0).  40 contexts of up to 2000
+// tokens, 8 heads of 128 in 4 bits to fp16, 97 MB: 23.7 us, 4.1 TB/s (a lane a unit after another 48); 3 of 20001 in 8 bits to fp32,
+// 148 MB: 35.7 us (with 32 bytes a lane, in two stores of half lines, 45).  Bound by HBM, four fifths of it writes.
 constexpr int kReadTokens = 32;
 template <typename T, int D, int UN>
 __global__ __launch_bounds__(256) void k_read_paged_q(PagedQArgs c, T* __restrict__ k_out, T* __restrict__ v_out,
                                                       const int32_t* __restrict__ seqs, const int32_t* __restrict__ positions,
-                                                      int64_t tokens, int32_t each)
+                                                      int64_t tokens, int32_t before, int32_t each)
 {
     constexpr int V = 16 / sizeof(T), per = D / V;
     struct __attribute__((aligned(16))) Out {
@@ -167,7 +170,7 @@ __global__ __launch_bounds__(256) void k_read_paged_q(PagedQArgs c, T* __restric
     const int32_t n = tokens - t0 < each ? (int32_t)(tokens - t0) : each, lane = threadIdx.x & 63;
     if ((int32_t)threadIdx.x < n) {
         const int64_t t = t0 + threadIdx.x;
-        rows[threadIdx.x] = paged_q_row(c, seqs ? seqs[t] : (int32_t)t, positions[t]);
+        rows[threadIdx.x] = paged_q_row(c, seqs ? seqs[t] : before + (int32_t)t, positions[t]);  // before: tokens of other launches
     }
     __syncthreads();
     const int32_t NG = D / c.group, glog = __builtin_ctz(c.group / V);
@@ -239,6 +242,11 @@ __global__ __launch_bounds__(256) void k_read_paged_q(PagedQArgs c, T* __restric
 // Loads of the next chunk are in flight while a chunk is worked on: V and the scales are free once they are in LDS, K once
 // the scores are there.  A tile past the end or on no page loads the first rows of page 0 instead; its scores
 // become -infinity and its scales 0, whatever they hold.
+// Measured in graphs: 32 contexts of 8192 keys, 32 heads on 8 of 128, 4 bits in groups of 32, 336 MB: 72 us, 4.6 TB/s (5.1 without the
+// merge); 32 of 4096, 8 heads on 8, 8 bits: 285 MB in 58.5 us; 96 from 1 to 8192 keys, 206 MB: 55.4 us.  Large ones are bound by
+// HBM, and 14 us of each call by what is not: lengths, pages, rows and the merge, each a round trip of its own.  At head_dim 64 a
+// chunk has half the bytes for the same scores, and the vector instructions count too (128 contexts of 8192 keys, 14 heads on 2,
+// 168 MB: 44 us).
 // ---------------------------------------------------------------------------
 template <int N>
 struct __attribute__((packed, aligned(4))) Words {
@@ -259,7 +267,8 @@ struct CodeMasks {
 __device__ __forceinline__ CodeMasks code_masks()
 {
     CodeMasks k{0x00f000f0u, 0x000f000fu, 0x54005400u, 0x64006400u};
-    asm("" : "+v"(k.mid), "+v"(k.low), "+s"(k.mid_one), "+s"(k.low_one));
+    asm("" : "+v"(k.mid), "+s"(k.mid_one));
+    asm("" : "+v"(k.low), "+s"(k.low_one));
     return k;
 }
 
@@ -798,7 +807,7 @@ int launch_read_paged_q(const PagedQArgs& c, void* k_out, void* v_out, const int
             const int64_t n = std::min(tokens - t, step), kd = t * c.KVH * c.D;
             hipLaunchKernelGGL(kern, dim3((unsigned)((n + each - 1) / each), (unsigned)parts), dim3(256), 0,
                                static_cast<hipStream_t>(stream), c, (T*)k_out + (k_out ? kd : 0), (T*)v_out + (v_out ? kd : 0),
-                               seqs ? seqs + t : nullptr, positions + t, n, (int32_t)each);
+                               seqs ? seqs + t : nullptr, positions + t, n, (int32_t)t, (int32_t)each);
         }
     };
     // 8 pieces a lane at a time where a block has as many, else 2 (40 contexts of up to 2000 tokens, 8 heads of 128, 23.6 us, 2
