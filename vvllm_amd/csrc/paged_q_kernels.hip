@@ -97,7 +97,8 @@ __global__ __launch_bounds__(512) void k_rope_append_paged_q(PagedQArgs c, T* q_
                                                              const float* __restrict__ rope, int32_t rope_positions)
 {
     constexpr int half = D / 2, per = D / 8;
-    const int32_t kvu = c.KVH * per, items = 2 * kvu + H * (half / 8);
+    // queries in waves of their own
+    const int32_t kvu = c.KVH * per, qi = (2 * kvu + 63) / 64 * 64, items = qi + H * (half / 8);
     const int64_t t = blockIdx.x;
     const int32_t s = seqs ? seqs[t] : (int32_t)t, p = positions[t];
     if (rope && p >= rope_positions) return;
@@ -105,6 +106,7 @@ __global__ __launch_bounds__(512) void k_rope_append_paged_q(PagedQArgs c, T* q_
     if (row < 0) return;
     const int lanes = c.group / 8;
     for (int32_t i = threadIdx.x; i < items; i += blockDim.x) {
+        if (i >= 2 * kvu && i < qi) continue;
         if (i < 2 * kvu) {
             const bool key = i < kvu;
             const int32_t j = key ? i : i - kvu, h = j / per, u = j - h * per;
@@ -133,7 +135,7 @@ __global__ __launch_bounds__(512) void k_rope_append_paged_q(PagedQArgs c, T* q_
             quantise8(x, bits, lanes, to, sm, u % lanes == 0);
             continue;
         }
-        const int32_t j = i - 2 * kvu, h = j / (half / 8), d = (j - h * (half / 8)) * 8;
+        const int32_t j = i - qi, h = j / (half / 8), d = (j - h * (half / 8)) * 8;
         const int64_t at = (t * H + h) * D + d;
         Eight<T> a = *reinterpret_cast<const Eight<T>*>(q + at), b = *reinterpret_cast<const Eight<T>*>(q + at + half);
         const f4* cs = reinterpret_cast<const f4*>(rope + ((int64_t)p * half + d) * 2);
@@ -772,7 +774,7 @@ int launch_rope_append_paged_q(const PagedQArgs& c, void* q_out, const void* q, 
                                const int32_t* seqs, const int32_t* positions, int64_t tokens, int64_t H, const float* rope,
                                int64_t rope_positions, int dtype, void* stream)
 {
-    const int64_t items = 2 * (int64_t)c.KVH * (c.D / 8) + H * (c.D / 16);
+    const int64_t items = (2 * (int64_t)c.KVH * (c.D / 8) + 63) / 64 * 64 + H * (c.D / 16);
     const int64_t threads = std::min<int64_t>((items + 63) / 64 * 64, tokens > 1024 ? 256 : 512);
     auto go = [&](auto kern, auto* type) {
         using T = std::remove_pointer_t<decltype(type)>;
