@@ -329,11 +329,30 @@ __global__ __launch_bounds__(1024) void k_attention_paged_merge(int32_t B, T* __
         den = den * f + l * e;
         M = mn;
     };
-    if (grp < GW) {
+    auto part = [&](int64_t i) {
+        const int64_t w = i < lead ? w0 + i : i < lead + full ? 4 * (f0 + i - lead) : 4 * k1 + i - lead - full;
+        return ws + ((w * 2 + (w == w0)) * hd.GT + hr) * (D + 4);
+    };
+    if constexpr (FAST) {  // four parts a group on their way at a time, the last ones again where there are fewer
+        for (int64_t i0 = wv * GW + (grp < GW ? grp : 0); i0 < parts; i0 += 4 * NW * GW) {
+            float m[4], l[4];
+            f4 o[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int64_t i = i0 + j * NW * GW;
+                const float* p = part(i < parts ? i : parts - 1);
+                m[j] = p[D];
+                l[j] = p[D + 1];
+                o[j] = *reinterpret_cast<const f4*>(p + 4 * d);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (i0 + j * NW * GW < parts) join(m[j], l[j], o[j]);
+        }
+    } else if (grp < GW) {
 #pragma unroll 4
         for (int64_t i = wv * GW + grp; i < parts; i += NW * GW) {
-            const int64_t w = i < lead ? w0 + i : i < lead + full ? 4 * (f0 + i - lead) : 4 * k1 + i - lead - full;
-            const float* p = ws + ((w * 2 + (w == w0)) * hd.GT + hr) * (D + 4);
+            const float* p = part(i);
             join(p[D], p[D + 1], *reinterpret_cast<const f4*>(p + 4 * d));
         }
     }
