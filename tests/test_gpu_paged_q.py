@@ -308,6 +308,13 @@ def test_attention_heads(gpu, dtype, H, KVH):
     check_attention(rng, [70, 1300, 9], 16, H, KVH, 64, 32, 4, 4, dtype)
 
 
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("lens", [[90, 17], [1300, 5]])
+def test_attention_many_kv_heads(gpu, dtype, lens):
+    rng = np.random.default_rng(31)
+    check_attention(rng, lens, 16, 600, 600, 64, 32, 4, 4, dtype)
+
+
 @pytest.mark.parametrize("page", [16, 32, 48, 80, 256, 1024])
 def test_attention_pages(gpu, page):
     rng = np.random.default_rng(page)
@@ -545,6 +552,25 @@ def test_two_graphs_of_one_stream(gpu):
         st.hip.hipGraphExecDestroy(e)
         st.hip.hipGraphDestroy(g)
     del st.keep
+    st.close()
+
+
+def test_short_contexts_captured(gpu):
+    """One launch, no workspace: captured on a stream that has made no call before, replayed with other lengths."""
+    rng = np.random.default_rng(32)
+    pg = PagesQ(rng, [500, 30, 0, 700], 16, 2, 128, 32, 8, 4, F16)
+    q = rng.normal(0, 2, (4, 12, 128)).astype(np.float16)
+    dq, do, st = capi.DevBuf.from_array(q), capi.DevBuf(q.nbytes), Stream()
+    replay = st.capture(lambda s: capi.call("vvh_attention_paged_q", pg.cache(), do.ptr, dq.ptr, pg.d_n.ptr, 700, 12, 0.125, s))
+    for lens in ([500, 30, 0, 700], [3, 0, 0, 64], [65, 17, -1, 640]):
+        pg.lens = np.array(lens, np.int32)
+        put(pg.d_n, pg.lens)
+        ref, tol = attention_q_ref(pg, q, 0.125, HALF[F16])
+        for _ in range(2):
+            capi.call("vvh_fill_normal", do.ptr, F16, q.size, 1, 0.0, 1.0, None)
+            capi.sync()
+            replay()
+            assert (np.abs(do.to_array(np.float16, q.shape) - ref) <= tol).all()
     st.close()
 
 
