@@ -421,6 +421,17 @@ def test_attention_of_any_scale(gpu, dtype, scale):
     assert (np.abs(got - ref) <= tol).all() and (got[2] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("scale", [np.nan, np.inf, -np.inf])
+def test_attention_of_a_scale_that_is_not_finite(gpu, dtype, scale):
+    """Rows that have a key are NaN, as the softmax of such scores; the others zeros."""
+    for lens in ([1, 0, 40], [3000, 0, 1]):
+        pg = PagesQ(np.random.default_rng(28), lens, 16, 2, 64, 32, 4, 4, dtype)
+        q = np.ones((3, 14, 64), NP[dtype])
+        got = run_attention(pg, q, scale=scale)
+        assert np.isnan(got[[0, 2]]).all() and (got[1] == 0).all()
+
+
 def test_attention_scores_that_differ_by_hundreds(gpu):
     rng = np.random.default_rng(18)
     check_attention(rng, [900, 2000], 16, 4, 2, 64, 32, 8, 4, F32, std=60.0)

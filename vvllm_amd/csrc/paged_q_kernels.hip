@@ -457,8 +457,9 @@ struct PagedQTiles {
         Operand q;  // worked out while the first chunk is on its way
         prepare(q0, lane, q);
         // scores to log2 units: positive (a negative scale turns q's sign), never 0, so that the maximum of the scores is
-        // that of the products and -infinity stays (2^-100 times any score is 0 for the exponential)
-        const float kl = fmaxf(__builtin_fabsf(__builtin_ldexpf(scale_log2, -q.e)), 0x1p-100f);
+        // that of the products and -infinity stays (2^-100 times any score is 0 for the exponential); a scale that is not
+        // finite makes the row NaN
+        const float kl = scale_log2 - scale_log2 == 0.0f ? fmaxf(__builtin_fabsf(__builtin_ldexpf(scale_log2, -q.e)), 0x1p-100f) : NAN;
         if (scale_log2 < 0.0f) {
 #pragma unroll
             for (int x = 0; x < DS; x++) {

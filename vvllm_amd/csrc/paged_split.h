@@ -1,9 +1,10 @@
 // Attention of one query per sequence over a paged cache, whatever its rows hold: a tile of up to 16 query heads of one kv
 // head is a wave's work on a chunk of keys, and here is how a batch's tiles and chunks are shared out and joined.  A class TL
 // of static members says the rest: Args (the cache; B, P, max_pages), T (queries and outputs), D, CH (keys of a chunk), HEAD
-// COLUMNS (a head's sums may be in several columns: put, store and join write what this code writes for the others), HEAD (chunks that the beginning of a tile is as long as: what comes before the first chunk's products counts in a batch of short contexts), VB
-// (bytes of LDS a wave), Q (a tile's queries in registers), load_q, tile (the chunks c0, c0 + cstep, ... below ke of sequence s
-// and kv head g), dim (of accumulator element (e, lane group, i)).
+// (chunks that the beginning of a tile is as long as: what comes before the first chunk's products counts in a batch of
+// short contexts), COLUMNS (a head's sums may be in several columns: put, store and join write what this code writes for the
+// others), VB (bytes of LDS a wave), Q (a tile's queries in registers), load_q, tile (the chunks c0, c0 + cstep, ... below ke
+// of sequence s and kv head g), dim (of accumulator element (e, lane group, i)).
 #pragma once
 
 #include <hip/hip_runtime.h>
