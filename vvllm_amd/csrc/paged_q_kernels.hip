@@ -227,15 +227,15 @@ __global__ __launch_bounds__(256) void k_read_paged_q(PagedQArgs c, T* __restric
 // ---------------------------------------------------------------------------
 // Attention on the matrix cores, a tile of up to 16 query heads of one kv head (paged_split.h says how tiles and chunks of keys
 // are shared out).  A wave takes CH keys at a time, in tiles of 16 that lie together in a page:
-//   S^T = K . q^T   A = K's codes c + b for a bias b that makes them fp16 values in one or two instructions a pair (CodeBias),
-//                   exact.  A group's sum begins at -b Q_g, Q_g the sum of the group's q, and is scaled in fp32:
-//                     score = sum_g s_g part_g + m_g Q_g.
+//   S^T = K . q^T   A = K's codes less their middle b (8 or 128) as fp16 values, exact.  A group's sum is scaled in fp32:
+//                     score = sum_g s_g part_g + (m_g + b s_g) Q_g, Q_g the sum of the group's q.
+//                   4-bit codes of fp16 rows are taken as 16 + c instead, and their sums begin at -16 Q_g.
 //                   q is scaled by a power of two to a largest of 2^10 .. 2^11 in its row (fp32: high and low part, 22 bits).
 //   softmax         online, in log2 units; maximum rounded up to an integer.
 //   O^T += V^T P^T  V's codes go through the wave's LDS region and its transposing reads of 4 and 8 bits, which give a lane the
-//                   codes of 16 (8) keys of one dim; taken with a bias again.  B = p s_g, the weights times their keys'
-//                   scales, as fp16 pairs high + low.  What the minima give, sum_k p m_g, is added up in fp32 beside, and what
-//                   the bias gives, b sum_k p s_g, by one more row of the product, whose A is 1.
+//                   codes of 16 (8) keys of one dim, less their middle b.  B = p s_g, the weights times their keys'
+//                   scales, as fp16 pairs high + low.  What the groups' middles give, sum_k p (m_g + b s_g), is added up in
+//                   fp32 beside.
 //                   Weights are times 2^14 over 2^es, a power of two above every scale so far, so that p s_g has fp16's range.
 // Column r of the products is head r / NGS and, of its groups, every NGS-th from r % NGS on: few heads leave columns free,
 // and scaling scores and weights is most of what a chunk costs (96 ragged contexts of 4 heads a kv head and 4 groups 116 us with a
@@ -255,49 +255,50 @@ struct __attribute__((packed, aligned(4))) Words {
     uint32_t w[N];
 };
 
-// What is added to a code of BITS bits to make an fp16 of it.  fp32 rows have the codes in the middle, and their minima moved by as
-// much (m - b s is the middle of the group's values, so that the two terms of a score are small).  fp16 rows take the cheapest,
-// 8 times as large, and its share out of the sums.  (The code's bits alone, an fp16 subnormal, would cost less yet, but the
-// matrix instruction keeps only about 17 bits of products of subnormals.)
-template <int BITS, bool TWO>
-constexpr float CodeBias = BITS == 8 ? (TWO ? -128.0f : 1024.0f) : (TWO ? -8.0f : 64.0f);
+// Codes are less their middle in the products, and minima moved by as much: m + b s is the middle of the group's values, so that
+// what sums are made of is not much larger than the values.  (A bias left in, 64 + c or 1024 + c, is fewer instructions, but sums of
+// n keys then hold n times the bias: fp16 outputs of 32 contexts of 32768 keys had a fourth of their elements rounded to a neighbour,
+// now 0.5 %, for 1 to 6 % of the time.  The code's bits alone, an fp16 subnormal, would cost less yet, but the matrix instruction
+// keeps only about 17 bits of products of subnormals.)
+template <int BITS>
+constexpr float CodeMiddle = BITS == 8 ? 128.0f : 8.0f;
 
 // Masks that the compiler knows nothing of: one in a vector and one in a scalar register are what v_and_or_b32 takes.
 struct CodeMasks {
-    uint32_t mid, low, mid_one, low_one;
+    uint32_t mid, low, high, mid_one, low_one, high_one;
 };
 __device__ __forceinline__ CodeMasks code_masks()
 {
-    CodeMasks k{0x00f000f0u, 0x000f000fu, 0x54005400u, 0x64006400u};
+    CodeMasks k{0x00f000f0u, 0x000f000fu, 0x03c003c0u, 0x54005400u, 0x64006400u, 0x4c004c00u};
     asm("" : "+v"(k.mid), "+s"(k.mid_one));
     asm("" : "+v"(k.low), "+s"(k.low_one));
+    asm("" : "+v"(k.high), "+s"(k.high_one));
     return k;
 }
 
-// 8 codes as an operand.  4 bits: code pairs (0, 4), (1, 5), (2, 6), (3, 7) of a word, the code in the mantissa's bits 4 to 7 (64 +
-// c), for fp32 rows also 0 to 3 (1024 + c), then less 72 or 1032; 8 bits: in order, in the mantissa's low bits (1024 + c), for
-// fp32 rows less 1152.
-template <bool TWO>
+// 8 codes less their middle as an operand.  4 bits: code pairs (0, 4), (1, 5), (2, 6), (3, 7) of a word, the code in the
+// mantissa's bits 4 to 7 (64 + c) or 0 to 3 (1024 + c), then less 72 or 1032; 8 bits: in order, in the mantissa's low bits (1024
+// + c), then less 1152.
 __device__ __forceinline__ h8 codes4(uint32_t w, const CodeMasks& k)
 {
-    if constexpr (TWO) {
-        const uint32_t v = w >> 8;
-        const h2 c72 = {(f16)72.0f, (f16)72.0f}, c1032 = {(f16)1032.0f, (f16)1032.0f};
-        const h2 a = __builtin_bit_cast(h2, (w & k.low) | k.low_one) - c1032, b = __builtin_bit_cast(h2, (w & k.mid) | k.mid_one) - c72;
-        const h2 c = __builtin_bit_cast(h2, (v & k.low) | k.low_one) - c1032, d = __builtin_bit_cast(h2, (v & k.mid) | k.mid_one) - c72;
-        return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-    }
-    return __builtin_bit_cast(h8, u4{(w << 4 & k.mid) | k.mid_one, (w & k.mid) | k.mid_one, (w >> 4 & k.mid) | k.mid_one,
-                                     (w >> 8 & k.mid) | k.mid_one});
+    const uint32_t v = w >> 8;
+    const h2 c72 = {(f16)72.0f, (f16)72.0f}, c1032 = {(f16)1032.0f, (f16)1032.0f};
+    const h2 a = __builtin_bit_cast(h2, (w & k.low) | k.low_one) - c1032, b = __builtin_bit_cast(h2, (w & k.mid) | k.mid_one) - c72;
+    const h2 c = __builtin_bit_cast(h2, (v & k.low) | k.low_one) - c1032, d = __builtin_bit_cast(h2, (v & k.mid) | k.mid_one) - c72;
+    return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
-template <bool TWO>
 __device__ __forceinline__ h8 codes8(uint32_t w0, uint32_t w1)
 {
     const u4 x = {__builtin_amdgcn_perm(0x64646464u, w0, 0x04010400u), __builtin_amdgcn_perm(0x64646464u, w0, 0x04030402u),
                   __builtin_amdgcn_perm(0x64646464u, w1, 0x04010400u), __builtin_amdgcn_perm(0x64646464u, w1, 0x04030402u)};
-    h8 y = __builtin_bit_cast(h8, x);
-    if constexpr (TWO) y -= (f16)1152.0f;
-    return y;
+    return __builtin_bit_cast(h8, x) - (f16)1152.0f;
+}
+// 4 bits, in the same order, as 16 + c (the mantissa's bits 6 to 9): for the sums of a key's dims, where 16 is next to the
+// largest code (128 contexts of 8192 keys, 14 heads on 2 of 64, 48.3 us, with the codes above 50.0).
+__device__ __forceinline__ h8 codes4_plus_16(uint32_t w, const CodeMasks& k)
+{
+    return __builtin_bit_cast(h8, u4{(w << 6 & k.high) | k.high_one, (w << 2 & k.high) | k.high_one,
+                                     (w >> 2 & k.high) | k.high_one, (w >> 6 & k.high) | k.high_one});
 }
 // High and low fp16 part of a pair of weights; minus: -1, in a register that the compiler knows nothing of, so that a
 // difference is one instruction that takes the fp16 as it is.
@@ -329,7 +330,7 @@ struct PagedQTiles {
     static constexpr int NP = (NG + NGS - 1) / NGS;                          // groups of a column
     static constexpr int SR = CH + 16, SW = NG * SR;                         // words of a group's scales in LDS, of a chunk's
     static constexpr int VB = CH * VP + 2 * SW * 4;
-    static constexpr bool TWO = sizeof(T) == 4;
+    static constexpr bool TWO = sizeof(T) == 4, PLUS16 = !TWO && KB == 4;
     // Lane (r, gr): dims 32 s + 8 gr .. + 7 of head r / NGS
     struct Q {
         Eight<T> v[DS];
@@ -381,14 +382,14 @@ struct PagedQTiles {
             }
         }
 #pragma unroll
-        for (int p = 0; p < NP; p++) x.sum[p] = sum_x32(sum_x16(x.sum[p]));
+        for (int p = 0; p < NP; p++) x.sum[p] = mx == INFINITY ? NAN : sum_x32(sum_x16(x.sum[p]));  // no score of it is a number
     }
 
-    // What a group's codes less their bias are added to: its minimum, for fp32 rows less the bias' share
+    // What a group's codes less their middle are added to
     template <int BITS>
     static __device__ __forceinline__ float middle(uint32_t sm)
     {
-        return TWO ? __builtin_fmaf(pair_scale(sm), -CodeBias<BITS, TWO>, pair_min(sm)) : pair_min(sm);
+        return __builtin_fmaf(pair_scale(sm), CodeMiddle<BITS>, pair_min(sm));
     }
 
     struct Spot {
@@ -412,8 +413,6 @@ struct PagedQTiles {
         asm("" : "+s"(minus));
         const CodeMasks masks = code_masks();
         acc.clear();
-        f4 ones = {};  // the row of ones
-        float ws[NP] = {};  // several groups a column: the sums of the weights themselves, in a register each
         float om[NP] = {}, m = -INFINITY, l = 0.0f, ref = 0x1p-30f;
         int es = -30;
 
@@ -505,11 +504,13 @@ struct PagedQTiles {
                 f4 part[NT];
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
-                    const float first = TWO ? 0.0f : -CodeBias<KB, TWO> * q.sum[p];
+                    const float first = PLUS16 ? -16.0f * q.sum[p] : 0.0f;
                     part[t] = f4{first, first, first, first};
 #pragma unroll
                     for (int x = p * NGS * GS; x < (p + 1) * NGS * GS && x < DS; x++) {
-                        const h8 a = KB == 4 ? codes4<TWO>(K[t].w[x], masks) : codes8<TWO>(K[t].w[2 * x % KW], K[t].w[(2 * x + 1) % KW]);
+                        const h8 a = PLUS16   ? codes4_plus_16(K[t].w[x], masks)
+                                     : KB == 4 ? codes4(K[t].w[x], masks)
+                                               : codes8(K[t].w[2 * x % KW], K[t].w[(2 * x + 1) % KW]);
                         if constexpr (TWO) part[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q.lo[x], part[t], 0, 0, 0);
                         part[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q.hi[x], part[t], 0, 0, 0);
                     }
@@ -519,7 +520,7 @@ struct PagedQTiles {
                     const u4 sm = *reinterpret_cast<const u4*>(lk + group_of(r, p) * SR + 16 * t + 4 * gr);
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const float y = __builtin_fmaf(middle<KB>(sm[i]), q.sum[p], p ? sc[t][i] : 0.0f);
+                        const float y = __builtin_fmaf(PLUS16 ? pair_min(sm[i]) : middle<KB>(sm[i]), q.sum[p], p ? sc[t][i] : 0.0f);
                         sc[t][i] = __builtin_fmaf(pair_scale(sm[i]), part[t][i], y);
                     }
                 }
@@ -558,12 +559,8 @@ struct PagedQTiles {
                 m = mn;
                 es = en;
                 l *= f;
-                ones *= f;
 #pragma unroll
-                for (int p = 0; p < NP; p++) {
-                    om[p] *= f;
-                    ws[p] *= f;
-                }
+                for (int p = 0; p < NP; p++) om[p] *= f;
 #pragma unroll
                 for (int e = 0; e < D / 16; e++) acc.o[e] *= f;
             }
@@ -587,11 +584,7 @@ struct PagedQTiles {
                     for (int i = 0; i < 4; i++)
                         om[p] = __builtin_fmaf(sc[t][i], middle<VBITS>(sm[t][i]), om[p]);
                 // + 0: one instruction that takes the scale as it is
-                auto w = [&](int t, int i) {
-                    const float x = __builtin_fmaf(sc[t][i], pair_scale(sm[t][i]), 0.0f);
-                    if constexpr (!TWO && NP > 1) ws[p] += x;
-                    return x;
-                };
+                auto w = [&](int t, int i) { return __builtin_fmaf(sc[t][i], pair_scale(sm[t][i]), 0.0f); };
 #pragma unroll
                 for (int u = 0; u < NT / 2; u++)
 #pragma unroll
@@ -602,15 +595,6 @@ struct PagedQTiles {
                         hi[u][i] = h;
                         lo[u][i] = o;
                     }
-                if constexpr (!TWO && NP == 1) {
-                    const f16 one = (f16)1.0f;
-                    const h8 row = {one, one, one, one, one, one, one, one};
-#pragma unroll
-                    for (int u = 0; u < NT / 2; u++) {
-                        ones = __builtin_amdgcn_mfma_f32_16x16x32_f16(row, __builtin_bit_cast(h8, lo[u]), ones, 0, 0, 0);
-                        ones = __builtin_amdgcn_mfma_f32_16x16x32_f16(row, __builtin_bit_cast(h8, hi[u]), ones, 0, 0, 0);
-                    }
-                }
 #pragma unroll
                 for (int e = p * NGS * GS * 2; e < (p + 1) * NGS * GS * 2 && e < D / 16; e++) {
                     h8 a[NT / 2];
@@ -619,13 +603,13 @@ struct PagedQTiles {
                         // nibble n of a lane: key 4 gr + n % 4 of tile n / 4
                         const char* src = lds + (16 * gr + 4 * (r & 3) + (r >> 2)) * VP + 8 * e;
                         const i2 w2 = __builtin_amdgcn_ds_read_tr4_b64_v2i32((__attribute__((address_space(3))) i2*)(src));
-                        a[0] = codes4<TWO>((uint32_t)w2[0], masks);
-                        a[1] = codes4<TWO>((uint32_t)w2[1], masks);
+                        a[0] = codes4((uint32_t)w2[0], masks);
+                        a[1] = codes4((uint32_t)w2[1], masks);
                     } else {
                         // byte n of a lane: key 4 gr + n % 4 of tile n / 4
                         const char* src = lds + (8 * gr + 2 * (r >> 1 & 3) + (r >> 3)) * VP + 16 * e + 8 * (r & 1);
                         const i2 w2 = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i2*)(src));
-                        a[0] = codes8<TWO>((uint32_t)w2[0], (uint32_t)w2[1]);
+                        a[0] = codes8((uint32_t)w2[0], (uint32_t)w2[1]);
                     }
 #pragma unroll
                     for (int u = 0; u < NT / 2; u++) {
@@ -637,10 +621,7 @@ struct PagedQTiles {
         }
         float ms[NP];
 #pragma unroll
-        for (int p = 0; p < NP; p++) {
-            ms[p] = sum_x32(sum_x16(om[p]));
-            if constexpr (!TWO) ms[p] = __builtin_fmaf(-CodeBias<VBITS, TWO>, NP == 1 ? ones[0] : sum_x32(sum_x16(ws[p])), ms[p]);
-        }
+        for (int p = 0; p < NP; p++) ms[p] = sum_x32(sum_x16(om[p]));
 #pragma unroll
         for (int e = 0; e < D / 16; e++) acc.o[e] += ms[e / (2 * GS) / NGS];
         acc.l = sum_x32(sum_x16(l));
