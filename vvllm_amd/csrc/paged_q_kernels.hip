@@ -5,6 +5,8 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
+#include <limits>
 #include <type_traits>
 
 #include "common.h"
@@ -231,7 +233,9 @@ __global__ __launch_bounds__(256) void k_read_paged_q(PagedQArgs c, T* __restric
 //                     score = sum_g s_g part_g + (m_g + b s_g) Q_g, Q_g the sum of the group's q.
 //                   4-bit codes of fp16 rows are taken as 16 + c instead, and their sums begin at -16 Q_g.
 //                   q is scaled by a power of two to a largest of 2^10 .. 2^11 in its row (fp32: high and low part, 22 bits).
-//   softmax         online, in log2 units; maximum rounded up to an integer.
+//   softmax         online, in log2 units less a reference: the maximum rounded up to an integer, so that references differ
+//                   exactly; from 2^20 on, where a score's last bit is a factor, the largest score itself, subtracted before
+//                   scores are taken to log2 units.  Finite inputs whose scores pass fp32's range so give the weights of their limit.
 //   O^T += V^T P^T  V's codes go through the wave's LDS region and its transposing reads of 4 and 8 bits, which give a lane the
 //                   codes of 16 (8) keys of one dim, less their middle b.  B = p s_g, the weights times their keys'
 //                   scales, as fp16 pairs high + low.  What the groups' middles give, sum_k p (m_g + b s_g), is added up in
@@ -413,7 +417,7 @@ struct PagedQTiles {
         asm("" : "+s"(minus));
         const CodeMasks masks = code_masks();
         acc.clear();
-        float om[NP] = {}, m = -INFINITY, l = 0.0f, ref = 0x1p-30f;
+        float om[NP] = {}, R = 0.0f, m = -INFINITY, l = 0.0f, ref = 0x1p-30f;  // the reference: score R, and m log2 units above it
         int es = -30;
 
         Words<KW> K[NT];
@@ -455,10 +459,15 @@ struct PagedQTiles {
         spot = look(c, s, c0 + cstep, lane);
         Operand q;  // worked out while the first chunk is on its way
         prepare(q0, lane, q);
-        // scores to log2 units: positive (a negative scale turns q's sign), never 0, so that the maximum of the scores is
-        // that of the products and -infinity stays (2^-100 times any score is 0 for the exponential); a scale that is not
-        // finite makes the row NaN
-        const float kl = scale_log2 - scale_log2 == 0.0f ? fmaxf(__builtin_fabsf(__builtin_ldexpf(scale_log2, -q.e)), 0x1p-100f) : NAN;
+        // Scores to log2 units: positive (a negative scale turns q's sign), never 0, so that the maximum of the scores is
+        // that of the products and -infinity stays.  Scores are below 2^44 and, but for those of queries rounded away, multiples of
+        // 2^-48: past these ends all weights are alike, or all but the largest's 0.  A scale that is not finite makes scores NaN.
+        const bool fine = scale_log2 - scale_log2 == 0.0f;
+        const float kl = fine ? __builtin_amdgcn_fmed3f(__builtin_fabsf(__builtin_ldexpf(scale_log2, -q.e)), 0x1p-100f, 0x1p80f) : 1.0f;
+        if (!fine) {
+#pragma unroll
+            for (int p = 0; p < NP; p++) q.sum[p] = NAN;
+        }
         if (scale_log2 < 0.0f) {
 #pragma unroll
             for (int x = 0; x < DS; x++) {
@@ -546,23 +555,36 @@ struct PagedQTiles {
 #pragma unroll
                 for (int i = 0; i < 4; i++) cm = fmaxf(cm, sc[t][i]);
             load_k();
-            cm = max_x32(max_x16(cm)) * kl;
-            if (__any(cm > m || smax > ref)) {  // a new maximum for some head, or a new largest scale
-                const float mn = __builtin_ceilf(fmaxf(m, cm));
+            cm = max_x32(max_x16(cm));
+            const bool more = (cm - R) * kl > m;
+            if (__any(more || smax > ref)) {  // a new maximum for some head, or a new largest scale
+                const float y = cm * kl;
+                const bool far = __builtin_fabsf(y) >= 0x1p20f;
+                const float Rn = far ? cm : 0.0f, mn = far ? 0.0f : __builtin_ceilf(y);
                 int en = es;
                 if (__any(smax > ref)) {
                     en = (int)(__builtin_bit_cast(uint32_t, group_max(smax, 64)) >> 23) - 126;
                     en = __builtin_amdgcn_readfirstlane(en < 16 ? en : 16);
                     ref = __builtin_ldexpf(1.0f, en);
                 }
-                const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn + (float)(es - en));
-                m = mn;
+                const float f = __builtin_amdgcn_exp2f((more ? __builtin_fmaf(R - Rn, kl, m - mn) : 0.0f) + (float)(es - en));
+                if (more) {
+                    R = Rn;
+                    m = mn;
+                }
                 es = en;
                 l *= f;
 #pragma unroll
                 for (int p = 0; p < NP; p++) om[p] *= f;
 #pragma unroll
                 for (int e = 0; e < D / 16; e++) acc.o[e] *= f;
+            }
+            if (uint64_t far = __ballot(R != 0.0f)) {
+                asm volatile("" : "+s"(far));  // a branch, as above
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) sc[t][i] -= R;
             }
             const float mb = m == -INFINITY ? 0.0f : m - 14.0f + (float)es;  // no key yet: every weight below is 0
 #pragma unroll
@@ -619,13 +641,17 @@ struct PagedQTiles {
                 }
             }
         }
+        // without the weights' power of two, exactly, so that parts of different ones join by their references alone
+        const float back = __builtin_ldexpf(1.0f, es);
         float ms[NP];
 #pragma unroll
-        for (int p = 0; p < NP; p++) ms[p] = sum_x32(sum_x16(om[p]));
+        for (int p = 0; p < NP; p++) ms[p] = sum_x32(sum_x16(om[p])) * back;
 #pragma unroll
-        for (int e = 0; e < D / 16; e++) acc.o[e] += ms[e / (2 * GS) / NGS];
-        acc.l = sum_x32(sum_x16(l));
-        acc.m = m == -INFINITY ? m : m + (float)es;
+        for (int e = 0; e < D / 16; e++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc.o[e][i] = __builtin_fmaf(acc.o[e][i], back, ms[e / (2 * GS) / NGS]);
+        acc.l = sum_x32(sum_x16(l)) * back;
+        acc.m = __builtin_fmaf(R, kl, m);
     }
 
     // The n heads' sums, from the columns of each dim's group: rows of `pitch` floats and their maxima and sums, which without
@@ -860,7 +886,9 @@ static void paged_q_go(const AttnPagedPlan& p, const PagedQArgs& c, typename TL:
 int launch_attention_paged_q(const AttnPagedPlan& p, const PagedQArgs& c, void* out, const void* q, const int32_t* lens, int64_t H,
                              float scale, float* ws, int dtype, void* stream)
 {
-    const float sl = (float)((double)scale * 1.4426950408889634);  // scores in log2 units
+    constexpr double most = std::numeric_limits<float>::max();
+    const double log2_units = (double)scale * 1.4426950408889634;  // a finite scale stays finite
+    const float sl = std::isfinite(scale) ? (float)std::clamp(log2_units, -most, most) : scale;
     auto run = [&](auto* t, auto d, auto ng, auto ngs) {
         using T = std::remove_pointer_t<decltype(t)>;
         constexpr int D = decltype(d)::value, NG = decltype(ng)::value, NGS = decltype(ngs)::value;
