@@ -11,7 +11,7 @@ def attention_q_bounds(pages, q, scale, tol_out):
     middles in fp32 (sizes |q| (2^bits |s| + |m|)), fp32 queries to 2^-23 of their largest, roundings of the scale and of the
     difference to the largest score, and 2^-21 for a weight's own (an exponential, a high and a low part).  Sums: two roundings
     each 16 keys and 64 at the end, of partial sums of sizes 2^bits |s| + |m|.  Weights times scales are kept to 2^-37 of the
-    largest scale, times codes of at most 2^(bits - 1)."""
+    largest scale and weight, times codes of at most 2^(bits - 1); n such roundings, at random, to 8 deviations sqrt(n / 3)."""
     B, H, D = q.shape
     ref, tol = np.zeros((B, H, D)), np.zeros((B, H, D))
     for s in range(B):
@@ -37,7 +37,8 @@ def attention_q_bounds(pages, q, scale, tol_out):
             least = (p * np.exp(-np.minimum(d, 700))).sum()
             tol[s, h] = off @ np.abs(v[:, g] - ref[s, h]) / least
             tol[s, h] += (len(p) / 8 + 64) * 2.0 ** -24 * (p @ vs[:, g])
-            tol[s, h] += len(p) * p.max() * 2.0 ** -37 * b[:, g, :, 0].max() * 2.0 ** (pages.vb - 1)
+            n = min(len(p), 8 * np.sqrt(len(p) / 3))
+            tol[s, h] += n * p.max() * 2.0 ** -37 * b[:, g, :, 0].max() * 2.0 ** (pages.vb - 1)
     return ref, tol + tol_out * np.abs(ref) + 2.0 ** -25
 
 
