@@ -645,8 +645,8 @@ VVH_API int vvh_read_paged_q(const vvh_paged_cache_q* cache, void* k_out, void* 
  * with codes are exact, sums and weights fp32, rounded once to the output.  Rows of the cache that no sequence has reached
  * may hold anything.  A NaN group of a key makes its heads' rows NaN, one of a value its dims (scales and minima that a
  * program packs itself are finite, of either sign, or NaN); a scale that is not finite makes every row with a position
- * NaN.  Weights times value scales are kept to 2^-39 of the largest scale of a kv head's keys: values of groups whose
- * scales are 2^-20 of another's keep about 15 bits.  At most 2^25 rows (num_seqs * num_heads).  Contexts over 1024 keys
+ * NaN.  Weights times value scales are kept to 2^-37 of the largest weight times the largest scale of a kv head's keys:
+ * values of groups whose scales are 2^-20 of another's keep about 15 bits.  At most 2^25 rows (num_seqs * num_heads).  Contexts over 1024 keys
  * (512 of 8-bit values) may be split, as max_len or the page table's capacity says, and their partial sums then use the
  * stream's workspace; its size depends only on the cache's sizes and bits, num_heads and max_len: make one such call
  * before capturing on the stream. */
