@@ -6,7 +6,7 @@ import pytest
 from paged_q import NP, PagesQ
 from paged_q_bounds import attention_q_bounds, plant
 from serving import HALF
-from test_gpu_paged_q import case, run_attention
+from test_gpu_paged_q import case, read_rows, run_attention
 from vvllm_amd import capi
 
 pytestmark = pytest.mark.gpu
@@ -120,3 +120,19 @@ def test_rows_whose_pages_are_all_gone(gpu, dtype, scale, n):
     got = run_attention(pg, np.ones((2, 6, 64), NP[dtype]), scale=scale)
     assert (got[0] == 0).all()
     assert np.isnan(got[1]).all() if not np.isfinite(scale) else np.isfinite(got[1]).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("D,group,kb,vb", FORMATS + [(64, 64, 8, 8), (128, 32, 4, 4)])
+@pytest.mark.parametrize("G", [1, 3, 16])
+@pytest.mark.parametrize("lens", [[1], [1] * 70, [1, 2000, 1, 0, 1]])
+def test_rows_of_one_key_are_the_row_read_back(gpu, dtype, D, group, kb, vb, G, lens):
+    """Its weight is 1, and m + s c fits fp32 where m and s come from values of one size: the same bits as vvh_read_paged_q."""
+    case("one key", dtype, D, group, kb, vb, G, lens)
+    rng = np.random.default_rng(44)
+    pg = PagesQ(rng, lens, 16, 2, D, group, kb, vb, dtype)
+    q = rng.normal(0, 2, (len(lens), 2 * G, D)).astype(NP[dtype])
+    got = run_attention(pg, q)
+    one = [s for s, n in enumerate(lens) if n == 1]
+    _, v = read_rows(pg, one, [0] * len(one))
+    np.testing.assert_array_equal(got[one], v.astype(np.float64).repeat(G, 1))

@@ -233,9 +233,9 @@ __global__ __launch_bounds__(256) void k_read_paged_q(PagedQArgs c, T* __restric
 //                     score = sum_g s_g part_g + (m_g + b s_g) Q_g, Q_g the sum of the group's q.
 //                   4-bit codes of fp16 rows are taken as 16 + c instead, and their sums begin at -16 Q_g.
 //                   q is scaled by a power of two to a largest of 2^10 .. 2^11 in its row (fp32: high and low part, 22 bits).
-//   softmax         online, in log2 units less a reference: the maximum rounded up to an integer, so that references differ
-//                   exactly; from 2^20 on, where a score's last bit is a factor, the largest score itself, subtracted before
-//                   scores are taken to log2 units.  Finite inputs whose scores pass fp32's range so give the weights of their limit.
+//   softmax         online; weights are powers of two of (score - R) kl, R the row's largest score when it last rose by a factor
+//                   of more than 2: subtracted before scores are taken to log2 units, so that a row of one key is exact, and scores
+//                   of any size, past fp32's range too, give the weights they stand for.
 //   O^T += V^T P^T  V's codes go through the wave's LDS region and its transposing reads of 4 and 8 bits, which give a lane the
 //                   codes of 16 (8) keys of one dim, less their middle b.  B = p s_g, the weights times their keys'
 //                   scales, as fp16 pairs high + low.  What the groups' middles give, sum_k p (m_g + b s_g), is added up in
@@ -417,7 +417,7 @@ struct PagedQTiles {
         asm("" : "+s"(minus));
         const CodeMasks masks = code_masks();
         acc.clear();
-        float om[NP] = {}, R = 0.0f, m = -INFINITY, l = 0.0f, ref = 0x1p-30f;  // the reference: score R, and m log2 units above it
+        float om[NP] = {}, R = -INFINITY, l = 0.0f, ref = 0x1p-30f;
         int es = -30;
 
         Words<KW> K[NT];
@@ -556,22 +556,16 @@ struct PagedQTiles {
                 for (int i = 0; i < 4; i++) cm = fmaxf(cm, sc[t][i]);
             load_k();
             cm = max_x32(max_x16(cm));
-            const bool more = (cm - R) * kl > m;
+            const bool more = (cm - R) * kl > 1.0f;
             if (__any(more || smax > ref)) {  // a new maximum for some head, or a new largest scale
-                const float y = cm * kl;
-                const bool far = __builtin_fabsf(y) >= 0x1p20f;
-                const float Rn = far ? cm : 0.0f, mn = far ? 0.0f : __builtin_ceilf(y);
                 int en = es;
                 if (__any(smax > ref)) {
                     en = (int)(__builtin_bit_cast(uint32_t, group_max(smax, 64)) >> 23) - 126;
                     en = __builtin_amdgcn_readfirstlane(en < 16 ? en : 16);
                     ref = __builtin_ldexpf(1.0f, en);
                 }
-                const float f = __builtin_amdgcn_exp2f((more ? __builtin_fmaf(R - Rn, kl, m - mn) : 0.0f) + (float)(es - en));
-                if (more) {
-                    R = Rn;
-                    m = mn;
-                }
+                const float f = __builtin_amdgcn_exp2f((more ? (R - cm) * kl : 0.0f) + (float)(es - en));
+                if (more) R = cm;
                 es = en;
                 l *= f;
 #pragma unroll
@@ -579,19 +573,12 @@ struct PagedQTiles {
 #pragma unroll
                 for (int e = 0; e < D / 16; e++) acc.o[e] *= f;
             }
-            if (uint64_t far = __ballot(R != 0.0f)) {
-                asm volatile("" : "+s"(far));  // a branch, as above
-#pragma unroll
-                for (int t = 0; t < NT; t++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) sc[t][i] -= R;
-            }
-            const float mb = m == -INFINITY ? 0.0f : m - 14.0f + (float)es;  // no key yet: every weight below is 0
+            const float Rb = R == -INFINITY ? 0.0f : R, up = (float)(14 - es);  // no key yet: every weight is 0
 #pragma unroll
             for (int t = 0; t < NT; t++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    sc[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][i], kl, -mb));
+                    sc[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][i] - Rb, kl, up));
                     l += sc[t][i];
                 }
             // ---- values
@@ -641,7 +628,7 @@ struct PagedQTiles {
                 }
             }
         }
-        // without the weights' power of two, exactly, so that parts of different ones join by their references alone
+        // without the weights' power of two, exactly, so that parts of different ones join by R alone
         const float back = __builtin_ldexpf(1.0f, es);
         float ms[NP];
 #pragma unroll
@@ -651,7 +638,7 @@ struct PagedQTiles {
 #pragma unroll
             for (int i = 0; i < 4; i++) acc.o[e][i] = __builtin_fmaf(acc.o[e][i], back, ms[e / (2 * GS) / NGS]);
         acc.l = sum_x32(sum_x16(l)) * back;
-        acc.m = __builtin_fmaf(R, kl, m);
+        acc.m = R * kl;
     }
 
     // The n heads' sums, from the columns of each dim's group: rows of `pitch` floats and their maxima and sums, which without
