@@ -136,3 +136,25 @@ def test_rows_of_one_key_are_the_row_read_back(gpu, dtype, D, group, kb, vb, G, 
     one = [s for s, n in enumerate(lens) if n == 1]
     _, v = read_rows(pg, one, [0] * len(one))
     np.testing.assert_array_equal(got[one], v.astype(np.float64).repeat(G, 1))
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("D,group,kb,vb", FORMATS + [(64, 64, 8, 8), (128, 32, 8, 8)])
+@pytest.mark.parametrize("G", [2, 16])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_queries_that_are_not_finite(gpu, dtype, D, group, kb, vb, G, bad):
+    """Their rows are NaN, in whichever group the value is, those without a position zeros, all others as they were."""
+    case("queries", dtype, D, group, kb, vb, G, bad)
+    rng = np.random.default_rng(45)
+    pg = PagesQ(rng, [1, 70, 2000, 0], 16, 2, D, group, kb, vb, dtype)
+    q = rng.normal(0, 2, (4, 2 * G, D)).astype(NP[dtype])
+    clean = run_attention(pg, q)
+    where = [(s, h, d) for s in range(4) for h, d in ((0, 0), (G, D - 1), (2 * G - 1, D // 2))]
+    for s, h, d in where:
+        q[s, h, d] = bad
+    got = run_attention(pg, q)
+    rows = np.zeros(got.shape[:2], bool)
+    for s, h, _ in where:
+        rows[s, h] = s < 3
+    assert np.isnan(got[rows]).all()
+    np.testing.assert_array_equal(got[~rows], clean[~rows])
