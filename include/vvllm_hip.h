@@ -637,19 +637,21 @@ VVH_API int vvh_rope_append_paged_q(const vvh_paged_cache_q* cache, void* q_out,
 /* Rows of the cache as the values that they stand for: row t of k_out and v_out [tokens, num_kv_heads, head_dim] (either
  * may be NULL) from position positions[t] of sequence seqs[t] (seqs NULL: sequence t); m + s c in fp32, rounded to dtype.
  * A token whose sequence, position or page is out of range leaves its rows as they are.  With the positions of a
- * sequence in order, vvh_attention then takes the rows: several queries, such as a prompt's next part. */
+ * sequence in order, vvh_attention then takes the rows: several queries, such as a prompt's next part, up to its 16000
+ * positions. */
 VVH_API int vvh_read_paged_q(const vvh_paged_cache_q* cache, void* k_out, void* v_out, const int32_t* seqs,
                              const int32_t* positions, size_t tokens, void* stream);
 /* vvh_attention_paged over a cache of codes: one query per sequence, lengths, positions without a page, rows without a
  * position and max_len as there.  Queries are used as given (fp32 ones to 22 bits of their row's largest), products
  * with codes are exact, sums and weights fp32, rounded once to the output.  Rows of the cache that no sequence has reached
  * may hold anything.  A NaN group of a key makes its heads' rows NaN, one of a value its dims (scales and minima that a
- * program packs itself are finite, of either sign, or NaN); a scale that is not finite makes every row with a position
- * NaN.  Weights times value scales are kept to 2^-37 of the largest weight times the largest scale of a kv head's keys:
- * values of groups whose scales are 2^-20 of another's keep about 15 bits.  At most 2^25 rows (num_seqs * num_heads).  Contexts over 1024 keys
- * (512 of 8-bit values) may be split, as max_len or the page table's capacity says, and their partial sums then use the
- * stream's workspace; its size depends only on the cache's sizes and bits, num_heads and max_len: make one such call
- * before capturing on the stream. */
+ * program packs itself are finite, of either sign, or NaN).  Of rows with a position, a query that is not finite makes its
+ * own NaN, a scale that is not finite every one; finite ones may give scores past fp32's range, whose weights are those of
+ * the scores all the same.  Weights times value scales are kept to 2^-37 of the largest weight times the largest scale of a
+ * kv head's keys: values of groups whose scales are 2^-20 of another's keep about 15 bits.  At most 2^25 rows (num_seqs *
+ * num_heads).  Contexts over 1024 keys (512 of 8-bit values) may be split, as max_len or the page table's capacity says,
+ * and their partial sums then use the stream's workspace; its size depends only on the cache's sizes and bits, num_heads
+ * and max_len: make one such call before capturing on the stream. */
 VVH_API int vvh_attention_paged_q(const vvh_paged_cache_q* cache, void* out, const void* q, const int32_t* lens,
                                   size_t max_len, size_t num_heads, float scale, void* stream);
 /* Linear of 4-bit weights: out[M,N] = inp[M,K] . W[N,K]^T + bias[N] (+

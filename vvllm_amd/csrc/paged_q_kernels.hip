@@ -248,11 +248,12 @@ __global__ __launch_bounds__(256) void k_read_paged_q(PagedQArgs c, T* __restric
 // Loads of the next chunk are in flight while a chunk is worked on: V and the scales are free once they are in LDS, K once
 // the scores are there.  A tile past the end or on no page loads the first rows of page 0 instead; its scores
 // become -infinity and its scales 0, whatever they hold.
-// Measured in graphs: 32 contexts of 8192 keys, 32 heads on 8 of 128, 4 bits in groups of 32, 336 MB: 72-75 us, 4.6 TB/s (5.1 without the
-// merge); 32 of 4096, 8 heads on 8, 8 bits: 285 MB in 58-61 us; 96 from 1 to 8192 keys, 206 MB: 54.1 us.  Large ones are bound by
-// HBM, and 14 us of each call by what is not: lengths, pages, rows and the merge, each a round trip of its own.  The same at
-// head_dim 64, where a chunk has half the bytes for as many scores: 128 contexts of 8192 keys, 14 heads on 2, 168 MB: 48 us, and
-// 256 of them 82 us, 4.9 TB/s for the difference.
+// Measured in graphs: 32 contexts of 8192 keys, 32 heads on 8 of 128, 4 bits in groups of 32, 336 MB: 72-75 us, 4.6 TB/s; 32 of
+// 4096, 8 heads on 8, 8 bits: 285 MB in 58-59 us; 96 from 1 to 8192 keys, 206 MB: 54.8 us.  Large ones are bound by HBM: 32
+// contexts of 2048, 4096, 8192 and 16384 keys take 28.2, 43.9, 74.5 and 133 us, 5.6 TB/s for the differences and 14 us beside,
+// 4.8 of them the merge, 4 what comes before the first rows (lengths, the search, pages).  The same at head_dim 64, where a chunk
+// has half the bytes for as many scores: 128 contexts of 8192 keys, 14 heads on 2, 168 MB: 48-49 us, and 256 of them 83-86, 4.5
+// to 4.8 TB/s for the difference.  32 of 8192 keys, 64 heads on 4, whose scales are applied per group: 58 us for 169 MB.
 // ---------------------------------------------------------------------------
 template <int N>
 struct __attribute__((packed, aligned(4))) Words {
